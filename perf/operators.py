@@ -313,6 +313,7 @@ def _quantized(out, lse, fmt):
     amax = x.abs().amax(-1, keepdim=True)
     exp = torch.frexp(amax / _PEAK[fmt])[1].clamp(min=-126)
     e = torch.where(amax <= _PEAK[fmt] * _two_to(exp - 1), exp - 1, exp)
+    e = torch.where(amax > 0, e, torch.full_like(e, -127))
     y = x * _two_to(-e)
     elements = y.to(torch.float8_e4m3fn) if fmt == "e4m3" else torch.round(y).to(torch.int8)
     return elements.flatten(-2), (e + 127).to(torch.uint8).squeeze(-1), lse
