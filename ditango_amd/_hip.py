@@ -18,7 +18,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libditango_hip.so"
 HOST_PATH = LIB_PATH.parent / "_ditango_host.so"
 
-DT_BF16, DT_FP32, DT_FP16 = 0, 1, 2
+DT_BF16, DT_FP32, DT_FP16, DT_BLOCK_E4M3, DT_BLOCK_INT8 = 0, 1, 2, 3, 4
 DT_LSE_BHS, DT_LSE_BSH = 0, 1
 DT_NORM_NONE, DT_NORM_RMS, DT_NORM_LAYER = 0, 1, 2
 DT_ROPE_NONE, DT_ROPE_INTERLEAVED, DT_ROPE_HALVES = 0, 1, 2
@@ -119,6 +119,11 @@ _SIGNATURES = {
     "dt_qk_norm_rope": (ctypes.c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i32, c_i32, c_i32, c_i32,
                                        c_i32, c_vp, c_vp, c_f32, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32,
                                        _P(c_i32), c_i32, c_i32, c_f32, c_vp]),
+    "dt_attn_window_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, _P(c_i64), _P(c_i64), _P(c_i64),
+                                          c_vp, c_f32, c_i32, c_vp, c_i64, c_vp]),
+    "dt_merge_block_states": (ctypes.c_int, [c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp]),
+    "dt_qk_norm_rope_axes": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_i32, _P(ctypes.c_uint64),
+                                            _P(ctypes.c_uint8), c_i32, _P(c_i32), c_i32, c_i32, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -449,6 +454,14 @@ def attn_states_merge(q: torch.Tensor, k_chunks: Sequence[torch.Tensor], v_chunk
                                      lambda need: _stream_counters(q.device, need), _stream())
 
 
+def attn_window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int, right: int, frame: int, sinks: int, q_begin: int,
+                    kv_lens: Optional[torch.Tensor] = None, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                    lse: Optional[torch.Tensor] = None):
+    """(out, lse) of ``dt_attn_window_fwd``; -1 stands for a border that is not there and for queries behind the keys."""
+    _here(q, "q")
+    return _host().attn_window(q, k, v, left, right, frame, sinks, q_begin, kv_lens, float(softmax_scale), out, lse, attn_workspace(q.device), _stream())
+
+
 def attn_sched_merge(q: torch.Tensor, table, dev_compute_ids: torch.Tensor, dev_count: torch.Tensor, max_jobs: int,
                      slot_out: torch.Tensor, slot_lse: torch.Tensor, diag: int, diag_out: torch.Tensor, diag_lse: torch.Tensor,
                      dst_dtype: torch.dtype, workspace: Optional[torch.Tensor] = None, q_prescaled: bool = False, row: int = 0,
@@ -514,6 +527,20 @@ def zero_rows_from(t: torch.Tensor, first_row: torch.Tensor) -> None:
     _host().zero_rows_from(t, first_row, _stream())
 
 
+def _here(t: torch.Tensor, name: str) -> None:
+    """The launch goes to the current device's stream: the tensors have to live there."""
+    _require(t.is_cuda, f"{name} must live on the GPU")
+    _require(t.get_device() == _current_device(), f"{name} lives on device {t.get_device()} but device {_current_device()} is current: make the "
+             "tensors' device current for this call")
+
+
+def merge_blocks(states, dst) -> None:
+    """Merge of states of any format into ``dst``; a state is ``(out, None, lse)`` of 16 or 32 bits or ``(elements, scales, lse)`` of 8.  One
+    state is copied."""
+    _here(dst[0], "the destination")
+    _host().merge_blocks(states, dst, _stream())
+
+
 # ---------------------------------------------------------------------------------------------
 # K4: schedule builder, rel-L1 sums
 # ---------------------------------------------------------------------------------------------
@@ -577,3 +604,14 @@ def qkv_project(text: torch.Tensor, video: torch.Tensor, heads: int, projections
     """q, k and v ``[B,T+V,heads,64]`` of ``text`` ``[B,T,K]`` and ``video`` ``[B,V,K]`` in one launch.  ``projections``: three of
     ``(weight, bias, norm, norm_weight, norm_bias, eps, rope)``; cos/sin fp32 ``[V,64]`` for those with ``rope``."""
     return _host().qkv_project(text, video, heads, projections, cos, sin, _stream())
+
+
+def rotary_table(turns: Sequence[int], axis_of_pair: Sequence[int], rope: int, sections: Sequence[int]):
+    """What ``qk_norm_rope_axes`` needs to know of the axes, for a caller to keep."""
+    return _host().RotaryTable(turns, axis_of_pair, rope, sections)
+
+
+def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: float, rounding: int = 0):
+    """q and k in one launch of ``dt_qk_norm_rope_axes``; ``tensors``: one or two of ``(x, weight, bias, out, out_scale)``."""
+    _here(tensors[0][0], "q")
+    return _host().qk_norm_rope_axes(tensors, positions, table, norm, float(eps), rounding, _stream())

@@ -28,7 +28,7 @@ HOST_PATH = LIB_DIR / "_ditango_host.so"             # Python extension: the hos
 PROBES_PATH = LIB_DIR / "libditango_probes.so"
 DEMO_PATH = LIB_DIR / "dt_capi_demo"
 RESOURCES_PATH = LIB_DIR / "kernel_resources.json"   # per-kernel registers / scratch / occupancy of the last build
-SOURCES = ["attn_fwd.hip", "attn_f32.hip", "state_ops.hip", "producer.hip", "qkv.hip", "capi.hip"]
+SOURCES = ["attn_fwd.hip", "attn_f32.hip", "attn_window.hip", "state_ops.hip", "state_blocks.hip", "producer.hip", "rotary.hip", "qkv.hip", "capi.hip"]
 PROBE_SOURCES = ["probes.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -89,7 +89,7 @@ def build_lib(verbose: bool = False, extra_flags=()) -> Path:
                  "-lc10", "-ltorch_python", f"-L{LIB_DIR}", "-lditango_hip", "-Wl,-rpath,$ORIGIN", "-o", str(HOST_PATH)]
     if verbose:
         print(" ".join(host_compile), flush=True)
-    with ThreadPoolExecutor(max_workers=7) as ex:
+    with ThreadPoolExecutor(max_workers=8) as ex:
         host = ex.submit(_run, host_compile)
         all_objs = list(ex.map(compile_one, SOURCES + PROBE_SOURCES))
         host.result()

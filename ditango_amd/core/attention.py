@@ -37,7 +37,7 @@ from .. import _hip
 from ..logger import init_logger
 from ..timer import get_timer
 from ..utils import get_timestep
-from .cache import proCache
+from .cache import merge_any, merge_cached, proCache
 from .config import get_config
 from .parallel_state import LocalRingGroup
 from .redundancy_map import get_redundancy_map
@@ -215,8 +215,8 @@ class proAttention:
         self.target_chunk_id = self.local_chunk_id // self.isp_size  # core/attention.py:27
         # pointers of all ring positions (each starts at position // isp_size = 0); see plan_call
         self._ring_targets = [x // self.isp_size for x in range(self.isp_size)]
-        self.cache = proCache(isp_size=self.isp_size, layer_id=layer_id)
         cfg = get_config()
+        self.cache = proCache(isp_size=self.isp_size, layer_id=layer_id, state_format=getattr(cfg, "state_format", None))
         self.use_ditango = cfg.use_ditango if cfg is not None else True
         self.small_ring_stride = 8
         self.measure_memory = False
@@ -260,6 +260,8 @@ class proAttention:
         if not self.dry_run and not self._exact_f32:
             query, key, value = _kernel_input(query), _kernel_input(key), _kernel_input(value)
         if rm is not None and rm.chunk_mask is not None and not self.dry_run:
+            if self.cache.state_format is not None:
+                return self._attn_masked_blocks(query, key, value)
             return self._attn_masked_f32(query, key, value) if self._exact_f32 else self._attn_masked(query, key, value)
         timestep = get_timestep()
         N, r = self.isp_size, self.local_chunk_id
@@ -385,7 +387,7 @@ class proAttention:
                     self.cache.store_block(job.store_slot, o, l)      # rounded to bf16 on its way into the cache
                 merge_outs.append(o)
                 merge_lses.append(l)
-            out, lse = _hip.merge_states(merge_outs, merge_lses, dst_dtype=self.out_dtype, dst_lse_bsh=True)
+            out, lse = merge_cached(merge_outs, merge_lses, self.out_dtype)
             self.last_lse = lse
             return out
         # the local chunk is (key, value); the others come from the ring stand-in
@@ -401,9 +403,14 @@ class proAttention:
             else:
                 cu_q, cu_kv_of = segments
                 cu_kv = [cu_kv_of(c) for c in needed]
-        states, out, lse = _hip.attn_states_merge(query, [k for k, _ in kv], [v for _, v in kv], jobs, self._MAX_JOB_CHUNKS,
-                                                  merge_outs, merge_lses, which, self.out_dtype, _hip.attn_workspace(query.device),
-                                                  self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
+        ks, vs, workspace = [k for k, _ in kv], [v for _, v in kv], _hip.attn_workspace(query.device)
+        if self.cache.state_format is None:
+            states, out, lse = _hip.attn_states_merge(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, merge_outs, merge_lses, which, self.out_dtype,
+                                                      workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
+        else:
+            states = _hip.attn_states(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
+            fresh = [states[i] for i in which]
+            out, lse = merge_cached(merge_outs + [o for o, _ in fresh], merge_lses + [l for _, l in fresh], self.out_dtype)
         for job, i in zip(plan.jobs, which):
             if job.store_slot is not None:
                 self.cache.store_block(job.store_slot, *states[i])  # :207-211
@@ -517,6 +524,46 @@ class proAttention:
             outs.append(o)
             lses.append(s)
         out, lse = _hip.merge_states(outs, lses, dst_dtype=self.out_dtype, dst_lse_bsh=True)
+        self.last_lse = lse
+        rm.record_out_redundancy(timestep=t, layer_id=l, curr_out=out)
+        return out
+
+    def _attn_masked_blocks(self, query, key, value) -> torch.Tensor:
+        """Mask mode with 8-bit states: the fresh ones are merged as they are and quantised into the arena."""
+        rm = get_redundancy_map()
+        t, l = get_timestep(), self.layer_id
+        C, diag = rm.chunk_mask.shape[2], rm.mask_diag
+        B, Sq, H, D = query.shape
+        cache = self.cache
+        row = rm.chunk_mask[t, l]
+        have_arena = cache.ensure_arena(C, B, Sq, H, D, query.device)
+        compute = ([diag] if 0 <= diag < C else []) + [c for c in range(C) if c != diag and (row[c] == 0 or not have_arena)]
+        reuse = [c for c in range(C) if c not in compute]
+        for c in reuse:
+            if not cache.arena_valid[c]:
+                raise RuntimeError(f"T{t}L{l}: mask asks to reuse chunk {c} but no state was ever stored for it")
+        local = self.local_chunk_id if (self.local_chunk_id == diag and key is not None) else -1
+        if not compute:
+            fresh = []
+        elif self._exact_f32:
+            fresh = self._job_states_f32(query, [(c,) for c in compute], key if local >= 0 else None, value)
+        else:
+            kv = [(key, value) if c == local else self.group.kv_chunk(c) for c in compute]
+            cu_q = cu_kv = dev_seg = None
+            if isinstance(self._segments, _DeviceSegmentSource):
+                dev_seg = self._segments.over(compute)
+            elif self._segments is not None:
+                cu_q, cu_kv_of = self._segments
+                cu_kv = [cu_kv_of(c) for c in compute]
+            fresh = _hip.attn_states(query, [_as4d(k, B) for k, _ in kv], [_as4d(v, B) for _, v in kv], [[i] for i in range(len(compute))],
+                                     self._MAX_JOB_CHUNKS, _hip.attn_workspace(query.device), self.q_prescaled, cu_q, cu_kv, dev_seg,
+                                     _kernel_input)
+        out, lse = merge_any([cache.arena_block(c) for c in reuse] + list(fresh), dst_dtype=self.out_dtype, dst_lse_bsh=True)
+        if have_arena:
+            for c, state in zip(compute, fresh):
+                if c != diag:
+                    merge_any([state], dst=cache.arena_block(c))
+                    cache.arena_valid[c] = True
         self.last_lse = lse
         rm.record_out_redundancy(timestep=t, layer_id=l, curr_out=out)
         return out

@@ -12,9 +12,13 @@ Two storage forms:
   (``_merge_blocks``) is one fused merge launch per new block, written in place;
 * a contiguous arena ``[C, B, Sq, H, D]`` / ``[C, B, H, Sq]`` plus one scratch
   state for the mask mode, addressed by chunk id from device-side schedules.
+
+With ``state_format`` ``"e4m3"`` or ``"int8"`` (also a key of the configuration) cached states take 8 bits an element and a scale for every
+32 (``BlockState``): half the memory again, and half the bytes of a merge.  Stores quantise, merges and loads read them as they are.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Callable, List, Optional, Tuple
 
 import torch
@@ -31,8 +35,66 @@ def _allocated_mb() -> float:
     return _hip._host().allocated_bytes(torch.cuda.current_device()) / (1024 * 1024) if torch.cuda.is_initialized() else 0.0
 
 
+STATE_FORMATS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+BLOCK = 32   # elements along D that share a scale
+
+
+@dataclass(frozen=True)
+class BlockState:
+    """An attention state in 8 bits: ``elements`` ``[B,S,H,D]`` (``torch.float8_e4m3fn`` or ``torch.int8``), ``scales`` uint8 ``[B,S,H,D/32]``, ``lse``
+    fp32 as in any state.  A value is ``element * 2 ** (scale - 127)``; the scale is the smallest for which the block's largest magnitude is
+    not above the format's largest element (448, 127).  Scale 255 marks a block that held an infinite or undefined value and reads as NaN."""
+    elements: torch.Tensor
+    scales: torch.Tensor
+    lse: torch.Tensor
+
+    @classmethod
+    def empty(cls, shape, state_format: str, device) -> "BlockState":
+        B, S, H, D = shape
+        return cls(torch.empty((B, S, H, D), dtype=STATE_FORMATS[state_format], device=device),
+                   torch.empty((B, S, H, D // BLOCK), dtype=torch.uint8, device=device),
+                   torch.empty((B, H, S), dtype=torch.float32, device=device))
+
+    @property
+    def shape(self):
+        return self.elements.shape
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.elements, self.scales, self.lse))
+
+
+def _parts(state):
+    return (state.elements, state.scales, state.lse) if isinstance(state, BlockState) else (state[0], None, state[1])
+
+
+def merge_any(states, *, dst=None, dst_dtype: torch.dtype = torch.float32, dst_lse_bsh: bool = False):
+    """N-way LSE merge of states of any format: each a ``BlockState`` or ``(out, lse)`` with out contiguous ``[B,S,H,D]`` (bf16, fp16, fp32) and
+    lse fp32 in ``[B,H,S]`` or ``[B,S,H(,1)]`` storage.  One pass over HBM for up to ``DT_MAX_MERGE`` states; a single one is copied.  Into ``dst`` --
+    a ``BlockState`` or ``(out, lse)``, one of the states among them -- or a new ``(out, lse)`` of ``dst_dtype``.  Returns the destination."""
+    if not states:
+        raise ValueError("need at least one state")
+    first = _parts(states[0])[0]
+    if dst is None:
+        B, S, H, D = first.shape
+        dst = (torch.empty((B, S, H, D), dtype=dst_dtype, device=first.device),
+               torch.empty((B, S, H, 1) if dst_lse_bsh else (B, H, S), dtype=torch.float32, device=first.device))
+    _hip.merge_blocks([_parts(s) for s in states], _parts(dst))
+    return dst
+
+
+def merge_cached(outs, lses, dst_dtype: torch.dtype):
+    """``_hip.merge_states`` with a ``[B,S,H,1]`` lse of what a cache hands out: tensors, or ``BlockState`` in the place of ``out``."""
+    if any(isinstance(o, BlockState) for o in outs):
+        return merge_any([o if isinstance(o, BlockState) else (o, l) for o, l in zip(outs, lses)], dst_dtype=dst_dtype, dst_lse_bsh=True)
+    return _hip.merge_states(outs, lses, dst_dtype=dst_dtype, dst_lse_bsh=True)
+
+
 class proCache:
-    def __init__(self, isp_size: int, layer_id: int):
+    def __init__(self, isp_size: int, layer_id: int, state_format: Optional[str] = None):
+        if state_format is not None and state_format not in STATE_FORMATS:
+            raise ValueError(f"state_format must be None or one of {sorted(STATE_FORMATS)}, got {state_format!r}")
+        self.state_format = state_format
         self.isp_size = isp_size
         self.curr_isp_stride = isp_size
         self.curr_block_num = isp_size
@@ -47,6 +109,7 @@ class proCache:
         # mask-mode arena
         self.arena_out: Optional[torch.Tensor] = None
         self.arena_lse: Optional[torch.Tensor] = None
+        self.arena_scales: Optional[torch.Tensor] = None   # under a state_format
         self.diag_out: Optional[torch.Tensor] = None
         self.diag_lse: Optional[torch.Tensor] = None
         self.arena_valid: List[bool] = []
@@ -76,8 +139,12 @@ class proCache:
         reference sizes an fp32 ``[..., D+1]`` tensor by allocating it, cache.py:89-101.)"""
         if self.block_size_mb is None:
             rows = tensor.numel() // tensor.shape[-1]
-            self.block_size_mb = rows * (2 * tensor.shape[-1] + 4) / (1024 ** 2)
+            self.block_size_mb = rows * self._row_bytes(tensor.shape[-1]) / (1024 ** 2)
         return self.block_size_mb
+
+    def _row_bytes(self, D: int) -> int:
+        """Bytes of a cached (token, head)."""
+        return 2 * D + 4 if self.state_format is None else D + D // BLOCK + 4
 
     def pass_memory_check(self, next_isp_stride: int, layer_id: int) -> bool:
         """cache.py:103-128"""
@@ -87,7 +154,9 @@ class proCache:
         for i, block in enumerate(self.out_block_cache):
             if block is not None:
                 active += 1
-                if self.block_size_mb is None and torch.is_tensor(block):  # (dry runs keep chunk-id tuples)
+                if self.block_size_mb is None and isinstance(block, BlockState):
+                    self.block_size_mb = block.nbytes / (1024 ** 2)
+                elif self.block_size_mb is None and torch.is_tensor(block):  # (dry runs keep chunk-id tuples)
                     mb = block.element_size() * block.nelement() / (1024 ** 2)
                     if self.lse_block_cache[i] is not None:
                         mb += self.lse_block_cache[i].element_size() * self.lse_block_cache[i].nelement() / (1024 ** 2)
@@ -126,7 +195,11 @@ class proCache:
             if len(outs) == 1:
                 new_out[i], new_lse[i] = outs[0], lses[0]
             elif len(outs) > 1:
-                _hip.merge_states(outs, lses, dst_out=outs[0], dst_lse=lses[0])
+                if any(isinstance(o, BlockState) for o in outs):
+                    merge_any([o if isinstance(o, BlockState) else (o, l) for o, l in zip(outs, lses)],
+                              dst=outs[0] if isinstance(outs[0], BlockState) else (outs[0], lses[0]))
+                else:
+                    _hip.merge_states(outs, lses, dst_out=outs[0], dst_lse=lses[0])
                 new_out[i], new_lse[i] = outs[0], lses[0]
         self.out_block_cache = new_out
         self.lse_block_cache = new_lse
@@ -154,6 +227,7 @@ class proCache:
             self.lse_block_cache[next_target_block_id] = None
 
     def get_block(self, block_id: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """(out, lse) of block ``block_id``, ``out`` a ``BlockState`` under a ``state_format``."""
         if block_id >= len(self.out_block_cache):
             logger.error(f"{get_timestep()} | Cache is not ready but trying to get cached value.")
         return self.out_block_cache[block_id], self.lse_block_cache[block_id]
@@ -162,8 +236,15 @@ class proCache:
         """Keep ``(out, lse)`` as block ``block_id``.  A state already in cache form
         (contiguous bf16 or fp16 ``out``, contiguous fp32 ``[B,H,S]`` ``lse`` -- what the
         attention kernel writes for a model that runs in that dtype) is adopted as is; anything
-        else goes through one ``dt_cache_store`` pass into fresh cache-form (bf16) tensors."""
+        else goes through one ``dt_cache_store`` pass into fresh cache-form (bf16) tensors.  Under a ``state_format`` it is
+        quantised in one pass, whatever it comes in."""
         B, S, H, D = out.shape
+        if self.state_format is not None:
+            state = BlockState.empty((B, S, H, D), self.state_format, out.device)
+            merge_any([(out.contiguous(), lse)], dst=state)
+            self.out_block_cache[block_id] = state
+            self.lse_block_cache[block_id] = state.lse
+            return
         in_cache_form = (out.dtype in _hip.HALF_DTYPES and out.is_contiguous() and lse.dtype == torch.float32
                          and tuple(lse.shape) == (B, H, S) and lse.is_contiguous())
         if not in_cache_form:
@@ -180,6 +261,8 @@ class proCache:
         o, l = self.get_block(block_id)
         if l is None:
             return None, None
+        if isinstance(o, BlockState):
+            return merge_any([o], dst_dtype=dtype, dst_lse_bsh=True)
         return _hip.cache_load(o, l, dtype, dst_lse_bsh=True)
 
     def clear(self) -> None:
@@ -191,7 +274,7 @@ class proCache:
         ``clear`` keeps them): frees the HBM a finished generation holds."""
         self.out_block_cache = [None] * self.curr_block_num
         self.lse_block_cache = [None] * self.curr_block_num
-        self.arena_out = self.arena_lse = self.diag_out = self.diag_lse = None
+        self.arena_out = self.arena_lse = self.diag_out = self.diag_lse = self.arena_scales = None
         self.arena_valid = []
         self.arena_refused = None
 
@@ -204,13 +287,16 @@ class proCache:
         (cache.py:103-128) -- and a layer without arena recomputes every chunk on every call, which is
         what the reference's guard falls back to (core/attention.py:97-98: stride forced to N)."""
         shape = (n_chunks, B, Sq, H, D)
+        if self.state_format is not None:
+            dtype = STATE_FORMATS[self.state_format]
         if (self.arena_out is not None and self.arena_out.shape == shape and self.arena_out.device == device
                 and self.arena_out.dtype == dtype):
             return True
         if self.arena_refused == shape:
             return False
-        self.arena_out = self.arena_lse = self.diag_out = self.diag_lse = None
-        need_mb = (n_chunks + 1) * B * Sq * H * (2 * D + 4) / (1024 ** 2)
+        self.arena_out = self.arena_lse = self.diag_out = self.diag_lse = self.arena_scales = None
+        # (8-bit states are quantised from fresh ones of their own, the diagonal's among them)
+        need_mb = (n_chunks + (self.state_format is None)) * B * Sq * H * self._row_bytes(D) / (1024 ** 2)
         now = self.memory_probe()
         if now + need_mb > self.memory_constraint:
             logger.warning(f"T{get_timestep()}L{self.layer_id} | Memory check failed: {now + need_mb:.0f} > "
@@ -220,10 +306,18 @@ class proCache:
             return False
         self.arena_out = torch.empty(shape, dtype=dtype, device=device)   # bf16, or fp16 for a model run in fp16
         self.arena_lse = torch.empty((n_chunks, B, H, Sq), dtype=torch.float32, device=device)
+        if self.state_format is not None:
+            self.arena_scales = torch.empty((n_chunks, B, Sq, H, D // BLOCK), dtype=torch.uint8, device=device)
+            self.arena_valid = [False] * n_chunks
+            return True
         self.diag_out = torch.empty((B, Sq, H, D), dtype=dtype, device=device)
         self.diag_lse = torch.empty((B, H, Sq), dtype=torch.float32, device=device)
         self.arena_valid = [False] * n_chunks
         return True
+
+    def arena_block(self, c: int) -> BlockState:
+        """Slot ``c`` of an 8-bit arena."""
+        return BlockState(self.arena_out[c], self.arena_scales[c], self.arena_lse[c])
 
     def report_cache_status(self, layer_id: int) -> None:
         """cache.py:131-207, condensed."""

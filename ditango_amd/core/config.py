@@ -29,6 +29,7 @@ _DEFAULTS = {
     "use_pab": False,
     "stride_dividers": [8, 4, 2, 1],
     "stride_percentiles": [20, 50, 80],
+    "state_format": None,   # cached attention states in 8 bits: "e4m3" or "int8" (core/cache.py)
 }
 
 

@@ -822,6 +822,142 @@ std::vector<Tensor> qkv_project(const Tensor& text_rows, const Tensor& video, in
   return outs;
 }
 
+// ---- operators of long videos -------------------------------------------------------------------------------------
+
+bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && b.is_cuda() && a.device() == b.device(); }
+
+// ditango_amd._hip.attn_window_fwd
+std::pair<Tensor, Tensor> attn_window(const Tensor& q, const Tensor& k, const Tensor& v, int32_t left, int32_t right, int32_t frame, int32_t sinks,
+                                      int32_t q_begin, const std::optional<Tensor>& kv_lens, double scale, std::optional<Tensor> out,
+                                      std::optional<Tensor> lse, const std::optional<Tensor>& workspace, uint64_t stream) {
+  const Dims d = check_bshd(q, {"q"}), dk = check_bshd(k, {"k"}), dv = check_bshd(v, {"v"});
+  REQUIRE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+  REQUIRE(same_device(q, k) && same_device(q, v), "q, k and v must be on one device");
+  REQUIRE(dk.B == d.B && dk.D == d.D && dv.B == dk.B && dv.S == dk.S && dv.H == dk.H && dv.D == dk.D && dk.H > 0 && d.H % dk.H == 0,
+          "k and v must be [B,Sk,Hk,D] with the batch and head dim of q and a number of heads that divides that of q");
+  REQUIRE(d.S < (1ll << 31) && dk.S < (1ll << 31), "too many tokens");
+  if (!out) out = new_out(d, q.scalar_type(), q);
+  if (!lse) lse = new_lse(d, false, q);
+  check_state(*out, *lse, d, q.scalar_type(), {"out"}, {"lse"});
+  REQUIRE(same_device(q, *out) && same_device(q, *lse), "out and lse must be on the device of q");
+  if (kv_lens)
+    REQUIRE(same_device(q, *kv_lens) && kv_lens->scalar_type() == at::kInt && kv_lens->is_contiguous() && shape_is(*kv_lens, {d.B}),
+            "kv_lens must be contiguous int32 [B] on the device of q");
+  if (q.numel() == 0) return {*out, *lse};
+  // (strides of dimensions of size one do not matter, and may be anything)
+  auto strides = [](const Tensor& t, int64_t (&s)[3]) {
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+  };
+  int64_t qs[3], ks[3], vs[3];
+  strides(q, qs);
+  strides(k, ks);
+  strides(v, vs);
+  const dt_window w = {left, right, frame, sinks, q_begin, static_cast<const int32_t*>(ptr(kv_lens))};
+  CALL(dt_attn_window_fwd, ptr(q), ptr(k), ptr(v), ptr(*out), static_cast<float*>(ptr(*lse)), (int32_t)d.B, (int32_t)d.S, (int32_t)dk.S, (int32_t)d.H,
+       (int32_t)dk.H, (int32_t)d.D, qs, ks, vs, &w, (float)scale, q.scalar_type() == at::kHalf ? DT_ATTN_FP16 : 0, ptr(workspace), bytes_of(workspace),
+       stream_of(stream));
+  return {*out, *lse};
+}
+
+// A state of any format: (out, lse) of 16 or 32 bits, or (elements, scales, lse) of 8.
+struct AnyState {
+  Tensor out, lse;
+  std::optional<Tensor> scales;
+};
+dt_state any_state(const AnyState& s, const Dims& d, const Tensor& like, const Name& name) {
+  int32_t dtype;
+  if (s.scales) {
+    const auto t = s.out.scalar_type();
+    REQUIRE(t == at::kFloat8_e4m3fn || t == at::kChar, name.str(), ": the elements of an 8-bit state must be float8_e4m3fn or int8");
+    dtype = t == at::kChar ? DT_BLOCK_INT8 : DT_BLOCK_E4M3;
+    REQUIRE(same_device(like, *s.scales) && s.scales->scalar_type() == at::kByte && s.scales->is_contiguous() && shape_is(*s.scales, {d.B, d.S, d.H, d.D / 32}),
+            name.str(), ": scales must be contiguous uint8 [B,Sq,H,D/32]");
+  } else {
+    dtype = dtype_code(s.out);
+  }
+  REQUIRE(same_device(like, s.out) && s.out.is_contiguous() && shape_is(s.out, {d.B, d.S, d.H, d.D}), name.str(),
+          " must be contiguous [B,Sq,H,D], all of them on one GPU");
+  REQUIRE(same_device(like, s.lse), name.str(), ": lse must be on the GPU of the states");
+  return {ptr(s.out), s.scales ? static_cast<uint8_t*>(ptr(*s.scales)) : nullptr, static_cast<float*>(ptr(s.lse)), dtype, lse_layout(s.lse, d.B, d.S, d.H)};
+}
+
+// Merge of states of any format into `dst`; more than one launch folds run in rounds through a running fp32 state.
+void merge_blocks(const std::vector<std::tuple<Tensor, std::optional<Tensor>, Tensor>>& states, const std::tuple<Tensor, std::optional<Tensor>, Tensor>& into,
+                  uint64_t stream) {
+  REQUIRE(!states.empty(), "need at least one state");
+  const Tensor& first = std::get<0>(states[0]);
+  REQUIRE(first.is_cuda() && first.dim() == 4, "states must be [B,Sq,H,D] on the GPU");
+  const Dims d{first.size(0), first.size(1), first.size(2), first.size(3)};
+  auto state = [&](const std::tuple<Tensor, std::optional<Tensor>, Tensor>& t, const Name& name) {
+    return any_state({std::get<0>(t), std::get<2>(t), std::get<1>(t)}, d, first, name);
+  };
+  const dt_state dst = state(into, {"destination"});
+  std::vector<dt_state> list;
+  Tensor run_out, run_lse;
+  for (size_t i = 0; i < states.size(); ++i) list.push_back(state(states[i], {"states", (int64_t)i}));
+  if (first.numel() == 0) return;
+  size_t at = 0;
+  while (list.size() - at > DT_MAX_MERGE) {
+    const bool again = run_out.defined();
+    if (!again) {
+      run_out = new_out(d, at::kFloat, first);
+      run_lse = new_lse(d, false, first);
+    }
+    const dt_state run = {ptr(run_out), nullptr, static_cast<float*>(ptr(run_lse)), DT_FP32, DT_LSE_BHS};
+    CALL(dt_merge_block_states, DT_MAX_MERGE, list.data() + at, &run, d.B, d.S, d.H, d.D, stream_of(stream));
+    at += DT_MAX_MERGE - 1;      // the last one's place takes the running state
+    list[at] = run;
+  }
+  CALL(dt_merge_block_states, (int32_t)(list.size() - at), list.data() + at, &dst, d.B, d.S, d.H, d.D, stream_of(stream));
+}
+
+// How a row's pairs turn: built once for a RotaryAxes object.
+struct RotaryTable {
+  std::vector<uint64_t> turns;
+  std::vector<uint8_t> axis;
+  int32_t rope;
+  std::vector<int32_t> sections;
+};
+
+// ditango_amd._hip.qk_norm_rope_axes.  A tensor: (x, weight, bias, out, scale).
+using RotaryRows = std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>, double>;
+std::vector<Tensor> qk_norm_rope_axes(const std::vector<RotaryRows>& tensors, const Tensor& positions, const RotaryTable& table, int32_t norm, double eps,
+                                      int32_t rounding, uint64_t stream) {
+  REQUIRE(tensors.size() == 1 || tensors.size() == 2, "one or two tensors are needed");
+  const Tensor& first = std::get<0>(tensors[0]);
+  const Dims d = check_bshd(first, {"q"});
+  dt_rotary_rows rows[2] = {};
+  std::vector<Tensor> outs;
+  const bool narrow = rounding & DT_WEIGHTS_16;
+  for (size_t i = 0; i < tensors.size(); ++i) {
+    const auto& [x, weight, bias, given, scale] = tensors[i];
+    const Dims dx = check_bshd(x, {i ? "k" : "q"});
+    REQUIRE(dx.B == d.B && dx.S == d.S && dx.D == d.D && x.scalar_type() == first.scalar_type() && same_device(x, first),
+            "q and k must have one dtype, device, batch, length and head dim");
+    for (const auto* t : {&weight, &bias})
+      REQUIRE(!*t || (same_device(**t, first) && (*t)->scalar_type() == (narrow ? x.scalar_type() : at::kFloat) && (*t)->is_contiguous() && (*t)->numel() == d.D),
+              "norm parameters must be ", narrow ? "of the tensors' dtype" : "fp32", ", [D] on the GPU");
+    outs.push_back(given ? *given : new_out(dx, x.scalar_type(), x));
+    const Tensor& y = outs.back();
+    REQUIRE(same_device(y, first) && y.scalar_type() == x.scalar_type() && y.is_contiguous() && shape_is(y, {dx.B, dx.S, dx.H, dx.D}),
+            "out must be a contiguous [B,S,H,D] in the dtype of its input");
+    rows[i] = {ptr(x), dx.B > 1 ? x.stride(0) : 0, dx.S > 1 ? x.stride(1) : 0, dx.H > 1 ? x.stride(2) : 0, ptr(y), ptr(weight), ptr(bias),
+               (int32_t)dx.H, (float)scale};
+  }
+  const int64_t n_axes = positions.size(-1);
+  REQUIRE(same_device(positions, first) && positions.scalar_type() == at::kInt && positions.is_contiguous() &&
+              (shape_is(positions, {d.S, n_axes}) || shape_is(positions, {d.B, d.S, n_axes})),
+          "positions must be contiguous int32 [S, axes] or [B, S, axes] on the device of q");
+  REQUIRE((int64_t)table.turns.size() == d.D / 2 && table.axis.size() == table.turns.size(), "the axes do not cover the head dim ", std::to_string(d.D));
+  REQUIRE(d.S < (1ll << 31) && d.B < (1ll << 31), "too many tokens");
+  if (first.numel() == 0) return outs;
+  if (first.scalar_type() == at::kHalf) rounding |= DT_IO_FP16;
+  CALL(dt_qk_norm_rope_axes, rows, (int32_t)tensors.size(), (int32_t)d.B, (int32_t)d.S, (int32_t)d.D, norm, (float)eps,
+       static_cast<const int32_t*>(ptr(positions)), positions.dim() == 3 ? positions.stride(0) : 0, (int32_t)n_axes, table.turns.data(),
+       table.axis.data(), table.rope, table.sections.data(), (int32_t)table.sections.size(), rounding, stream_of(stream));
+  return outs;
+}
+
 // ---- host state of a call -------------------------------------------------------------------------------------
 
 // Element [row, col] of a 2-D int64 tensor in host memory, or nothing where it is another one or the place is not there.
@@ -890,6 +1026,13 @@ PYBIND11_MODULE(_ditango_host, m) {
   m.def("zero_rows_from", &zero_rows_from);
   m.def("qk_norm_rope", &qk_norm_rope);
   m.def("qkv_project", &qkv_project);
+  m.def("attn_window", &attn_window);
+  m.def("merge_blocks", &merge_blocks);
+  py::class_<RotaryTable>(m, "RotaryTable")
+      .def(py::init([](const std::vector<uint64_t>& turns, const std::vector<uint8_t>& axis, int32_t rope, const std::vector<int32_t>& sections) {
+        return RotaryTable{turns, axis, rope, sections};
+      }));
+  m.def("qk_norm_rope_axes", &qk_norm_rope_axes);
   m.def("element", &element);
   m.def("allocated_bytes", &allocated_bytes);
 }

@@ -1,0 +1,304 @@
+// QK norm and rotation by positions on several axes (gfx950): what producer.hip does with cos / sin tables, for q and k in one launch and
+// from the tokens' int32 positions.
+//
+// A pair (a, b) of a head row at position n on its axis turns by t = n f / 2 pi full turns.  f / 2 pi comes as a 64-bit fraction F of a
+// turn, so n F mod 2^64 is the angle of any 32-bit position to 2^-32 of a turn: integers have no range reduction to lose bits in.  Its upper half, as
+// a signed fraction, splits into the nearest quarter turn and x = 2 pi r, |x| <= pi / 4, and
+//   sin x = x - x^3/3! + x^5/5! - x^7/7! + x^9/9!       (next term 1.8e-9)
+//   cos x = 1 - x^2/2! + x^4/4! - x^6/6! + x^8/8! - x^10/10!  (next term 1.2e-10).
+//
+// HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row, so that an angle is computed once
+// for the kHeads heads of a lane group: 8 neighbours with interleaved pairs, two runs of 4 half a section apart with rotate-half.
+#include "producer_math.h"
+
+namespace dt {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+constexpr int kHeads = 4;         // heads of a lane group
+constexpr int kMostAxes = 8;
+
+struct Rows {
+  const uint16_t* x;
+  uint16_t* y;
+  int64_t sb, ss, sh;
+  const void *w, *bias;
+  float scale;
+  int32_t H, groups;              // groups of kHeads heads
+};
+struct RotaryArgs {
+  Rows rows[2];
+  const int32_t* pos;
+  int64_t pos_sb;
+  int32_t S, n_axes, norm, w16, halves;
+  float eps;
+  uint32_t items;                 // B * S * groups of both
+  Quotient by_groups, by_s;
+  uint8_t a0[16], b0[16];         // first element of a lane's two runs of 4 (halves)
+  uint8_t axis[64];               // of pair 4 lane + i
+  uint64_t turns[64];
+};
+
+// sin and cos of (t / 2^32) turns.
+__device__ __forceinline__ void sin_cos(uint32_t t, float& sn, float& cs) {
+  const uint32_t q = (t + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(t - (q << 30)) * 1.46291807926715968e-9f;   // 2 pi / 2^32
+  const float z = x * x;
+  float s = __builtin_fmaf(z, 2.7557319224e-6f, -1.9841269841e-4f);
+  s = __builtin_fmaf(z, s, 8.3333333333e-3f);
+  s = __builtin_fmaf(z, s, -1.6666666667e-1f);
+  s = __builtin_fmaf(z * x, s, x);
+  float c = __builtin_fmaf(z, -2.7557319224e-7f, 2.4801587302e-5f);
+  c = __builtin_fmaf(z, c, -1.3888888889e-3f);
+  c = __builtin_fmaf(z, c, 4.1666666667e-2f);
+  c = __builtin_fmaf(z, c, -0.5f);
+  c = __builtin_fmaf(z, c, 1.f);
+  const float u = q & 1 ? c : s, v = q & 1 ? s : c;      // quarter turns: (s, c) -> (c, -s) -> (-s, -c) -> (-c, s)
+  sn = q & 2 ? -u : u;
+  cs = (q + 1) & 2 ? -v : v;
+}
+
+template <bool kHalf>
+__device__ __forceinline__ void load_weights4(const void* base, bool w16, int d, float* v) {
+  if (w16) {   // uniform
+    const u32x2 r = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(base) + d);
+    float u[8];
+    unpack8<kHalf>(u32x4{r.x, r.y, 0u, 0u}, u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = u[i];
+  } else {
+    const f32x4 r = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = r[i];
+  }
+}
+
+template <int D, bool kHalf, bool kHalves>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const RotaryArgs a) {
+  constexpr int G = D / 8;
+  const int c = threadIdx.x % G;
+  const uint32_t item = blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  if (item >= a.items) return;   // a lane group leaves as a whole; the exchanges below stay inside a group
+  const uint32_t bs = quotient(item, a.by_groups);
+  int hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups));
+  const bool second = hg >= a.rows[0].groups;
+  if (second) hg -= a.rows[0].groups;
+  const Rows& t = second ? a.rows[1] : a.rows[0];
+  const uint32_t b = quotient(bs, a.by_s), s = bs - b * (uint32_t)a.S;
+  const int h0 = hg * kHeads, nh = min(t.H - h0, kHeads);
+  const int ea = kHalves ? a.a0[c] : 8 * c, eb = kHalves ? a.b0[c] : 8 * c + 4;
+
+  const uint16_t* xp = t.x + (int64_t)b * t.sb + (int64_t)s * t.ss + (int64_t)h0 * t.sh;
+  u32x4 raw[kHeads];
+#pragma unroll
+  for (int r = 0; r < kHeads; ++r) {
+    raw[r] = u32x4{0, 0, 0, 0};
+    if (r < nh) {
+      const uint16_t* p = xp + (int64_t)r * t.sh;
+      if constexpr (kHalves) {
+        const u32x2 lo = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + ea));
+        const u32x2 hi = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + eb));
+        raw[r] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      } else {
+        raw[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + ea));
+      }
+    }
+  }
+  // the angles of this lane's pairs; t mod 2^32 of the upper half of n F
+  float sn[4], cs[4];
+  {
+    const int32_t* pos = a.pos + (int64_t)b * a.pos_sb + (int64_t)s * a.n_axes;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t n = pos[a.axis[4 * c + i]];
+      const uint64_t f = a.turns[4 * c + i];
+      const uint32_t lo = (uint32_t)f, hi = (uint32_t)(f >> 32);
+      sin_cos(__umulhi((uint32_t)n, lo) + (uint32_t)n * hi - (n < 0 ? lo : 0u), sn[i], cs[i]);
+    }
+  }
+  float w[8], bias[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = 1.f;
+    bias[i] = 0.f;
+  }
+  if (a.norm != DT_NORM_NONE && t.w) {
+    load_weights4<kHalf>(t.w, a.w16 != 0, ea, w);
+    load_weights4<kHalf>(t.w, a.w16 != 0, eb, w + 4);
+  }
+  if (a.norm == DT_NORM_LAYER && t.bias) {
+    load_weights4<kHalf>(t.bias, a.w16 != 0, ea, bias);
+    load_weights4<kHalf>(t.bias, a.w16 != 0, eb, bias + 4);
+  }
+  float mean[kHeads] = {}, rs[kHeads] = {}, ss[kHeads];
+  if (a.norm != DT_NORM_NONE) {   // uniform
+#pragma unroll
+    for (int r = 0; r < kHeads; ++r) {
+      float v[8];
+      unpack8<kHalf>(raw[r], v);
+      if (a.norm == DT_NORM_LAYER) {
+        mean[r] = row_sum<G>(v) * (1.0f / D);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] -= mean[r];
+      }
+      ss[r] = row_squares<G>(v);
+    }
+    inverse_rms4<D>(ss[0], ss[1], ss[2], ss[3], a.eps, rs);
+  }
+  uint16_t* yp = t.y + ((int64_t)bs * t.H + h0) * D;
+#pragma unroll
+  for (int r = 0; r < kHeads; ++r) {
+    if (r >= nh) break;
+    float v[8];
+    unpack8<kHalf>(raw[r], v);
+    if (a.norm != DT_NORM_NONE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = layer_norm(v[i], mean[r], rs[r], w[i], bias[i]);   // (rms: mean 0, bias 0)
+    }
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ia = kHalves ? i : 2 * i, ib = kHalves ? 4 + i : 2 * i + 1;
+      y[ia] = rotated(v[ia], -v[ib], cs[i], sn[i]) * t.scale;
+      y[ib] = rotated(v[ib], v[ia], cs[i], sn[i]) * t.scale;
+    }
+    const u32x4 o = u32x4{pack2<kHalf>(y[0], y[1]), pack2<kHalf>(y[2], y[3]), pack2<kHalf>(y[4], y[5]), pack2<kHalf>(y[6], y[7])};
+    uint16_t* q = yp + r * D;
+    if constexpr (kHalves) {
+      __builtin_nontemporal_store(u32x2{o.x, o.y}, reinterpret_cast<u32x2*>(q + ea));
+      __builtin_nontemporal_store(u32x2{o.z, o.w}, reinterpret_cast<u32x2*>(q + eb));
+    } else {
+      __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(q + ea));
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace dt
+
+using namespace dt;
+
+extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, int32_t S, int32_t D, int32_t norm, float eps,
+                                    const int32_t* positions, int64_t pos_stride_b, int32_t n_axes, const uint64_t* turns,
+                                    const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections, int32_t n_sections,
+                                    int32_t rounding, void* stream) {
+  if (!rows || n_rows < 1 || n_rows > 2 || B <= 0 || S <= 0) {
+    set_error("need one or two tensors and positive B and S (got %d, %d, %d)", n_rows, B, S);
+    return DT_ERR_INVALID;
+  }
+  if (D != 64 && D != 128) {
+    set_error("head dim %d not built (64 and 128 are)", D);
+    return DT_ERR_UNSUPPORTED;
+  }
+  if (norm < DT_NORM_NONE || norm > DT_NORM_LAYER || (rope != DT_ROPE_INTERLEAVED && rope != DT_ROPE_HALVES) ||
+      (rounding & ~(DT_IO_FP16 | DT_WEIGHTS_16))) {
+    set_error("bad norm / rope / rounding code (%d, %d, %d)", norm, rope, rounding);
+    return DT_ERR_INVALID;
+  }
+  if (!positions || n_axes < 1 || n_axes > kMostAxes || !turns || !axis_of_pair || pos_stride_b < 0) {
+    set_error("positions, turns and axis_of_pair must be non-null, with 1..%d axes and a stride that is not negative", kMostAxes);
+    return DT_ERR_INVALID;
+  }
+  RotaryArgs a{};
+  for (int j = 0; j < D / 2; ++j)
+    if (axis_of_pair[j] >= n_axes) {
+      set_error("pair %d is on axis %d of %d", j, axis_of_pair[j], n_axes);
+      return DT_ERR_INVALID;
+    }
+  int pair_of[64];      // of run element 4 lane + i
+  if (rope == DT_ROPE_HALVES) {
+    const int32_t whole[1] = {D};
+    if (n_sections == 0) {
+      sections = whole;
+      n_sections = 1;
+    }
+    if (n_sections < 0 || n_sections > DT_MAX_SECTIONS || !sections) {
+      set_error("rotate-half RoPE takes 0..%d sections", DT_MAX_SECTIONS);
+      return DT_ERR_INVALID;
+    }
+    int lo = 0, lane = 0;
+    for (int i = 0; i < n_sections; ++i) {
+      if (sections[i] <= 0 || (sections[i] & 7) || sections[i] > D - lo) {
+        set_error("section %d has %d elements: need positive multiples of 8 that sum to %d", i, sections[i], D);
+        return DT_ERR_INVALID;
+      }
+      for (int e = 0; e < sections[i] / 2; e += 4, ++lane) {
+        a.a0[lane] = (uint8_t)(lo + e);
+        a.b0[lane] = (uint8_t)(lo + sections[i] / 2 + e);
+        for (int k = 0; k < 4; ++k) pair_of[4 * lane + k] = lo / 2 + e + k;
+      }
+      lo += sections[i];
+    }
+    if (lo != D) {
+      set_error("sections sum to %d, head dim is %d", lo, D);
+      return DT_ERR_INVALID;
+    }
+  } else {
+    for (int j = 0; j < D / 2; ++j) pair_of[j] = j;
+  }
+  for (int j = 0; j < D / 2; ++j) {
+    a.axis[j] = axis_of_pair[pair_of[j]];
+    a.turns[j] = turns[pair_of[j]];
+  }
+  for (int i = 0; i < n_rows; ++i) {
+    const dt_rotary_rows& r = rows[i];
+    if (r.H <= 0 || !r.x || !r.y || !aligned16(r.x) || !aligned16(r.y) || ((r.stride_b | r.stride_s | r.stride_h) & 7)) {
+      set_error("tensor %d: x and y must be non-null, 16-byte aligned, with strides that are multiples of 8 elements and a positive number of heads", i);
+      return DT_ERR_INVALID;
+    }
+    if (!(r.out_scale > 0.0f) || !(r.out_scale < INFINITY)) {
+      set_error("out_scale must be positive and finite (1 for none)");
+      return DT_ERR_INVALID;
+    }
+    if ((r.weight && !aligned16(r.weight)) || (r.bias && !aligned16(r.bias))) {
+      set_error("weight and bias must be 16-byte aligned");
+      return DT_ERR_INVALID;
+    }
+    Rows& d = a.rows[i];
+    d.x = static_cast<const uint16_t*>(r.x);
+    d.y = static_cast<uint16_t*>(r.y);
+    d.sb = r.stride_b; d.ss = r.stride_s; d.sh = r.stride_h;
+    d.w = r.weight; d.bias = r.bias;
+    d.scale = r.out_scale;
+    d.H = r.H;
+    d.groups = (r.H - 1) / kHeads + 1;
+  }
+  const int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
+  const __int128 items = (__int128)B * S * groups;
+  if (items >= (1ll << 31)) {
+    set_error("too many rows");
+    return DT_ERR_INVALID;
+  }
+  a.pos = positions;
+  a.pos_sb = pos_stride_b;
+  a.S = S;
+  a.n_axes = n_axes;
+  a.norm = norm;
+  a.w16 = (rounding & DT_WEIGHTS_16) != 0;
+  a.eps = eps;
+  a.items = (uint32_t)items;
+  a.by_groups = quotient_by((int32_t)groups);
+  a.by_s = quotient_by(S);
+  const int per_wg = kThreads / (D / 8);
+  const dim3 grid((unsigned)((items + per_wg - 1) / per_wg)), block(kThreads);
+  const hipStream_t st = (hipStream_t)stream;
+  const bool half = (rounding & DT_IO_FP16) != 0, halves = rope == DT_ROPE_HALVES;
+#define DT_LAUNCH(D, half, halves) hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves>), grid, block, 0, st, a)
+#define DT_LAUNCH_D(D)                                                           \
+  do {                                                                           \
+    if (half && halves) DT_LAUNCH(D, true, true);                                \
+    else if (half) DT_LAUNCH(D, true, false);                                    \
+    else if (halves) DT_LAUNCH(D, false, true);                                  \
+    else DT_LAUNCH(D, false, false);                                             \
+  } while (0)
+  if (D == 128) DT_LAUNCH_D(128);
+  else DT_LAUNCH_D(64);
+#undef DT_LAUNCH_D
+#undef DT_LAUNCH
+  return hip_fail(hipGetLastError(), "qk_norm_rope_axes launch");
+}

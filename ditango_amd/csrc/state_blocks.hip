@@ -1,0 +1,350 @@
+// Attention states in 8 bits (gfx950): stored, read back, and merged with states of any other format.
+//
+// Blocks of 32 elements along D carry one scale byte.  With M the largest element of the format (448 for e4m3, 127 for int8) and amax the
+// block's largest magnitude,
+//   e = the smallest integer >= -127 with amax <= M 2^e,   scale byte = e + 127,   element = rne(x 2^-e),   value = element 2^e,
+// so nothing saturates, the scaling itself is exact and any arithmetic gives the same elements.  A block that holds an infinite or
+// undefined value has scale byte 255 and reads as undefined (a format without such values must not make numbers of them).
+//
+// The merge is that of the 16-bit states: lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i, fp32 sums, one pass; a single
+// state is copied.  Bound by HBM: D + D / 32 + 4 bytes a row and 8-bit state instead of 2 D + 4.
+//
+// A lane owns 8 consecutive elements, so 4 lanes hold a block and its maximum is two exchanges inside a quad; a row's lanes are
+// neighbours in a wavefront.  States come sorted by the size of their elements, each size in batches whose loads are in flight together.
+#include <algorithm>
+
+#include "dt_common.h"
+#include "state_rows.h"
+
+namespace dt {
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;
+constexpr int kBlock = 32;   // elements of a scale
+
+struct BlockArgs {
+  const void* out[DT_MAX_MERGE];        // 8-bit states first, then 16-bit ones, then fp32 ones
+  const uint8_t* scales[DT_MAX_MERGE];  // [B,Sq,H,D/32] of the 8-bit ones
+  const float* lse[DT_MAX_MERGE];
+  uint64_t bsh_mask;    // bit i: lse[i] is [B,Sq,H] (else [B,H,Sq])
+  uint64_t kind_mask;   // bit i: int8 instead of e4m3, IEEE half instead of bfloat16
+  int32_t n8, n16, n;   // states below n8 are 8-bit, below n16 at most 16-bit
+  void* dst;
+  uint8_t* dst_scales;
+  float* dst_lse;       // may be null
+  int32_t dst_dtype, dst_bsh;
+  RowIndex at;
+};
+
+__device__ __forceinline__ float scale_of(uint32_t byte) {   // 2^(byte - 127); byte 0 is below the normal numbers, 255 infinite
+  return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+
+// Raw 8 elements of a lane.
+template <int kBytes> struct Raw;
+template <> struct Raw<1> { u32x2 x; uint32_t scale; };
+template <> struct Raw<2> { u32x4 x; };
+template <> struct Raw<4> { u32x4 x, y; };
+
+template <int kBytes>
+__device__ __forceinline__ void load(const BlockArgs& a, int i, int64_t elem, Raw<kBytes>& r) {
+  const uint8_t* p = static_cast<const uint8_t*>(a.out[i]) + elem * kBytes;
+  if constexpr (kBytes == 1) {
+    r.x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+    r.scale = a.scales[i][elem / kBlock];
+  } else {
+    r.x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    if constexpr (kBytes == 4) r.y = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p) + 1);
+  }
+}
+
+// acc += w x
+template <int kBytes>
+__device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, float (&acc)[8]) {
+  float x[8];
+  if constexpr (kBytes == 1) {
+    w *= scale_of(r.scale);       // (0 times the infinite scale would not leave a state without weight out)
+    if (kind) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)(r.x[e / 4] << (24 - 8 * (e % 4))) >> 24);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.x[e / 4], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.x[e / 4], true);
+        x[e] = lo.x;
+        x[e + 1] = lo.y;
+        x[e + 2] = hi.x;
+        x[e + 3] = hi.y;
+      }
+    }
+  } else if constexpr (kBytes == 2) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t word = r.x[e];   // (a bit cast of the vector's element itself reads its first one)
+      if (kind) {
+        const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      } else {
+        x[2 * e] = __uint_as_float(word << 16);
+        x[2 * e + 1] = __uint_as_float(word & 0xffff0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = __uint_as_float(r.x[e]);
+      x[4 + e] = __uint_as_float(r.y[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(w, x[e], acc[e]);
+}
+
+struct Sums {
+  float acc[8], m, den;
+};
+
+template <int kBytes, int NB>
+__device__ __forceinline__ void batch(const BlockArgs& a, int i0, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+  Raw<kBytes> r[NB];
+  float l[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    load<kBytes>(a, i0 + j, elem, r[j]);
+    l[j] = a.lse[i0 + j][(a.bsh_mask >> (i0 + j)) & 1 ? row : bhs];
+  }
+  float m = s.m;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) m = fmaxf(m, l[j]);
+  if (!(m > -INFINITY)) {          // no state with a key so far
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      if (l[j] != l[j]) s.den = l[j];   // (an undefined one stays in the result)
+    return;
+  }
+  const float rescale = __expf(s.m - m);
+  s.den *= rescale;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s.acc[e] *= rescale;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const float w = __expf(l[j] - m);
+    s.den += w;
+    if (w != 0.f) add<kBytes>(r[j], (a.kind_mask >> (i0 + j)) & 1, w, s.acc);   // without weight, whatever it holds
+  }
+  s.m = m;
+}
+template <int kBytes, int NB>
+__device__ __forceinline__ void rest(const BlockArgs& a, int i0, int n, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+  if constexpr (NB >= 1) {
+    if (n == NB) batch<kBytes, NB>(a, i0, elem, row, bhs, s);
+    else rest<kBytes, NB - 1>(a, i0, n, elem, row, bhs, s);
+  }
+}
+template <int kBytes>
+__device__ __forceinline__ void states(const BlockArgs& a, int i0, int i1, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+  for (; i0 + kBatch <= i1; i0 += kBatch) batch<kBytes, kBatch>(a, i0, elem, row, bhs, s);
+  rest<kBytes, kBatch - 1>(a, i0, i1 - i0, elem, row, bhs, s);
+}
+
+// The other lanes of a quad: lane ^ 1, lane ^ 2.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kCtrl, 0xf, 0xf, true);
+}
+
+// 8 elements in the destination's format.  (Lanes of a quad are all here: a row has 8 or 16.)
+__device__ __forceinline__ void store(const BlockArgs& a, int64_t elem, const float (&x)[8]) {
+  uint8_t* p = static_cast<uint8_t*>(a.dst);
+  if (a.dst_dtype == DT_FP32) {
+    f32x4 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = x[e];
+      hi[e] = x[4 + e];
+    }
+    __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(p + elem * 4));
+    __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(p + elem * 4) + 1);
+  } else if (a.dst_dtype == DT_BF16 || a.dst_dtype == DT_FP16) {
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f32x2 f;
+      f.x = x[2 * e];
+      f.y = x[2 * e + 1];
+      w[e] = a.dst_dtype == DT_FP16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2))
+                                    : __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+    }
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p + elem * 2));
+  } else {
+    uint32_t top = 0;     // magnitudes compare like their bits, infinite and undefined ones above all others
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+    top = max(top, dpp<0xb1>(top));
+    top = max(top, dpp<0x4e>(top));
+    const bool int8 = a.dst_dtype == DT_BLOCK_INT8, finite = top < 0x7f800000u;
+    // amax = 1.f 2^n is at most M 2^(n - 8) with M = 1.75 2^8, at most M 2^(n - 6) with M = 1.984375 2^6, or needs one more
+    const int n = (int)(top >> 23) - 127;
+    const int e = max(n - (int8 ? 6 : 8) + ((top & 0x7fffffu) > (int8 ? 0x7e0000u : 0x600000u) ? 1 : 0), -127);
+    const float inv = finite ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = finite ? x[i] * inv : 0.f;
+    u32x2 w;
+    if (int8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v |= ((uint32_t)(int32_t)__builtin_rintf(y[4 * i + b]) & 0xffu) << (8 * b);
+        w[i] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], v, true);
+      }
+    }
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x2*>(p + elem));
+    if ((threadIdx.x & 3) == 0) a.dst_scales[elem / kBlock] = finite ? (uint8_t)(e + 127) : 255;
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs a) {
+  const int64_t elem = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8, row64 = elem / D;
+  if (row64 >= a.at.rows) return;
+  const uint32_t row = (uint32_t)row64, bhs = bhs_of(a.at, row);
+  Sums s;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s.acc[e] = 0.f;
+  s.m = -INFINITY;
+  s.den = 0.f;
+  states<1>(a, 0, a.n8, elem, row, bhs, s);
+  states<2>(a, a.n8, a.n16, elem, row, bhs, s);
+  states<4>(a, a.n16, a.n, elem, row, bhs, s);
+  const float inv = s.den != 0.f ? 1.f / s.den : 0.f;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = s.acc[e] * inv;
+  store(a, elem, x);
+  if (a.dst_lse != nullptr && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
+}
+
+// One state into another format, its lse bit for bit.
+template <int D, int kBytes>
+__global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a) {
+  const int64_t elem = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8, row64 = elem / D;
+  if (row64 >= a.at.rows) return;
+  Raw<kBytes> r;
+  load<kBytes>(a, 0, elem, r);
+  const bool with_lse = a.dst_lse != nullptr && elem % D == 0;
+  const uint32_t row = (uint32_t)row64, bhs = bhs_of(a.at, row);
+  float l = 0.f;
+  if (with_lse) l = a.lse[0][a.bsh_mask & 1 ? row : bhs];
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = -0.f;       // (-0 + -0 keeps its sign)
+  add<kBytes>(r, a.kind_mask & 1, 1.f, x);
+  store(a, elem, x);
+  if (with_lse) a.dst_lse[a.dst_bsh ? row : bhs] = l;
+}
+
+bool is_block(int dtype) { return dtype == DT_BLOCK_E4M3 || dtype == DT_BLOCK_INT8; }
+int element_bytes(int dtype) { return is_block(dtype) ? 1 : dtype == DT_FP32 ? 4 : 2; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_state(const dt_state& s, const char* what, int i) {
+  if (s.dtype < DT_BF16 || s.dtype > DT_BLOCK_INT8 || (s.lse_layout != DT_LSE_BHS && s.lse_layout != DT_LSE_BSH)) {
+    set_error("%s %d: bad dtype %d or lse layout %d", what, i, s.dtype, s.lse_layout);
+    return DT_ERR_INVALID;
+  }
+  if (!s.out || !aligned16(s.out) || !s.lse || (is_block(s.dtype) && !s.scales)) {
+    set_error("%s %d: out must be non-null and 16-byte aligned, lse and the scales of an 8-bit state non-null", what, i);
+    return DT_ERR_INVALID;
+  }
+  return DT_OK;
+}
+
+}  // namespace
+}  // namespace dt
+
+using namespace dt;
+
+extern "C" int dt_merge_block_states(int32_t n, const dt_state* states, const dt_state* dst, int32_t B, int32_t Sq, int32_t H, int32_t D,
+                                     void* stream) {
+  if (n < 1 || n > DT_MAX_MERGE || !states || !dst) {
+    set_error("%d states: need 1..%d, and a destination", n, DT_MAX_MERGE);
+    return DT_ERR_INVALID;
+  }
+  if (B <= 0 || Sq <= 0 || H <= 0) {
+    set_error("B, Sq, H must be positive (got %d, %d, %d)", B, Sq, H);
+    return DT_ERR_INVALID;
+  }
+  if (D != 64 && D != 128) {
+    set_error("head dim %d not built (64 and 128 are)", D);
+    return DT_ERR_UNSUPPORTED;
+  }
+  // (a grid holds fewer than 2^32 lanes)
+  const __int128 rows = (__int128)B * Sq * H;
+  if (rows * (D / 8) > (1ll << 32) - kThreads || rows >= (1ll << 31)) {
+    set_error("too many rows (%d x %d x %d)", B, Sq, H);
+    return DT_ERR_INVALID;
+  }
+  if (int rc = check_state(*dst, "destination", 0)) return rc;
+  for (int i = 0; i < n; ++i)
+    if (int rc = check_state(states[i], "state", i)) return rc;
+  BlockArgs a{};
+  int at = 0;
+  for (const int bytes : {1, 2, 4}) {
+    for (int i = 0; i < n; ++i) {
+      const dt_state& s = states[i];
+      if (element_bytes(s.dtype) != bytes) continue;
+      a.out[at] = s.out;
+      a.scales[at] = s.scales;
+      a.lse[at] = s.lse;
+      if (s.lse_layout == DT_LSE_BSH) a.bsh_mask |= 1ull << at;
+      if (s.dtype == DT_BLOCK_INT8 || s.dtype == DT_FP16) a.kind_mask |= 1ull << at;
+      ++at;
+    }
+    if (bytes == 1) a.n8 = at;
+    if (bytes == 2) a.n16 = at;
+  }
+  a.n = n;
+  a.dst = dst->out;
+  a.dst_scales = dst->scales;
+  a.dst_lse = dst->lse;
+  a.dst_dtype = dst->dtype;
+  a.dst_bsh = dst->lse_layout == DT_LSE_BSH;
+  a.at = row_index(B, Sq, H);
+  const dim3 grid((unsigned)(((int64_t)a.at.rows * (D / 8) + kThreads - 1) / kThreads)), block(kThreads);
+  const hipStream_t st = (hipStream_t)stream;
+#define DT_LAUNCH(kernel) hipLaunchKernelGGL(kernel, grid, block, 0, st, a)
+  if (n > 1) {
+    if (D == 128) DT_LAUNCH((merge_blocks_kernel<128>));
+    else DT_LAUNCH((merge_blocks_kernel<64>));
+  } else {
+    const int bytes = element_bytes(states[0].dtype);
+    if (D == 128) {
+      if (bytes == 1) DT_LAUNCH((copy_blocks_kernel<128, 1>));
+      else if (bytes == 2) DT_LAUNCH((copy_blocks_kernel<128, 2>));
+      else DT_LAUNCH((copy_blocks_kernel<128, 4>));
+    } else {
+      if (bytes == 1) DT_LAUNCH((copy_blocks_kernel<64, 1>));
+      else if (bytes == 2) DT_LAUNCH((copy_blocks_kernel<64, 2>));
+      else DT_LAUNCH((copy_blocks_kernel<64, 4>));
+    }
+  }
+#undef DT_LAUNCH
+  return hip_fail(hipGetLastError(), "merge_blocks launch");
+}

@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "dt_common.h"
+#include "state_rows.h"
 
 namespace dt {
 
@@ -450,11 +451,6 @@ __global__ __launch_bounds__(kThreads) void merge_states_kernel(const MergeArgs 
 // D = 64 48.2 -> 38.0, 2222 x 48, D = 64 17.5 -> 13.1.  Workgroups of 512 and 1024 lanes 68.6 and 68.8.  One block
 // state alone (the first of a loop) is 24 bytes an element and bound by the instructions of so many lanes: it stays there (43.4;
 // 57 here).
-struct RowIndex {         // row ((b * Sq) + s) * H + h of B * Sq * H < 2^31 -> its place in the [B,H,Sq] layout
-  int32_t Sq, H;
-  uint32_t rows;          // B * Sq * H
-  Quotient by_h, by_s;
-};
 struct UpdateArgs {
   const float* run;
   const float* run_lse;
@@ -468,25 +464,6 @@ struct UpdateArgs {
 constexpr int kUpdateThreads = 256;
 constexpr int kUpdateGroup = 64;   // workgroups that follow each other on one XCD (1: 3 % slower, 8: the same)
 
-__device__ __forceinline__ uint32_t bhs_of(const RowIndex& at, uint32_t row) {
-  const uint32_t bs = quotient(row, at.by_h), h = row - bs * (uint32_t)at.H;
-  const uint32_t b = quotient(bs, at.by_s), q = bs - b * (uint32_t)at.Sq;
-  return (b * (uint32_t)at.H + h) * (uint32_t)at.Sq + q;
-}
-__device__ __forceinline__ uint32_t bsh_of(const RowIndex& at, uint32_t row) {   // the other way round
-  const uint32_t bh = quotient(row, at.by_s), q = row - bh * (uint32_t)at.Sq;
-  const uint32_t b = quotient(bh, at.by_h), h = bh - b * (uint32_t)at.H;
-  return (b * (uint32_t)at.Sq + q) * (uint32_t)at.H + h;
-}
-static RowIndex row_index(int B, int Sq, int H) {
-  RowIndex at{};
-  at.Sq = Sq;
-  at.H = H;
-  at.rows = (uint32_t)((int64_t)B * Sq * H);
-  at.by_h = quotient_by(H);
-  at.by_s = quotient_by(Sq);
-  return at;
-}
 // A grid holds fewer than 2^32 lanes, and these kernels take D / 4 of them a row.
 static bool lanes_fit(int B, int Sq, int H, int D) { return (int64_t)B * Sq * H * (D / 4) <= (1ll << 32) - kUpdateThreads; }
 static dim3 lane_grid(const RowIndex& at, int D) {

@@ -15,6 +15,9 @@ The reference's executors run these as chains of eager torch ops right before
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
+from decimal import Decimal, localcontext
+from functools import cached_property, lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -81,6 +84,104 @@ def prepare_qk(x: torch.Tensor, *, norm: Optional[str] = None, weight: Optional[
                              rope=_ROPES[rope], cos=cos, sin=sin, rope_begin=rope_begin, rope_end=rope_end,
                              sections=sections, rounding=rounding, out=out,
                              out_scale=1.0 if fold_softmax_scale is None else folded_scale(x.shape[-1], fold_softmax_scale))
+
+
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+
+
+@lru_cache(maxsize=64)
+def _turns_of(dim: int, base: float) -> Tuple[int, ...]:
+    """base ** (-2 j / dim) / (2 pi), j < dim / 2, in units of 2^-64."""
+    with localcontext() as ctx:
+        ctx.prec = 50      # (a chain of at most 63 products loses 2 of the 50 digits, 2^64 has 20)
+        step, f, turns = Decimal(base) ** (Decimal(-2) / Decimal(dim)), Decimal(2) ** 64 / (2 * _PI), []
+        for _ in range(dim // 2):
+            turns.append(int(f.to_integral_value()))
+            f *= step
+    return tuple(turns)
+
+
+@dataclass(frozen=True)
+class RotaryAxes:
+    """How a head row turns with a token's position on several axes, e.g. (time, height, width).
+
+    Axis ``i`` has ``dims[i]`` elements of the row and turns their pair ``j`` by ``position * bases[i] ** (-2 j / dims[i])``; ``base`` is one
+    number for all axes or one for each.  ``pairing``: ``"interleaved"`` (neighbours; CogVideoX ``(16, 24, 24)``, HunyuanVideo ``(16, 56,
+    56)`` with base 256) or ``"rotate_half"`` (the halves of each axis' section; Step-Video ``(64, 32, 32)``).  ``halves="head"`` pairs the
+    two halves of the whole row instead, whose pairs the axes then share out in order.  Keep the object: it holds the frequencies as 64-bit
+    fractions of a turn, which are exact for any position."""
+    dims: Tuple[int, ...]
+    base: object = 10000.0
+    pairing: str = "interleaved"
+    halves: str = "axis"
+
+    def __post_init__(self):
+        object.__setattr__(self, "dims", tuple(int(d) for d in self.dims))
+        base = tuple(float(b) for b in self.base) if isinstance(self.base, (tuple, list)) else (float(self.base),) * len(self.dims)
+        object.__setattr__(self, "base", base)
+        if sum(self.dims) not in (64, 128) or not 1 <= len(self.dims) <= 8 or len(base) != len(self.dims):
+            raise ValueError(f"dims must be 1 to 8 axes that sum to 64 or 128, with one base or one each; got {self.dims} and {self.base}")
+        if not all(b > 1 and math.isfinite(b) for b in base):
+            raise ValueError(f"bases must be finite and above 1, got {base}")
+        if self.pairing not in ("interleaved", "rotate_half") or self.halves not in ("axis", "head"):
+            raise ValueError(f"unknown pairing {self.pairing!r} or halves {self.halves!r}")
+        by_section = self.pairing == "rotate_half" and self.halves == "axis"
+        step = 8 if by_section else 2
+        if any(d <= 0 or d % step for d in self.dims):
+            raise ValueError(f"{self.pairing} axes need positive multiples of {step} elements, got {self.dims}")
+
+    @cached_property
+    def turns(self):
+        """(fraction of a turn a step of the position is, times 2^64; axis) of every pair."""
+        turns = [t for d, b in zip(self.dims, self.base) for t in _turns_of(d, b)]
+        axis = [i for i, d in enumerate(self.dims) for _ in range(d // 2)]
+        return turns, axis
+
+    @property
+    def sections(self):
+        return list(self.dims) if self.pairing == "rotate_half" and self.halves == "axis" else []
+
+    @cached_property
+    def table(self):
+        """The axes as the binding takes them."""
+        return _hip.rotary_table(*self.turns, _ROPES[self.pairing], self.sections)
+
+
+def prepare_qk_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, axes: RotaryAxes, *, norm: Optional[str] = None,
+                    q_weight: Optional[torch.Tensor] = None, q_bias: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                    out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None, fold_softmax_scale: Optional[float] = None):
+    """``prepare_qk`` of q ``[B,S,H,D]`` and k ``[B,S,Hk,D]`` in one launch, rotated by ``positions`` int32 ``[S, axes]`` or ``[B, S, axes]`` on the
+    GPU instead of by tables that somebody has to build: any place in time, height and width, far into a rollout as exactly as at its
+    start.  A token at the origin of every axis (text) is not turned.  Returns (q, k), contiguous, in their dtype, computed in fp32
+    and rounded once; k may be ``None``.  ``norm``, weights, ``out`` and ``fold_softmax_scale`` (q only) as in ``prepare_qk``."""
+    if norm not in _NORMS:
+        raise ValueError(f"unknown norm {norm!r}")
+    if positions.dtype is not torch.int32:
+        raise ValueError(f"positions must be int32, got {positions.dtype}")
+    if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes.dims):
+        raise ValueError(f"positions must be [S, {len(axes.dims)}] or [B, S, {len(axes.dims)}] for these axes, got {tuple(positions.shape)}")
+    given = (None, None) if out is None else out
+    tensors = [(q, q_weight, q_bias, given[0])] + ([] if k is None else [(k, k_weight, k_bias, given[1])])
+    params = [t for _, w, b, _ in tensors for t in (w, b)]
+    rounding = 0
+    if any(t is not None for t in params) and _read_in_place(q, None, None) and all(_read_in_place(q, t, None) for t in params):
+        rounding = _hip.DT_WEIGHTS_16
+    else:
+        tensors = [(x, _f32(w, x.device), _f32(b, x.device), y) for x, w, b, y in tensors]
+    scale = 1.0 if fold_softmax_scale is None else folded_scale(q.shape[-1], fold_softmax_scale)
+    done = _hip.qk_norm_rope_axes([(*t, scale if i == 0 else 1.0) for i, t in enumerate(tensors)],
+                                  positions if positions.is_contiguous() else positions.contiguous(), axes.table, _NORMS[norm], eps, rounding)
+    return done[0], (done[1] if k is not None else None)
+
+
+def grid_positions(f: int, h: int, w: int, *, text: int = 0, first_frame: int = 0, device=None) -> torch.Tensor:
+    """int32 ``[text + f*h*w, 3]``: ``text`` tokens at the origin, then the tokens of ``f`` frames of ``h`` x ``w``, row by row, from frame
+    ``first_frame`` of a rollout on.  A sequence-parallel rank slices the rows of its shard."""
+    grid = torch.cartesian_prod(torch.arange(first_frame, first_frame + f, dtype=torch.int32), torch.arange(h, dtype=torch.int32),
+                                torch.arange(w, dtype=torch.int32)).view(-1, 3)
+    pos = torch.cat((torch.zeros(text, 3, dtype=torch.int32), grid))
+    return pos if device is None else pos.to(device)
 
 
 def folded_scale(head_dim: int, softmax_scale: float = 0.0) -> float:

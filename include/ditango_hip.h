@@ -37,6 +37,8 @@ extern "C" {
 #define DT_BF16 0
 #define DT_FP32 1
 #define DT_FP16 2 /* IEEE binary16 */
+#define DT_BLOCK_E4M3 3 /* 8-bit states of dt_merge_block_states: e4m3 elements, a scale for every 32 */
+#define DT_BLOCK_INT8 4 /* ... int8 elements */
 
 #define DT_LSE_BHS 0
 #define DT_LSE_BSH 1
@@ -547,6 +549,75 @@ int dt_qkv_project(const void* text, int64_t text_stride_b, int64_t text_stride_
                    const void* video, int64_t video_stride_b, int64_t video_stride_s, int32_t V,
                    int32_t B, int32_t K, int32_t H, int32_t D, const dt_projection* proj,
                    const float* cos, const float* sin, int32_t rounding, void* stream);
+
+/*
+ * Attention in a window: query row i of a sample stands at position p = q_begin + i among the sample's keys (q_begin = -1: behind them,
+ * p = len - Sq + i) and sees the frames of `frame` tokens from `left` in front of its own to `right` behind it, and the first `sinks` keys
+ * wherever it stands.  Frames are counted from key `sinks`: with start = sinks + floor((p - sinks) / frame) * frame, key j is visible where
+ *   j < len,  j < start + (right + 1) * frame  (right = -1: no border),  j < sinks or j >= start - left * frame  (left = -1: no border).
+ * frame = 1 is a window of tokens, right = 0 a causal one.  len is Sk, or kv_lens[b] (device int32 [B], read by the kernel and clamped to
+ * 0..Sk; NULL: Sk): keys behind it, padding or rows of a cache that are not written yet, may hold anything.
+ * The result is a state as of dt_attn_chunk_fwd, out [B,Sq,H,D] contiguous in the dtype of q, lse fp32 [B,H,Sq]: softmax over the visible keys;
+ * a row that sees none gets out = 0, lse = -inf.  A masked key adds nothing, whatever it and its value hold.
+ * q [B,Sq,H,D], k and v [B,Sk,Hk,D] with element strides {batch, token, head} of their own (HOST arrays of 3; multiples of 8, token strides of
+ * k and v at most 2^23), H a multiple of Hk: query heads h share key head h / (H / Hk).  bfloat16, or IEEE half with DT_ATTN_FP16.
+ * workspace: device memory, 16-byte aligned; launches of few rows cut long windows into parts that leave partial states there and a
+ * second kernel that adds them up.  dt_attn_workspace_bytes() is plenty, without it (NULL) nothing is cut.  Launches that share a workspace must not
+ * overlap on the GPU.  No counterpart in the reference (its chunks are attended to whole).
+ */
+typedef struct {
+  int32_t left, right, frame, sinks, q_begin;
+  const int32_t* kv_lens;
+} dt_window;
+int dt_attn_window_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int32_t B, int32_t Sq, int32_t Sk,
+                       int32_t H, int32_t Hk, int32_t D, const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, const dt_window* window, float softmax_scale, int32_t flags,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention states in 8 bits, for a cache of half the size (core/cache.py:75-84 keeps fp32 states): the merge of n states of any dtype
+ * into one of any dtype, in one pass; n = 1 copies (stores, loads) with the lse bit for bit.
+ * out is [B,Sq,H,D] contiguous, 16-byte aligned.  DT_BLOCK_E4M3 (OCP e4m3) and DT_BLOCK_INT8 have scales uint8 [B,Sq,H,D/32], one for every 32
+ * elements along D: value = element * 2^(scale - 127), with the smallest scale for which no magnitude of the block is above the largest
+ * element (448, 127), and elements rounded to nearest even.  A block that holds an infinite or undefined value has scale 255 and reads as NaN.
+ * The other dtypes take scales = NULL.  States whose lse is -inf contribute nothing, whatever they hold.  dst may be one of the states (the
+ * same pointers, dtype and layout).  states is a HOST array; n <= DT_MAX_MERGE.
+ */
+typedef struct {
+  void* out;
+  uint8_t* scales;
+  float* lse;
+  int32_t dtype, lse_layout;
+} dt_state;
+int dt_merge_block_states(int32_t n, const dt_state* states, const dt_state* dst, int32_t B, int32_t Sq, int32_t H, int32_t D,
+                          void* stream);
+
+/*
+ * dt_qk_norm_rope for positions on several axes (time, height, width) instead of tables, on up to two tensors (q and k, whose heads may
+ * differ in number) in one launch: executor/hunyuanvideo/hunyuan_transformer.py:177-191 and executor/step/blocks.py:66-75 with the tables that
+ * executor/step/rope.py:13-90 builds for a whole clip.
+ * positions: device int32, position of token s of batch b on axis i at [b * pos_stride_b + s * n_axes + i]; negative ones turn backwards.
+ * Pair j of a row, j < D / 2, turns by positions[axis_of_pair[j]] * turns[j] / 2^64 full turns (HOST arrays; turns[j] is its frequency over 2 pi as a
+ * fraction of 2^64, so that any position's angle is right to 2^-32 of a turn).  Pairs are elements (2j, 2j+1) with DT_ROPE_INTERLEAVED and
+ * (lo + i, lo + len/2 + i), j = lo/2 + i, in each of the sections of DT_ROPE_HALVES (lengths multiples of 8 that sum to D; n_sections = 0: one of D):
+ *   y_a = x_a cos - x_b sin,  y_b = x_b cos + x_a sin,
+ * on the normalised row (norm, weight, bias, eps as in dt_qk_norm_rope), in fp32, times out_scale, rounded once.
+ * x is 16-bit [B,S,H,D] with strides that are multiples of 8, y [B,S,H,D] contiguous, weight and bias [D] or NULL, all of them 16-byte aligned;
+ * y may alias x where x is contiguous.  rounding: DT_IO_FP16 and DT_WEIGHTS_16 only.
+ */
+typedef struct {
+  const void* x;
+  int64_t stride_b, stride_s, stride_h;
+  void* y;
+  const void *weight, *bias;
+  int32_t H;
+  float out_scale;
+} dt_rotary_rows;
+#define DT_MAX_SECTIONS 8
+int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, int32_t S, int32_t D, int32_t norm, float eps,
+                         const int32_t* positions, int64_t pos_stride_b, int32_t n_axes, const uint64_t* turns,
+                         const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections, int32_t n_sections,
+                         int32_t rounding, void* stream);
 
 #ifdef __cplusplus
 }
