@@ -9,8 +9,8 @@
 //
 // Work: rows of one key head are the queries of all query heads that share it (row = query * group + head in group), so shared heads
 // fill the matrix instructions of a single token.  Two forms:
-//   * shared tiles: a workgroup of 4 wavefronts, 32 rows each, walks the 64-key tiles that some of its 128 rows see: the sinks' tiles,
-//     then the window's.  Two workgroups a CU; one does its softmax while the other has the matrix pipe.
+//   * shared tiles: a workgroup of 8 wavefronts, 32 rows each, walks the 64-key tiles that some of its 256 rows see: the sinks' tiles,
+//     then the window's.  Its two groups of 4 run a phase apart: while one has its products on the matrix pipe, the other does its softmax.
 //   * few rows: the 4 wavefronts of a workgroup share 32 rows and take 32-key tiles of their own in turn, and the window is cut into
 //     `parts` workgroups; states meet in the LDS, those of the parts in a fold kernel behind the launch.
 // A wavefront leaves out tiles that none of its rows sees, and only a tile with a border in it is masked.
@@ -23,10 +23,10 @@
 namespace dt {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
-constexpr int kRowsShared = kWaves * 32;   // rows of a workgroup, shared tiles
-constexpr int kRowsFew = 32;               // ... few rows
+constexpr int kWavesShared = 8;
+constexpr int kRowsShared = kWavesShared * 32;   // rows of a workgroup, shared tiles
+constexpr int kWavesFew = 4;
+constexpr int kRowsFew = 32;                     // ... few rows
 constexpr int kXcds = 8;
 // A tile's sum of a lane's probabilities above which the tile is redone with its exact maximum: below it no probability exceeds 2^12,
 // which the 16-bit operand and the fp32 sums hold as well as one below 1.
@@ -62,6 +62,11 @@ __device__ __forceinline__ Span span_of(const WindowArgs& a, int len, int s) {
   r.hi = a.right < 0 ? len : min(max(start + a.right, 0), len);
   return r;
 }
+// The same for a query of all lanes, in scalar registers.
+__device__ __forceinline__ Span uniform_span(const WindowArgs& a, int len, int s) {
+  const Span r = span_of(a, len, __builtin_amdgcn_readfirstlane(s));
+  return {__builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi)};
+}
 __device__ __forceinline__ int keys_of(const WindowArgs& a, int b) {
   return a.kv_lens ? min(max(a.kv_lens[b], 0), a.Sk) : a.Sk;   // nothing on the host has looked at the list
 }
@@ -80,7 +85,11 @@ __device__ __forceinline__ TileList tiles_of(const WindowArgs& a, const Span& fi
 }
 
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void wait_loads_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ void wait_lds_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 template <int D, int NKB>
 struct Tiles {
@@ -118,8 +127,8 @@ struct RowState {
     const int row = min(row0 + col, a.rows - 1);
     const int s = row / a.group, g = row - s * a.group;
     mine = span_of(a, len, s);
-    first = span_of(a, len, __builtin_amdgcn_readfirstlane(min(row0, a.rows - 1) / a.group));
-    last = span_of(a, len, __builtin_amdgcn_readfirstlane(min(row0 + 31, a.rows - 1) / a.group));
+    first = uniform_span(a, len, min(row0, a.rows - 1) / a.group);
+    last = uniform_span(a, len, min(row0 + 31, a.rows - 1) / a.group);
     sinks = a.sinks;
     const uint16_t* q = a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * a.group + g) * a.q_sh + 8 * hh;
 #pragma unroll
@@ -141,9 +150,9 @@ struct RowState {
   }
 
   // Whether a row of the wavefront sees a key of [k0, k0 + kKeys); whether all of them see all.
-  __device__ __forceinline__ bool needs(int k0) const { return k0 < last.hi && (k0 + T::kKeys > first.lo || k0 < sinks); }
+  __device__ __forceinline__ bool needs(int k0) const { return (k0 < last.hi) & ((k0 + T::kKeys > first.lo) | (k0 < sinks)); }
   __device__ __forceinline__ bool whole(int k0) const {
-    return k0 + T::kKeys <= first.hi && (k0 >= last.lo || k0 + T::kKeys <= sinks);
+    return (k0 + T::kKeys <= first.hi) & ((k0 >= last.lo) | (k0 + T::kKeys <= sinks));
   }
 
   __device__ __forceinline__ ex8 v_frag(const uint8_t* vt, int db, int step) const {
@@ -173,10 +182,8 @@ struct RowState {
     sum = s0 + s1;
   }
 
-  // The tile of keys k0 .. in the LDS at kt and vt.
-  __device__ __forceinline__ void tile(const uint8_t* kt, const uint8_t* vt, int k0, int lane) {
-    const int hh = lane >> 5;
-    f32x16 s[NKB];
+  // S^T = K Q^T of the tile at kt.
+  __device__ __forceinline__ void scores(const uint8_t* kt, f32x16 (&s)[NKB]) const {
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
@@ -184,24 +191,24 @@ struct RowState {
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) {
-        const ex8 ka = *reinterpret_cast<const ex8*>(kt + kld[i] + kb * 32 * T::kRowBytes);
-        s[kb] = E::mfma(ka, qf[i], s[kb]);
-      }
-    const bool masked = !whole(k0);   // uniform
+      for (int kb = 0; kb < NKB; ++kb) s[kb] = E::mfma(*reinterpret_cast<const ex8*>(kt + kld[i] + kb * 32 * T::kRowBytes), qf[i], s[kb]);
+  }
+
+  // Scores of the keys k0 .. -> probabilities.
+  __device__ __forceinline__ void softmax(f32x16 (&s)[NKB], ex8 (&p)[NKB][2], int k0, bool masked, int lane) {
     if (masked) {
       asm volatile("" ::: "memory");   // keeps this a real branch
+      const int hh = lane >> 5;
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = k0 + 32 * kb + 16 * (r >> 3) + 8 * hh + (r & 7);
-          if (!(key < mine.hi && (key >= mine.lo || key < sinks))) s[kb][r] = -INFINITY;
+          s[kb][r] = (key < mine.hi) & ((key >= mine.lo) | (key < sinks)) ? s[kb][r] : -INFINITY;
         }
     }
     // Probabilities relative to the reference that the sums are scaled to.  The tile's own maximum is looked for only where the sum of
     // the probabilities, needed anyway, says that the reference lags too far behind (or is not there yet: the sum is inf or NaN).
-    ex8 p[NKB][2];
     float sum;
     softmax_pass(s, m_ref * c, p, sum);
     if (__builtin_expect(__any(!(sum <= kSumLimit)), 0)) {
@@ -222,10 +229,10 @@ struct RowState {
       softmax_pass(s, m_new > -INFINITY ? m_new * c : 0.f, p, sum);
     }
     l_run += sum;
-    if (masked && any_not_finite(vt, lane)) {
-      visible_only(vt, p, k0, lane);
-      return;
-    }
+  }
+
+  // O^T += V^T P^T of the tile at vt.
+  __device__ __forceinline__ void values(const uint8_t* vt, const ex8 (&p)[NKB][2]) {
 #pragma unroll
     for (int step = 0; step < 2 * NKB; ++step)
 #pragma unroll
@@ -233,11 +240,13 @@ struct RowState {
   }
 
   // A masked key's probability is 0, which an infinite or undefined value of V would turn into NaN.  Tiles with masked keys are looked
-  // through (a wavefront reads all of the tile: 192 more vector instructions), and one with such a value adds up visible keys only.
+  // through (a wavefront reads all of the tile: 192 more vector instructions).  Where there is such a value, few rows multiply the tile with
+  // zeros in their place and then add them, as they are, to the rows that see them (the weight of a visible key is above 0); shared tiles, whose
+  // loop has no registers for that, compute the 32 rows once more behind it (rows_one_by_one).
+  static constexpr uint32_t kExp = kHalf ? 0x7c007c00u : 0x7f807f80u, kOne = kHalf ? 0x04000400u : 0x00800080u;
   __device__ __forceinline__ bool any_not_finite(const uint8_t* vt, int lane) const {
-    constexpr uint32_t kExp = kHalf ? 0x7c007c00u : 0x7f807f80u, kOne = kHalf ? 0x04000400u : 0x00800080u;
     uint32_t over = 0;
-#pragma unroll
+#pragma unroll 2
     for (int i = 0; i < T::kBytes / 1024; ++i) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(vt + i * 1024 + lane * 16);
 #pragma unroll
@@ -245,18 +254,22 @@ struct RowState {
     }
     return __any((over & 0x80008000u) != 0);
   }
-  __device__ __forceinline__ void visible_only(const uint8_t* vt, const ex8 (&p)[NKB][2], int k0, int lane) {
+  __device__ __forceinline__ void values_not_finite(const uint8_t* vt, const ex8 (&p)[NKB][2], int k0, int lane) {
+#pragma unroll
+    for (int step = 0; step < 2 * NKB; ++step)
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) {
+        u32x4 v = __builtin_bit_cast(u32x4, v_frag(vt, db, step));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bad = ((v[e] & kExp) + kOne) & 0x80008000u;     // sign bits of the elements to leave out
+          v[e] &= ~((bad << 1) - (bad >> 15));
+        }
+        o[db] = E::mfma(__builtin_bit_cast(ex8, v), p[step >> 1][step & 1], o[db]);
+      }
     const int hh = lane >> 5;
 #pragma unroll 1
     for (int key = 0; key < T::kKeys; ++key) {
-      const int at = (key >> 5) * 16 + ((key >> 4) & 1) * 8 + (key & 7), from = (key >> 3) & 1;
-      float w = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (at == kb * 16 + r) w = (float)p[kb][r >> 3][r & 7];
-      w = __shfl(w, (lane & 31) + 32 * from);
       const int j = k0 + key;
       const bool seen = j < mine.hi && (j >= mine.lo || j < sinks);
       const uint8_t* row = vt + key * T::kRowBytes;
@@ -266,8 +279,10 @@ struct RowState {
         for (int g = 0; g < 4; ++g) {
           const typename E::x4 v = *reinterpret_cast<const typename E::x4*>(row + 64 * (db ^ T::swz_v(key)) + 16 * g + 8 * hh);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (seen) o[db][4 * g + e] = __builtin_fmaf(w, (float)v[e], o[db][4 * g + e]);
+          for (int e = 0; e < 4; ++e) {
+            const float f = (float)v[e];
+            if (seen && !(__builtin_fabsf(f) < INFINITY)) o[db][4 * g + e] += f;
+          }
         }
     }
   }
@@ -280,36 +295,62 @@ struct Loader {
   const uint16_t *k, *v;       // of this batch and key head
   int64_t k_ss, v_ss;
   uint32_t k_off, v_off;       // lane's bytes within block 0
-  int len;
 
-  __device__ __forceinline__ void open(const WindowArgs& a, int b, int hk, int keys, int lane) {
+  __device__ __forceinline__ void open(const WindowArgs& a, int b, int hk, int lane) {
     k = a.k + b * a.k_sb + hk * a.k_sh;
     v = a.v + b * a.v_sb + hk * a.v_sh;
     k_ss = a.k_ss;
     v_ss = a.v_ss;
-    len = keys;
     const int row = lane / T::kRowLanes, chunk = lane % T::kRowLanes;
     k_off = row * (uint32_t)(2 * k_ss) + 16 * (chunk ^ T::swz_k(row));
     v_off = row * (uint32_t)(2 * v_ss) + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
   }
-  // Blocks b0, b0 + step .. of the tile at key k0 into the LDS at kt and vt.  The descriptor ends behind the last key there is, rows
-  // behind it arrive as zeros; its base is the tile's, so that no offset needs more than 32 bits however long the cache is.
+  // Blocks b0, b0 + step .. of the tile at `from`, `left` keys in front of the last there is, into the LDS at `to`.  The descriptor ends behind the
+  // last key, rows behind it arrive as zeros (all of them where left <= 0); its base is the tile's, so that no offset needs more than 32 bits
+  // however long the cache is.  (The row is part of the lane's offset: a scalar offset beyond the descriptor's end would wrap its range check.)
   template <int kCount>
-  __device__ __forceinline__ void issue(int k0, int b0, int step, uint32_t kt, uint32_t vt) const {
-    const int valid = min(len - k0, T::kKeys);
-    const uint32_t kb = 2 * (uint32_t)k_ss, vb = 2 * (uint32_t)v_ss;
-    const u32x4 rk = make_rsrc(k + (int64_t)k0 * k_ss, valid > 0 ? (valid - 1) * kb + T::kRowBytes : 0u);
-    const u32x4 rv = make_rsrc(v + (int64_t)k0 * v_ss, valid > 0 ? (valid - 1) * vb + T::kRowBytes : 0u);
+  __device__ __forceinline__ void issue(const uint16_t* from, int left, uint32_t off, uint32_t flip, uint32_t row, int b0, int step, uint32_t to) const {
+    const uint32_t valid = left >= T::kKeys ? (T::kKeys - 1) * row + T::kRowBytes : left > 0 ? (left - 1) * row + T::kRowBytes : 0u;
+    const u32x4 r = make_rsrc(from, valid);
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
       const int blk = b0 + i * step;
-      load_block_to_lds(rk, (k_off ^ (64u * (blk & T::kBlockXor))) + blk * T::kBlockRows * kb, 0, kt + blk * 1024);
+      load_block_to_lds(r, (off ^ (64u * (blk & flip))) + blk * T::kBlockRows * row, 0, to + blk * 1024);
     }
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int blk = b0 + i * step;
-      load_block_to_lds(rv, v_off + blk * T::kBlockRows * vb, 0, vt + blk * 1024);
+  }
+  template <int kCount>
+  __device__ __forceinline__ void issue_k(const uint16_t* from, int left, int b0, int step, uint32_t to) const {
+    issue<kCount>(from, left, k_off, T::kBlockXor, 2 * (uint32_t)k_ss, b0, step, to);
+  }
+  template <int kCount>
+  __device__ __forceinline__ void issue_v(const uint16_t* from, int left, int b0, int step, uint32_t to) const {
+    issue<kCount>(from, left, v_off, 0u, 2 * (uint32_t)v_ss, b0, step, to);
+  }
+};
+
+// Walks a workgroup's tiles: the sinks', then the window's.  Behind the last one `left` is 0.
+template <int kTile>
+struct Cursor {
+  const uint16_t* from;
+  int key, left, t;
+  __device__ __forceinline__ void open(const TileList& list, const uint16_t* base, int64_t ss, int len) {
+    t = 0;
+    seek(list, base, ss, len, list.n_sink > 0 ? 0 : list.w0);
+  }
+  __device__ __forceinline__ void next(const TileList& list, const uint16_t* base, int64_t ss, int len) {
+    ++t;
+    if (__builtin_expect(t == list.n_sink || t >= list.n, 0)) {
+      seek(list, base, ss, len, list.w0);
+    } else {
+      key += kTile;
+      left -= kTile;
+      from += kTile * ss;
     }
+  }
+  __device__ __forceinline__ void seek(const TileList& list, const uint16_t* base, int64_t ss, int len, int tile) {
+    key = tile * kTile;
+    from = base + key * ss;
+    left = t < list.n ? len - key : 0;
   }
 };
 
@@ -327,97 +368,283 @@ __device__ __forceinline__ bool item_of(const WindowArgs& a, int rows, Item& it)
   it.row0 = (a.row_tiles - 1 - (t - unit * a.row_tiles)) * rows;
   it.b = unit / a.Hk;
   it.hk = unit - it.b * a.Hk;
+  for (int* x : {&it.index, &it.part, &it.row0, &it.b, &it.hk}) *x = __builtin_amdgcn_readfirstlane(*x);
   return true;
 }
 
 typedef __attribute__((address_space(3))) uint8_t* lds_ptr_t;
 
+// Phases of the shared tiles.  Group g (0 or 1) does the softmax of tile t in phase 2t + g and its products -- O^T += V^T P^T of tile t, then
+// S^T = K Q^T of tile t + 1 -- in phase 2t + g + 1; a barrier ends every phase.  V of tile t and K of tile t + 1, read together, are pair t:
+//   * read in phases 2t (the products' first fragments, ahead of the barrier) to 2t + 2;
+//   * in buffer t % 4.  A softmax phase of tile t begins with the loads of pair t + 2, whose buffer was last read in phase 2t - 2 (pair t - 2);
+//   * waited for by both groups at the end of phase 2t - 1, where the pair behind it, t + 1, may still be on its way: a barrier lies between
+//     every wavefront's wait and anybody's read.
+// The first scores' K, tile 0, is the second half of pair -1, in buffer 3.  Past the last tile, loads go on with empty descriptors.
+constexpr int kPairs = 4;
+
 template <int D>
 struct SharedLds {
-  static constexpr int kStagePitch = 2 * D + 16;
-  static constexpr int kBytes = 4 * Tiles<D, 2>::kBytes;
-  static_assert(kWaves * 32 * kStagePitch <= kBytes, "the epilogue's rows fit the tile buffers");
+  typedef Tiles<D, 2> T;
+  static constexpr int kPair = 2 * T::kBytes;            // V, then K
+  static constexpr int kStage = kPairs * kPair;          // rows of the result, half of the columns, 32 x D bytes a wavefront
+  static constexpr int kBytes = kStage + kWavesShared * 32 * D;
+  static constexpr int kLoads = 2 * T::kBlocks / kWavesShared;   // of a wavefront, a pair
+  // a row's 16-byte chunks in the staging rows
+  __device__ static constexpr int swz_o(int row) { return D == 128 ? ((row >> 1) & 7) : ((row >> 2) & 3); }
 };
 
+template <int N>
+__device__ __forceinline__ void wait_all_but() {
+  static_assert(N == 2 || N == 4, "loads of a pair");
+  if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+}
+// Ends a phase: what it has made goes through the statement, so that the compiler keeps the work on its side of the barrier.
+template <typename V>
+__device__ __forceinline__ void end_softmax(V (&p)[2][2]) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : "+v"(p[0][0]), "+v"(p[0][1]), "+v"(p[1][0]), "+v"(p[1][1]) : : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int NO>
+__device__ __forceinline__ void end_products(f32x16 (&s)[2], f32x16 (&o)[NO]) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]), "+v"(s[1]) : : "memory");
+  if constexpr (NO == 4) asm volatile("s_barrier" : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]) : : "memory");
+  else asm volatile("s_barrier" : "+v"(o[0]), "+v"(o[1]) : : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The 32 rows of a wavefront without matrix instructions, visible keys only, from the maxima (in powers of two) and inverse sums that lane r and
+// r + 32 hold of row r: a lane has a key's score, then its columns.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void attn_window_kernel(const WindowArgs a) {
-  typedef Tiles<D, 2> T;
+__device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item& it, int len, int row0, float m, float inv, int lane) {
   typedef Elem<kHalf> E;
+  constexpr int kCols = D / 64;
+  const uint16_t* k = a.k + it.b * a.k_sb + it.hk * a.k_sh;
+  const uint16_t* v = a.v + it.b * a.v_sb + it.hk * a.v_sh + lane * kCols;
+#pragma unroll 1
+  for (int r = 0; r < 32 && row0 + r < a.rows; ++r) {
+    const int s = (row0 + r) / a.group, head = it.hk * a.group + row0 + r - s * a.group;
+    const Span span = uniform_span(a, len, s);
+    const uint16_t* q = a.q + it.b * a.q_sb + s * a.q_ss + head * a.q_sh;
+    const float top = __shfl(m, r), norm = __shfl(inv, r);
+    float acc[kCols] = {};
+    const int sinks = min(a.sinks, min(span.lo, span.hi));
+#pragma unroll 1
+    for (int j0 = sinks > 0 ? 0 : span.lo; j0 < span.hi; j0 = j0 < sinks && j0 + 64 >= sinks ? max(span.lo, sinks) : j0 + 64) {
+      const int end = min(j0 < sinks ? sinks : span.hi, j0 + 64);
+      float score = 0.f;
+      if (j0 + lane < end) {
+        const uint16_t* row = k + (int64_t)(j0 + lane) * a.k_ss;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 8) {
+          const typename E::x8 x = *reinterpret_cast<const typename E::x8*>(q + d), y = *reinterpret_cast<const typename E::x8*>(row + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) score = __builtin_fmaf((float)x[e], (float)y[e], score);
+        }
+      }
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, a.scale_log2, -top));
+#pragma unroll 1
+      for (int j = j0; j < end; ++j) {
+        const float wj = __shfl(w, j - j0);
+        const uint16_t* row = v + (int64_t)j * a.v_ss;
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(wj, (float)*reinterpret_cast<const typename E::t*>(row + e), acc[e]);
+      }
+    }
+    typename E::t* out = reinterpret_cast<typename E::t*>(a.out) + (((int64_t)it.b * a.Sq + s) * a.H + head) * D + lane * kCols;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) out[e] = (typename E::t)(acc[e] * norm);
+  }
+}
+
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_window_kernel(const WindowArgs a) {
+  typedef Tiles<D, 2> T;
+  typedef SharedLds<D> S;
+  typedef Elem<kHalf> E;
+  typedef typename E::x8 ex8;
   extern __shared__ __align__(1024) uint8_t lds[];
   Item it;
   if (!item_of(a, kRowsShared, it)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int group = wave >> 2;
   const int len = keys_of(a, it.b);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  const Span first = span_of(a, len, it.row0 / a.group);
-  const Span last = span_of(a, len, min(it.row0 + kRowsShared - 1, a.rows - 1) / a.group);
-  const TileList list = tiles_of<T::kKeys>(a, first, last);
-  auto key_of = [&](int t) __attribute__((always_inline)) { return (t < list.n_sink ? t : list.w0 + t - list.n_sink) * T::kKeys; };
+  const TileList list = tiles_of<T::kKeys>(a, uniform_span(a, len, it.row0 / a.group),
+                                           uniform_span(a, len, min(it.row0 + kRowsShared - 1, a.rows - 1) / a.group));
+  const int n = list.n;
   Loader<D, 2> ld;
-  ld.open(a, it.b, it.hk, len, lane);
-  constexpr int kPer = T::kBlocks / kWaves;
-  auto issue = [&](int t) __attribute__((always_inline)) {
-    const uint32_t at = lds0 + (t & 1) * 2 * T::kBytes;
-    ld.template issue<kPer>(key_of(t), wave, kWaves, at, at + T::kBytes);
+  ld.open(a, it.b, it.hk, lane);
+  constexpr int kPer = T::kBlocks / kWavesShared;
+  Cursor<T::kKeys> kc, vc;
+  kc.open(list, ld.k, ld.k_ss, len);
+  vc.open(list, ld.v, ld.v_ss, len);
+  auto pair_at = [&](int t) __attribute__((always_inline)) { return (t & (kPairs - 1)) * S::kPair; };
+  auto load_k = [&](int pair) __attribute__((always_inline)) {
+    ld.template issue_k<kPer>(kc.from, kc.left, wave, kWavesShared, lds0 + pair_at(pair) + T::kBytes);
+    kc.next(list, ld.k, ld.k_ss, len);
   };
-  if (list.n > 0) issue(0);
+  auto load_pair = [&](int t) __attribute__((always_inline)) {
+    ld.template issue_v<kPer>(vc.from, vc.left, wave, kWavesShared, lds0 + pair_at(t));
+    vc.next(list, ld.v, ld.v_ss, len);
+    load_k(t);
+  };
   RowState<D, kHalf, 2> st;
   const int row0 = it.row0 + 32 * wave;
+  bool hurt = false;     // values that are infinite or undefined in a tile that some row does not see whole
+  if (n > 0) load_k(-1);
   st.open(a, it.b, it.hk, row0, len, lane);
-  for (int t = 0; t < list.n; ++t) {
-    wait_loads_barrier();        // the tile is there, and nobody reads the one before any more
-    if (t + 1 < list.n) issue(t + 1);
-    const int k0 = key_of(t);
-    if (st.needs(k0)) {
-      const uint8_t* kt = lds + (t & 1) * 2 * T::kBytes;
-      st.tile(kt, kt + T::kBytes, k0, lane);
+  if (n > 0) {
+    f32x16 s[2];
+    ex8 p[2][2];
+    // The products of a tile and the scores of the next as one stream of MFMAs, fed by reads from the LDS that run kRing fragments ahead.
+    constexpr int kPV = D / 32 * 4, kQK = D / 16 * 2, kRing = 4;
+    ex8 ring[kRing];
+    auto products = [&](const uint8_t* vt) __attribute__((always_inline)) {
+      const uint8_t* kt = vt + T::kBytes;
+      auto frag = [&](int i) __attribute__((always_inline)) -> ex8 {
+        if (i < kPV) return st.v_frag(vt, i % (D / 32), i / (D / 32));
+        return *reinterpret_cast<const ex8*>(kt + st.kld[(i - kPV) >> 1] + ((i - kPV) & 1) * 32 * T::kRowBytes);
+      };
+#pragma unroll
+      for (int i = 0; i < kPV + kQK; ++i) {
+        const ex8 cur = ring[i % kRing];
+        if (i + kRing < kPV + kQK) ring[i % kRing] = frag(i + kRing);
+        if (i < kPV) {
+          const int step = i / (D / 32);
+          st.o[i % (D / 32)] = E::mfma(cur, p[step >> 1][step & 1], st.o[i % (D / 32)]);
+        } else {
+          const int kb = (i - kPV) & 1, at = (i - kPV) >> 1;
+          if (at == 0) {
+            f32x16 zero;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+            s[kb] = E::mfma(cur, st.qf[at], zero);
+          } else {
+            s[kb] = E::mfma(cur, st.qf[at], s[kb]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kPV - kRing; ++i) {   // behind an MFMA the two reads of a fragment of V, or the one of a fragment of K
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kQK; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kRing, 0);
+    };
+    auto prefill = [&](const uint8_t* vt) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) ring[i] = st.v_frag(vt, i % (D / 32), i / (D / 32));
+    };
+    // Q and K of tile 0 are here; pairs 0 and 1 on their way
+    wait_loads();
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.qf[i]));
+    load_pair(0);
+    load_pair(1);
+    wait_lds_barrier();
+    if (group == 1) {
+      wait_all_but<S::kLoads>();
+      wait_lds_barrier();
     }
+    st.scores(lds + pair_at(-1) + T::kBytes, s);
+    if (group == 0) wait_all_but<S::kLoads>();
+    end_products(s, st.o);
+    int k0 = list.n_sink > 0 ? 0 : list.w0 * T::kKeys;
+    auto probabilities = [&](int t, bool masked) __attribute__((always_inline)) {
+      if (__builtin_expect(st.needs(k0), 1)) {
+        st.softmax(s, p, k0, masked, lane);
+      } else {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i >> 1][i & 1] = __builtin_bit_cast(ex8, u32x4{0u, 0u, 0u, 0u});
+      }
+    };
+    // (the last tile is apart: with a way out in the middle of the loop, the compiler moves O^T to other registers and back in every turn)
+    for (int t = 0; t < n - 1; ++t) {
+      __builtin_amdgcn_s_setprio(D == 64 ? 0 : 1);
+      load_pair(t + 2);
+      const bool masked = !st.whole(k0);
+      const uint8_t* vt = lds + pair_at(t);
+      probabilities(t, masked);
+      prefill(vt);
+      if (group == 1) wait_all_but<S::kLoads>();
+      end_softmax(p);
+      __builtin_amdgcn_s_setprio(0);
+      if (masked) hurt |= st.any_not_finite(vt, lane);
+      products(vt);
+      if (group == 0) wait_all_but<S::kLoads>();
+      end_products(s, st.o);
+      k0 = t + 1 == list.n_sink ? list.w0 * T::kKeys : k0 + T::kKeys;
+    }
+    const bool masked = !st.whole(k0);
+    const uint8_t* vt = lds + pair_at(n - 1);
+    probabilities(n - 1, masked);
+    end_softmax(p);
+    if (masked) hurt |= st.any_not_finite(vt, lane);
+    st.values(vt, p);
+    // group 1's last products are the last thing that happens in the buffers
+    if (group == 0) wait_lds_barrier();
   }
-  // Rows of the result through the LDS, so that a store covers whole lines.
+  // Rows of the result through the LDS, so that a store covers whole lines: half of the columns at a time.
   const int col = lane & 31, hh = lane >> 5;
   const float l = st.l_run + __shfl_xor(st.l_run, 32);
   const float inv = l != 0.f ? 1.f / l : 0.f;      // (an undefined sum stays one)
-  wait_loads_barrier();
-  constexpr int kPitch = SharedLds<D>::kStagePitch;
-  uint8_t* stage = lds + wave * 32 * kPitch;
-#pragma unroll
-  for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      typename E::x4 h;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(st.o[db][4 * g + e] * inv);
-      *reinterpret_cast<typename E::x4*>(stage + col * kPitch + 64 * db + 16 * g + 8 * hh) = h;
-    }
-  __builtin_amdgcn_wave_barrier();
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   if (hh == 0 && row0 + col < a.rows) {
     const int s = (row0 + col) / a.group, g = row0 + col - s * a.group;
     a.lse[((int64_t)it.b * a.H + it.hk * a.group + g) * a.Sq + s] =
         l != 0.f ? (st.m_ref * st.c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
   }
+  if (__builtin_expect(hurt, 0)) {
+    rows_one_by_one<D, kHalf>(a, it, len, row0, st.m_ref * st.c, inv, lane);
+    wait_loads();
+    return;
+  }
+  uint8_t* stage = lds + S::kStage + wave * 32 * D;
+  constexpr int kChunks = D / 16, kPass = 64 / kChunks;       // 16-byte chunks of half a row, rows of a store
 #pragma unroll
-  for (int i = 0; i < 32 / (64 / T::kRowLanes); ++i) {
-    const int r = i * (64 / T::kRowLanes) + lane / T::kRowLanes, chunk = lane % T::kRowLanes;
-    const int row = row0 + r;
-    if (row < a.rows) {
-      const int s = row / a.group, g = row - s * a.group;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * kPitch + 16 * chunk);
-      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.out + (((int64_t)it.b * a.Sq + s) * a.H + it.hk * a.group + g) * D + 8 * chunk));
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        typename E::x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(st.o[half * (D / 64) + i][4 * g + e] * inv);
+        *reinterpret_cast<typename E::x4*>(stage + col * D + (((4 * i + g) ^ S::swz_o(col)) << 4) + 8 * hh) = h;
+      }
+#pragma unroll
+    for (int i = 0; i < 32 / kPass; ++i) {
+      const int r = i * kPass + lane / kChunks, chunk = lane % kChunks;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * D + ((chunk ^ S::swz_o(r)) << 4));
+      const int row = row0 + r;
+      if (row < a.rows) {
+        const int s = row / a.group, g = row - s * a.group;
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.out + (((int64_t)it.b * a.Sq + s) * a.H + it.hk * a.group + g) * D + half * (D / 2) + 8 * chunk));
+      }
     }
   }
+  wait_loads();     // (loads past the last tile store zeros: before the LDS is another workgroup's)
 }
 
 // Few rows.  The LDS holds two tiles (K and V) of each wavefront, then the four states.
 template <int D>
 struct FewLds {
-  static constexpr int kBytes = kWaves * 4 * Tiles<D, 1>::kBytes;
-  static_assert(kWaves * 32 * D * 4 <= kBytes, "the states fit the tile buffers");
-  static constexpr int kAll = kBytes + kWaves * 256;      // and a maximum and a sum a row and wavefront
+  static constexpr int kBytes = kWavesFew * 4 * Tiles<D, 1>::kBytes;
+  static_assert(kWavesFew * 32 * D * 4 <= kBytes, "the states fit the tile buffers");
+  static constexpr int kAll = kBytes + kWavesFew * 256;      // and a maximum and a sum a row and wavefront
 };
 
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kThreads) void attn_window_few_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const WindowArgs a) {
   typedef Tiles<D, 1> T;
   typedef Elem<kHalf> E;
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -435,18 +662,27 @@ __global__ __launch_bounds__(kThreads) void attn_window_few_kernel(const WindowA
   uint8_t* mine = lds + wave * 4 * T::kBytes;
   const uint32_t mine0 = (uint32_t)(uintptr_t)(lds_ptr_t)mine;
   Loader<D, 1> ld;
-  ld.open(a, it.b, it.hk, len, lane);
+  ld.open(a, it.b, it.hk, lane);
   auto issue = [&](int t, int buf) __attribute__((always_inline)) {
     const uint32_t at = mine0 + buf * 2 * T::kBytes;
-    ld.template issue<T::kBlocks>(key_of(t), 0, 1, at, at + T::kBytes);
+    const int k0 = key_of(t);
+    ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, len - k0, 0, 1, at);
+    ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, len - k0, 0, 1, at + T::kBytes);
   };
   int buf = 0;
   if (t0 + wave < t1) issue(t0 + wave, 0);
-  for (int t = t0 + wave; t < t1; t += kWaves, buf ^= 1) {
+  for (int t = t0 + wave; t < t1; t += kWavesFew, buf ^= 1) {
     wait_loads();
-    if (t + kWaves < t1) issue(t + kWaves, buf ^ 1);
+    if (t + kWavesFew < t1) issue(t + kWavesFew, buf ^ 1);
     const uint8_t* kt = mine + buf * 2 * T::kBytes;
-    st.tile(kt, kt + T::kBytes, key_of(t), lane);
+    const int k0 = key_of(t);
+    const bool masked = !st.whole(k0);
+    f32x16 s[1];
+    typename E::x8 p[1][2];
+    st.scores(kt, s);
+    st.softmax(s, p, k0, masked, lane);
+    if (masked && st.any_not_finite(kt + T::kBytes, lane)) st.values_not_finite(kt + T::kBytes, p, k0, lane);
+    else st.values(kt + T::kBytes, p);
   }
   // The four states as they lie in the registers; a wavefront then adds up its quarter of the columns.
   float l = st.l_run + __shfl_xor(st.l_run, 32);
@@ -468,15 +704,15 @@ __global__ __launch_bounds__(kThreads) void attn_window_few_kernel(const WindowA
     ml[wave * 64 + 32 + col] = l;
   }
   __syncthreads();
-  float m[kWaves], w[kWaves], top = -INFINITY;
+  float m[kWavesFew], w[kWavesFew], top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < kWavesFew; ++i) {
     m[i] = ml[i * 64 + col];
     top = fmaxf(top, m[i]);
   }
   l = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < kWavesFew; ++i) {
     w[i] = m[i] > -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;    // a state without a key
     if (m[i] > -INFINITY) l = __builtin_fmaf(w[i], ml[i * 64 + 32 + col], l);
   }
@@ -492,7 +728,7 @@ __global__ __launch_bounds__(kThreads) void attn_window_few_kernel(const WindowA
     const int q = wave * (D / 32) + i;             // group of 4 registers: d = 8 q + 4 hh ..
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kWaves; ++j) {
+    for (int j = 0; j < kWavesFew; ++j) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * (32 * D * 4)) + lane * 4 + q * 256);
       if (m[j] > -INFINITY)
 #pragma unroll
@@ -567,7 +803,7 @@ int cus() {
 }
 
 template <typename Kernel>
-int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int lds, hipStream_t stream) {
+int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int waves, int lds, hipStream_t stream) {
   // more than 64 KB of LDS has to be allowed once per kernel and device
   static thread_local int allowed_dev = -1;
   int dev = 0;
@@ -578,14 +814,14 @@ int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int lds, hipStream
       return rc;
     allowed_dev = dev;
   }
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), lds, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(waves * 64), lds, stream, a);
   return hip_fail(hipGetLastError(), "attn_window launch");
 }
 
 template <int D, bool kHalf>
 int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t shared = units * ((a.rows + kRowsShared - 1) / kRowsShared);
-  const bool few = shared < 2 * n_cus;
+  const bool few = shared < (D == 64 ? 2 : 1) * n_cus;
   a.row_tiles = (a.rows + (few ? kRowsFew : kRowsShared) - 1) / (few ? kRowsFew : kRowsShared);
   int64_t items = units * a.row_tiles;
   a.parts = 1;
@@ -595,13 +831,13 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
     const int64_t tiles = (seen + 31) / 32;
     const int64_t slots = (int64_t)n_cus * (D == 64 ? 2 : 1);
     const int64_t bytes = items * (32 * (D + 2) * 4);
-    int64_t most = std::min<int64_t>(64, tiles / (2 * kWaves));
+    int64_t most = std::min<int64_t>(64, tiles / (2 * kWavesFew));
     if (!workspace || bytes <= 0) most = 1;
     else most = std::min(most, workspace_bytes / bytes);
     // rounds of the chip x tiles of a workgroup
-    int64_t best = (items + slots - 1) / slots * ((tiles + kWaves - 1) / kWaves);
+    int64_t best = (items + slots - 1) / slots * ((tiles + kWavesFew - 1) / kWavesFew);
     for (int64_t p = 2; p <= most; ++p) {
-      const int64_t cost = (items * p + slots - 1) / slots * ((tiles + kWaves * p - 1) / (kWaves * p) + 2) + 4;
+      const int64_t cost = (items * p + slots - 1) / slots * ((tiles + kWavesFew * p - 1) / (kWavesFew * p) + 2) + 4;
       if (cost < best) {
         best = cost;
         a.parts = (int)p;
@@ -620,8 +856,8 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
     a.part_ml = a.part_out + items * 32 * D;
   }
   const unsigned grid = (unsigned)(a.per_xcd * kXcds);
-  if (!few) return launch(attn_window_kernel<D, kHalf>, a, grid, SharedLds<D>::kBytes, stream);
-  if (int rc = launch(attn_window_few_kernel<D, kHalf>, a, grid, FewLds<D>::kAll, stream)) return rc;
+  if (!few) return launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream);
+  if (int rc = launch(attn_window_few_kernel<D, kHalf>, a, grid, kWavesFew, FewLds<D>::kAll, stream)) return rc;
   if (a.parts == 1) return DT_OK;
   const int64_t rows = items / a.parts * 32;
   const unsigned fold = (unsigned)((rows * (D / 4) + 255) / 256);
