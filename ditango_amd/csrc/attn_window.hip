@@ -43,8 +43,10 @@ struct WindowArgs {
   int32_t frame, sinks, q_begin;
   const int32_t* kv_lens;       // device [B], or null: Sk
   float scale_log2;
-  int32_t rows, row_tiles, parts, items, per_xcd;
-  float* part_out;              // parts > 1: [item][row 32][D] sums, and [item][row 32] (maximum in powers of two, sum)
+  int32_t rows, row_tiles, items, per_xcd;
+  // An XCD's items from tail_start on, tail of them, are cut along the keys into `ways` workgroups each
+  int32_t tail_start, tail, ways;
+  float* part_out;              // [part][row of a tile][D] sums, and [part][row] (maximum in powers of two, sum)
   float* part_ml;
 };
 
@@ -71,18 +73,19 @@ __device__ __forceinline__ int keys_of(const WindowArgs& a, int b) {
   return a.kv_lens ? min(max(a.kv_lens[b], 0), a.Sk) : a.Sk;   // nothing on the host has looked at the list
 }
 
-// Tiles of kTile keys that rows between two queries see: [0, n_sink) and [w0, w0 + n - n_sink).
-struct TileList {
-  int n_sink, w0, n;
-};
+// Tiles of kTile keys that rows between two queries see, [0, n_sink) and [w0, ...), and of that list a part, [begin, end).
 template <int kTile>
-__device__ __forceinline__ TileList tiles_of(const WindowArgs& a, const Span& first, const Span& last) {
-  TileList t;
-  t.n_sink = (min(a.sinks, last.hi) + kTile - 1) / kTile;
-  t.w0 = max(first.lo / kTile, t.n_sink);
-  t.n = t.n_sink + max((last.hi + kTile - 1) / kTile - t.w0, 0);
-  return t;
-}
+struct TileList {
+  int n_sink, w0, begin, end;
+  __device__ __forceinline__ TileList(const WindowArgs& a, const Span& first, const Span& last, int part, int ways) {
+    n_sink = (min(a.sinks, last.hi) + kTile - 1) / kTile;
+    w0 = max(first.lo / kTile, n_sink);
+    const int n = n_sink + max((last.hi + kTile - 1) / kTile - w0, 0);
+    begin = (int)((int64_t)n * part / ways);
+    end = (int)((int64_t)n * (part + 1) / ways);
+  }
+  __device__ __forceinline__ int key(int t) const { return (t < n_sink ? t : w0 + t - n_sink) * kTile; }
+};
 
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void wait_lds_barrier() {
@@ -167,17 +170,22 @@ struct RowState {
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        f32x2 e;
-        e.x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -mc));
-        e.y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r + 1], c, -mc));
-        s0 += e.x;
-        s1 += e.y;
-        // P goes to the second product in the tensors' 16 bits, as q, k and v come: half a step relative to each probability.  The sum
-        // is that of the fp32 values.
-        const ex2 h = __builtin_convertvector(e, ex2);
-        p[kb][r >> 3][r & 7] = h.x;
-        p[kb][r >> 3][(r & 7) + 1] = h.y;
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) {
+          f32x2 e;
+          e.x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * half + r], c, -mc));
+          e.y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * half + r + 1], c, -mc));
+          s0 += e.x;
+          s1 += e.y;
+          // P goes to the second product in the tensors' 16 bits, as q, k and v come: half a step relative to each probability.  The
+          // sum is that of the fp32 values.
+          const ex2 h = __builtin_convertvector(e, ex2);
+          p[kb][half][r] = h.x;
+          p[kb][half][r + 1] = h.y;
+        }
+        // (rounded and added here: the compiler otherwise holds them in fp32, beside the scores, until the sum's branch is decided)
+        asm volatile("" : "+v"(p[kb][half]), "+v"(s0), "+v"(s1));
       }
     sum = s0 + s1;
   }
@@ -328,47 +336,60 @@ struct Loader {
   }
 };
 
-// Walks a workgroup's tiles: the sinks', then the window's.  Behind the last one `left` is 0.
+// Walks a list's tiles.  Behind the last one `left` is 0.
 template <int kTile>
 struct Cursor {
   const uint16_t* from;
-  int key, left, t;
-  __device__ __forceinline__ void open(const TileList& list, const uint16_t* base, int64_t ss, int len) {
-    t = 0;
-    seek(list, base, ss, len, list.n_sink > 0 ? 0 : list.w0);
+  int left, t;
+  __device__ __forceinline__ void open(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
+    t = list.begin;
+    seek(list, base, ss, len);
   }
-  __device__ __forceinline__ void next(const TileList& list, const uint16_t* base, int64_t ss, int len) {
+  __device__ __forceinline__ void next(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
     ++t;
-    if (__builtin_expect(t == list.n_sink || t >= list.n, 0)) {
-      seek(list, base, ss, len, list.w0);
+    if (__builtin_expect(t == list.n_sink || t >= list.end, 0)) {
+      seek(list, base, ss, len);
     } else {
-      key += kTile;
       left -= kTile;
       from += kTile * ss;
     }
   }
-  __device__ __forceinline__ void seek(const TileList& list, const uint16_t* base, int64_t ss, int len, int tile) {
-    key = tile * kTile;
+  __device__ __forceinline__ void seek(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
+    const int key = t < list.end ? list.key(t) : 0;
     from = base + key * ss;
-    left = t < list.n ? len - key : 0;
+    left = t < list.end ? len - key : 0;
   }
 };
 
-// The workgroup's item: part, rows (the last ones first: under a causal border without a window they see most), batch and key head.
+// The workgroup's item: rows (the last ones first: under a causal border without a window they see most), batch and key head, and of its tiles
+// the part [n part / ways, n (part + 1) / ways).
 struct Item {
-  int index, part, row0, b, hk;
+  int row0, b, hk, part, ways, slot;    // slot: of the part's state in the workspace
 };
-__device__ __forceinline__ bool item_of(const WindowArgs& a, int rows, Item& it) {
-  const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds;
-  it.index = xcd * a.per_xcd + at;      // an XCD works through neighbouring items, which share keys in its L2
-  if (it.index >= a.items) return false;
-  const int t = it.index / a.parts;
-  it.part = it.index - t * a.parts;
-  const int unit = t / a.row_tiles;
-  it.row0 = (a.row_tiles - 1 - (t - unit * a.row_tiles)) * rows;
+__device__ __forceinline__ bool item_at(const WindowArgs& a, int xcd, int idx, int rows, Item& it) {
+  const int item = xcd * a.per_xcd + idx;      // an XCD works through neighbouring items, which share keys in its L2
+  if (idx >= a.per_xcd || item >= a.items) return false;
+  const int unit = item / a.row_tiles;
+  it.row0 = (a.row_tiles - 1 - (item - unit * a.row_tiles)) * rows;
   it.b = unit / a.Hk;
   it.hk = unit - it.b * a.Hk;
-  for (int* x : {&it.index, &it.part, &it.row0, &it.b, &it.hk}) *x = __builtin_amdgcn_readfirstlane(*x);
+  return true;
+}
+__device__ __forceinline__ bool item_of(const WindowArgs& a, int rows, Item& it) {
+  const int xcd = blockIdx.x % kXcds;
+  int idx = blockIdx.x / kXcds;
+  it.part = 0;
+  it.ways = 1;
+  it.slot = 0;
+  if (idx >= a.tail_start) {
+    const int k = idx - a.tail_start;
+    idx = a.tail_start + k / a.ways;
+    it.part = k % a.ways;
+    it.ways = a.ways;
+    it.slot = xcd * a.tail * a.ways + k;
+  }
+  if (!item_at(a, xcd, idx, rows, it)) return false;
+  for (int* x : {&it.row0, &it.b, &it.hk, &it.part, &it.ways, &it.slot}) *x = __builtin_amdgcn_readfirstlane(*x);
   return true;
 }
 
@@ -419,7 +440,7 @@ __device__ __forceinline__ void end_products(f32x16 (&s)[2], f32x16 (&o)[NO]) {
 // The 32 rows of a wavefront without matrix instructions, visible keys only, from the maxima (in powers of two) and inverse sums that lane r and
 // r + 32 hold of row r: a lane has a key's score, then its columns.
 template <int D, bool kHalf>
-__device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item& it, int len, int row0, float m, float inv, int lane) {
+__device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item& it, int len, int row0, float m, float inv, int begin, int end, int lane) {
   typedef Elem<kHalf> E;
   constexpr int kCols = D / 64;
   const uint16_t* k = a.k + it.b * a.k_sb + it.hk * a.k_sh;
@@ -431,12 +452,14 @@ __device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item&
     const uint16_t* q = a.q + it.b * a.q_sb + s * a.q_ss + head * a.q_sh;
     const float top = __shfl(m, r), norm = __shfl(inv, r);
     float acc[kCols] = {};
-    const int sinks = min(a.sinks, min(span.lo, span.hi));
+    // keys [begin, end) of them: in front of the window, and in it
+    const int lo = max(span.lo, begin), hi = min(span.hi, end);
+    const int sinks = min(min(a.sinks, end), min(span.lo, span.hi));
 #pragma unroll 1
-    for (int j0 = sinks > 0 ? 0 : span.lo; j0 < span.hi; j0 = j0 < sinks && j0 + 64 >= sinks ? max(span.lo, sinks) : j0 + 64) {
-      const int end = min(j0 < sinks ? sinks : span.hi, j0 + 64);
+    for (int j0 = begin < sinks ? begin : lo; j0 < hi || j0 < sinks; j0 = j0 < sinks && j0 + 64 >= sinks ? max(lo, sinks) : j0 + 64) {
+      const int stop = min(j0 < sinks ? sinks : hi, j0 + 64);
       float score = 0.f;
-      if (j0 + lane < end) {
+      if (j0 + lane < stop) {
         const uint16_t* row = k + (int64_t)(j0 + lane) * a.k_ss;
 #pragma unroll 1
         for (int d = 0; d < D; d += 8) {
@@ -447,16 +470,22 @@ __device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item&
       }
       const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, a.scale_log2, -top));
 #pragma unroll 1
-      for (int j = j0; j < end; ++j) {
+      for (int j = j0; j < stop; ++j) {
         const float wj = __shfl(w, j - j0);
         const uint16_t* row = v + (int64_t)j * a.v_ss;
 #pragma unroll
         for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(wj, (float)*reinterpret_cast<const typename E::t*>(row + e), acc[e]);
       }
     }
-    typename E::t* out = reinterpret_cast<typename E::t*>(a.out) + (((int64_t)it.b * a.Sq + s) * a.H + head) * D + lane * kCols;
+    if (it.ways > 1) {
+      float* part = a.part_out + ((int64_t)it.slot * kRowsShared + row0 % kRowsShared + r) * D + lane * kCols;
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) out[e] = (typename E::t)(acc[e] * norm);
+      for (int e = 0; e < kCols; ++e) part[e] = acc[e];
+    } else {
+      typename E::t* out = reinterpret_cast<typename E::t*>(a.out) + (((int64_t)it.b * a.Sq + s) * a.H + head) * D + lane * kCols;
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) out[e] = (typename E::t)(acc[e] * norm);
+    }
   }
 }
 
@@ -473,9 +502,9 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   const int group = wave >> 2;
   const int len = keys_of(a, it.b);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  const TileList list = tiles_of<T::kKeys>(a, uniform_span(a, len, it.row0 / a.group),
-                                           uniform_span(a, len, min(it.row0 + kRowsShared - 1, a.rows - 1) / a.group));
-  const int n = list.n;
+  const TileList<T::kKeys> list(a, uniform_span(a, len, it.row0 / a.group),
+                                uniform_span(a, len, min(it.row0 + kRowsShared - 1, a.rows - 1) / a.group), it.part, it.ways);
+  const int n = list.end - list.begin;
   Loader<D, 2> ld;
   ld.open(a, it.b, it.hk, lane);
   constexpr int kPer = T::kBlocks / kWavesShared;
@@ -558,7 +587,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     st.scores(lds + pair_at(-1) + T::kBytes, s);
     if (group == 0) wait_all_but<S::kLoads>();
     end_products(s, st.o);
-    int k0 = list.n_sink > 0 ? 0 : list.w0 * T::kKeys;
+    int k0 = list.key(list.begin);
     auto probabilities = [&](int t, bool masked) __attribute__((always_inline)) {
       if (__builtin_expect(st.needs(k0), 1)) {
         st.softmax(s, p, k0, masked, lane);
@@ -583,7 +612,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       products(vt);
       if (group == 0) wait_all_but<S::kLoads>();
       end_products(s, st.o);
-      k0 = t + 1 == list.n_sink ? list.w0 * T::kKeys : k0 + T::kKeys;
+      k0 = list.begin + t + 1 == list.n_sink ? list.w0 * T::kKeys : k0 + T::kKeys;
     }
     const bool masked = !st.whole(k0);
     const uint8_t* vt = lds + pair_at(n - 1);
@@ -598,13 +627,36 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   const int col = lane & 31, hh = lane >> 5;
   const float l = st.l_run + __shfl_xor(st.l_run, 32);
   const float inv = l != 0.f ? 1.f / l : 0.f;      // (an undefined sum stays one)
+  if (it.ways > 1) {
+    // A part's sums, fp32.  (Where they have to be computed once more, they are those of the keys of the part.)
+    const int64_t at = (int64_t)it.slot * kRowsShared + 32 * wave + col;
+    if (__builtin_expect(hurt, 0)) {
+      rows_one_by_one<D, kHalf>(a, it, len, row0, st.m_ref * st.c, inv, list.begin < list.end ? list.key(list.begin) : 0, list.begin < list.end ? list.key(list.end - 1) + T::kKeys : 0, lane);
+    } else if (row0 + col < a.rows) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = st.o[db][4 * g + e];
+          *reinterpret_cast<f32x4*>(a.part_out + at * D + 32 * db + 8 * g + 4 * hh) = x;
+        }
+    }
+    if (hh == 0 && row0 + col < a.rows) {
+      a.part_ml[at * 2] = st.m_ref * st.c;
+      a.part_ml[at * 2 + 1] = l;
+    }
+    wait_loads();
+    return;
+  }
   if (hh == 0 && row0 + col < a.rows) {
     const int s = (row0 + col) / a.group, g = row0 + col - s * a.group;
     a.lse[((int64_t)it.b * a.H + it.hk * a.group + g) * a.Sq + s] =
         l != 0.f ? (st.m_ref * st.c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
   }
   if (__builtin_expect(hurt, 0)) {
-    rows_one_by_one<D, kHalf>(a, it, len, row0, st.m_ref * st.c, inv, lane);
+    rows_one_by_one<D, kHalf>(a, it, len, row0, st.m_ref * st.c, inv, 0, len, lane);
     wait_loads();
     return;
   }
@@ -655,27 +707,24 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
   const int len = keys_of(a, it.b);
   RowState<D, kHalf, 1> st;
   st.open(a, it.b, it.hk, it.row0, len, lane);
-  const TileList list = tiles_of<T::kKeys>(a, st.first, st.last);
-  auto key_of = [&](int t) __attribute__((always_inline)) { return (t < list.n_sink ? t : list.w0 + t - list.n_sink) * T::kKeys; };
-  // the part's tiles, and of them every fourth
-  const int t0 = (int)((int64_t)list.n * it.part / a.parts), t1 = (int)((int64_t)list.n * (it.part + 1) / a.parts);
+  const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every fourth tile
   uint8_t* mine = lds + wave * 4 * T::kBytes;
   const uint32_t mine0 = (uint32_t)(uintptr_t)(lds_ptr_t)mine;
   Loader<D, 1> ld;
   ld.open(a, it.b, it.hk, lane);
   auto issue = [&](int t, int buf) __attribute__((always_inline)) {
     const uint32_t at = mine0 + buf * 2 * T::kBytes;
-    const int k0 = key_of(t);
+    const int k0 = list.key(t);
     ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, len - k0, 0, 1, at);
     ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, len - k0, 0, 1, at + T::kBytes);
   };
   int buf = 0;
-  if (t0 + wave < t1) issue(t0 + wave, 0);
-  for (int t = t0 + wave; t < t1; t += kWavesFew, buf ^= 1) {
+  if (list.begin + wave < list.end) issue(list.begin + wave, 0);
+  for (int t = list.begin + wave; t < list.end; t += kWavesFew, buf ^= 1) {
     wait_loads();
-    if (t + kWavesFew < t1) issue(t + kWavesFew, buf ^ 1);
+    if (t + kWavesFew < list.end) issue(t + kWavesFew, buf ^ 1);
     const uint8_t* kt = mine + buf * 2 * T::kBytes;
-    const int k0 = key_of(t);
+    const int k0 = list.key(t);
     const bool masked = !st.whole(k0);
     f32x16 s[1];
     typename E::x8 p[1][2];
@@ -722,7 +771,7 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int64_t head = it.hk * a.group + g0;
   uint16_t* out = a.out + (((int64_t)it.b * a.Sq + s) * a.H + head) * D;
-  const int64_t part_row = (int64_t)it.index * 32 + col;
+  const int64_t part_row = (int64_t)it.slot * kRowsFew + col;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     const int q = wave * (D / 32) + i;             // group of 4 registers: d = 8 q + 4 hh ..
@@ -735,7 +784,7 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
         for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);
     }
     if (!live) continue;
-    if (a.parts > 1) {
+    if (it.ways > 1) {
       *reinterpret_cast<f32x4*>(a.part_out + part_row * D + 8 * q + 4 * hh) = sum;
     } else {
       typename E::x4 h;
@@ -745,7 +794,7 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
     }
   }
   if (wave == 0 && hh == 0 && live) {
-    if (a.parts > 1) {
+    if (it.ways > 1) {
       a.part_ml[part_row * 2] = top;
       a.part_ml[part_row * 2 + 1] = l;
     } else {
@@ -756,22 +805,23 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
 
 // Adds up the parts of a row: a lane group of D / 4 lanes a row.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(256) void attn_window_fold_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(256) void attn_window_fold_kernel(const WindowArgs a, int tile_rows) {
   typedef Elem<kHalf> E;
   constexpr int kLanes = D / 4;
   const int c = threadIdx.x % kLanes;
   const int64_t at = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  const int tile = (int)(at / 32), r = (int)(at % 32);
-  if (tile >= a.items / a.parts) return;
-  const int unit = tile / a.row_tiles;
-  const int row = (a.row_tiles - 1 - (tile - unit * a.row_tiles)) * kRowsFew + r;
+  const int unit = (int)(at / tile_rows), r = (int)(at % tile_rows);     // of the items that are cut
+  if (unit >= kXcds * a.tail) return;
+  Item it;
+  if (!item_at(a, unit / a.tail, a.tail_start + unit % a.tail, tile_rows, it)) return;
+  const int row = it.row0 + r;
   if (row >= a.rows) return;
   float top = -INFINITY, l = 0.f;
-  const int64_t first = (int64_t)tile * a.parts * 32 + r;
-  for (int p = 0; p < a.parts; ++p) top = fmaxf(top, a.part_ml[(first + 32 * p) * 2]);
+  const int64_t first = (int64_t)unit * a.ways * tile_rows + r;
+  for (int p = 0; p < a.ways; ++p) top = fmaxf(top, a.part_ml[(first + tile_rows * p) * 2]);
   f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < a.parts; ++p) {
-    const int64_t i = first + 32 * p;
+  for (int p = 0; p < a.ways; ++p) {
+    const int64_t i = first + tile_rows * p;
     const float m = a.part_ml[i * 2];
     if (!(m > -INFINITY)) continue;
     const float w = __builtin_amdgcn_exp2f(m - top);
@@ -780,7 +830,7 @@ __global__ __launch_bounds__(256) void attn_window_fold_kernel(const WindowArgs 
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w, x[e], sum[e]);
   }
-  const int s = row / a.group, b = unit / a.Hk, h = (unit - b * a.Hk) * a.group + row - s * a.group;
+  const int s = row / a.group, b = it.b, h = it.hk * a.group + row - s * a.group;
   const float inv = l != 0.f ? 1.f / l : 0.f;
   typename E::x4 o;
 #pragma unroll
@@ -818,50 +868,57 @@ int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int waves, int lds
   return hip_fail(hipGetLastError(), "attn_window launch");
 }
 
+// Cuts an XCD's last items, `tail` of them, into `ways` workgroups along the keys, where that is estimated to end sooner.  us: `tile` a tile of
+// the form's, `once` an item beside its tiles.
+void plan_tail(WindowArgs& a, int D, int tile_rows, int64_t slots, int64_t tiles, double tile, double once, void* workspace, int64_t workspace_bytes) {
+  a.per_xcd = (a.items + kXcds - 1) / kXcds;
+  a.tail_start = a.per_xcd;
+  a.tail = 0;
+  a.ways = 1;
+  const int64_t tail = a.per_xcd % slots == 0 ? slots : a.per_xcd % slots;     // (a launch of whole rounds is cut in its last one, if at all)
+  double best = tile * tiles + once;
+  for (int ways = 2; ways <= 64 && tiles >= 4 * ways; ++ways) {
+    const int64_t bytes = kXcds * tail * ways * tile_rows * (D + 2) * 4;
+    if (!workspace || bytes > workspace_bytes) break;
+    // the parts' states go to memory and back at some 4 bytes a ns, in a launch behind this one
+    const double cost = (double)((tail * ways + slots - 1) / slots) * (tile * ((tiles + ways - 1) / ways) + once) + 5.0 + 2.0 * bytes / 4.0e6;
+    if (cost < best) {
+      best = cost;
+      a.ways = ways;
+    }
+  }
+  if (a.ways == 1) return;
+  a.tail = (int32_t)tail;
+  a.tail_start = a.per_xcd - a.tail;
+  a.part_out = static_cast<float*>(workspace);
+  a.part_ml = a.part_out + kXcds * tail * a.ways * tile_rows * D;
+}
+
 template <int D, bool kHalf>
 int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   const int64_t shared = units * ((a.rows + kRowsShared - 1) / kRowsShared);
   const bool few = shared < (D == 64 ? 2 : 1) * n_cus;
-  a.row_tiles = (a.rows + (few ? kRowsFew : kRowsShared) - 1) / (few ? kRowsFew : kRowsShared);
-  int64_t items = units * a.row_tiles;
-  a.parts = 1;
-  if (few) {
-    // keys that a row tile may see, in tiles
-    const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + kRowsFew + 2 * a.frame);
-    const int64_t tiles = (seen + 31) / 32;
-    const int64_t slots = (int64_t)n_cus * (D == 64 ? 2 : 1);
-    const int64_t bytes = items * (32 * (D + 2) * 4);
-    int64_t most = std::min<int64_t>(64, tiles / (2 * kWavesFew));
-    if (!workspace || bytes <= 0) most = 1;
-    else most = std::min(most, workspace_bytes / bytes);
-    // rounds of the chip x tiles of a workgroup
-    int64_t best = (items + slots - 1) / slots * ((tiles + kWavesFew - 1) / kWavesFew);
-    for (int64_t p = 2; p <= most; ++p) {
-      const int64_t cost = (items * p + slots - 1) / slots * ((tiles + kWavesFew * p - 1) / (kWavesFew * p) + 2) + 4;
-      if (cost < best) {
-        best = cost;
-        a.parts = (int)p;
-      }
-    }
-    items *= a.parts;
-  }
+  const int tile_rows = few ? kRowsFew : kRowsShared;
+  a.row_tiles = (a.rows + tile_rows - 1) / tile_rows;
+  const int64_t items = units * a.row_tiles;
   if (items > (1 << 28)) {
     set_error("too many query tiles (%lld)", (long long)items);
     return DT_ERR_INVALID;
   }
   a.items = (int32_t)items;
-  a.per_xcd = (a.items + kXcds - 1) / kXcds;
-  if (a.parts > 1) {
-    a.part_out = static_cast<float*>(workspace);
-    a.part_ml = a.part_out + items * 32 * D;
-  }
-  const unsigned grid = (unsigned)(a.per_xcd * kXcds);
-  if (!few) return launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream);
-  if (int rc = launch(attn_window_few_kernel<D, kHalf>, a, grid, kWavesFew, FewLds<D>::kAll, stream)) return rc;
-  if (a.parts == 1) return DT_OK;
-  const int64_t rows = items / a.parts * 32;
-  const unsigned fold = (unsigned)((rows * (D / 4) + 255) / 256);
-  hipLaunchKernelGGL((attn_window_fold_kernel<D, kHalf>), dim3(fold), dim3(256), 0, stream, a);
+  // keys that a row tile sees, at most
+  const int64_t rows = tile_rows / a.group + 1;
+  const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + rows / a.frame * a.frame);
+  const int64_t slots = (int64_t)n_cus / kXcds * (D == 64 ? 2 : 1);
+  if (few) plan_tail(a, D, tile_rows, slots, (seen + 32 * kWavesFew - 1) / (32 * kWavesFew), 1.5, 4.0, workspace, workspace_bytes);
+  else plan_tail(a, D, tile_rows, slots, (seen + 63) / 64, D == 64 ? 0.55 : 0.75, 5.0, workspace, workspace_bytes);
+  const unsigned grid = (unsigned)(kXcds * (a.tail_start + a.tail * a.ways));
+  if (int rc = few ? launch(attn_window_few_kernel<D, kHalf>, a, grid, kWavesFew, FewLds<D>::kAll, stream)
+                   : launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream))
+    return rc;
+  if (a.ways == 1) return DT_OK;
+  const int64_t folded = (int64_t)kXcds * a.tail * tile_rows;
+  hipLaunchKernelGGL((attn_window_fold_kernel<D, kHalf>), dim3((unsigned)((folded * (D / 4) + 255) / 256)), dim3(256), 0, stream, a, tile_rows);
   return hip_fail(hipGetLastError(), "attn_window fold launch");
 }
 

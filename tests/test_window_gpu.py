@@ -70,6 +70,8 @@ CASES = [
     (2, 700, 900, 32, 16, dict(left=1, right=0, frame=128, sinks=70, q_begin=190)),
     (3, 600, 777, 40, 40, dict(left=None, right=0, sinks=0)),
     (1, 1500, 1600, 64, 8, dict(left=2, right=2, frame=100, sinks=100, q_begin=100)),
+    (1, 2100, 2100, 66, 66, dict(left=None, right=0)),                # ... with a last round that is cut along the keys
+    (1, 2100, 2300, 70, 70, dict(left=9, right=3, frame=100, sinks=150, q_begin=200)),
 ]
 
 
@@ -97,19 +99,20 @@ def test_lengths_on_the_gpu(hip, D, Sq, H):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("Sq, H", [(48, 2), (700, 64)])
-def test_masked_values_add_nothing(hip, Sq, H, dtype):
+@pytest.mark.parametrize("Sq, H, Hk, left", [(48, 2, 1, 6), (700, 64, 1, 6), (2100, 66, 66, 6), (2100, 66, 66, 1500)])
+def test_masked_values_add_nothing(hip, Sq, H, Hk, left, dtype):
     """Infinities and NaN in values and keys that some rows see and others do not."""
-    q, k, v = _tensors(1, Sq, Sq, H, 1, 64, dtype, seed=1)
+    q, k, v = _tensors(1, Sq, Sq, H, Hk, 64, dtype, seed=1)
     v[0, 20, 0, 5] = float("inf")
     v[0, 33, 0, 7] = float("nan")
     v[0, 2, 0, 9] = float("-inf")
     k[0, 41] = float("nan")
-    w = dict(left=6, right=0, sinks=1)
+    w = dict(left=left, right=0, sinks=1)
     out, lse = _run(q, k, v, **w)
-    seen = L.visible(Sq, Sq, Sq, 6, 0, 1, 1, None)
+    seen = L.visible(Sq, Sq, Sq, left, 0, 1, 1, None)
     hurt = seen[:, 41]
-    assert bool(out[0, hurt.to(DEV)].isnan().all()) and bool(lse[0, :, hurt.to(DEV)].isnan().all())
+    assert bool(out[0, hurt.to(DEV), 0].isnan().all()) and bool(lse[0, 0, hurt.to(DEV)].isnan().all())
+    out, q, k, v = out[:, :, :2], q[:, :, :2], k[:, :, :1 if Hk == 1 else 2], v[:, :, :1 if Hk == 1 else 2]      # (the others have nothing special)
     keep = (~hurt).nonzero()[:, 0].to(DEV)
     o, l, weight, top = L.window_attention(q, k, v, **w)
     got, want = out[0, keep].double(), o[0, keep]
