@@ -11,9 +11,9 @@
 // fill the matrix instructions of a single token.  Two forms:
 //   * shared tiles: a workgroup of 8 wavefronts, 32 rows each, walks the 64-key tiles that some of its 256 rows see: the sinks' tiles,
 //     then the window's.  Its two groups of 4 run a phase apart: while one has its products on the matrix pipe, the other does its softmax.
-//   * few rows: the 4 wavefronts of a workgroup share 32 rows and take 32-key tiles of their own in turn, and the window is cut into
-//     `parts` workgroups; states meet in the LDS, those of the parts in a fold kernel behind the launch.
-// A wavefront leaves out tiles that none of its rows sees, and only a tile with a border in it is masked.
+//   * few rows: the 8 wavefronts of a workgroup share 32 rows and take 32-key tiles of their own in turn; their states meet in the LDS.
+// Only a tile with a border in it is masked.  The last round of workgroups, or all of them, may be cut into parts along the keys, whose states a
+// kernel behind the launch adds up.
 #include <algorithm>
 #include <cmath>
 
@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kWavesShared = 8;
 constexpr int kRowsShared = kWavesShared * 32;   // rows of a workgroup, shared tiles
-constexpr int kWavesFew = 4;
+constexpr int kWavesFew = 8;
 constexpr int kRowsFew = 32;                     // ... few rows
 constexpr int kXcds = 8;
 // A tile's sum of a lane's probabilities above which the tile is redone with its exact maximum: below it no probability exceeds 2^12,
@@ -687,16 +687,25 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   wait_loads();     // (loads past the last tile store zeros: before the LDS is another workgroup's)
 }
 
-// Few rows.  The LDS holds two tiles (K and V) of each wavefront, then the four states.
+// Few rows.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is on its way while it
+// has the softmax and the values of this one, V of the next from there on, and while it waits the other seven have theirs (8 x 16 KB a CU at
+// D = 128; four wavefronts with two tiles each were 48 KB a us and CU, this is 70).
 template <int D>
 struct FewLds {
-  static constexpr int kBytes = kWavesFew * 4 * Tiles<D, 1>::kBytes;
-  static_assert(kWavesFew * 32 * D * 4 <= kBytes, "the states fit the tile buffers");
+  static constexpr int kTile = 2 * Tiles<D, 1>::kBytes;
+  static constexpr int kBytes = kWavesFew * kTile;
+  static_assert(32 * D * 4 <= kTile, "a state fits its wavefront's tile");
   static constexpr int kAll = kBytes + kWavesFew * 256;      // and a maximum and a sum a row and wavefront
 };
+template <int N>
+__device__ __forceinline__ void wait_oldest() {     // all loads but those of the newest half tile
+  static_assert(N == 4 || N == 8, "blocks of a half tile");
+  if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+}
 
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_few_kernel(const WindowArgs a) {
   typedef Tiles<D, 1> T;
   typedef Elem<kHalf> E;
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -707,38 +716,46 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
   const int len = keys_of(a, it.b);
   RowState<D, kHalf, 1> st;
   st.open(a, it.b, it.hk, it.row0, len, lane);
-  const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every fourth tile
-  uint8_t* mine = lds + wave * 4 * T::kBytes;
-  const uint32_t mine0 = (uint32_t)(uintptr_t)(lds_ptr_t)mine;
+  const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every eighth tile
+  const uint8_t* kt = lds + wave * FewLds<D>::kTile;
+  const uint8_t* vt = kt + T::kBytes;
+  const uint32_t kt0 = (uint32_t)(uintptr_t)(lds_ptr_t)(lds + wave * FewLds<D>::kTile);
   Loader<D, 1> ld;
   ld.open(a, it.b, it.hk, lane);
-  auto issue = [&](int t, int buf) __attribute__((always_inline)) {
-    const uint32_t at = mine0 + buf * 2 * T::kBytes;
+  auto load_k = [&](int t) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
     const int k0 = list.key(t);
-    ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, len - k0, 0, 1, at);
-    ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, len - k0, 0, 1, at + T::kBytes);
+    ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, t < list.end ? len - k0 : 0, 0, 1, kt0);
   };
-  int buf = 0;
-  if (list.begin + wave < list.end) issue(list.begin + wave, 0);
-  for (int t = list.begin + wave; t < list.end; t += kWavesFew, buf ^= 1) {
-    wait_loads();
-    if (t + kWavesFew < list.end) issue(t + kWavesFew, buf ^ 1);
-    const uint8_t* kt = mine + buf * 2 * T::kBytes;
+  auto load_v = [&](int t) __attribute__((always_inline)) {
+    const int k0 = list.key(t);
+    ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, t < list.end ? len - k0 : 0, 0, 1, kt0 + T::kBytes);
+  };
+  int t = list.begin + wave;
+  if (t < list.end) {
+    load_k(t);
+    load_v(t);
+  }
+  for (; t < list.end; t += kWavesFew) {
     const int k0 = list.key(t);
     const bool masked = !st.whole(k0);
     f32x16 s[1];
     typename E::x8 p[1][2];
+    wait_oldest<T::kBlocks>();
     st.scores(kt, s);
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");      // (the tile has been read)
+    load_k(t + kWavesFew);
     st.softmax(s, p, k0, masked, lane);
-    if (masked && st.any_not_finite(kt + T::kBytes, lane)) st.values_not_finite(kt + T::kBytes, p, k0, lane);
-    else st.values(kt + T::kBytes, p);
+    wait_oldest<T::kBlocks>();
+    if (masked && st.any_not_finite(vt, lane)) st.values_not_finite(vt, p, k0, lane);
+    else st.values(vt, p);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    load_v(t + kWavesFew);
   }
-  // The four states as they lie in the registers; a wavefront then adds up its quarter of the columns.
+  // The states as they lie in the registers; a wavefront then adds up its share of the columns.
   float l = st.l_run + __shfl_xor(st.l_run, 32);
   wait_loads();
-  float* slot = reinterpret_cast<float*>(lds + wave * (32 * D * 4)) + lane * 4;
+  float* slot = reinterpret_cast<float*>(lds + wave * FewLds<D>::kTile) + lane * 4;
   float* ml = reinterpret_cast<float*>(lds + FewLds<D>::kBytes);
-  __syncthreads();
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -773,12 +790,12 @@ __global__ __launch_bounds__(kWavesFew * 64) void attn_window_few_kernel(const W
   uint16_t* out = a.out + (((int64_t)it.b * a.Sq + s) * a.H + head) * D;
   const int64_t part_row = (int64_t)it.slot * kRowsFew + col;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int q = wave * (D / 32) + i;             // group of 4 registers: d = 8 q + 4 hh ..
+  for (int i = 0; i < D / 8 / kWavesFew; ++i) {
+    const int q = wave * (D / 8 / kWavesFew) + i;  // group of 4 registers: d = 8 q + 4 hh ..
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kWavesFew; ++j) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * (32 * D * 4)) + lane * 4 + q * 256);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D>::kTile) + lane * 4 + q * 256);
       if (m[j] > -INFINITY)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);
@@ -868,36 +885,52 @@ int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int waves, int lds
   return hip_fail(hipGetLastError(), "attn_window launch");
 }
 
-// Cuts an XCD's last items, `tail` of them, into `ways` workgroups along the keys, where that is estimated to end sooner.  us: `tile` a tile of
-// the form's, `once` an item beside its tiles.
-void plan_tail(WindowArgs& a, int D, int tile_rows, int64_t slots, int64_t tiles, double tile, double once, void* workspace, int64_t workspace_bytes) {
-  a.per_xcd = (a.items + kXcds - 1) / kXcds;
-  a.tail_start = a.per_xcd;
-  a.tail = 0;
-  a.ways = 1;
-  const int64_t tail = a.per_xcd % slots == 0 ? slots : a.per_xcd % slots;     // (a launch of whole rounds is cut in its last one, if at all)
-  double best = tile * tiles + once;
-  for (int ways = 2; ways <= 64 && tiles >= 4 * ways; ++ways) {
-    const int64_t bytes = kXcds * tail * ways * tile_rows * (D + 2) * 4;
-    if (!workspace || bytes > workspace_bytes) break;
-    // the parts' states go to memory and back at some 4 bytes a ns, in a launch behind this one
-    const double cost = (double)((tail * ways + slots - 1) / slots) * (tile * ((tiles + ways - 1) / ways) + once) + 5.0 + 2.0 * bytes / 4.0e6;
-    if (cost < best) {
-      best = cost;
-      a.ways = ways;
-    }
+// How a launch runs: the form, and how the last round of workgroups (all of them, in a launch of less than one) is cut along the keys.  By
+// estimate, from what the forms take here (us; the chip idle but for them, and full):
+//   a step of few rows (32 rows, 256 keys) kStepFew, of shared tiles (256 rows, 64 keys) kStepShared, with one workgroup a CU (D = 64:
+//   kStepFull with two); an item beside its steps kOnce; parts, their states' way to memory and back and the kernel that adds them
+//   up, kFold + 2 bytes / 6.7 TB/s.
+struct Plan {
+  bool few;
+  int ways;
+  int64_t tail, tiles;
+  double us;
+};
+constexpr double kStepShared[2] = {1.4, 1.15}, kStepFew[2] = {1.6, 1.0}, kStepFull = 2.0, kOnceShared = 8.0, kOnceFew = 5.0, kFold = 8.0;
+
+template <int D>
+Plan plan_form(const WindowArgs& a, bool few, int64_t units, int n_cus, int64_t workspace_bytes) {
+  const int rows = few ? kRowsFew : kRowsShared;
+  const int64_t row_tiles = (a.rows + rows - 1) / rows, per_xcd = (units * row_tiles + kXcds - 1) / kXcds, cus = std::max(n_cus / kXcds, 1);
+  const int64_t slots = cus * (D == 64 ? 2 : 1);
+  // keys that a row tile sees, at most
+  const int64_t queries = std::min<int64_t>(rows / a.group + 1, a.Sq);
+  const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + queries / a.frame * a.frame);
+  const int step = few ? 32 * kWavesFew : 64;
+  const int64_t tiles = (seen + step - 1) / step;
+  auto item = [&](int64_t n, int64_t workgroups) {     // us of an item of n steps, that many on an XCD
+    const double one = few ? kStepFew[D == 64] : kStepShared[D == 64];
+    return (workgroups > cus ? kStepFull : one) * n + (few ? kOnceFew : kOnceShared);
+  };
+  Plan best{few, 1, 0, tiles, 0.0};
+  const int64_t tail = (per_xcd - 1) % slots + 1;
+  const double before = (double)(per_xcd / slots - (per_xcd % slots == 0)) * item(tiles, slots);
+  best.us = before + item(tiles, tail);
+  for (int ways = 2; ways <= 64 && tiles >= 2 * ways; ++ways) {
+    const int64_t bytes = kXcds * tail * ways * rows * (D + 2) * 4;
+    if (bytes > workspace_bytes) break;
+    const double us = before + (double)((tail * ways + slots - 1) / slots) * item((tiles + ways - 1) / ways, std::min(tail * ways, slots)) + kFold +
+                      2.0 * bytes / 6.7e6;
+    if (us < best.us) best = Plan{few, ways, tail, tiles, us};
   }
-  if (a.ways == 1) return;
-  a.tail = (int32_t)tail;
-  a.tail_start = a.per_xcd - a.tail;
-  a.part_out = static_cast<float*>(workspace);
-  a.part_ml = a.part_out + kXcds * tail * a.ways * tile_rows * D;
+  return best;
 }
 
 template <int D, bool kHalf>
 int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  const int64_t shared = units * ((a.rows + kRowsShared - 1) / kRowsShared);
-  const bool few = shared < (D == 64 ? 2 : 1) * n_cus;
+  const Plan shared = plan_form<D>(a, false, units, n_cus, workspace ? workspace_bytes : 0), some = plan_form<D>(a, true, units, n_cus, workspace ? workspace_bytes : 0);
+  const Plan& plan = some.us < shared.us ? some : shared;
+  const bool few = plan.few;
   const int tile_rows = few ? kRowsFew : kRowsShared;
   a.row_tiles = (a.rows + tile_rows - 1) / tile_rows;
   const int64_t items = units * a.row_tiles;
@@ -906,12 +939,14 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
     return DT_ERR_INVALID;
   }
   a.items = (int32_t)items;
-  // keys that a row tile sees, at most
-  const int64_t rows = tile_rows / a.group + 1;
-  const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + rows / a.frame * a.frame);
-  const int64_t slots = (int64_t)n_cus / kXcds * (D == 64 ? 2 : 1);
-  if (few) plan_tail(a, D, tile_rows, slots, (seen + 32 * kWavesFew - 1) / (32 * kWavesFew), 1.5, 4.0, workspace, workspace_bytes);
-  else plan_tail(a, D, tile_rows, slots, (seen + 63) / 64, D == 64 ? 0.55 : 0.75, 5.0, workspace, workspace_bytes);
+  a.per_xcd = (a.items + kXcds - 1) / kXcds;
+  a.ways = plan.ways;
+  a.tail = (int32_t)plan.tail;
+  a.tail_start = a.per_xcd - a.tail;
+  if (a.ways > 1) {
+    a.part_out = static_cast<float*>(workspace);
+    a.part_ml = a.part_out + kXcds * plan.tail * a.ways * tile_rows * D;
+  }
   const unsigned grid = (unsigned)(kXcds * (a.tail_start + a.tail * a.ways));
   if (int rc = few ? launch(attn_window_few_kernel<D, kHalf>, a, grid, kWavesFew, FewLds<D>::kAll, stream)
                    : launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream))
