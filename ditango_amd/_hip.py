@@ -120,7 +120,7 @@ _SIGNATURES = {
                                        c_i32, c_vp, c_vp, c_f32, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32,
                                        _P(c_i32), c_i32, c_i32, c_f32, c_vp]),
     "dt_attn_window_fwd": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, _P(c_i64), _P(c_i64), _P(c_i64),
-                                          c_vp, c_f32, c_i32, c_vp, c_i64, c_vp]),
+                                          c_vp, c_f32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
     "dt_merge_block_states": (ctypes.c_int, [c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp]),
     "dt_qk_norm_rope_axes": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_i32, _P(ctypes.c_uint64),
                                             _P(ctypes.c_uint8), c_i32, _P(c_i32), c_i32, c_i32, c_vp]),
@@ -459,7 +459,10 @@ def attn_window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int
                     lse: Optional[torch.Tensor] = None):
     """(out, lse) of ``dt_attn_window_fwd``; -1 stands for a border that is not there and for queries behind the keys."""
     _here(q, "q")
-    return _host().attn_window(q, k, v, left, right, frame, sinks, q_begin, kv_lens, float(softmax_scale), out, lse, attn_workspace(q.device), _stream())
+    workspace, counters = attn_scratch(q.device)
+    if counters is None:
+        counters = _stream_counters(q.device, 1)      # (none under capture)
+    return _host().attn_window(q, k, v, left, right, frame, sinks, q_begin, kv_lens, float(softmax_scale), out, lse, workspace, counters, _stream())
 
 
 def attn_sched_merge(q: torch.Tensor, table, dev_compute_ids: torch.Tensor, dev_count: torch.Tensor, max_jobs: int,

@@ -345,23 +345,7 @@ __device__ __forceinline__ void prefetch_args(uint64_t args) {
       : "memory");
 }
 
-// ---- states that meet inside a launch ----------------------------------------------------------
-// What another workgroup of the launch reads (states and partial states of a merging launch) is stored and loaded with the
-// device-scope bit: past the L1 and the XCD's L2, so that behind the writer's s_waitcnt vmcnt(0) it is where every XCD finds
-// it.  The fences of an acquire and release at device scope do the same to whole caches: the invalidation alone, executed by
-// one wavefront per merge, took the keys and values of the XCD's other workgroups out of its L2 and cost 4 us per work
-// item (two samples of 24 heads x 1861 queries x 3 of 8 chunks 242 -> 261 us); counting and waiting cost nothing that shows.
-constexpr int kNt = 2, kDevice = 16, kDeviceNt = kDevice | kNt;   // cache-policy bits of a raw buffer access: nt, sc1
-typedef __amdgpu_buffer_rsrc_t Rsrc;
-__device__ __forceinline__ Rsrc buffer_of(const void* base, uint32_t valid_bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, valid_bytes, kRsrcFlags);
-}
-__device__ __forceinline__ void store_device(float* p, float x) {
-  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float load_device(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
+// ---- states that meet inside a launch (see attn_tiles.h) ----------------------------------------
 // This wavefront's contribution (device-scope stores) is complete: counts it.  True for the last of `expected`, whose
 // device-scope loads then see the contributions of the others, and for which the counter is back at zero.
 __device__ __forceinline__ bool arrive_last(uint32_t* counter, int expected) {

@@ -11,9 +11,9 @@
 // fill the matrix instructions of a single token.  Two forms:
 //   * shared tiles: a workgroup of 8 wavefronts, 32 rows each, walks the 64-key tiles that some of its 256 rows see: the sinks' tiles,
 //     then the window's.  Its two groups of 4 run a phase apart: while one has its products on the matrix pipe, the other does its softmax.
-//   * few rows: the 8 wavefronts of a workgroup share 32 rows and take 32-key tiles of their own in turn; their states meet in the LDS.
-// Only a tile with a border in it is masked.  The last round of workgroups, or all of them, may be cut into parts along the keys, whose states a
-// kernel behind the launch adds up.
+//   * few rows: the 8 (or 4) wavefronts of a workgroup share 32 rows and take 32-key tiles of their own in turn; their states meet in the LDS.
+// Only a tile with a border in it is masked.  The last round of workgroups, or all of them, may be cut into parts along the keys, whose states the
+// last one of an item adds up (few rows, with counters) or a kernel behind the launch.
 #include <algorithm>
 #include <cmath>
 
@@ -25,8 +25,7 @@ namespace {
 
 constexpr int kWavesShared = 8;
 constexpr int kRowsShared = kWavesShared * 32;   // rows of a workgroup, shared tiles
-constexpr int kWavesFew = 8;
-constexpr int kRowsFew = 32;                     // ... few rows
+constexpr int kRowsFew = 32;                     // ... few rows, 4 or 8 wavefronts
 constexpr int kXcds = 8;
 // A tile's sum of a lane's probabilities above which the tile is redone with its exact maximum: below it no probability exceeds 2^12,
 // which the 16-bit operand and the fp32 sums hold as well as one below 1.
@@ -48,6 +47,7 @@ struct WindowArgs {
   int32_t tail_start, tail, ways;
   float* part_out;              // [part][row of a tile][D] sums, and [part][row] (maximum in powers of two, sum)
   float* part_ml;
+  uint32_t* counters;           // of an item's parts that are done, zero before and after the launch; null: a kernel adds them up
 };
 
 struct Span {
@@ -687,15 +687,16 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   wait_loads();     // (loads past the last tile store zeros: before the LDS is another workgroup's)
 }
 
-// Few rows.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is on its way while it
-// has the softmax and the values of this one, V of the next from there on, and while it waits the other seven have theirs (8 x 16 KB a CU at
-// D = 128; four wavefronts with two tiles each were 48 KB a us and CU, this is 70).
-template <int D>
+// Few rows, W wavefronts.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is on its
+// way while it has the softmax and the values of this one, V of the next from there on, and while it waits the others have theirs (8 x 16 KB a
+// CU at D = 128; four wavefronts with two tiles each were 48 KB a us and CU, this is 70).
+template <int D, int W>
 struct FewLds {
   static constexpr int kTile = 2 * Tiles<D, 1>::kBytes;
-  static constexpr int kBytes = kWavesFew * kTile;
+  static constexpr int kBytes = W * kTile;
   static_assert(32 * D * 4 <= kTile, "a state fits its wavefront's tile");
-  static constexpr int kAll = kBytes + kWavesFew * 256;      // and a maximum and a sum a row and wavefront
+  static constexpr int kFlag = kBytes + W * 256;             // behind a maximum and a sum a row and wavefront
+  static constexpr int kAll = kFlag + 16;
 };
 template <int N>
 __device__ __forceinline__ void wait_oldest() {     // all loads but those of the newest half tile
@@ -704,8 +705,8 @@ __device__ __forceinline__ void wait_oldest() {     // all loads but those of th
   else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
 }
 
-template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_few_kernel(const WindowArgs a) {
+template <int D, bool kHalf, int W>
+__global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kernel(const WindowArgs a) {
   typedef Tiles<D, 1> T;
   typedef Elem<kHalf> E;
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -716,10 +717,10 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
   const int len = keys_of(a, it.b);
   RowState<D, kHalf, 1> st;
   st.open(a, it.b, it.hk, it.row0, len, lane);
-  const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every eighth tile
-  const uint8_t* kt = lds + wave * FewLds<D>::kTile;
+  const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every W-th tile
+  const uint8_t* kt = lds + wave * FewLds<D, W>::kTile;
   const uint8_t* vt = kt + T::kBytes;
-  const uint32_t kt0 = (uint32_t)(uintptr_t)(lds_ptr_t)(lds + wave * FewLds<D>::kTile);
+  const uint32_t kt0 = (uint32_t)(uintptr_t)(lds_ptr_t)(lds + wave * FewLds<D, W>::kTile);
   Loader<D, 1> ld;
   ld.open(a, it.b, it.hk, lane);
   auto load_k = [&](int t) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
@@ -735,7 +736,7 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
     load_k(t);
     load_v(t);
   }
-  for (; t < list.end; t += kWavesFew) {
+  for (; t < list.end; t += W) {
     const int k0 = list.key(t);
     const bool masked = !st.whole(k0);
     f32x16 s[1];
@@ -743,19 +744,19 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
     wait_oldest<T::kBlocks>();
     st.scores(kt, s);
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");      // (the tile has been read)
-    load_k(t + kWavesFew);
+    load_k(t + W);
     st.softmax(s, p, k0, masked, lane);
     wait_oldest<T::kBlocks>();
     if (masked && st.any_not_finite(vt, lane)) st.values_not_finite(vt, p, k0, lane);
     else st.values(vt, p);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    load_v(t + kWavesFew);
+    load_v(t + W);
   }
   // The states as they lie in the registers; a wavefront then adds up its share of the columns.
   float l = st.l_run + __shfl_xor(st.l_run, 32);
   wait_loads();
-  float* slot = reinterpret_cast<float*>(lds + wave * FewLds<D>::kTile) + lane * 4;
-  float* ml = reinterpret_cast<float*>(lds + FewLds<D>::kBytes);
+  float* slot = reinterpret_cast<float*>(lds + wave * FewLds<D, W>::kTile) + lane * 4;
+  float* ml = reinterpret_cast<float*>(lds + FewLds<D, W>::kBytes);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -770,15 +771,15 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
     ml[wave * 64 + 32 + col] = l;
   }
   __syncthreads();
-  float m[kWavesFew], w[kWavesFew], top = -INFINITY;
+  float m[W], w[W], top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kWavesFew; ++i) {
+  for (int i = 0; i < W; ++i) {
     m[i] = ml[i * 64 + col];
     top = fmaxf(top, m[i]);
   }
   l = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWavesFew; ++i) {
+  for (int i = 0; i < W; ++i) {
     w[i] = m[i] > -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;    // a state without a key
     if (m[i] > -INFINITY) l = __builtin_fmaf(w[i], ml[i * 64 + 32 + col], l);
   }
@@ -788,21 +789,24 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int64_t head = it.hk * a.group + g0;
   uint16_t* out = a.out + (((int64_t)it.b * a.Sq + s) * a.H + head) * D;
+  const bool meet = it.ways > 1 && a.counters != nullptr;
   const int64_t part_row = (int64_t)it.slot * kRowsFew + col;
+  constexpr uint32_t kPartBytes = kRowsFew * D * 4;
+  const Rsrc part = buffer_of(a.part_out + (int64_t)it.slot * (kRowsFew * D), kPartBytes);
 #pragma unroll
-  for (int i = 0; i < D / 8 / kWavesFew; ++i) {
-    const int q = wave * (D / 8 / kWavesFew) + i;  // group of 4 registers: d = 8 q + 4 hh ..
+  for (int i = 0; i < D / 8 / W; ++i) {
+    const int q = wave * (D / 8 / W) + i;  // group of 4 registers: d = 8 q + 4 hh ..
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kWavesFew; ++j) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D>::kTile) + lane * 4 + q * 256);
+    for (int j = 0; j < W; ++j) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D, W>::kTile) + lane * 4 + q * 256);
       if (m[j] > -INFINITY)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);
     }
     if (!live) continue;
     if (it.ways > 1) {
-      *reinterpret_cast<f32x4*>(a.part_out + part_row * D + 8 * q + 4 * hh) = sum;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), part, (col * D + 8 * q + 4 * hh) * 4, 0, kDevice);
     } else {
       typename E::x4 h;
 #pragma unroll
@@ -812,12 +816,75 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_window_f
   }
   if (wave == 0 && hh == 0 && live) {
     if (it.ways > 1) {
-      a.part_ml[part_row * 2] = top;
-      a.part_ml[part_row * 2 + 1] = l;
+      store_device(a.part_ml + part_row * 2, top);
+      store_device(a.part_ml + part_row * 2 + 1, l);
     } else {
       a.lse[((int64_t)it.b * a.H + head) * a.Sq + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
     }
   }
+  if (!meet) return;
+  // The last of the item's parts adds them all up, each lane the columns it has stored of its own part's.
+  int* flag = reinterpret_cast<int*>(lds + FewLds<D, W>::kFlag);
+  wait_loads();                // (stores as well)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* counter = a.counters + it.slot / it.ways;
+    const bool last = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == it.ways;
+    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  if (!*flag || !live) return;
+  const int slot0 = it.slot - it.part;
+  const float* mls = a.part_ml + ((int64_t)slot0 * kRowsFew + col) * 2;
+  const float* parts = a.part_out + (int64_t)slot0 * (kRowsFew * D);
+  constexpr int kCols = D / 8 / W, kSome = 4;          // parts under way together
+  top = -INFINITY;
+  for (int p0 = 0; p0 < it.ways; p0 += kSome) {
+    float x[kSome];
+#pragma unroll
+    for (int p = 0; p < kSome; ++p) x[p] = load_device(mls + min(p0 + p, it.ways - 1) * (2 * kRowsFew));
+#pragma unroll
+    for (int p = 0; p < kSome; ++p) top = fmaxf(top, x[p]);
+  }
+  f32x4 sum[kCols];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  l = 0.f;
+  for (int p0 = 0; p0 < it.ways; p0 += kSome) {
+    float pm[kSome], pl[kSome];
+    f32x4 x[kSome][kCols];
+#pragma unroll
+    for (int p = 0; p < kSome; ++p) {
+      const int at = min(p0 + p, it.ways - 1);
+      pm[p] = load_device(mls + at * (2 * kRowsFew));
+      pl[p] = load_device(mls + at * (2 * kRowsFew) + 1);
+      const Rsrc from = buffer_of(parts + (int64_t)at * (kRowsFew * D), kPartBytes);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+        x[p][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (col * D + 8 * (wave * kCols + i) + 4 * hh) * 4, 0, kDevice));
+    }
+#pragma unroll
+    for (int p = 0; p < kSome; ++p) {
+      if (p0 + p >= it.ways || !(pm[p] > -INFINITY)) continue;       // (a part without a key has stored nothing of use)
+      const float wp = __builtin_amdgcn_exp2f(pm[p] - top);
+      l = __builtin_fmaf(wp, pl[p], l);
+#pragma unroll
+      for (int i = 0; i < kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(wp, x[p][i][e], sum[i][e]);
+    }
+  }
+  const float norm = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    typename E::x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(sum[i][e] * norm);
+    *reinterpret_cast<typename E::x4*>(out + 8 * (wave * kCols + i) + 4 * hh) = h;
+  }
+  if (wave == 0 && hh == 0)
+    a.lse[((int64_t)it.b * a.H + head) * a.Sq + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
 // Adds up the parts of a row: a lane group of D / 4 lanes a row.
@@ -886,52 +953,59 @@ int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int waves, int lds
 }
 
 // How a launch runs: the form, and how the last round of workgroups (all of them, in a launch of less than one) is cut along the keys.  By
-// estimate, from what the forms take here (us; the chip idle but for them, and full):
-//   a step of few rows (32 rows, 256 keys) kStepFew, of shared tiles (256 rows, 64 keys) kStepShared, with one workgroup a CU (D = 64:
-//   kStepFull with two); an item beside its steps kOnce; parts, their states' way to memory and back and the kernel that adds them
-//   up, kFold + 2 bytes / 6.7 TB/s.
+// estimate, from what the forms take here, in us: a step -- 64 keys of shared tiles, a 32-key tile of every wavefront of few rows -- with up to
+// eight wavefronts a CU, and with more (D = 64); an item beside its steps; parts, their states' way to memory and back, 2 bytes / 6.7 TB/s, and the
+// kernel that adds them up, or the last of them that does.
+struct Form {
+  int rows, keys, per_cu;       // rows of a workgroup, keys of its step, workgroups a CU
+  double step, full, once;
+};
+template <int D>
+constexpr Form kForms[3] = {
+    {kRowsShared, 64, D == 64 ? 2 : 1, D == 64 ? 1.15 : 1.4, 2.0, 8.0},
+    {kRowsFew, 256, D == 64 ? 2 : 1, D == 64 ? 1.0 : 1.6, 2.0, 5.0},
+    {kRowsFew, 128, D == 64 ? 4 : 2, D == 64 ? 1.0 : 1.6, 2.0, 4.0},
+};
 struct Plan {
-  bool few;
-  int ways;
-  int64_t tail, tiles;
+  int form, ways;
+  int64_t tail;
   double us;
 };
-constexpr double kStepShared[2] = {1.4, 1.15}, kStepFew[2] = {1.6, 1.0}, kStepFull = 2.0, kOnceShared = 8.0, kOnceFew = 5.0, kFold = 8.0;
 
 template <int D>
-Plan plan_form(const WindowArgs& a, bool few, int64_t units, int n_cus, int64_t workspace_bytes) {
-  const int rows = few ? kRowsFew : kRowsShared;
-  const int64_t row_tiles = (a.rows + rows - 1) / rows, per_xcd = (units * row_tiles + kXcds - 1) / kXcds, cus = std::max(n_cus / kXcds, 1);
-  const int64_t slots = cus * (D == 64 ? 2 : 1);
+Plan plan_form(const WindowArgs& a, int form, int64_t units, int n_cus, int64_t workspace_bytes) {
+  const Form& f = kForms<D>[form];
+  const int64_t row_tiles = (a.rows + f.rows - 1) / f.rows, per_xcd = (units * row_tiles + kXcds - 1) / kXcds, cus = std::max(n_cus / kXcds, 1);
+  const int64_t slots = cus * f.per_cu;
   // keys that a row tile sees, at most
-  const int64_t queries = std::min<int64_t>(rows / a.group + 1, a.Sq);
+  const int64_t queries = std::min<int64_t>(f.rows / a.group + 1, a.Sq);
   const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + queries / a.frame * a.frame);
-  const int step = few ? 32 * kWavesFew : 64;
-  const int64_t tiles = (seen + step - 1) / step;
-  auto item = [&](int64_t n, int64_t workgroups) {     // us of an item of n steps, that many on an XCD
-    const double one = few ? kStepFew[D == 64] : kStepShared[D == 64];
-    return (workgroups > cus ? kStepFull : one) * n + (few ? kOnceFew : kOnceShared);
+  const int64_t steps = (seen + f.keys - 1) / f.keys;
+  auto item = [&](int64_t n, int64_t workgroups) {     // us of an item of n steps, that many at once on an XCD
+    return (D == 64 && 2 * workgroups > slots ? f.full : f.step) * n + f.once;
   };
-  Plan best{few, 1, 0, tiles, 0.0};
   const int64_t tail = (per_xcd - 1) % slots + 1;
-  const double before = (double)(per_xcd / slots - (per_xcd % slots == 0)) * item(tiles, slots);
-  best.us = before + item(tiles, tail);
-  for (int ways = 2; ways <= 64 && tiles >= 2 * ways; ++ways) {
-    const int64_t bytes = kXcds * tail * ways * rows * (D + 2) * 4;
+  const double before = (double)((per_xcd - tail) / slots) * item(steps, slots);
+  Plan best{form, 1, 0, before + item(steps, tail)};
+  for (int ways = 2; ways <= 64 && steps >= 2 * ways; ++ways) {
+    const int64_t bytes = kXcds * tail * ways * f.rows * (D + 2) * 4;
     if (bytes > workspace_bytes) break;
-    const double us = before + (double)((tail * ways + slots - 1) / slots) * item((tiles + ways - 1) / ways, std::min(tail * ways, slots)) + kFold +
+    const double fold = form != 0 && a.counters ? 3.0 : 8.0;
+    const double us = before + (double)((tail * ways + slots - 1) / slots) * item((steps + ways - 1) / ways, std::min(tail * ways, slots)) + fold +
                       2.0 * bytes / 6.7e6;
-    if (us < best.us) best = Plan{few, ways, tail, tiles, us};
+    if (us < best.us) best = Plan{form, ways, tail, us};
   }
   return best;
 }
 
 template <int D, bool kHalf>
-int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  const Plan shared = plan_form<D>(a, false, units, n_cus, workspace ? workspace_bytes : 0), some = plan_form<D>(a, true, units, n_cus, workspace ? workspace_bytes : 0);
-  const Plan& plan = some.us < shared.us ? some : shared;
-  const bool few = plan.few;
-  const int tile_rows = few ? kRowsFew : kRowsShared;
+int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, int64_t n_counters, hipStream_t stream) {
+  Plan plan = plan_form<D>(a, 0, units, n_cus, workspace ? workspace_bytes : 0);
+  for (int form : {1, 2}) {
+    const Plan other = plan_form<D>(a, form, units, n_cus, workspace ? workspace_bytes : 0);
+    if (other.us < plan.us) plan = other;
+  }
+  const int tile_rows = kForms<D>[plan.form].rows;
   a.row_tiles = (a.rows + tile_rows - 1) / tile_rows;
   const int64_t items = units * a.row_tiles;
   if (items > (1 << 28)) {
@@ -947,11 +1021,12 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
     a.part_out = static_cast<float*>(workspace);
     a.part_ml = a.part_out + kXcds * plan.tail * a.ways * tile_rows * D;
   }
+  if (plan.form == 0 || kXcds * plan.tail > n_counters) a.counters = nullptr;
   const unsigned grid = (unsigned)(kXcds * (a.tail_start + a.tail * a.ways));
-  if (int rc = few ? launch(attn_window_few_kernel<D, kHalf>, a, grid, kWavesFew, FewLds<D>::kAll, stream)
-                   : launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream))
-    return rc;
-  if (a.ways == 1) return DT_OK;
+  const int rc = plan.form == 0   ? launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream)
+                 : plan.form == 1 ? launch(attn_window_few_kernel<D, kHalf, 8>, a, grid, 8, FewLds<D, 8>::kAll, stream)
+                                  : launch(attn_window_few_kernel<D, kHalf, 4>, a, grid, 4, FewLds<D, 4>::kAll, stream);
+  if (rc != DT_OK || a.ways == 1 || a.counters) return rc;
   const int64_t folded = (int64_t)kXcds * a.tail * tile_rows;
   hipLaunchKernelGGL((attn_window_fold_kernel<D, kHalf>), dim3((unsigned)((folded * (D / 4) + 255) / 256)), dim3(256), 0, stream, a, tile_rows);
   return hip_fail(hipGetLastError(), "attn_window fold launch");
@@ -967,7 +1042,7 @@ using namespace dt;
 extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int32_t B, int32_t Sq, int32_t Sk,
                                   int32_t H, int32_t Hk, int32_t D, const int64_t* q_strides, const int64_t* k_strides,
                                   const int64_t* v_strides, const dt_window* window, float softmax_scale, int32_t flags, void* workspace,
-                                  int64_t workspace_bytes, void* stream) {
+                                  int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream) {
   if (B <= 0 || Sq <= 0 || Sk < 0 || H <= 0 || Hk <= 0 || H % Hk) {
     set_error("B, Sq, H, Hk must be positive, Sk not negative and H a multiple of Hk (got %d, %d, %d, %d, %d)", B, Sq, Sk, H, Hk);
     return DT_ERR_INVALID;
@@ -1008,6 +1083,10 @@ extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, v
     set_error("workspace must be 16-byte aligned with a non-negative size");
     return DT_ERR_INVALID;
   }
+  if (counters && ((reinterpret_cast<uintptr_t>(counters) & 3) || n_counters < 0)) {
+    set_error("counters must be 4-byte aligned with a non-negative number");
+    return DT_ERR_INVALID;
+  }
   const int64_t rows = (int64_t)Sq * (H / Hk), units = (int64_t)B * Hk;
   if (rows > (1ll << 30) || units > (1ll << 28) || units * ((rows + 31) / 32) > (1ll << 28)) {
     set_error("too many query rows");
@@ -1030,6 +1109,7 @@ extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, v
   a.kv_lens = w.kv_lens;
   a.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   a.rows = (int32_t)rows;
+  a.counters = counters;
   const int n_cus = cus();
   if (n_cus <= 0) {
     set_error("no current device");
@@ -1038,8 +1118,8 @@ extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, v
   const hipStream_t st = (hipStream_t)stream;
   const bool half = (flags & DT_ATTN_FP16) != 0;
   if (D == 128)
-    return half ? launch_dim<128, true>(a, units, n_cus, workspace, workspace_bytes, st)
-                : launch_dim<128, false>(a, units, n_cus, workspace, workspace_bytes, st);
-  return half ? launch_dim<64, true>(a, units, n_cus, workspace, workspace_bytes, st)
-              : launch_dim<64, false>(a, units, n_cus, workspace, workspace_bytes, st);
+    return half ? launch_dim<128, true>(a, units, n_cus, workspace, workspace_bytes, n_counters, st)
+                : launch_dim<128, false>(a, units, n_cus, workspace, workspace_bytes, n_counters, st);
+  return half ? launch_dim<64, true>(a, units, n_cus, workspace, workspace_bytes, n_counters, st)
+              : launch_dim<64, false>(a, units, n_cus, workspace, workspace_bytes, n_counters, st);
 }

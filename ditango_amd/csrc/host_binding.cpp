@@ -829,7 +829,8 @@ bool same_device(const Tensor& a, const Tensor& b) { return a.is_cuda() && b.is_
 // ditango_amd._hip.attn_window_fwd
 std::pair<Tensor, Tensor> attn_window(const Tensor& q, const Tensor& k, const Tensor& v, int32_t left, int32_t right, int32_t frame, int32_t sinks,
                                       int32_t q_begin, const std::optional<Tensor>& kv_lens, double scale, std::optional<Tensor> out,
-                                      std::optional<Tensor> lse, const std::optional<Tensor>& workspace, uint64_t stream) {
+                                      std::optional<Tensor> lse, const std::optional<Tensor>& workspace, const std::optional<Tensor>& counters,
+                                      uint64_t stream) {
   const Dims d = check_bshd(q, {"q"}), dk = check_bshd(k, {"k"}), dv = check_bshd(v, {"v"});
   REQUIRE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
   REQUIRE(same_device(q, k) && same_device(q, v), "q, k and v must be on one device");
@@ -855,7 +856,7 @@ std::pair<Tensor, Tensor> attn_window(const Tensor& q, const Tensor& k, const Te
   const dt_window w = {left, right, frame, sinks, q_begin, static_cast<const int32_t*>(ptr(kv_lens))};
   CALL(dt_attn_window_fwd, ptr(q), ptr(k), ptr(v), ptr(*out), static_cast<float*>(ptr(*lse)), (int32_t)d.B, (int32_t)d.S, (int32_t)dk.S, (int32_t)d.H,
        (int32_t)dk.H, (int32_t)d.D, qs, ks, vs, &w, (float)scale, q.scalar_type() == at::kHalf ? DT_ATTN_FP16 : 0, ptr(workspace), bytes_of(workspace),
-       stream_of(stream));
+       static_cast<uint32_t*>(ptr(counters)), counters ? counters->numel() : 0, stream_of(stream));
   return {*out, *lse};
 }
 

@@ -561,9 +561,10 @@ int dt_qkv_project(const void* text, int64_t text_stride_b, int64_t text_stride_
  * a row that sees none gets out = 0, lse = -inf.  A masked key adds nothing, whatever it and its value hold.
  * q [B,Sq,H,D], k and v [B,Sk,Hk,D] with element strides {batch, token, head} of their own (HOST arrays of 3; multiples of 8, token strides of
  * k and v at most 2^23), H a multiple of Hk: query heads h share key head h / (H / Hk).  bfloat16, or IEEE half with DT_ATTN_FP16.
- * workspace: device memory, 16-byte aligned; launches of few rows cut long windows into parts that leave partial states there and a
- * second kernel that adds them up.  dt_attn_workspace_bytes() is plenty, without it (NULL) nothing is cut.  Launches that share a workspace must not
- * overlap on the GPU.  No counterpart in the reference (its chunks are attended to whole).
+ * workspace: device memory, 16-byte aligned; launches that leave part of the GPU idle cut their windows into parts, which leave partial states
+ * there.  dt_attn_workspace_bytes() is plenty, without it (NULL) nothing is cut.  counters: n_counters words of device memory that are
+ * zero; every launch leaves them at zero.  With them, the last part of a few rows adds the parts up, without (NULL, or too few) a second kernel.
+ * Launches that share either must not overlap on the GPU.  No counterpart in the reference (its chunks are attended to whole).
  */
 typedef struct {
   int32_t left, right, frame, sinks, q_begin;
@@ -572,7 +573,7 @@ typedef struct {
 int dt_attn_window_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int32_t B, int32_t Sq, int32_t Sk,
                        int32_t H, int32_t Hk, int32_t D, const int64_t* q_strides, const int64_t* k_strides,
                        const int64_t* v_strides, const dt_window* window, float softmax_scale, int32_t flags,
-                       void* workspace, int64_t workspace_bytes, void* stream);
+                       void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream);
 
 /*
  * Attention states in 8 bits, for a cache of half the size (core/cache.py:75-84 keeps fp32 states): the merge of n states of any dtype

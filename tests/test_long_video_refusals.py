@@ -28,14 +28,14 @@ class Rows(ctypes.Structure):
 def test_window_arguments():
     lib = _hip.load_library()
     ok = dict(q=4096, k=4096, v=4096, out=4096, lse=4096, B=1, Sq=4, Sk=4, H=4, Hk=2, D=64, qs=(512, 128, 64), ks=(512, 128, 64), vs=(512, 128, 64),
-              left=1, right=0, frame=1, sinks=0, q_begin=-1, flags=0, ws=None, bytes=0)
+              left=1, right=0, frame=1, sinks=0, q_begin=-1, flags=0, ws=None, bytes=0, counters=None, n=0)
 
     def call(**kw):
         a = {**ok, **kw}
         s = [None if a[n] is None else (ctypes.c_int64 * 3)(*a[n]) for n in ("qs", "ks", "vs")]
         w = Window(a["left"], a["right"], a["frame"], a["sinks"], a["q_begin"], None)
         return lib.dt_attn_window_fwd(a["q"], a["k"], a["v"], a["out"], a["lse"], a["B"], a["Sq"], a["Sk"], a["H"], a["Hk"], a["D"], *s,
-                                      ctypes.cast(ctypes.pointer(w), ctypes.c_void_p), 0.0, a["flags"], a["ws"], a["bytes"], None)
+                                      ctypes.cast(ctypes.pointer(w), ctypes.c_void_p), 0.0, a["flags"], a["ws"], a["bytes"], a["counters"], a["n"], None)
 
     for kw in (dict(B=0), dict(Sq=0), dict(Sk=-1), dict(H=0), dict(Hk=0), dict(Hk=3)):
         assert "must be positive" in _err(lib, call(**kw))
@@ -55,6 +55,8 @@ def test_window_arguments():
         assert "flags" in _err(lib, call(flags=flags))
     for kw in (dict(ws=4104, bytes=1024), dict(ws=4096, bytes=-1)):
         assert "workspace" in _err(lib, call(**kw))
+    for kw in (dict(counters=4098, n=4), dict(counters=4096, n=-1)):
+        assert "counters" in _err(lib, call(**kw))
     assert "too many" in _err(lib, call(Sq=1 << 29, H=64, Hk=2))
 
 
