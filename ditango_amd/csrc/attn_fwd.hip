@@ -196,14 +196,6 @@ __device__ __forceinline__ void load_next_block_to_lds(u32x4 rsrc, uint32_t lane
                : "v"(lane_off), "s"(r), "s"(__builtin_amdgcn_readfirstlane(uniform_off))
                : "memory");
 }
-// The same from an address of each lane's own.
-__device__ __forceinline__ void load_rows_to_lds(const uint16_t* from, uint32_t lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-               :
-               : "v"(from), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
-               : "memory", "m0");
-}
-
 // Segment boundaries are read through the constant address space, i.e. with scalar loads: the lists were
 // written before the launch and the address is uniform.  (As a vector load the compiler follows it with
 // vmcnt(0), which inside the loop would also wait for every tile load in flight.)

@@ -94,6 +94,14 @@ __device__ __forceinline__ void load_block_to_lds(u32x4 rsrc, uint32_t lane_off,
                : "memory", "m0");
 }
 
+// The same from an address of each lane's own.
+__device__ __forceinline__ void load_rows_to_lds(const uint16_t* from, uint32_t lds_addr) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(from), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+               : "memory", "m0");
+}
+
 // ---- states that meet inside a launch ----------------------------------------------------------
 // What another workgroup of the launch reads (states and partial states of a merging launch) is stored and loaded with the
 // device-scope bit: past the L1 and the XCD's L2, so that behind the writer's s_waitcnt vmcnt(0) it is where every XCD finds

@@ -43,6 +43,7 @@ struct WindowArgs {
   const int32_t* kv_lens;       // device [B], or null: Sk
   float scale_log2;
   int32_t rows, row_tiles, items, per_xcd;
+  Quotient by_group, by_frame;
   // An XCD's items from tail_start on, tail of them, are cut along the keys into `ways` workgroups each
   int32_t tail_start, tail, ways;
   float* part_out;              // [part][row of a tile][D] sums, and [part][row] (maximum in powers of two, sum)
@@ -56,8 +57,7 @@ struct Span {
 __device__ __forceinline__ Span span_of(const WindowArgs& a, int len, int s) {
   const int p = (a.q_begin >= 0 ? a.q_begin : len - a.Sq) + s;
   const int x = p - a.sinks;
-  int f = x / a.frame;
-  if (f * a.frame > x) --f;
+  const int f = x >= 0 ? (int)quotient(x, a.by_frame) : -1 - (int)quotient(-1 - x, a.by_frame);
   const int start = a.sinks + f * a.frame;
   Span r;
   r.lo = a.left < 0 ? 0 : max(start - a.left, 0);
@@ -69,6 +69,7 @@ __device__ __forceinline__ Span uniform_span(const WindowArgs& a, int len, int s
   const Span r = span_of(a, len, __builtin_amdgcn_readfirstlane(s));
   return {__builtin_amdgcn_readfirstlane(r.lo), __builtin_amdgcn_readfirstlane(r.hi)};
 }
+__device__ __forceinline__ int query_of(const WindowArgs& a, int row) { return (int)quotient(row, a.by_group); }
 __device__ __forceinline__ int keys_of(const WindowArgs& a, int b) {
   return a.kv_lens ? min(max(a.kv_lens[b], 0), a.Sk) : a.Sk;   // nothing on the host has looked at the list
 }
@@ -125,17 +126,19 @@ struct RowState {
   Span mine, first, last;       // of this lane's query, of the wavefront's first and last (spans never go back along the rows)
   int sinks;
 
-  __device__ __forceinline__ void open(const WindowArgs& a, int b, int hk, int row0, int len, int lane) {
+  __device__ __forceinline__ void open(const WindowArgs& a, int b, int hk, int row0, int len, int lane, bool read_q) {
     const int col = lane & 31, hh = lane >> 5;
     const int row = min(row0 + col, a.rows - 1);
-    const int s = row / a.group, g = row - s * a.group;
+    const int s = query_of(a, row), g = row - s * a.group;
     mine = span_of(a, len, s);
-    first = uniform_span(a, len, min(row0, a.rows - 1) / a.group);
-    last = uniform_span(a, len, min(row0 + 31, a.rows - 1) / a.group);
+    first = uniform_span(a, len, query_of(a, min(row0, a.rows - 1)));
+    last = uniform_span(a, len, query_of(a, min(row0 + 31, a.rows - 1)));
     sinks = a.sinks;
-    const uint16_t* q = a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * a.group + g) * a.q_sh + 8 * hh;
+    if (read_q) {
+      const uint16_t* q = a.q + b * a.q_sb + s * a.q_ss + (int64_t)(hk * a.group + g) * a.q_sh + 8 * hh;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) qf[i] = *reinterpret_cast<const ex8*>(q + 16 * i);
+      for (int i = 0; i < D / 16; ++i) qf[i] = *reinterpret_cast<const ex8*>(q + 16 * i);
+    }
     c = a.scale_log2;
     m_ref = -INFINITY;
     l_run = 0.f;
@@ -206,13 +209,19 @@ struct RowState {
   __device__ __forceinline__ void softmax(f32x16 (&s)[NKB], ex8 (&p)[NKB][2], int k0, bool masked, int lane) {
     if (masked) {
       asm volatile("" ::: "memory");   // keeps this a real branch
-      const int hh = lane >> 5;
+      // A key's place behind `lo` as an unsigned number is below the span's length inside it alone; one of the sinks is below `some`.
+      const int at = k0 + 8 * (lane >> 5);
+      int from = at - mine.lo, some = min(sinks, mine.hi) - at;
+      const uint32_t length = (uint32_t)max(mine.hi - mine.lo, 0);
+      asm volatile("" : "+v"(from), "+v"(some));     // (sums of them and the keys' places would otherwise be kept through the loop)
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * kb + 16 * (r >> 3) + 8 * hh + (r & 7);
-          s[kb][r] = (key < mine.hi) & ((key >= mine.lo) | (key < sinks)) ? s[kb][r] : -INFINITY;
+          const int key = 32 * kb + 16 * (r >> 3) + (r & 7);
+          const bool seen = ((uint32_t)(from + key) < length) | (key < some);
+          s[kb][r] = seen ? s[kb][r] : -INFINITY;
+          asm volatile("" : "+v"(s[kb][r]));     // one comparison and choice after the other: 90 spilled scalars otherwise
         }
     }
     // Probabilities relative to the reference that the sums are scaled to.  The tile's own maximum is looked for only where the sum of
@@ -248,14 +257,15 @@ struct RowState {
   }
 
   // A masked key's probability is 0, which an infinite or undefined value of V would turn into NaN.  Tiles with masked keys are looked
-  // through (a wavefront reads all of the tile: 192 more vector instructions).  Where there is such a value, few rows multiply the tile with
-  // zeros in their place and then add them, as they are, to the rows that see them (the weight of a visible key is above 0); shared tiles, whose
-  // loop has no registers for that, compute the 32 rows once more behind it (rows_one_by_one).
+  // through (3 instructions for 8 values, by the four wavefronts of a group together where tiles are shared).  Where there is such a value, few
+  // rows multiply the tile with zeros in their place and then add them, as they are, to the rows that see them (the weight of a visible key is
+  // above 0); shared tiles, whose loop has no registers for that, compute the 32 rows once more behind it (rows_one_by_one).
   static constexpr uint32_t kExp = kHalf ? 0x7c007c00u : 0x7f807f80u, kOne = kHalf ? 0x04000400u : 0x00800080u;
+  template <int kBlocks = T::kBlocks>
   __device__ __forceinline__ bool any_not_finite(const uint8_t* vt, int lane) const {
     uint32_t over = 0;
 #pragma unroll 2
-    for (int i = 0; i < T::kBytes / 1024; ++i) {
+    for (int i = 0; i < kBlocks; ++i) {
       const u32x4 x = *reinterpret_cast<const u32x4*>(vt + i * 1024 + lane * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) over |= (x[e] & kExp) + kOne;   // an exponent of ones carries into the sign's bit
@@ -417,9 +427,10 @@ struct SharedLds {
 
 template <int N>
 __device__ __forceinline__ void wait_all_but() {
-  static_assert(N == 2 || N == 4, "loads of a pair");
+  static_assert(N == 2 || N == 4 || N == 8, "loads of a pair or two");
   if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
 }
 // Ends a phase: what it has made goes through the statement, so that the compiler keeps the work on its side of the barrier.
 template <typename V>
@@ -447,7 +458,7 @@ __device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item&
   const uint16_t* v = a.v + it.b * a.v_sb + it.hk * a.v_sh + lane * kCols;
 #pragma unroll 1
   for (int r = 0; r < 32 && row0 + r < a.rows; ++r) {
-    const int s = (row0 + r) / a.group, head = it.hk * a.group + row0 + r - s * a.group;
+    const int s = query_of(a, row0 + r), head = it.hk * a.group + row0 + r - s * a.group;
     const Span span = uniform_span(a, len, s);
     const uint16_t* q = a.q + it.b * a.q_sb + s * a.q_ss + head * a.q_sh;
     const float top = __shfl(m, r), norm = __shfl(inv, r);
@@ -502,8 +513,8 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   const int group = wave >> 2;
   const int len = keys_of(a, it.b);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  const TileList<T::kKeys> list(a, uniform_span(a, len, it.row0 / a.group),
-                                uniform_span(a, len, min(it.row0 + kRowsShared - 1, a.rows - 1) / a.group), it.part, it.ways);
+  const Span all_first = uniform_span(a, len, query_of(a, it.row0)), all_last = uniform_span(a, len, query_of(a, min(it.row0 + kRowsShared - 1, a.rows - 1)));
+  const TileList<T::kKeys> list(a, all_first, all_last, it.part, it.ways);
   const int n = list.end - list.begin;
   Loader<D, 2> ld;
   ld.open(a, it.b, it.hk, lane);
@@ -524,8 +535,34 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   RowState<D, kHalf, 2> st;
   const int row0 = it.row0 + 32 * wave;
   bool hurt = false;     // values that are infinite or undefined in a tile that some row does not see whole
-  if (n > 0) load_k(-1);
-  st.open(a, it.b, it.hk, row0, len, lane);
+  // The wavefront's rows of Q come as whole lines through the LDS: half of them through its staging rows, a quarter each through its own shares
+  // of V of pairs 3 and 2, which nothing but its own later loads writes.  (As fragments from memory, a load instruction touches 32 lines for 32
+  // bytes each, and the compiler's wait for them would be one for every tile load behind them.)
+  constexpr int kQuarter = kPer, kQRows = T::kBlockRows;      // 1 KB blocks, rows of one
+  auto q_at = [&](int blk) __attribute__((always_inline)) {
+    const int quarter = blk / kQuarter, i = blk % kQuarter;
+    return quarter < 2 ? S::kStage + wave * 32 * D + blk * 1024 : pair_at(5 - quarter) + (wave + kWavesShared * i) * 1024;
+  };
+  // (row r is in block r / kQRows; the quarters lie apart)
+  auto q_row = [&](int r) __attribute__((always_inline)) {
+    const int in_half = S::kStage + wave * 32 * D + r * T::kRowBytes;
+    const int blk = r / kQRows, i = blk % kQuarter;
+    const int apart = (blk / kQuarter == 2 ? pair_at(3) : pair_at(2)) + (wave + kWavesShared * i) * 1024 + r % kQRows * T::kRowBytes;
+    return r < 16 ? in_half : apart;
+  };
+  if (n > 0) {
+    const uint16_t* q = a.q + it.b * a.q_sb + (int64_t)it.hk * a.group * a.q_sh;
+#pragma unroll
+    for (int blk = 0; blk < 4 * kQuarter; ++blk) {
+      const int r = blk * kQRows + lane / T::kRowLanes, row = min(row0 + r, a.rows - 1);
+      const int s = query_of(a, row), g = row - s * a.group;
+      load_rows_to_lds(q + s * a.q_ss + g * a.q_sh + 8 * ((lane % T::kRowLanes) ^ T::swz_k(r)), lds0 + q_at(blk));
+    }
+    load_k(-1);
+    load_pair(0);
+    load_pair(1);
+  }
+  st.open(a, it.b, it.hk, row0, len, lane, false);
   if (n > 0) {
     f32x16 s[2];
     ex8 p[2][2];
@@ -573,12 +610,15 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
 #pragma unroll
       for (int i = 0; i < kRing; ++i) ring[i] = st.v_frag(vt, i % (D / 32), i / (D / 32));
     };
-    // Q and K of tile 0 are here; pairs 0 and 1 on their way
-    wait_loads();
+    // Q and K of tile 0 are here, pairs 0 and 1 on their way
+    wait_all_but<2 * S::kLoads>();
+    {
+      const int r = lane & 31, hh = lane >> 5;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) st.qf[i] = *reinterpret_cast<const ex8*>(lds + q_row(r) + 16 * ((2 * i + hh) ^ T::swz_k(r)));
+    }
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.qf[i]));
-    load_pair(0);
-    load_pair(1);
     wait_lds_barrier();
     if (group == 1) {
       wait_all_but<S::kLoads>();
@@ -588,6 +628,8 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     if (group == 0) wait_all_but<S::kLoads>();
     end_products(s, st.o);
     int k0 = list.key(list.begin);
+    // what the group's wavefronts have found in a tile's values, each in a quarter of them: in staging rows, which are free until the end
+    int* flags = reinterpret_cast<int*>(lds + S::kStage + group * 4 * 32 * D);
     auto probabilities = [&](int t, bool masked) __attribute__((always_inline)) {
       if (__builtin_expect(st.needs(k0), 1)) {
         st.softmax(s, p, k0, masked, lane);
@@ -603,12 +645,17 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       load_pair(t + 2);
       const bool masked = !st.whole(k0);
       const uint8_t* vt = lds + pair_at(t);
+      if (__builtin_expect(!((k0 + T::kKeys <= all_first.hi) & ((k0 >= all_last.lo) | (k0 + T::kKeys <= a.sinks))), 0)) {   // masked for some wavefront
+        constexpr int kShare = T::kBlocks / 4;
+        const bool bad = st.template any_not_finite<kShare>(vt + (wave & 3) * kShare * 1024, lane);
+        if (lane == 0) flags[wave & 3] = bad;
+      }
       probabilities(t, masked);
       prefill(vt);
       if (group == 1) wait_all_but<S::kLoads>();
       end_softmax(p);
       __builtin_amdgcn_s_setprio(0);
-      if (masked) hurt |= st.any_not_finite(vt, lane);
+      if (masked) hurt |= (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
       products(vt);
       if (group == 0) wait_all_but<S::kLoads>();
       end_products(s, st.o);
@@ -651,7 +698,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     return;
   }
   if (hh == 0 && row0 + col < a.rows) {
-    const int s = (row0 + col) / a.group, g = row0 + col - s * a.group;
+    const int s = query_of(a, row0 + col), g = row0 + col - s * a.group;
     a.lse[((int64_t)it.b * a.H + it.hk * a.group + g) * a.Sq + s] =
         l != 0.f ? (st.m_ref * st.c + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
   }
@@ -679,7 +726,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * D + ((chunk ^ S::swz_o(r)) << 4));
       const int row = row0 + r;
       if (row < a.rows) {
-        const int s = row / a.group, g = row - s * a.group;
+        const int s = query_of(a, row), g = row - s * a.group;
         __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.out + (((int64_t)it.b * a.Sq + s) * a.H + it.hk * a.group + g) * D + half * (D / 2) + 8 * chunk));
       }
     }
@@ -716,7 +763,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
   const int col = lane & 31, hh = lane >> 5;
   const int len = keys_of(a, it.b);
   RowState<D, kHalf, 1> st;
-  st.open(a, it.b, it.hk, it.row0, len, lane);
+  st.open(a, it.b, it.hk, it.row0, len, lane, true);
   const TileList<T::kKeys> list(a, st.first, st.last, it.part, it.ways);   // and of the part every W-th tile
   const uint8_t* kt = lds + wave * FewLds<D, W>::kTile;
   const uint8_t* vt = kt + T::kBytes;
@@ -785,7 +832,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
   }
   const int row = it.row0 + col;
   const bool live = row < a.rows;
-  const int s = min(row, a.rows - 1) / a.group, g0 = min(row, a.rows - 1) - s * a.group;
+  const int s = query_of(a, min(row, a.rows - 1)), g0 = min(row, a.rows - 1) - s * a.group;
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int64_t head = it.hk * a.group + g0;
   uint16_t* out = a.out + (((int64_t)it.b * a.Sq + s) * a.H + head) * D;
@@ -914,7 +961,7 @@ __global__ __launch_bounds__(256) void attn_window_fold_kernel(const WindowArgs 
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w, x[e], sum[e]);
   }
-  const int s = row / a.group, b = it.b, h = it.hk * a.group + row - s * a.group;
+  const int s = query_of(a, row), b = it.b, h = it.hk * a.group + row - s * a.group;
   const float inv = l != 0.f ? 1.f / l : 0.f;
   typename E::x4 o;
 #pragma unroll
@@ -1109,6 +1156,8 @@ extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, v
   a.kv_lens = w.kv_lens;
   a.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   a.rows = (int32_t)rows;
+  a.by_group = quotient_by(a.group);
+  a.by_frame = quotient_by(a.frame);
   a.counters = counters;
   const int n_cus = cus();
   if (n_cus <= 0) {
