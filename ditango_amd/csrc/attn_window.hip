@@ -323,12 +323,15 @@ struct Loader {
     k_off = row * (uint32_t)(2 * k_ss) + 16 * (chunk ^ T::swz_k(row));
     v_off = row * (uint32_t)(2 * v_ss) + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
   }
-  // Blocks b0, b0 + step .. of the tile at `from`, `left` keys in front of the last there is, into the LDS at `to`.  The descriptor ends behind the
-  // last key, rows behind it arrive as zeros (all of them where left <= 0); its base is the tile's, so that no offset needs more than 32 bits
-  // however long the cache is.  (The row is part of the lane's offset: a scalar offset beyond the descriptor's end would wrap its range check.)
+  // Bytes of a tile in front of key `left` of the sample's: rows behind the last key arrive as zeros.
+  __device__ __forceinline__ static uint32_t bytes(int left, int64_t ss) {
+    return left > 0 ? (uint32_t)(min(left, T::kKeys) - 1) * (2 * (uint32_t)ss) + T::kRowBytes : 0u;
+  }
+  // Blocks b0, b0 + step .. of the tile at `from`, of which `valid` bytes are there, into the LDS at `to`.  The descriptor's base is the tile's, so
+  // that no offset needs more than 32 bits however long the cache is.  (The row is part of the lane's offset: a scalar offset beyond the
+  // descriptor's end would wrap its range check.)
   template <int kCount>
-  __device__ __forceinline__ void issue(const uint16_t* from, int left, uint32_t off, uint32_t flip, uint32_t row, int b0, int step, uint32_t to) const {
-    const uint32_t valid = left >= T::kKeys ? (T::kKeys - 1) * row + T::kRowBytes : left > 0 ? (left - 1) * row + T::kRowBytes : 0u;
+  __device__ __forceinline__ void issue(const uint16_t* from, uint32_t valid, uint32_t off, uint32_t flip, uint32_t row, int b0, int step, uint32_t to) const {
     const u32x4 r = make_rsrc(from, valid);
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
@@ -337,37 +340,36 @@ struct Loader {
     }
   }
   template <int kCount>
-  __device__ __forceinline__ void issue_k(const uint16_t* from, int left, int b0, int step, uint32_t to) const {
-    issue<kCount>(from, left, k_off, T::kBlockXor, 2 * (uint32_t)k_ss, b0, step, to);
+  __device__ __forceinline__ void issue_k(const uint16_t* from, uint32_t valid, int b0, int step, uint32_t to) const {
+    issue<kCount>(from, valid, k_off, T::kBlockXor, 2 * (uint32_t)k_ss, b0, step, to);
   }
   template <int kCount>
-  __device__ __forceinline__ void issue_v(const uint16_t* from, int left, int b0, int step, uint32_t to) const {
-    issue<kCount>(from, left, v_off, 0u, 2 * (uint32_t)v_ss, b0, step, to);
+  __device__ __forceinline__ void issue_v(const uint16_t* from, uint32_t valid, int b0, int step, uint32_t to) const {
+    issue<kCount>(from, valid, v_off, 0u, 2 * (uint32_t)v_ss, b0, step, to);
   }
 };
 
-// Walks a list's tiles.  Behind the last one `left` is 0.
-template <int kTile>
+// Walks a list's tiles: where a tile lies and how many bytes of it there are, 0 behind the last one.  Between two stops -- the first tile of the
+// window, the last one, which may end early -- a step is an addition and a comparison.
+template <int D, int NKB>
 struct Cursor {
+  typedef Tiles<D, NKB> T;
   const uint16_t* from;
-  int left, t;
-  __device__ __forceinline__ void open(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
+  uint32_t valid;
+  int t, stop;
+  __device__ __forceinline__ void open(const TileList<T::kKeys>& list, const uint16_t* base, int64_t ss, int len) {
     t = list.begin;
     seek(list, base, ss, len);
   }
-  __device__ __forceinline__ void next(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
-    ++t;
-    if (__builtin_expect(t == list.n_sink || t >= list.end, 0)) {
-      seek(list, base, ss, len);
-    } else {
-      left -= kTile;
-      from += kTile * ss;
-    }
+  __device__ __forceinline__ void next(const TileList<T::kKeys>& list, const uint16_t* base, int64_t ss, int len) {
+    from += T::kKeys * ss;
+    if (__builtin_expect(++t == stop, 0)) seek(list, base, ss, len);
   }
-  __device__ __forceinline__ void seek(const TileList<kTile>& list, const uint16_t* base, int64_t ss, int len) {
+  __device__ __forceinline__ void seek(const TileList<T::kKeys>& list, const uint16_t* base, int64_t ss, int len) {
     const int key = t < list.end ? list.key(t) : 0;
     from = base + key * ss;
-    left = t < list.end ? len - key : 0;
+    valid = t < list.end ? Loader<D, NKB>::bytes(len - key, ss) : 0u;
+    stop = t >= list.end - 1 ? t + 1 : t < list.n_sink ? min(list.n_sink, list.end - 1) : list.end - 1;
   }
 };
 
@@ -519,16 +521,16 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   Loader<D, 2> ld;
   ld.open(a, it.b, it.hk, lane);
   constexpr int kPer = T::kBlocks / kWavesShared;
-  Cursor<T::kKeys> kc, vc;
+  Cursor<D, 2> kc, vc;
   kc.open(list, ld.k, ld.k_ss, len);
   vc.open(list, ld.v, ld.v_ss, len);
   auto pair_at = [&](int t) __attribute__((always_inline)) { return (t & (kPairs - 1)) * S::kPair; };
   auto load_k = [&](int pair) __attribute__((always_inline)) {
-    ld.template issue_k<kPer>(kc.from, kc.left, wave, kWavesShared, lds0 + pair_at(pair) + T::kBytes);
+    ld.template issue_k<kPer>(kc.from, kc.valid, wave, kWavesShared, lds0 + pair_at(pair) + T::kBytes);
     kc.next(list, ld.k, ld.k_ss, len);
   };
   auto load_pair = [&](int t) __attribute__((always_inline)) {
-    ld.template issue_v<kPer>(vc.from, vc.left, wave, kWavesShared, lds0 + pair_at(t));
+    ld.template issue_v<kPer>(vc.from, vc.valid, wave, kWavesShared, lds0 + pair_at(t));
     vc.next(list, ld.v, ld.v_ss, len);
     load_k(t);
   };
@@ -630,8 +632,10 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     int k0 = list.key(list.begin);
     // what the group's wavefronts have found in a tile's values, each in a quarter of them: in staging rows, which are free until the end
     int* flags = reinterpret_cast<int*>(lds + S::kStage + group * 4 * 32 * D);
-    auto probabilities = [&](int t, bool masked) __attribute__((always_inline)) {
-      if (__builtin_expect(st.needs(k0), 1)) {
+    // keys from which on, and up to which, a tile is seen whole by all rows of the workgroup
+    const uint32_t inside = (uint32_t)max(all_first.hi - (T::kKeys - 1) - all_last.lo, 0);
+    auto probabilities = [&](bool need, bool masked) __attribute__((always_inline)) {
+      if (__builtin_expect(need, 1)) {
         st.softmax(s, p, k0, masked, lane);
       } else {
         asm volatile("" ::: "memory");
@@ -643,14 +647,16 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     for (int t = 0; t < n - 1; ++t) {
       __builtin_amdgcn_s_setprio(D == 64 ? 0 : 1);
       load_pair(t + 2);
-      const bool masked = !st.whole(k0);
       const uint8_t* vt = lds + pair_at(t);
-      if (__builtin_expect(!((k0 + T::kKeys <= all_first.hi) & ((k0 >= all_last.lo) | (k0 + T::kKeys <= a.sinks))), 0)) {   // masked for some wavefront
+      bool masked = false, need = true;
+      if (__builtin_expect((uint32_t)(k0 - all_last.lo) >= inside, 0)) {
+        masked = !st.whole(k0);
+        need = st.needs(k0);
         constexpr int kShare = T::kBlocks / 4;
         const bool bad = st.template any_not_finite<kShare>(vt + (wave & 3) * kShare * 1024, lane);
         if (lane == 0) flags[wave & 3] = bad;
       }
-      probabilities(t, masked);
+      probabilities(need, masked);
       prefill(vt);
       if (group == 1) wait_all_but<S::kLoads>();
       end_softmax(p);
@@ -663,7 +669,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     }
     const bool masked = !st.whole(k0);
     const uint8_t* vt = lds + pair_at(n - 1);
-    probabilities(n - 1, masked);
+    probabilities(st.needs(k0), masked);
     end_softmax(p);
     if (masked) hurt |= st.any_not_finite(vt, lane);
     st.values(vt, p);
@@ -772,11 +778,11 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
   ld.open(a, it.b, it.hk, lane);
   auto load_k = [&](int t) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
     const int k0 = list.key(t);
-    ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, t < list.end ? len - k0 : 0, 0, 1, kt0);
+    ld.template issue_k<T::kBlocks>(ld.k + k0 * ld.k_ss, t < list.end ? ld.bytes(len - k0, ld.k_ss) : 0u, 0, 1, kt0);
   };
   auto load_v = [&](int t) __attribute__((always_inline)) {
     const int k0 = list.key(t);
-    ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, t < list.end ? len - k0 : 0, 0, 1, kt0 + T::kBytes);
+    ld.template issue_v<T::kBlocks>(ld.v + k0 * ld.v_ss, t < list.end ? ld.bytes(len - k0, ld.v_ss) : 0u, 0, 1, kt0 + T::kBytes);
   };
   int t = list.begin + wave;
   if (t < list.end) {
