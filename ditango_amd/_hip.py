@@ -458,11 +458,11 @@ def attn_window_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int
                     kv_lens: Optional[torch.Tensor] = None, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
                     lse: Optional[torch.Tensor] = None):
     """(out, lse) of ``dt_attn_window_fwd``; -1 stands for a border that is not there and for queries behind the keys."""
-    _here(q, "q")
+    stream = _stream_at(q, "q")
     workspace, counters = attn_scratch(q.device)
     if counters is None:
         counters = _stream_counters(q.device, 1)      # (none under capture)
-    return _host().attn_window(q, k, v, left, right, frame, sinks, q_begin, kv_lens, float(softmax_scale), out, lse, workspace, counters, _stream())
+    return _host().attn_window(q, k, v, left, right, frame, sinks, q_begin, kv_lens, float(softmax_scale), out, lse, workspace, counters, stream)
 
 
 def attn_sched_merge(q: torch.Tensor, table, dev_compute_ids: torch.Tensor, dev_count: torch.Tensor, max_jobs: int,
@@ -530,18 +530,19 @@ def zero_rows_from(t: torch.Tensor, first_row: torch.Tensor) -> None:
     _host().zero_rows_from(t, first_row, _stream())
 
 
-def _here(t: torch.Tensor, name: str) -> None:
-    """The launch goes to the current device's stream: the tensors have to live there."""
+def _stream_at(t: torch.Tensor, name: str) -> int:
+    """The current device's current stream, which the tensors have to live on."""
     _require(t.is_cuda, f"{name} must live on the GPU")
-    _require(t.get_device() == _current_device(), f"{name} lives on device {t.get_device()} but device {_current_device()} is current: make the "
-             "tensors' device current for this call")
+    device = _current_device()
+    if t.get_device() != device:
+        raise DitangoHipError(f"{name} lives on device {t.get_device()} but device {device} is current: make the tensors' device current for this call")
+    return _raw_stream(device)
 
 
-def merge_blocks(states, dst) -> None:
-    """Merge of states of any format into ``dst``; a state is ``(out, None, lse)`` of 16 or 32 bits or ``(elements, scales, lse)`` of 8.  One
-    state is copied."""
-    _here(dst[0], "the destination")
-    _host().merge_blocks(states, dst, _stream())
+def merge_blocks(states, dst, dst_dtype: torch.dtype = torch.float32, dst_lse_bsh: bool = False):
+    """Merge of states of any format into ``dst``, or a new state of ``dst_dtype`` (8-bit where that is ``torch.float8_e4m3fn`` or ``torch.int8``); a
+    state is ``(out, None, lse)`` of 16 or 32 bits or ``(elements, scales, lse)`` of 8.  One state is copied.  Returns the destination."""
+    return _host().merge_blocks(states, dst, dst_dtype, dst_lse_bsh, _stream_at(states[0][0], "states[0]"))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -614,7 +615,6 @@ def rotary_table(turns: Sequence[int], axis_of_pair: Sequence[int], rope: int, s
     return _host().RotaryTable(turns, axis_of_pair, rope, sections)
 
 
-def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: float, rounding: int = 0):
+def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: float):
     """q and k in one launch of ``dt_qk_norm_rope_axes``; ``tensors``: one or two of ``(x, weight, bias, out, out_scale)``."""
-    _here(tensors[0][0], "q")
-    return _host().qk_norm_rope_axes(tensors, positions, table, norm, float(eps), rounding, _stream())
+    return _host().qk_norm_rope_axes(tensors, positions, table, norm, eps, _stream_at(tensors[0][0], "q"))

@@ -74,13 +74,13 @@ def merge_any(states, *, dst=None, dst_dtype: torch.dtype = torch.float32, dst_l
     a ``BlockState`` or ``(out, lse)``, one of the states among them -- or a new ``(out, lse)`` of ``dst_dtype``.  Returns the destination."""
     if not states:
         raise ValueError("need at least one state")
-    first = _parts(states[0])[0]
-    if dst is None:
-        B, S, H, D = first.shape
-        dst = (torch.empty((B, S, H, D), dtype=dst_dtype, device=first.device),
-               torch.empty((B, S, H, 1) if dst_lse_bsh else (B, H, S), dtype=torch.float32, device=first.device))
-    _hip.merge_blocks([_parts(s) for s in states], _parts(dst))
-    return dst
+    out, _, lse = _hip.merge_blocks([_parts(s) for s in states], None if dst is None else _parts(dst), dst_dtype, dst_lse_bsh)
+    return (out, lse) if dst is None else dst
+
+
+def quantized(out: torch.Tensor, lse: torch.Tensor, state_format: str) -> BlockState:
+    """The state ``(out, lse)`` of any format in 8 bits."""
+    return BlockState(*_hip.merge_blocks([(out, None, lse)], None, STATE_FORMATS[state_format]))
 
 
 def merge_cached(outs, lses, dst_dtype: torch.dtype):
@@ -238,13 +238,12 @@ class proCache:
         attention kernel writes for a model that runs in that dtype) is adopted as is; anything
         else goes through one ``dt_cache_store`` pass into fresh cache-form (bf16) tensors.  Under a ``state_format`` it is
         quantised in one pass, whatever it comes in."""
-        B, S, H, D = out.shape
         if self.state_format is not None:
-            state = BlockState.empty((B, S, H, D), self.state_format, out.device)
-            merge_any([(out.contiguous(), lse)], dst=state)
+            state = quantized(out.contiguous(), lse, self.state_format)
             self.out_block_cache[block_id] = state
             self.lse_block_cache[block_id] = state.lse
             return
+        B, S, H, D = out.shape
         in_cache_form = (out.dtype in _hip.HALF_DTYPES and out.is_contiguous() and lse.dtype == torch.float32
                          and tuple(lse.shape) == (B, H, S) and lse.is_contiguous())
         if not in_cache_form:

@@ -882,21 +882,27 @@ dt_state any_state(const AnyState& s, const Dims& d, const Tensor& like, const N
   return {ptr(s.out), s.scales ? static_cast<uint8_t*>(ptr(*s.scales)) : nullptr, static_cast<float*>(ptr(s.lse)), dtype, lse_layout(s.lse, d.B, d.S, d.H)};
 }
 
-// Merge of states of any format into `dst`; more than one launch folds run in rounds through a running fp32 state.
-void merge_blocks(const std::vector<std::tuple<Tensor, std::optional<Tensor>, Tensor>>& states, const std::tuple<Tensor, std::optional<Tensor>, Tensor>& into,
-                  uint64_t stream) {
+// Merge of states of any format into `into`; more than one launch folds run in rounds through a running fp32 state.  Without `into`, a new state: of
+// `dst_dtype`, or 8-bit where that is float8_e4m3fn or int8.
+using StateParts = std::tuple<Tensor, std::optional<Tensor>, Tensor>;
+StateParts merge_blocks(const std::vector<StateParts>& states, std::optional<StateParts> into, at::ScalarType dst_dtype, bool dst_bsh, uint64_t stream) {
   REQUIRE(!states.empty(), "need at least one state");
   const Tensor& first = std::get<0>(states[0]);
   REQUIRE(first.is_cuda() && first.dim() == 4, "states must be [B,Sq,H,D] on the GPU");
   const Dims d{first.size(0), first.size(1), first.size(2), first.size(3)};
-  auto state = [&](const std::tuple<Tensor, std::optional<Tensor>, Tensor>& t, const Name& name) {
+  auto state = [&](const StateParts& t, const Name& name) {
     return any_state({std::get<0>(t), std::get<2>(t), std::get<1>(t)}, d, first, name);
   };
-  const dt_state dst = state(into, {"destination"});
+  if (!into) {
+    std::optional<Tensor> scales;
+    if (dst_dtype == at::kFloat8_e4m3fn || dst_dtype == at::kChar) scales = empty({d.B, d.S, d.H, d.D / 32}, first.options().dtype(at::kByte));
+    into = StateParts{new_out(d, dst_dtype, first), scales, new_lse(d, dst_bsh, first)};
+  }
+  const dt_state dst = state(*into, {"destination"});
   std::vector<dt_state> list;
   Tensor run_out, run_lse;
   for (size_t i = 0; i < states.size(); ++i) list.push_back(state(states[i], {"states", (int64_t)i}));
-  if (first.numel() == 0) return;
+  if (first.numel() == 0) return *into;
   size_t at = 0;
   while (list.size() - at > DT_MAX_MERGE) {
     const bool again = run_out.defined();
@@ -910,6 +916,7 @@ void merge_blocks(const std::vector<std::tuple<Tensor, std::optional<Tensor>, Te
     list[at] = run;
   }
   CALL(dt_merge_block_states, (int32_t)(list.size() - at), list.data() + at, &dst, d.B, d.S, d.H, d.D, stream_of(stream));
+  return *into;
 }
 
 // How a row's pairs turn: built once for a RotaryAxes object.
@@ -923,26 +930,36 @@ struct RotaryTable {
 // ditango_amd._hip.qk_norm_rope_axes.  A tensor: (x, weight, bias, out, scale).
 using RotaryRows = std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>, double>;
 std::vector<Tensor> qk_norm_rope_axes(const std::vector<RotaryRows>& tensors, const Tensor& positions, const RotaryTable& table, int32_t norm, double eps,
-                                      int32_t rounding, uint64_t stream) {
+                                      uint64_t stream) {
   REQUIRE(tensors.size() == 1 || tensors.size() == 2, "one or two tensors are needed");
   const Tensor& first = std::get<0>(tensors[0]);
   const Dims d = check_bshd(first, {"q"});
   dt_rotary_rows rows[2] = {};
-  std::vector<Tensor> outs;
-  const bool narrow = rounding & DT_WEIGHTS_16;
+  std::vector<Tensor> outs, kept;
+  // norm parameters in the tensors' own type are widened by the kernel as it reads them; others become fp32 here
+  bool narrow = true;
+  for (const auto& t : tensors)
+    for (const auto* p : {&std::get<1>(t), &std::get<2>(t)})
+      if (*p) {
+        REQUIRE((*p)->numel() == d.D && at::isFloatingType((*p)->scalar_type()), "norm parameters must be floating-point [D]");
+        narrow = narrow && (*p)->scalar_type() == first.scalar_type() && same_device(**p, first) && (*p)->is_contiguous() &&
+                 reinterpret_cast<uintptr_t>(ptr(**p)) % 16 == 0;
+      }
+  auto parameter = [&](const std::optional<Tensor>& p) -> const void* {
+    if (!p || narrow) return ptr(p);
+    kept.push_back(p->detach().to(first.options().dtype(at::kFloat)).contiguous());
+    return ptr(kept.back());
+  };
   for (size_t i = 0; i < tensors.size(); ++i) {
     const auto& [x, weight, bias, given, scale] = tensors[i];
     const Dims dx = check_bshd(x, {i ? "k" : "q"});
     REQUIRE(dx.B == d.B && dx.S == d.S && dx.D == d.D && x.scalar_type() == first.scalar_type() && same_device(x, first),
             "q and k must have one dtype, device, batch, length and head dim");
-    for (const auto* t : {&weight, &bias})
-      REQUIRE(!*t || (same_device(**t, first) && (*t)->scalar_type() == (narrow ? x.scalar_type() : at::kFloat) && (*t)->is_contiguous() && (*t)->numel() == d.D),
-              "norm parameters must be ", narrow ? "of the tensors' dtype" : "fp32", ", [D] on the GPU");
     outs.push_back(given ? *given : new_out(dx, x.scalar_type(), x));
     const Tensor& y = outs.back();
     REQUIRE(same_device(y, first) && y.scalar_type() == x.scalar_type() && y.is_contiguous() && shape_is(y, {dx.B, dx.S, dx.H, dx.D}),
             "out must be a contiguous [B,S,H,D] in the dtype of its input");
-    rows[i] = {ptr(x), dx.B > 1 ? x.stride(0) : 0, dx.S > 1 ? x.stride(1) : 0, dx.H > 1 ? x.stride(2) : 0, ptr(y), ptr(weight), ptr(bias),
+    rows[i] = {ptr(x), dx.B > 1 ? x.stride(0) : 0, dx.S > 1 ? x.stride(1) : 0, dx.H > 1 ? x.stride(2) : 0, ptr(y), parameter(weight), parameter(bias),
                (int32_t)dx.H, (float)scale};
   }
   const int64_t n_axes = positions.size(-1);
@@ -952,7 +969,7 @@ std::vector<Tensor> qk_norm_rope_axes(const std::vector<RotaryRows>& tensors, co
   REQUIRE((int64_t)table.turns.size() == d.D / 2 && table.axis.size() == table.turns.size(), "the axes do not cover the head dim ", std::to_string(d.D));
   REQUIRE(d.S < (1ll << 31) && d.B < (1ll << 31), "too many tokens");
   if (first.numel() == 0) return outs;
-  if (first.scalar_type() == at::kHalf) rounding |= DT_IO_FP16;
+  const int32_t rounding = (first.scalar_type() == at::kHalf ? DT_IO_FP16 : 0) | (narrow ? DT_WEIGHTS_16 : 0);
   CALL(dt_qk_norm_rope_axes, rows, (int32_t)tensors.size(), (int32_t)d.B, (int32_t)d.S, (int32_t)d.D, norm, (float)eps,
        static_cast<const int32_t*>(ptr(positions)), positions.dim() == 3 ? positions.stride(0) : 0, (int32_t)n_axes, table.turns.data(),
        table.axis.data(), table.rope, table.sections.data(), (int32_t)table.sections.size(), rounding, stream_of(stream));

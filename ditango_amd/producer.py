@@ -161,17 +161,11 @@ def prepare_qk_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch
         raise ValueError(f"positions must be int32, got {positions.dtype}")
     if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes.dims):
         raise ValueError(f"positions must be [S, {len(axes.dims)}] or [B, S, {len(axes.dims)}] for these axes, got {tuple(positions.shape)}")
-    given = (None, None) if out is None else out
-    tensors = [(q, q_weight, q_bias, given[0])] + ([] if k is None else [(k, k_weight, k_bias, given[1])])
-    params = [t for _, w, b, _ in tensors for t in (w, b)]
-    rounding = 0
-    if any(t is not None for t in params) and _read_in_place(q, None, None) and all(_read_in_place(q, t, None) for t in params):
-        rounding = _hip.DT_WEIGHTS_16
-    else:
-        tensors = [(x, _f32(w, x.device), _f32(b, x.device), y) for x, w, b, y in tensors]
-    scale = 1.0 if fold_softmax_scale is None else folded_scale(q.shape[-1], fold_softmax_scale)
-    done = _hip.qk_norm_rope_axes([(*t, scale if i == 0 else 1.0) for i, t in enumerate(tensors)],
-                                  positions if positions.is_contiguous() else positions.contiguous(), axes.table, _NORMS[norm], eps, rounding)
+    q_out, k_out = (None, None) if out is None else out
+    tensors = [(q, q_weight, q_bias, q_out, 1.0 if fold_softmax_scale is None else folded_scale(q.shape[-1], fold_softmax_scale))]
+    if k is not None:
+        tensors.append((k, k_weight, k_bias, k_out, 1.0))
+    done = _hip.qk_norm_rope_axes(tensors, positions if positions.is_contiguous() else positions.contiguous(), axes.table, _NORMS[norm], eps)
     return done[0], (done[1] if k is not None else None)
 
 
