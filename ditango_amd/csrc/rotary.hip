@@ -3,12 +3,11 @@
 //
 // A pair (a, b) of a head row at position n on its axis turns by t = n f / 2 pi full turns.  f / 2 pi comes as a 64-bit fraction F of a
 // turn, so n F mod 2^64 is the angle of any 32-bit position to 2^-32 of a turn: integers have no range reduction to lose bits in.  Its upper half, as
-// a signed fraction, splits into the nearest quarter turn and x = 2 pi r, |x| <= pi / 4, and
-//   sin x = x - x^3/3! + x^5/5! - x^7/7! + x^9/9!       (next term 1.8e-9)
-//   cos x = 1 - x^2/2! + x^4/4! - x^6/6! + x^8/8! - x^10/10!  (next term 1.2e-10).
+// a signed fraction of a turn in fp32, is what the sine and cosine instructions take; they are off by 1.9e-7 at most, the fraction's rounding
+// included (4 million fractions all round the turn), where the row's 16 bits are off by 2^-9 to 2^-12 of a value.
 //
-// HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row, so that an angle is computed once
-// for the kHeads heads of a lane group: 8 neighbours with interleaved pairs, two runs of 4 half a section apart with rotate-half.
+// HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
+// runs of 4 half a section apart with rotate-half.  It has their angles once for the kHeads heads of its lane group.
 #include "producer_math.h"
 
 namespace dt {
@@ -41,25 +40,6 @@ struct RotaryArgs {
   uint8_t axis[64];               // of pair 4 lane + i
   uint64_t turns[64];
 };
-
-// sin and cos of (t / 2^32) turns.
-__device__ __forceinline__ void sin_cos(uint32_t t, float& sn, float& cs) {
-  const uint32_t q = (t + 0x20000000u) >> 30;
-  const float x = (float)(int32_t)(t - (q << 30)) * 1.46291807926715968e-9f;   // 2 pi / 2^32
-  const float z = x * x;
-  float s = __builtin_fmaf(z, 2.7557319224e-6f, -1.9841269841e-4f);
-  s = __builtin_fmaf(z, s, 8.3333333333e-3f);
-  s = __builtin_fmaf(z, s, -1.6666666667e-1f);
-  s = __builtin_fmaf(z * x, s, x);
-  float c = __builtin_fmaf(z, -2.7557319224e-7f, 2.4801587302e-5f);
-  c = __builtin_fmaf(z, c, -1.3888888889e-3f);
-  c = __builtin_fmaf(z, c, 4.1666666667e-2f);
-  c = __builtin_fmaf(z, c, -0.5f);
-  c = __builtin_fmaf(z, c, 1.f);
-  const float u = q & 1 ? c : s, v = q & 1 ? s : c;      // quarter turns: (s, c) -> (c, -s) -> (-s, -c) -> (-c, s)
-  sn = q & 2 ? -u : u;
-  cs = (q + 1) & 2 ? -v : v;
-}
 
 template <bool kHalf>
 __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d, float* v) {
@@ -116,7 +96,10 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
       const int32_t n = pos[a.axis[4 * c + i]];
       const uint64_t f = a.turns[4 * c + i];
       const uint32_t lo = (uint32_t)f, hi = (uint32_t)(f >> 32);
-      sin_cos(__umulhi((uint32_t)n, lo) + (uint32_t)n * hi - (n < 0 ? lo : 0u), sn[i], cs[i]);
+      const uint32_t t32 = __umulhi((uint32_t)n, lo) + (uint32_t)n * hi - (n < 0 ? lo : 0u);
+      const float turn = (float)(int32_t)t32 * 2.3283064365386963e-10f;     // 2^-32
+      sn[i] = __builtin_amdgcn_sinf(turn);
+      cs[i] = __builtin_amdgcn_cosf(turn);
     }
   }
   float w[8], bias[8];
