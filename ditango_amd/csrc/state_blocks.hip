@@ -27,7 +27,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;
 constexpr int kBlock = 32;   // elements of a scale
 
 struct BlockArgs {
@@ -44,6 +43,11 @@ struct BlockArgs {
   RowIndex at;
 };
 
+// The arguments where they arrive, in the kernarg segment: indexed in unrolled batches of a by-value parameter, the optimiser makes a private copy
+// of the tables for every lane (8 states a batch: 122 -> 1950 us).
+typedef const BlockArgs __attribute__((address_space(4))) KernArgs;
+__device__ __forceinline__ KernArgs& kernel_args() { return *(KernArgs*)__builtin_amdgcn_kernarg_segment_ptr(); }
+
 __device__ __forceinline__ float scale_of(uint32_t byte) {   // 2^(byte - 127); byte 0 is below the normal numbers, 255 infinite
   return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
@@ -55,7 +59,7 @@ template <> struct Raw<2> { u32x4 x; };
 template <> struct Raw<4> { u32x4 x, y; };
 
 template <int kBytes>
-__device__ __forceinline__ void load(const BlockArgs& a, int i, int64_t elem, Raw<kBytes>& r) {
+__device__ __forceinline__ void load(KernArgs& a, int i, int64_t elem, Raw<kBytes>& r) {
   const uint8_t* p = static_cast<const uint8_t*>(a.out[i]) + elem * kBytes;
   if constexpr (kBytes == 1) {
     r.x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
@@ -66,19 +70,21 @@ __device__ __forceinline__ void load(const BlockArgs& a, int i, int64_t elem, Ra
   }
 }
 
-// acc += w x
+// acc += w x; a weight of 0 leaves x out, whatever it is
 template <int kBytes>
 __device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, float (&acc)[8]) {
+  const bool there = w != 0.f;
   float x[8];
   if constexpr (kBytes == 1) {
-    w *= scale_of(r.scale);       // (0 times the infinite scale would not leave a state without weight out)
+    w = there ? w * scale_of(r.scale) : 0.f;       // (the scale may be infinite)
+    const uint32_t word[2] = {r.x.x, r.x.y};
     if (kind) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)(r.x[e / 4] << (24 - 8 * (e % 4))) >> 24);
+      for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)(word[e / 4] << (24 - 8 * (e % 4))) >> 24);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.x[e / 4], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.x[e / 4], true);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[e / 4], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[e / 4], true);
         x[e] = lo.x;
         x[e + 1] = lo.y;
         x[e + 2] = hi.x;
@@ -88,7 +94,7 @@ __device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, fl
   } else if constexpr (kBytes == 2) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t word = r.x[e];   // (a bit cast of the vector's element itself reads its first one)
+      const uint32_t word = there ? r.x[e] : 0u;   // (a bit cast of the vector's element itself reads its first one)
       if (kind) {
         const f32x2 f = __builtin_convertvector(__builtin_bit_cast(f16x2, word), f32x2);
         x[2 * e] = f.x;
@@ -101,8 +107,8 @@ __device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, fl
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[e] = __uint_as_float(r.x[e]);
-      x[4 + e] = __uint_as_float(r.y[e]);
+      x[e] = there ? __uint_as_float(r.x[e]) : 0.f;
+      x[4 + e] = there ? __uint_as_float(r.y[e]) : 0.f;
     }
   }
 #pragma unroll
@@ -113,47 +119,47 @@ struct Sums {
   float acc[8], m, den;
 };
 
+// NB states' loads are in flight together, and nothing between them and the folding branches: behind a branch on the lse the compiler would issue
+// the other loads after the lse's have come.
 template <int kBytes, int NB>
-__device__ __forceinline__ void batch(const BlockArgs& a, int i0, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+__device__ __forceinline__ void batch(int i0, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+  KernArgs& a = kernel_args();
   Raw<kBytes> r[NB];
   float l[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    load<kBytes>(a, i0 + j, elem, r[j]);
     l[j] = a.lse[i0 + j][(a.bsh_mask >> (i0 + j)) & 1 ? row : bhs];
+    load<kBytes>(a, i0 + j, elem, r[j]);
   }
+  __builtin_amdgcn_sched_barrier(0);
+  const uint32_t kinds = (uint32_t)(a.kind_mask >> i0);
   float m = s.m;
 #pragma unroll
   for (int j = 0; j < NB; ++j) m = fmaxf(m, l[j]);
-  if (!(m > -INFINITY)) {          // no state with a key so far
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-      if (l[j] != l[j]) s.den = l[j];   // (an undefined one stays in the result)
-    return;
-  }
-  const float rescale = __expf(s.m - m);
+  const float top = m > -INFINITY ? m : 0.f;       // (no state with a key so far: all weights are 0; an undefined lse stays one)
+  const float rescale = __expf(s.m - top);
   s.den *= rescale;
 #pragma unroll
   for (int e = 0; e < 8; ++e) s.acc[e] *= rescale;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const float w = __expf(l[j] - m);
+    const float w = __expf(l[j] - top);
     s.den += w;
-    if (w != 0.f) add<kBytes>(r[j], (a.kind_mask >> (i0 + j)) & 1, w, s.acc);   // without weight, whatever it holds
+    add<kBytes>(r[j], (kinds >> j) & 1, w, s.acc);
   }
   s.m = m;
 }
 template <int kBytes, int NB>
-__device__ __forceinline__ void rest(const BlockArgs& a, int i0, int n, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+__device__ __forceinline__ void rest(int i0, int n, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
   if constexpr (NB >= 1) {
-    if (n == NB) batch<kBytes, NB>(a, i0, elem, row, bhs, s);
-    else rest<kBytes, NB - 1>(a, i0, n, elem, row, bhs, s);
+    if (n == NB) batch<kBytes, NB>(i0, elem, row, bhs, s);
+    else rest<kBytes, NB - 1>(i0, n, elem, row, bhs, s);
   }
 }
-template <int kBytes>
-__device__ __forceinline__ void states(const BlockArgs& a, int i0, int i1, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
-  for (; i0 + kBatch <= i1; i0 += kBatch) batch<kBytes, kBatch>(a, i0, elem, row, bhs, s);
-  rest<kBytes, kBatch - 1>(a, i0, i1 - i0, elem, row, bhs, s);
+template <int kBytes, int kBatch>
+__device__ __forceinline__ void states(int i0, int i1, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+  for (; i0 + kBatch <= i1; i0 += kBatch) batch<kBytes, kBatch>(i0, elem, row, bhs, s);
+  rest<kBytes, kBatch - 1>(i0, i1 - i0, elem, row, bhs, s);
 }
 
 // The other lanes of a quad: lane ^ 1, lane ^ 2.
@@ -162,18 +168,30 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kCtrl, 0xf, 0xf, true);
 }
 
-// 8 elements in the destination's format.  (Lanes of a quad are all here: a row has 8 or 16.)
-__device__ __forceinline__ void store(const BlockArgs& a, int64_t elem, const float (&x)[8]) {
+// 8 elements in the destination's format; all lanes of a wavefront, `live` those whose row is there (a quad's are, or are not, together).
+__device__ __forceinline__ void store(KernArgs& a, int64_t elem, bool live, int64_t elems, const float (&x)[8]) {
   uint8_t* p = static_cast<uint8_t*>(a.dst);
   if (a.dst_dtype == DT_FP32) {
+    // A lane's 32 bytes as two stores would each write every other 16 bytes of a line (9 % more bytes written): through the LDS, whole kilobytes.
+    __shared__ f32x4 stage[kThreads / 64][128];
     f32x4 lo, hi;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       lo[e] = x[e];
       hi[e] = x[4 + e];
     }
-    __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(p + elem * 4));
-    __builtin_nontemporal_store(hi, reinterpret_cast<f32x4*>(p + elem * 4) + 1);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    stage[wave][2 * lane] = lo;
+    stage[wave][2 * lane + 1] = hi;
+    __builtin_amdgcn_wave_barrier();
+    const int64_t first = elem - 8 * lane;       // of the wavefront
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x4 y = stage[wave][64 * i + lane];
+      if (first + 256 * i + 4 * lane < elems) __builtin_nontemporal_store(y, reinterpret_cast<f32x4*>(p + (first + 256 * i + 4 * lane) * 4));
+    }
+  } else if (!live) {
+    return;
   } else if (a.dst_dtype == DT_BF16 || a.dst_dtype == DT_FP16) {
     u32x4 w;
 #pragma unroll
@@ -220,43 +238,71 @@ __device__ __forceinline__ void store(const BlockArgs& a, int64_t elem, const fl
   }
 }
 
+// The first element of this lane.  The lse of consecutive queries share a line of the [B,H,Sq] layout, and workgroups go to the 8 XCDs in turn: so
+// that a line is read into one L2 only, kGroup workgroups that follow each other in memory are of one XCD.
+constexpr int kGroup = 64;
+__device__ __forceinline__ int64_t first_elem() {
+  uint32_t wg = blockIdx.x;
+  constexpr uint32_t kSpan = 8 * kGroup;
+  if ((wg / kSpan + 1) * kSpan <= gridDim.x) wg = wg / kSpan * kSpan + (wg & 7u) * kGroup + (wg % kSpan >> 3);
+  return ((int64_t)wg * kThreads + threadIdx.x) * 8;
+}
+
+__device__ __forceinline__ RowIndex rows_of(KernArgs& a) {
+  RowIndex at;
+  at.Sq = a.at.Sq;
+  at.H = a.at.H;
+  at.rows = a.at.rows;
+  at.by_h = {a.at.by_h.mul, a.at.by_h.shift};
+  at.by_s = {a.at.by_s.mul, a.at.by_s.shift};
+  return at;
+}
+
 template <int D>
-__global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs a) {
-  const int64_t elem = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8, row64 = elem / D;
-  if (row64 >= a.at.rows) return;
-  const uint32_t row = (uint32_t)row64, bhs = bhs_of(a.at, row);
+__global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs args_by_value) {
+  (void)args_by_value;
+  KernArgs& a = kernel_args();
+  const RowIndex at = rows_of(a);
+  const int64_t elems = (int64_t)at.rows * D, elem = first_elem();
+  const bool live = elem < elems;
+  const int64_t from = live ? elem : 0;          // (lanes behind the last row read the first one's and store nothing)
+  const uint32_t row = (uint32_t)(from / D), bhs = bhs_of(at, row);
   Sums s;
 #pragma unroll
   for (int e = 0; e < 8; ++e) s.acc[e] = 0.f;
   s.m = -INFINITY;
   s.den = 0.f;
-  states<1>(a, 0, a.n8, elem, row, bhs, s);
-  states<2>(a, a.n8, a.n16, elem, row, bhs, s);
-  states<4>(a, a.n16, a.n, elem, row, bhs, s);
+  states<1, 4>(0, a.n8, from, row, bhs, s);
+  states<2, 4>(a.n8, a.n16, from, row, bhs, s);
+  states<4, 2>(a.n16, a.n, from, row, bhs, s);
   const float inv = s.den != 0.f ? 1.f / s.den : 0.f;
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = s.acc[e] * inv;
-  store(a, elem, x);
-  if (a.dst_lse != nullptr && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
+  store(a, elem, live, elems, x);
+  if (live && a.dst_lse != nullptr && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
 }
 
 // One state into another format, its lse bit for bit.
 template <int D, int kBytes>
-__global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a) {
-  const int64_t elem = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 8, row64 = elem / D;
-  if (row64 >= a.at.rows) return;
+__global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs args_by_value) {
+  (void)args_by_value;
+  KernArgs& a = kernel_args();
+  const RowIndex at = rows_of(a);
+  const int64_t elems = (int64_t)at.rows * D, elem = first_elem();
+  const bool live = elem < elems;
+  const int64_t from = live ? elem : 0;
   Raw<kBytes> r;
-  load<kBytes>(a, 0, elem, r);
-  const bool with_lse = a.dst_lse != nullptr && elem % D == 0;
-  const uint32_t row = (uint32_t)row64, bhs = bhs_of(a.at, row);
+  load<kBytes>(a, 0, from, r);
+  const bool with_lse = live && a.dst_lse != nullptr && elem % D == 0;
+  const uint32_t row = (uint32_t)(from / D), bhs = bhs_of(at, row);
   float l = 0.f;
   if (with_lse) l = a.lse[0][a.bsh_mask & 1 ? row : bhs];
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = -0.f;       // (-0 + -0 keeps its sign)
   add<kBytes>(r, a.kind_mask & 1, 1.f, x);
-  store(a, elem, x);
+  store(a, elem, live, elems, x);
   if (with_lse) a.dst_lse[a.dst_bsh ? row : bhs] = l;
 }
 
