@@ -46,6 +46,27 @@ def test_store_and_load(hip, fmt, D, dtype, bsh):
             assert torch.equal(o.cpu().double(), L.value(state.elements.cpu(), state.scales.cpu().int() - 127))
 
 
+@pytest.mark.parametrize("D, S", [(128, 2741), (64, 5481)])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_large_state_is_its_pieces(hip, fmt, D, S):
+    """More rows than a launch of the small form: the same bits as piece by piece, and back, in every type."""
+    from ditango_amd.core.cache import BlockState, merge_any, quantized
+    g = torch.Generator().manual_seed(S)
+    for dtype in (torch.float32, torch.bfloat16):
+        out, lse = _state(g, 1, S, 12, D, dtype)
+        state = quantized(out, lse, fmt)
+        assert torch.equal(state.lse, lse)
+        for a in range(0, S, 700):
+            piece = quantized(out[:, a:a + 700].contiguous(), lse[:, :, a:a + 700].contiguous(), fmt)
+            assert torch.equal(piece.elements.view(torch.uint8), state.elements[:, a:a + 700].contiguous().view(torch.uint8))
+            assert torch.equal(piece.scales, state.scales[:, a:a + 700])
+        for dst in (torch.float32, torch.bfloat16):
+            back, l = merge_any([state], dst_dtype=dst, dst_lse_bsh=True)
+            assert torch.equal(l.squeeze(-1).transpose(1, 2), lse)
+            want = state.elements.float().unflatten(-1, (-1, 32)) * torch.exp2(state.scales.float() - 127).unsqueeze(-1)
+            assert torch.equal(back.float(), want.flatten(-2))
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_rows_at_the_ends_of_the_range(hip, fmt):
     from ditango_amd.core.cache import BlockState, merge_any
