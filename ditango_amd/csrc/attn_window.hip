@@ -43,7 +43,7 @@ struct WindowArgs {
   const int32_t* kv_lens;       // device [B], or null: Sk
   float scale_log2;
   int32_t rows, row_tiles, items, per_xcd;
-  Quotient by_group, by_frame;
+  Quotient by_group, by_frame, by_tiles, by_heads, by_ways;
   // An XCD's items from tail_start on, tail of them, are cut along the keys into `ways` workgroups each
   int32_t tail_start, tail, ways;
   float* part_out;              // [part][row of a tile][D] sums, and [part][row] (maximum in powers of two, sum)
@@ -381,9 +381,9 @@ struct Item {
 __device__ __forceinline__ bool item_at(const WindowArgs& a, int xcd, int idx, int rows, Item& it) {
   const int item = xcd * a.per_xcd + idx;      // an XCD works through neighbouring items, which share keys in its L2
   if (idx >= a.per_xcd || item >= a.items) return false;
-  const int unit = item / a.row_tiles;
+  const int unit = (int)quotient(item, a.by_tiles);
   it.row0 = (a.row_tiles - 1 - (item - unit * a.row_tiles)) * rows;
-  it.b = unit / a.Hk;
+  it.b = (int)quotient(unit, a.by_heads);
   it.hk = unit - it.b * a.Hk;
   return true;
 }
@@ -395,8 +395,9 @@ __device__ __forceinline__ bool item_of(const WindowArgs& a, int rows, Item& it)
   it.slot = 0;
   if (idx >= a.tail_start) {
     const int k = idx - a.tail_start;
-    idx = a.tail_start + k / a.ways;
-    it.part = k % a.ways;
+    const int whole = (int)quotient(k, a.by_ways);
+    idx = a.tail_start + whole;
+    it.part = k - whole * a.ways;
     it.ways = a.ways;
     it.slot = xcd * a.tail * a.ways + k;
   }
@@ -675,6 +676,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     st.values(vt, p);
     // group 1's last products are the last thing that happens in the buffers
     if (group == 0) wait_lds_barrier();
+    wait_loads();     // those past the last tile, which store zeros: before the LDS is another workgroup's (and not behind the result's stores)
   }
   // Rows of the result through the LDS, so that a store covers whole lines: half of the columns at a time.
   const int col = lane & 31, hh = lane >> 5;
@@ -700,7 +702,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       a.part_ml[at * 2] = st.m_ref * st.c;
       a.part_ml[at * 2 + 1] = l;
     }
-    wait_loads();
     return;
   }
   if (hh == 0 && row0 + col < a.rows) {
@@ -710,7 +711,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   }
   if (__builtin_expect(hurt, 0)) {
     rows_one_by_one<D, kHalf>(a, it, len, row0, st.m_ref * st.c, inv, 0, len, lane);
-    wait_loads();
     return;
   }
   uint8_t* stage = lds + S::kStage + wave * 32 * D;
@@ -737,7 +737,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       }
     }
   }
-  wait_loads();     // (loads past the last tile store zeros: before the LDS is another workgroup's)
 }
 
 // Few rows, W wavefronts.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is on its
@@ -1068,6 +1067,9 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
   a.items = (int32_t)items;
   a.per_xcd = (a.items + kXcds - 1) / kXcds;
   a.ways = plan.ways;
+  a.by_ways = quotient_by(a.ways);
+  a.by_tiles = quotient_by(a.row_tiles);
+  a.by_heads = quotient_by(a.Hk);
   a.tail = (int32_t)plan.tail;
   a.tail_start = a.per_xcd - a.tail;
   if (a.ways > 1) {
