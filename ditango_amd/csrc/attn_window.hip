@@ -30,6 +30,7 @@ constexpr int kXcds = 8;
 // A tile's sum of a lane's probabilities above which the tile is redone with its exact maximum: below it no probability exceeds 2^12,
 // which the 16-bit operand and the fp32 sums hold as well as one below 1.
 constexpr float kSumLimit = 4096.0f;
+constexpr int64_t kMostItems = (1 << 23) - (1 << 17);      // a grid holds fewer than 2^32 lanes, 512 a workgroup; 2^17 workgroups for parts
 constexpr int32_t kMostTokens = 1 << 29;   // positions, spans and lengths: their sums stay in 32 bits
 
 struct WindowArgs {
@@ -407,6 +408,10 @@ __device__ __forceinline__ bool item_of(const WindowArgs& a, int rows, Item& it)
 }
 
 typedef __attribute__((address_space(3))) uint8_t* lds_ptr_t;
+
+// The weight of a state with maximum m and sum l beside others of which the largest maximum is `top`.  Without a maximum there was no key and the
+// sum is 0, or only undefined scores, and the sum is undefined: it is then the weight.
+__device__ __forceinline__ float weight_of(float m, float l, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : l; }
 
 // Phases of the shared tiles.  Group g (0 or 1) does the softmax of tile t in phase 2t + g and its products -- O^T += V^T P^T of tile t, then
 // S^T = K Q^T of tile t + 1 -- in phase 2t + g + 1; a barrier ends every phase.  V of tile t and K of tile t + 1, read together, are pair t:
@@ -832,8 +837,9 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
   l = 0.f;
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    w[i] = m[i] > -INFINITY ? __builtin_amdgcn_exp2f(m[i] - top) : 0.f;    // a state without a key
-    if (m[i] > -INFINITY) l = __builtin_fmaf(w[i], ml[i * 64 + 32 + col], l);
+    const float li = ml[i * 64 + 32 + col];
+    w[i] = weight_of(m[i], li, top);
+    l = __builtin_fmaf(w[i], li, l);
   }
   const int row = it.row0 + col;
   const bool live = row < a.rows;
@@ -852,7 +858,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D, W>::kTile) + lane * 4 + q * 256);
-      if (m[j] > -INFINITY)
+      if (w[j] != 0.f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);
     }
@@ -918,8 +924,8 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
     }
 #pragma unroll
     for (int p = 0; p < kSome; ++p) {
-      if (p0 + p >= it.ways || !(pm[p] > -INFINITY)) continue;       // (a part without a key has stored nothing of use)
-      const float wp = __builtin_amdgcn_exp2f(pm[p] - top);
+      if (p0 + p >= it.ways) continue;
+      const float wp = weight_of(pm[p], pl[p], top);
       l = __builtin_fmaf(wp, pl[p], l);
 #pragma unroll
       for (int i = 0; i < kCols; ++i)
@@ -958,10 +964,8 @@ __global__ __launch_bounds__(256) void attn_window_fold_kernel(const WindowArgs 
   f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int p = 0; p < a.ways; ++p) {
     const int64_t i = first + tile_rows * p;
-    const float m = a.part_ml[i * 2];
-    if (!(m > -INFINITY)) continue;
-    const float w = __builtin_amdgcn_exp2f(m - top);
-    l = __builtin_fmaf(w, a.part_ml[i * 2 + 1], l);
+    const float li = a.part_ml[i * 2 + 1], w = weight_of(a.part_ml[i * 2], li, top);
+    l = __builtin_fmaf(w, li, l);
     const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_out + i * D + 4 * c);
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w, x[e], sum[e]);
@@ -988,8 +992,8 @@ int cus() {
   return cached;
 }
 
-template <typename Kernel>
-int launch(Kernel kernel, const WindowArgs& a, unsigned grid, int waves, int lds, hipStream_t stream) {
+template <void (*kernel)(const WindowArgs)>
+int launch(const WindowArgs& a, unsigned grid, int waves, int lds, hipStream_t stream) {
   // more than 64 KB of LDS has to be allowed once per kernel and device
   static thread_local int allowed_dev = -1;
   int dev = 0;
@@ -1054,17 +1058,13 @@ template <int D, bool kHalf>
 int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t workspace_bytes, int64_t n_counters, hipStream_t stream) {
   Plan plan = plan_form<D>(a, 0, units, n_cus, workspace ? workspace_bytes : 0);
   for (int form : {1, 2}) {
+    if (units * ((a.rows + kRowsFew - 1) / kRowsFew) > kMostItems) break;
     const Plan other = plan_form<D>(a, form, units, n_cus, workspace ? workspace_bytes : 0);
     if (other.us < plan.us) plan = other;
   }
   const int tile_rows = kForms<D>[plan.form].rows;
   a.row_tiles = (a.rows + tile_rows - 1) / tile_rows;
-  const int64_t items = units * a.row_tiles;
-  if (items > (1 << 28)) {
-    set_error("too many query tiles (%lld)", (long long)items);
-    return DT_ERR_INVALID;
-  }
-  a.items = (int32_t)items;
+  a.items = (int32_t)(units * a.row_tiles);
   a.per_xcd = (a.items + kXcds - 1) / kXcds;
   a.ways = plan.ways;
   a.by_ways = quotient_by(a.ways);
@@ -1078,9 +1078,9 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
   }
   if (plan.form == 0 || kXcds * plan.tail > n_counters) a.counters = nullptr;
   const unsigned grid = (unsigned)(kXcds * (a.tail_start + a.tail * a.ways));
-  const int rc = plan.form == 0   ? launch(attn_window_kernel<D, kHalf>, a, grid, kWavesShared, SharedLds<D>::kBytes, stream)
-                 : plan.form == 1 ? launch(attn_window_few_kernel<D, kHalf, 8>, a, grid, 8, FewLds<D, 8>::kAll, stream)
-                                  : launch(attn_window_few_kernel<D, kHalf, 4>, a, grid, 4, FewLds<D, 4>::kAll, stream);
+  const int rc = plan.form == 0   ? launch<attn_window_kernel<D, kHalf>>(a, grid, kWavesShared, SharedLds<D>::kBytes, stream)
+                 : plan.form == 1 ? launch<attn_window_few_kernel<D, kHalf, 8>>(a, grid, 8, FewLds<D, 8>::kAll, stream)
+                                  : launch<attn_window_few_kernel<D, kHalf, 4>>(a, grid, 4, FewLds<D, 4>::kAll, stream);
   if (rc != DT_OK || a.ways == 1 || a.counters) return rc;
   const int64_t folded = (int64_t)kXcds * a.tail * tile_rows;
   hipLaunchKernelGGL((attn_window_fold_kernel<D, kHalf>), dim3((unsigned)((folded * (D / 4) + 255) / 256)), dim3(256), 0, stream, a, tile_rows);
@@ -1143,7 +1143,7 @@ extern "C" int dt_attn_window_fwd(const void* q, const void* k, const void* v, v
     return DT_ERR_INVALID;
   }
   const int64_t rows = (int64_t)Sq * (H / Hk), units = (int64_t)B * Hk;
-  if (rows > (1ll << 30) || units > (1ll << 28) || units * ((rows + 31) / 32) > (1ll << 28)) {
+  if (rows > (1ll << 30) || units > kMostItems || units * ((rows + kRowsShared - 1) / kRowsShared) > kMostItems) {
     set_error("too many query rows");
     return DT_ERR_INVALID;
   }

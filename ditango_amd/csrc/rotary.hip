@@ -253,7 +253,7 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
   }
   const int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
   const __int128 items = (__int128)B * S * groups;
-  if (items >= (1ll << 31)) {
+  if (items * (D / 8) > (1ll << 32) - kThreads || items >= (1ll << 31)) {      // (a grid holds fewer than 2^32 lanes)
     set_error("too many rows");
     return DT_ERR_INVALID;
   }

@@ -38,7 +38,7 @@ struct BlockArgs {
   int32_t n8, n16, n;   // states below n8 are 8-bit, below n16 at most 16-bit
   void* dst;
   uint8_t* dst_scales;
-  float* dst_lse;       // may be null
+  float* dst_lse;
   int32_t dst_dtype, dst_bsh;
   RowIndex at;
 };
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs 
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = s.acc[e] * inv;
   store(a, elem, live, elems, x);
-  if (live && a.dst_lse != nullptr && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
+  if (live && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
 }
 
 // One state into another format, its lse bit for bit.  From kManyWorkgroups workgroups on, with twice the elements each: a state of 14 882 x 24
@@ -295,7 +295,6 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
   KernArgs& a = kernel_args();
   const RowIndex at = rows_of(a);
   const int64_t elems = (int64_t)at.rows * D, elem = first_elem<kUnits>();
-  const bool with_lse = a.dst_lse != nullptr;
   Raw<kBytes> r[kUnits];
   float l[kUnits];
   uint32_t bhs[kUnits];
@@ -304,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
     const int64_t e = elem + u * (kThreads * 8), from = e < elems ? e : 0;
     load<kBytes>(a, 0, from, r[u]);
     bhs[u] = bhs_of(at, (uint32_t)(from / D));
-    if (with_lse && e % D == 0) l[u] = a.lse[0][a.bsh_mask & 1 ? (uint32_t)(from / D) : bhs[u]];
+    if (e % D == 0) l[u] = a.lse[0][a.bsh_mask & 1 ? (uint32_t)(from / D) : bhs[u]];
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -316,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
     for (int i = 0; i < 8; ++i) x[i] = -0.f;       // (-0 + -0 keeps its sign)
     add<kBytes>(r[u], a.kind_mask & 1, 1.f, x);
     store(a, e, live, elems, x);
-    if (with_lse && live && e % D == 0) a.dst_lse[a.dst_bsh ? (uint32_t)(e / D) : bhs[u]] = l[u];
+    if (live && e % D == 0) a.dst_lse[a.dst_bsh ? (uint32_t)(e / D) : bhs[u]] = l[u];
   }
 }
 

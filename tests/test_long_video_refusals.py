@@ -164,3 +164,17 @@ def test_memory_of_a_cached_row():
     assert proCache(8, 0).set_block_size_mb(x) * 2 ** 20 == 16 * 260
     assert proCache(8, 0, state_format="int8").set_block_size_mb(x) * 2 ** 20 == 16 * 136
     assert BlockState.empty(x.shape, "e4m3", "cpu").nbytes == 16 * 136
+
+
+def test_grids_beyond_the_launchers_are_refused():
+    """A grid holds fewer than 2^32 lanes: more rows than that are refused before the launch, not by it."""
+    lib = _hip.load_library()
+    strides = (ctypes.c_int64 * 3)(0, 128, 64)
+    w = Window(1, 0, 1, 0, -1, None)
+    for B, Sq in ((1 << 23, 1), (1 << 13, 1 << 18)):
+        assert "too many query rows" in _err(lib, lib.dt_attn_window_fwd(4096, 4096, 4096, 4096, 4096, B, Sq, 4, 2, 2, 64, strides, strides, strides,
+                                                                         ctypes.cast(ctypes.pointer(w), ctypes.c_void_p), 0.0, 0, None, 0, None, 0, None))
+    rows = (Rows * 1)(Rows(4096, 0, 0, 0, 4096, None, None, 1, 1.0))
+    for D, S in ((64, 1 << 15), (128, 1 << 14)):
+        assert "too many rows" in _err(lib, lib.dt_qk_norm_rope_axes(ctypes.cast(rows, ctypes.c_void_p), 1, 1 << 14, S, D, 1, 1e-6, 4096, 0, 3,
+                                                                     (ctypes.c_uint64 * 64)(), (ctypes.c_uint8 * 64)(), 1, None, 0, 0, None))

@@ -246,3 +246,34 @@ def test_the_step_adapter_hands_it_out(hip):
             layer.attn_processor("window")(q, k, v, causal=True, right=1)
     finally:
         parallel_state.destroy_local_groups()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq, Sk, H, Hk, left", [(1, 30000, 2, 2, None), (3, 40, 4, 2, 11), (70, 5000, 2, 2, 3000), (700, 900, 64, 1, 150), (2100, 2100, 66, 66, 1500)])
+def test_undefined_scores_stay_undefined(hip, Sq, Sk, H, Hk, left, D, captured):
+    """A query that holds a NaN, and the queries that see a key that does, become NaN, in the lse as well, however the keys are shared out; no other does."""
+    from ditango_amd.window import window_attention
+    q, k, v = _tensors(1, Sq, Sk, H, Hk, D, torch.bfloat16, seed=12)
+    w = dict(left=left, right=0)
+    query, key = (0, 0), (Sk - 1 - Sq // 2, Hk - 1)
+    q2, k2 = q.clone(), k.clone()
+    q2[0, query[0], query[1], D - 3] = math.nan
+    k2[0, key[0], key[1], 7] = math.nan
+    window_attention(q2, k2, v, **w)
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = window_attention(q2, k2, v, **w)
+        graph.replay()
+        torch.cuda.synchronize()
+    else:
+        out, lse = _run(q2, k2, v, **w)
+    at = torch.arange(Sq, device=DEV) + Sk - Sq
+    sees = (at >= key[0]) & (at - (Sk if left is None else left) <= key[0])
+    nan = torch.zeros(1, H, Sq, dtype=torch.bool, device=DEV)
+    nan[0, key[1] * (H // Hk):(key[1] + 1) * (H // Hk)] = sees
+    nan[0, query[1], query[0]] = True
+    assert torch.equal(lse.isnan(), nan) and torch.equal(out.isnan(), nan.transpose(1, 2)[..., None].expand_as(out))
+    _check(torch.where(out.isnan(), L.window_attention(q, k, v, **w)[0].to(out.dtype), out), torch.where(nan, L.window_attention(q, k, v, **w)[1].float(), lse), q, k, v, **w)
