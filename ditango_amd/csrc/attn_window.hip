@@ -210,20 +210,34 @@ struct RowState {
   __device__ __forceinline__ void softmax(f32x16 (&s)[NKB], ex8 (&p)[NKB][2], int k0, bool masked, int lane) {
     if (masked) {
       asm volatile("" ::: "memory");   // keeps this a real branch
-      // A key's place behind `lo` as an unsigned number is below the span's length inside it alone; one of the sinks is below `some`.
+      // One border after the other, as most such tiles have only one of them.  Keys in front of the window but for the sinks are hidden: the place
+      // behind the last sink, as an unsigned number, is then below that of the window.
       const int at = k0 + 8 * (lane >> 5);
-      int from = at - mine.lo, some = min(sinks, mine.hi) - at;
-      const uint32_t length = (uint32_t)max(mine.hi - mine.lo, 0);
-      asm volatile("" : "+v"(from), "+v"(some));     // (sums of them and the keys' places would otherwise be kept through the loop)
+      if (k0 < last.lo) {
+        int some = max(sinks - at, 0);
+        uint32_t hidden = (uint32_t)max(mine.lo - at - some, 0);
+        asm volatile("" : "+v"(some), "+v"(hidden));     // (their sums with the keys' places would otherwise be kept through the loop)
 #pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
+        for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = 32 * kb + 16 * (r >> 3) + (r & 7);
-          const bool seen = ((uint32_t)(from + key) < length) | (key < some);
-          s[kb][r] = seen ? s[kb][r] : -INFINITY;
-          asm volatile("" : "+v"(s[kb][r]));     // one comparison and choice after the other: 90 spilled scalars otherwise
-        }
+          for (int r = 0; r < 16; ++r) {
+            const int key = 32 * kb + 16 * (r >> 3) + (r & 7);
+            s[kb][r] = (uint32_t)(key - some) < hidden ? -INFINITY : s[kb][r];
+            asm volatile("" : "+v"(s[kb][r]));     // one comparison and choice after the other: 90 spilled scalars otherwise
+          }
+      }
+      if (k0 + T::kKeys > first.hi) {
+        int end = mine.hi - at;
+        asm volatile("" : "+v"(end));
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = 32 * kb + 16 * (r >> 3) + (r & 7);
+            s[kb][r] = key < end ? s[kb][r] : -INFINITY;
+            asm volatile("" : "+v"(s[kb][r]));
+          }
+      }
     }
     // Probabilities relative to the reference that the sums are scaled to.  The tile's own maximum is looked for only where the sum of
     // the probabilities, needed anyway, says that the reference lags too far behind (or is not there yet: the sum is inf or NaN).
