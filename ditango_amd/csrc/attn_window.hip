@@ -271,20 +271,21 @@ struct RowState {
       for (int db = 0; db < D / 32; ++db) o[db] = E::mfma(v_frag(vt, db, step), p[step >> 1][step & 1], o[db]);
   }
 
-  // A masked key's probability is 0, which an infinite or undefined value of V would turn into NaN.  Tiles with masked keys are looked
-  // through (3 instructions for 8 values, by the four wavefronts of a group together where tiles are shared).  Where there is such a value, few
-  // rows multiply the tile with zeros in their place and then add them, as they are, to the rows that see them (the weight of a visible key is
-  // above 0); shared tiles, whose loop has no registers for that, compute the 32 rows once more behind it (rows_one_by_one).
+  // A masked key's probability is 0, which an infinite or undefined value of V would turn into NaN.  Few rows look tiles with masked keys through
+  // (3 instructions for 8 values); where there is such a value, they multiply the tile with zeros in their place and then add them, as they are, to
+  // the rows that see them (the weight of a visible key is above 0).  Shared tiles look at the sums instead, once: where one of a defined weight is
+  // not finite and a tile with masked keys holds such a value, they compute the 32 rows once more (rows_one_by_one).
   static constexpr uint32_t kExp = kHalf ? 0x7c007c00u : 0x7f807f80u, kOne = kHalf ? 0x04000400u : 0x00800080u;
-  template <int kBlocks = T::kBlocks>
+  __device__ __forceinline__ static uint32_t ones(const u32x4& x) {     // sign bits where an element's exponent is all ones, whose carry they are
+    uint32_t over = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) over |= (x[e] & kExp) + kOne;
+    return over;
+  }
   __device__ __forceinline__ bool any_not_finite(const uint8_t* vt, int lane) const {
     uint32_t over = 0;
 #pragma unroll 2
-    for (int i = 0; i < kBlocks; ++i) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(vt + i * 1024 + lane * 16);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) over |= (x[e] & kExp) + kOne;   // an exponent of ones carries into the sign's bit
-    }
+    for (int i = 0; i < T::kBlocks; ++i) over |= ones(*reinterpret_cast<const u32x4*>(vt + i * 1024 + lane * 16));
     return __any((over & 0x80008000u) != 0);
   }
   __device__ __forceinline__ void values_not_finite(const uint8_t* vt, const ex8 (&p)[NKB][2], int k0, int lane) {
@@ -522,6 +523,23 @@ __device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item&
   }
 }
 
+// Whether a tile that some row of the wavefront does not see whole holds infinite or undefined values.
+template <int D, bool kHalf>
+__device__ __forceinline__ bool masked_not_finite(const WindowArgs& a, const Item& it, const RowState<D, kHalf, 2>& st, const TileList<64>& list, int len, int lane) {
+  typedef RowState<D, kHalf, 2> State;
+  typedef Tiles<D, 2> T;
+  const uint16_t* v = a.v + it.b * a.v_sb + it.hk * a.v_sh + 8 * (lane % T::kRowLanes);
+  uint32_t over = 0;
+#pragma unroll 1
+  for (int t = list.begin; t < list.end; ++t) {
+    const int k0 = list.key(t);
+    if (st.whole(k0)) continue;
+#pragma unroll 1
+    for (int j = k0 + lane / T::kRowLanes; j < min(k0 + T::kKeys, len); j += T::kBlockRows) over |= State::ones(*reinterpret_cast<const u32x4*>(v + j * a.v_ss));
+  }
+  return __any((over & 0x80008000u) != 0);
+}
+
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_window_kernel(const WindowArgs a) {
   typedef Tiles<D, 2> T;
@@ -556,7 +574,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   };
   RowState<D, kHalf, 2> st;
   const int row0 = it.row0 + 32 * wave;
-  bool hurt = false;     // values that are infinite or undefined in a tile that some row does not see whole
   // The wavefront's rows of Q come as whole lines through the LDS: half of them through its staging rows, a quarter each through its own shares
   // of V of pairs 3 and 2, which nothing but its own later loads writes.  (As fragments from memory, a load instruction touches 32 lines for 32
   // bytes each, and the compiler's wait for them would be one for every tile load behind them.)
@@ -650,8 +667,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     if (group == 0) wait_all_but<S::kLoads>();
     end_products(s, st.o);
     int k0 = list.key(list.begin);
-    // what the group's wavefronts have found in a tile's values, each in a quarter of them: in staging rows, which are free until the end
-    int* flags = reinterpret_cast<int*>(lds + S::kStage + group * 4 * 32 * D);
     // keys from which on, and up to which, a tile is seen whole by all rows of the workgroup
     const uint32_t inside = (uint32_t)max(all_first.hi - (T::kKeys - 1) - all_last.lo, 0);
     auto probabilities = [&](bool need, bool masked) __attribute__((always_inline)) {
@@ -672,16 +687,12 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
       if (__builtin_expect((uint32_t)(k0 - all_last.lo) >= inside, 0)) {
         masked = !st.whole(k0);
         need = st.needs(k0);
-        constexpr int kShare = T::kBlocks / 4;
-        const bool bad = st.template any_not_finite<kShare>(vt + (wave & 3) * kShare * 1024, lane);
-        if (lane == 0) flags[wave & 3] = bad;
       }
       probabilities(need, masked);
       prefill(vt);
       if (group == 1) wait_all_but<S::kLoads>();
       end_softmax(p);
       __builtin_amdgcn_s_setprio(0);
-      if (masked) hurt |= (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
       products(vt);
       if (group == 0) wait_all_but<S::kLoads>();
       end_products(s, st.o);
@@ -691,7 +702,6 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     const uint8_t* vt = lds + pair_at(n - 1);
     probabilities(st.needs(k0), masked);
     end_softmax(p);
-    if (masked) hurt |= st.any_not_finite(vt, lane);
     st.values(vt, p);
     // group 1's last products are the last thing that happens in the buffers
     if (group == 0) wait_lds_barrier();
@@ -701,6 +711,12 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   const int col = lane & 31, hh = lane >> 5;
   const float l = st.l_run + __shfl_xor(st.l_run, 32);
   const float inv = l != 0.f ? 1.f / l : 0.f;      // (an undefined sum stays one)
+  float undefined = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) undefined = __builtin_fmaf(st.o[i][r], 0.f, undefined);
+  const bool hurt = __builtin_expect(__any(undefined != 0.f && l == l), 0) && masked_not_finite<D, kHalf>(a, it, st, list, len, lane);
   if (it.ways > 1) {
     // A part's sums, fp32.  (Where they have to be computed once more, they are those of the keys of the part.)
     const int64_t at = (int64_t)it.slot * kRowsShared + 32 * wave + col;
