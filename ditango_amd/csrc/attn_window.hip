@@ -1041,7 +1041,7 @@ int launch(const WindowArgs& a, unsigned grid, int waves, int lds, hipStream_t s
 // How a launch runs: the form, and how the last round of workgroups (all of them, in a launch of less than one) is cut along the keys.  By
 // estimate, from what the forms take here, in us: a step -- 64 keys of shared tiles, a 32-key tile of every wavefront of few rows -- with up to
 // eight wavefronts a CU, and with more (D = 64); an item beside its steps; parts, their states' way to memory and back, 2 bytes / 6.7 TB/s, and the
-// kernel that adds them up, or the last of them that does.
+// kernel that adds them up, or the last of them that does, 0.4 us a part (2 heads of 64, a token over 20 000: 20.9 us without that term, 13.3 with).
 struct Form {
   int rows, keys, per_cu;       // rows of a workgroup, keys of its step, workgroups a CU
   double step, full, once;
@@ -1076,7 +1076,7 @@ Plan plan_form(const WindowArgs& a, int form, int64_t units, int n_cus, int64_t 
   for (int ways = 2; ways <= 64 && steps >= 2 * ways; ++ways) {
     const int64_t bytes = kXcds * tail * ways * f.rows * (D + 2) * 4;
     if (bytes > workspace_bytes) break;
-    const double fold = form != 0 && a.counters ? 3.0 : 8.0;
+    const double fold = form != 0 && a.counters ? 2.0 + 0.4 * ways : 8.0;
     const double us = before + (double)((tail * ways + slots - 1) / slots) * item((steps + ways - 1) / ways, std::min(tail * ways, slots)) + fold +
                       2.0 * bytes / 6.7e6;
     if (us < best.us) best = Plan{form, ways, tail, us};
