@@ -559,6 +559,7 @@ int dt_qkv_project(const void* text, int64_t text_stride_b, int64_t text_stride_
  * 0..Sk; NULL: Sk): keys behind it, padding or rows of a cache that are not written yet, may hold anything.
  * The result is a state as of dt_attn_chunk_fwd, out [B,Sq,H,D] contiguous in the dtype of q, lse fp32 [B,H,Sq]: softmax over the visible keys;
  * a row that sees none gets out = 0, lse = -inf.  A masked key adds nothing, whatever it and its value hold.
+ * out may be q where that is contiguous, and shares no memory with k or v.
  * q [B,Sq,H,D], k and v [B,Sk,Hk,D] with element strides {batch, token, head} of their own (HOST arrays of 3; multiples of 8, token strides of
  * k and v at most 2^23), H a multiple of Hk: query heads h share key head h / (H / Hk).  bfloat16, or IEEE half with DT_ATTN_FP16.
  * workspace: device memory, 16-byte aligned; launches that leave part of the GPU idle cut their windows into parts, which leave partial states

@@ -223,3 +223,19 @@ def test_no_rows(hip):
     o, l = torch.empty(1, 0, 4, 64, device=DEV), torch.empty(1, 4, 0, device=DEV)
     state = BlockState.empty(o.shape, "int8", DEV)
     assert merge_any([(o, l)], dst=state) is state and merge_any([state])[0].shape == (1, 0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_merged_into_one_of_the_states_and_with_itself(hip, fmt, dtype):
+    """The destination is a 16- or 32-bit state among 8-bit ones; a state that appears twice counts twice."""
+    from ditango_amd.core.cache import merge_any, quantized
+    g = torch.Generator().manual_seed(21)
+    for B, S, H, D in ((1, 3, 1, 64), (2, 411, 5, 128)):
+        o, l = _state(g, B, S, H, D, dtype, 0.3)
+        state = quantized(*_state(g, B, S, H, D, torch.float32, 0.3), fmt)
+        want = merge_any([state, (o, l), state], dst_dtype=dtype)
+        own = (L.value(state.elements.cpu(), state.scales.cpu().int() - 127), state.lse.cpu())
+        _check_merge(want[0], want[1], [own, (o.cpu(), l.cpu()), own], dtype)
+        got = merge_any([state, (o, l), state], dst=(o, l))
+        assert got[0] is o and torch.equal(o, want[0]) and torch.equal(l, want[1])

@@ -277,3 +277,38 @@ def test_undefined_scores_stay_undefined(hip, Sq, Sk, H, Hk, left, D, captured):
     nan[0, query[1], query[0]] = True
     assert torch.equal(lse.isnan(), nan) and torch.equal(out.isnan(), nan.transpose(1, 2)[..., None].expand_as(out))
     _check(torch.where(out.isnan(), L.window_attention(q, k, v, **w)[0].to(out.dtype), out), torch.where(nan, L.window_attention(q, k, v, **w)[1].float(), lse), q, k, v, **w)
+
+
+@pytest.mark.parametrize("Sq, Sk, H, Hk, w", [(1, 3000, 4, 2, dict(left=1000, right=0, sinks=70)), (700, 900, 64, 1, dict(left=150, right=3, sinks=5)),
+                                              (2100, 2100, 66, 66, dict(left=2, right=1, frame=300, sinks=100, q_begin=0)), (2100, 2100, 66, 66, dict(left=None, right=0))])
+def test_undefined_values_where_rows_do_and_do_not_see_them(hip, Sq, Sk, H, Hk, w):
+    """Heads of 128: values without a finite magnitude in tiles that are seen whole, in part and not at all, in every key head."""
+    q, k, v = _tensors(1, Sq, Sk, H, Hk, 128, torch.bfloat16, seed=13, sigma=1.0)
+    for i in range(Hk):
+        v[0, (37 * i + 1) % Sk, i, i % 128] = float("nan")
+        v[0, (911 * i + 500) % Sk, i, (i + 64) % 128] = float("inf")
+        v[0, Sk - 1 - i % 3, i, (i + 9) % 128] = float("-inf")
+    _check(*_run(q, k, v, **w), q, k, v, **w)
+
+
+def test_keys_that_batches_and_heads_share_by_stride(hip):
+    """Expanded tensors: strides of 0 along the batch, the heads and (one key) the tokens."""
+    q, k, v = _tensors(3, 50, 200, 4, 1, 64, torch.bfloat16, seed=14)
+    k, v = k[:1].expand(3, -1, 4, -1), v[:1].expand(3, -1, 4, -1)
+    got = _run(q, k, v, left=70, right=0, sinks=3)
+    want = _run(q, k.contiguous(), v.contiguous(), left=70, right=0, sinks=3)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = (k[:, :1].expand(-1, 90, -1, -1), v[:, :1].expand(-1, 90, -1, -1))
+    got, want = _run(q, *one, left=20, right=5), _run(q, *(t.contiguous() for t in one), left=20, right=5)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_results_over_the_queries(hip):
+    """``out`` may be q: a row is read before anything of it is written, also where several workgroups share it."""
+    from ditango_amd.window import window_attention
+    for Sq, Sk, H in ((1, 9000, 2), (40, 9000, 2), (2100, 2100, 66)):
+        q, k, v = _tensors(1, Sq, Sk, H, H, 64, torch.bfloat16, seed=15)
+        want = _run(q, k, v, left=None, right=0)
+        out, lse = window_attention(q, k, v, left=None, right=0, out=q)
+        torch.cuda.synchronize()
+        assert out.data_ptr() == q.data_ptr() and torch.equal(q, want[0]) and torch.equal(lse, want[1])
