@@ -7,7 +7,8 @@
 // included (4 million fractions all round the turn), where the row's 16 bits are off by 2^-9 to 2^-12 of a value.
 //
 // HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
-// runs of 4 half a section apart with rotate-half.  It has their angles once for the kHeads heads of its lane group.
+// runs of 4 half a section apart with rotate-half.  It has their angles once for the kHeads heads of its lane group.  14 882 tokens x (24 + 24) heads of
+// 128 with an RMS norm: 68.0 us, 5.4 TB/s (two launches of the kernel with tables: 68.2, and the tables' making).
 #include "producer_math.h"
 
 namespace dt {

@@ -8,6 +8,7 @@
 //
 // The merge is that of the 16-bit states: lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i, fp32 sums, one pass; a single
 // state is copied.  Bound by HBM: D + D / 32 + 4 bytes a row and 8-bit state instead of 2 D + 4.
+// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 108.6 us, 6.1 TB/s; one stored and loaded 55.0 us, 5.2 TB/s.
 //
 // A lane owns 8 consecutive elements, so 4 lanes hold a block and its maximum is two exchanges inside a quad; a row's lanes are
 // neighbours in a wavefront.  States come sorted by the size of their elements, each size in batches whose loads are in flight together.
