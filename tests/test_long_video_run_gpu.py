@@ -173,3 +173,29 @@ def test_a_layer_without_room_for_its_arena_recomputes(env):
         update_timestep(t)
         outs.append(attn.attn(q, ks[0], vs[0]))
     assert attn.cache.arena_out is None and torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_many_ragged_chunks_under_a_mask(env, fmt):
+    """More chunks than one launch addresses, some without a key, some steps that compute nothing but the own chunk."""
+    from ditango_amd.core.attention import proAttention
+    from ditango_amd.core.parallel_state import get_usp_group
+    from ditango_amd.utils import update_timestep
+    C, T, H, S, D = 70, 3, 2, 40, 64
+    rm = env(C, 5, T, 1, state_format=fmt)
+    mask = (np.random.default_rng(1).random((T, 1, C)) < 0.5).astype(np.uint8)
+    mask[0], mask[2] = 0, 1
+    rm.set_chunk_mask(mask, diag=5)
+    group = get_usp_group()
+    small, plain = proAttention(0, group), proAttention(0, group)
+    plain.cache = type(plain.cache)(C, 0)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    lens = [0 if c % 11 == 3 else 1 + (c * 17) % 60 for c in range(C)]
+    for t in range(T):
+        update_timestep(t)
+        q = torch.randn(2, S, H, D, generator=g, device=DEV).bfloat16()
+        ks, vs = ([torch.randn(2, n, H, D, generator=g, device=DEV).bfloat16() for n in lens] for _ in range(2))
+        group.set_kv_chunks(ks, vs)
+        a, b = (x.attn(q, ks[5], vs[5]) for x in (plain, small))
+        assert float((plain.last_lse - small.last_lse).abs().max()) < 1e-4
+        assert float((a - b).abs().max()) <= _bound(fmt, 6.0, 1)
