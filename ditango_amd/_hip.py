@@ -532,10 +532,11 @@ def zero_rows_from(t: torch.Tensor, first_row: torch.Tensor) -> None:
 
 def _stream_at(t: torch.Tensor, name: str) -> int:
     """The current device's current stream, which the tensors have to live on."""
-    _require(t.is_cuda, f"{name} must live on the GPU")
-    device = _current_device()
-    if t.get_device() != device:
-        raise DitangoHipError(f"{name} lives on device {t.get_device()} but device {device} is current: make the tensors' device current for this call")
+    device = t.get_device()
+    if device < 0:
+        raise DitangoHipError(f"{name} must live on the GPU")
+    if device != _current_device():
+        raise DitangoHipError(f"{name} lives on device {device} but device {_current_device()} is current: make the tensors' device current for this call")
     return _raw_stream(device)
 
 

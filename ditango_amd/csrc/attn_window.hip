@@ -507,12 +507,19 @@ __device__ __forceinline__ void rows_one_by_one(const WindowArgs& a, const Item&
         }
       }
       const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(score, a.scale_log2, -top));
-#pragma unroll 1
-      for (int j = j0; j < stop; ++j) {
-        const float wj = __shfl(w, j - j0);
-        const uint16_t* row = v + (int64_t)j * a.v_ss;
+      for (int j = j0; j < stop; j += 8) {
+        typename E::t x[8][kCols];
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(wj, (float)*reinterpret_cast<const typename E::t*>(row + e), acc[e]);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < kCols; ++e) x[i][e] = reinterpret_cast<const typename E::t*>(v + (int64_t)min(j + i, stop - 1) * a.v_ss)[e];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float wj = __shfl(w, j + i - j0);
+#pragma unroll
+          for (int e = 0; e < kCols; ++e)
+            if (j + i < stop) acc[e] = __builtin_fmaf(wj, (float)x[i][e], acc[e]);
+        }
       }
     }
     if (it.ways > 1) {

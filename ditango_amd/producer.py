@@ -159,7 +159,7 @@ def prepare_qk_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch
         raise ValueError(f"unknown norm {norm!r}")
     if positions.dtype is not torch.int32:
         raise ValueError(f"positions must be int32, got {positions.dtype}")
-    if positions.dim() not in (2, 3) or positions.shape[-1] != len(axes.dims):
+    if not 2 <= positions.dim() <= 3 or positions.size(-1) != len(axes.dims):
         raise ValueError(f"positions must be [S, {len(axes.dims)}] or [B, S, {len(axes.dims)}] for these axes, got {tuple(positions.shape)}")
     q_out, k_out = (None, None) if out is None else out
     tensors = [(q, q_weight, q_bias, q_out, 1.0 if fold_softmax_scale is None else folded_scale(q.shape[-1], fold_softmax_scale))]

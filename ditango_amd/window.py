@@ -17,9 +17,13 @@ from . import _hip
 def _limit(name: str, value: Optional[int]) -> int:
     if value is None:
         return -1
-    if isinstance(value, bool) or not hasattr(value, "__index__") or not 0 <= value.__index__() < 1 << 31:
+    if type(value) is not int:
+        if isinstance(value, bool) or not hasattr(value, "__index__"):
+            raise ValueError(f"{name} must be None or a whole number of at least 0, got {value!r}")
+        value = value.__index__()
+    if not 0 <= value < 1 << 31:
         raise ValueError(f"{name} must be None or a whole number of at least 0, got {value!r}")
-    return value.__index__()
+    return value
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: Optional[int] = None, right: Optional[int] = None,
