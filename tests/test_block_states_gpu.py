@@ -239,3 +239,27 @@ def test_merged_into_one_of_the_states_and_with_itself(hip, fmt, dtype):
         _check_merge(want[0], want[1], [own, (o.cpu(), l.cpu()), own], dtype)
         got = merge_any([state, (o, l), state], dst=(o, l))
         assert got[0] is o and torch.equal(o, want[0]) and torch.equal(l, want[1])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_more_than_2_to_the_31_elements(hip, fmt):
+    """A state of 2.3 billion elements, stored, merged and loaded, against pieces of its end on their own."""
+    from ditango_amd.core.cache import BlockState, merge_any, quantized
+    S, H, D, n = 140_001, 128, 128, 33
+    out = torch.empty(1, S, H, D, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(3))
+    lse = torch.randn(1, H, S, device=DEV)
+    state = quantized(out, lse, fmt)
+    ends = [slice(0, n), slice(S - n, S)]
+    for at in ends:
+        o, l = out[:, at].contiguous(), lse[:, :, at].contiguous()
+        piece = quantized(o, l, fmt)
+        part = BlockState(state.elements[:, at], state.scales[:, at], state.lse[:, :, at])
+        assert torch.equal(part.elements.view(torch.uint8), piece.elements.view(torch.uint8)) and torch.equal(part.scales, piece.scales)
+        assert torch.equal(part.lse, piece.lse)
+    both = merge_any([state, (out, lse)], dst_dtype=torch.bfloat16)
+    back = merge_any([state], dst_dtype=torch.bfloat16)
+    for at in ends:
+        o, l = out[:, at].contiguous(), lse[:, :, at].contiguous()
+        piece = quantized(o, l, fmt)
+        for whole, want in ((both, merge_any([piece, (o, l)], dst_dtype=torch.bfloat16)), (back, merge_any([piece], dst_dtype=torch.bfloat16))):
+            assert torch.equal(whole[0][:, at], want[0]) and torch.equal(whole[1][:, :, at], want[1])

@@ -161,3 +161,16 @@ def test_no_tokens(hip):
     q = torch.empty(2, 0, 4, 64, dtype=torch.bfloat16, device=DEV)
     y, k = prepare_qk_axes(q, q[:, :, :2], torch.empty(0, 3, dtype=torch.int32, device=DEV), RotaryAxes(dims=(16, 24, 24)))
     assert y.shape == (2, 0, 4, 64) and k.shape == (2, 0, 2, 64)
+
+
+def test_more_than_2_to_the_31_elements(hip):
+    """The end of a sequence of 2.3 billion elements, against the same tokens on their own."""
+    from ditango_amd.producer import RotaryAxes, grid_positions, prepare_qk_axes
+    S, H, D, n = 140_001, 128, 128, 37
+    q = torch.empty(1, S, H, D, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(4))
+    axes, pos = RotaryAxes(dims=(16, 56, 56), base=256.0), grid_positions(1, 140_001, 1, device=DEV)
+    k = q[:, :, :2]
+    got = prepare_qk_axes(q, k, pos, axes, norm="rms")
+    for at in (slice(0, n), slice(S - n, S)):
+        want = prepare_qk_axes(q[:, at], k[:, at], pos[at].contiguous(), axes, norm="rms")
+        assert torch.equal(got[0][:, at], want[0]) and torch.equal(got[1][:, at], want[1])

@@ -66,7 +66,7 @@ CASES = [
     (1, 65, 300, 2, 2, dict(left=10, right=None, sinks=300)),
     (1, 64, 64, 1, 1, dict(left=2, right=0, frame=1 << 29, sinks=0)),
     (1, 33, 97, 1, 1, dict(left=(1 << 31) - 1, right=(1 << 31) - 1, frame=1 << 29)),
-    (2, 1030, 1030, 32, 32, dict(left=99, right=20, sinks=6)),        # enough rows for workgroups of 128
+    (2, 1030, 1030, 32, 32, dict(left=99, right=20, sinks=6)),        # enough rows for workgroups of 256
     (2, 700, 900, 32, 16, dict(left=1, right=0, frame=128, sinks=70, q_begin=190)),
     (3, 600, 777, 40, 40, dict(left=None, right=0, sinks=0)),
     (1, 1500, 1600, 64, 8, dict(left=2, right=2, frame=100, sinks=100, q_begin=100)),
