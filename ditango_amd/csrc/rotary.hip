@@ -7,7 +7,7 @@
 // included (4 million fractions all round the turn), where the row's 16 bits are off by 2^-9 to 2^-12 of a value.
 //
 // HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
-// runs of 4 half a section apart with rotate-half.  It has their angles once for the kHeads heads of its lane group.  14 882 tokens x (24 + 24) heads of
+// runs of 4 half a section apart with rotate-half.  It has their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of
 // 128 with an RMS norm: 68.0 us, 5.4 TB/s (two launches of the kernel with tables: 68.2, and the tables' making).
 #include "producer_math.h"
 
@@ -18,7 +18,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;         // heads of a lane group
+// A lane group takes 4 heads of a token, or 8: the angles and the loads in front of them are then shared by twice as many rows.  Eight where groups of four
+// make more than kManyWorkgroups workgroups and eight leave no more lanes idle.  us with 4 and with 8, q and k of 24 heads of 128: 600 tokens (450 workgroups)
+// 6.0 / 6.0, 1200 8.3 / 7.8, 2400 15.6 / 12.0, 4800 25.8 / 23.2, 14 882 69.1 / 66.2; of 12 heads, 2400 tokens 8.2 / 9.2.  Twelve need scratch.
+constexpr unsigned kManyWorkgroups = 640;
 constexpr int kMostAxes = 8;
 
 struct Rows {
@@ -27,7 +30,7 @@ struct Rows {
   int64_t sb, ss, sh;
   const void *w, *bias;
   float scale;
-  int32_t H, groups;              // groups of kHeads heads
+  int32_t H, groups;              // groups of heads that a lane group takes
 };
 struct RotaryArgs {
   Rows rows[2];
@@ -57,7 +60,7 @@ __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d,
   }
 }
 
-template <int D, bool kHalf, bool kHalves>
+template <int D, bool kHalf, bool kHalves, int kHeads>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const RotaryArgs a) {
   constexpr int G = D / 8;
   const int c = threadIdx.x % G;
@@ -130,7 +133,13 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
       }
       ss[r] = row_squares<G>(v);
     }
-    inverse_rms4<D>(ss[0], ss[1], ss[2], ss[3], a.eps, rs);
+#pragma unroll
+    for (int r = 0; r < kHeads; r += 4) {
+      float four[4];
+      inverse_rms4<D>(ss[r], ss[r + 1], ss[r + 2], ss[r + 3], a.eps, four);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rs[r + i] = four[i];
+    }
   }
   uint16_t* yp = t.y + ((int64_t)bs * t.H + h0) * D;
 #pragma unroll
@@ -250,13 +259,20 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
     d.w = r.weight; d.bias = r.bias;
     d.scale = r.out_scale;
     d.H = r.H;
-    d.groups = (r.H - 1) / kHeads + 1;
+    d.groups = (r.H - 1) / 4 + 1;
   }
-  const int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
-  const __int128 items = (__int128)B * S * groups;
+  int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
+  __int128 items = (__int128)B * S * groups;
   if (items * (D / 8) > (1ll << 32) - kThreads || items >= (1ll << 31)) {      // (a grid holds fewer than 2^32 lanes)
     set_error("too many rows");
     return DT_ERR_INVALID;
+  }
+  const int per_wg = kThreads / (D / 8);
+  const bool eight = items > (int64_t)kManyWorkgroups * per_wg && a.rows[0].groups % 2 == 0 && a.rows[1].groups % 2 == 0;
+  if (eight) {
+    for (Rows& r : a.rows) r.groups /= 2;
+    groups /= 2;
+    items /= 2;
   }
   a.pos = positions;
   a.pos_sb = pos_stride_b;
@@ -268,11 +284,14 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
   a.items = (uint32_t)items;
   a.by_groups = quotient_by((int32_t)groups);
   a.by_s = quotient_by(S);
-  const int per_wg = kThreads / (D / 8);
   const dim3 grid((unsigned)((items + per_wg - 1) / per_wg)), block(kThreads);
   const hipStream_t st = (hipStream_t)stream;
   const bool half = (rounding & DT_IO_FP16) != 0, halves = rope == DT_ROPE_HALVES;
-#define DT_LAUNCH(D, half, halves) hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves>), grid, block, 0, st, a)
+#define DT_LAUNCH(D, half, halves)                                                                                    \
+  do {                                                                                                                \
+    if (eight) hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves, 8>), grid, block, 0, st, a);             \
+    else hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves, 4>), grid, block, 0, st, a);                   \
+  } while (0)
 #define DT_LAUNCH_D(D)                                                           \
   do {                                                                           \
     if (half && halves) DT_LAUNCH(D, true, true);                                \

@@ -174,3 +174,24 @@ def test_more_than_2_to_the_31_elements(hip):
     for at in (slice(0, n), slice(S - n, S)):
         want = prepare_qk_axes(q[:, at], k[:, at], pos[at].contiguous(), axes, norm="rms")
         assert torch.equal(got[0][:, at], want[0]) and torch.equal(got[1][:, at], want[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("norm", [None, "rms", "layer_norm"])
+@pytest.mark.parametrize("axes", range(len(AXES)))
+def test_a_long_sequence_is_its_pieces(hip, axes, norm, dtype):
+    """Long launches give a lane group eight heads, short ones four: the same bits, q with and without k, also where heads do not fill a group."""
+    from ditango_amd.producer import RotaryAxes, prepare_qk_axes
+    g = torch.Generator().manual_seed(40 + axes)
+    axes = RotaryAxes(**AXES[axes])
+    D, n = sum(axes.dims), 50
+    w, b = (torch.randn(D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    p = dict(norm=norm, q_weight=w, k_weight=b, q_bias=b if norm == "layer_norm" else None, fold_softmax_scale=0.3)
+    for B, S, H, Hk in ((2, 2401, 24, 8), (1, 5003, 22, 5), (1, 3001, 45, None)):
+        q = torch.randn(B, S, H, D, generator=g).to(dtype).to(DEV)
+        k = None if Hk is None else torch.randn(B, S, Hk, D, generator=g).to(dtype).to(DEV)
+        pos = _positions(g, (B, S, len(axes.dims)), 3000)
+        whole = prepare_qk_axes(q, k, pos, axes, **p)
+        for at in (slice(0, n), slice(S // 2, S // 2 + n), slice(S - n, S)):
+            piece = prepare_qk_axes(q[:, at], None if k is None else k[:, at], pos[:, at], axes, **p)
+            assert torch.equal(whole[0][:, at], piece[0]) and (k is None or torch.equal(whole[1][:, at], piece[1]))
