@@ -8,7 +8,7 @@
 //
 // The merge is that of the 16-bit states: lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i, fp32 sums, one pass; a single
 // state is copied.  Bound by HBM: D + D / 32 + 4 bytes a row and 8-bit state instead of 2 D + 4.
-// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 108.6 us, 6.1 TB/s; one stored and loaded 55.0 us, 5.2 TB/s.
+// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 108.6 us, 6.1 TB/s; one stored and loaded 52.6 us, 5.4 TB/s.
 //
 // A lane owns 8 consecutive elements, so 4 lanes hold a block and its maximum is two exchanges inside a quad; a row's lanes are
 // neighbours in a wavefront.  States come sorted by the size of their elements, each size in batches whose loads are in flight together.
@@ -215,25 +215,23 @@ __device__ __forceinline__ void store(KernArgs& a, int64_t elem, bool live, int6
     const int n = (int)(top >> 23) - 127;
     const int e = max(n - (int8 ? 6 : 8) + ((top & 0x7fffffu) > (int8 ? 0x7e0000u : 0x600000u) ? 1 : 0), -127);
     const float inv = finite ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = finite ? x[i] * inv : 0.f;
     u32x2 w;
     if (int8) {
+      // 1.5 2^23 added, a float's lowest bits are the nearest even integer
+      uint32_t v[8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t v = 0;
+      for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__builtin_fmaf(x[i], inv, 12582912.f));
 #pragma unroll
-        for (int b = 0; b < 4; ++b) v |= ((uint32_t)(int32_t)__builtin_rintf(y[4 * i + b]) & 0xffu) << (8 * b);
-        w[i] = v;
-      }
+      for (int i = 0; i < 2; ++i)
+        w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(v[4 * i + 3], v[4 * i + 2], 0x0c0c0400u), __builtin_amdgcn_perm(v[4 * i + 1], v[4 * i], 0x0c0c0400u), 0x05040100u);
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        int v = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], v, true);
+        const int v = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+        w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, v, true);
       }
     }
+    if (!finite) w = u32x2{0u, 0u};
     __builtin_nontemporal_store(w, reinterpret_cast<u32x2*>(p + elem));
     if ((threadIdx.x & 3) == 0) a.dst_scales[elem / kBlock] = finite ? (uint8_t)(e + 127) : 255;
   }
@@ -285,8 +283,8 @@ __global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs 
   if (live && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
 }
 
-// One state into another format, its lse bit for bit.  From kManyWorkgroups workgroups on, with twice the elements each: a state of 14 882 x 24
-// heads of 128 stored and loaded 62.2 -> 57.1 us (four times as many: 58.8).
+// One state into another format, its lse bit for bit.  From kManyWorkgroups workgroups on, with twice the elements each.  A state of 14 882 x 24 heads of
+// 128, int8, stored and loaded: 52.6 us (one unit a lane 54.0, four 54.7; with the lse in the rows' first lanes 56.0).
 constexpr unsigned kManyWorkgroups = 2048;
 constexpr int kCopyUnits = 2;
 // kUnits times kThreads lanes' elements a workgroup.
@@ -296,15 +294,23 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
   KernArgs& a = kernel_args();
   const RowIndex at = rows_of(a);
   const int64_t elems = (int64_t)at.rows * D, elem = first_elem<kUnits>();
+  // an lse in one layout on both sides is a flat range of its own, of which a workgroup moves what its elements' rows are in number
+  constexpr uint32_t kRows = kThreads * 8 * kUnits / D;
+  const bool flat = (a.bsh_mask & 1) == (a.dst_bsh ? 1u : 0u);
+  const uint32_t mine = (uint32_t)((elem - 8 * (int64_t)threadIdx.x) / D) + threadIdx.x;
+  const bool moves = flat && threadIdx.x < kRows && mine < at.rows;
   Raw<kBytes> r[kUnits];
   float l[kUnits];
   uint32_t bhs[kUnits];
+  if (moves) l[0] = a.lse[0][mine];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     const int64_t e = elem + u * (kThreads * 8), from = e < elems ? e : 0;
     load<kBytes>(a, 0, from, r[u]);
-    bhs[u] = bhs_of(at, (uint32_t)(from / D));
-    if (e % D == 0) l[u] = a.lse[0][a.bsh_mask & 1 ? (uint32_t)(from / D) : bhs[u]];
+    if (!flat) {
+      bhs[u] = bhs_of(at, (uint32_t)(from / D));
+      if (e % D == 0) l[u] = a.lse[0][a.bsh_mask & 1 ? (uint32_t)(from / D) : bhs[u]];
+    }
   }
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -316,8 +322,9 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
     for (int i = 0; i < 8; ++i) x[i] = -0.f;       // (-0 + -0 keeps its sign)
     add<kBytes>(r[u], a.kind_mask & 1, 1.f, x);
     store(a, e, live, elems, x);
-    if (live && e % D == 0) a.dst_lse[a.dst_bsh ? (uint32_t)(e / D) : bhs[u]] = l[u];
+    if (!flat && live && e % D == 0) a.dst_lse[a.dst_bsh ? (uint32_t)(e / D) : bhs[u]] = l[u];
   }
+  if (moves) a.dst_lse[mine] = l[0];
 }
 
 bool is_block(int dtype) { return dtype == DT_BLOCK_E4M3 || dtype == DT_BLOCK_INT8; }
