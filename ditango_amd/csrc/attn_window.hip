@@ -16,7 +16,7 @@
 // last one of an item adds up (few rows, with counters) or a kernel behind the launch.
 //
 // Large launches are bound by the package's power cap: 14 400 queries of 24 heads of 128 over 8 frames of 3600 of 57 600 keys and the first frame 4.73 ms, 1.21
-// PFLOP/s of visible pairs at 1.57 GHz, MFMAs busy 71 % of the cycles (a library product of 16384^3: 1.36 PFLOP/s); 48 heads of 64, 17 550 queries over 5 frames of 1350
+// PFLOP/s of visible pairs at 1.60 GHz, MFMAs busy 73 % of the cycles (a library product of 16384^3: 1.36 PFLOP/s); 48 heads of 64, 17 550 queries over 5 frames of 1350
 // 1.41 ms, 0.97 PFLOP/s (vector ALU 76 %).  Single tokens by HBM: 4 x 24 heads of 128 over 4160 keys 44.2 us, 4.6 TB/s with the launch.
 #include <algorithm>
 #include <cmath>
