@@ -8,7 +8,7 @@
 //
 // The merge is that of the 16-bit states: lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i, fp32 sums, one pass; a single
 // state is copied.  Bound by HBM: D + D / 32 + 4 bytes a row and 8-bit state instead of 2 D + 4.
-// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 108.6 us, 6.1 TB/s; one stored and loaded 52.6 us, 5.4 TB/s.
+// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 101.4 us, 6.5 TB/s; one stored and loaded 52.6 us, 5.4 TB/s.
 //
 // A lane owns 8 consecutive elements, so 4 lanes hold a block and its maximum is two exchanges inside a quad; a row's lanes are
 // neighbours in a wavefront.  States come sorted by the size of their elements, each size in batches whose loads are in flight together.
@@ -42,6 +42,7 @@ struct BlockArgs {
   float* dst_lse;
   int32_t dst_dtype, dst_bsh;
   RowIndex at;
+  Quotient by_h_tiles, by_s_tiles;      // tiles of rows (merges)
 };
 
 // The arguments where they arrive, in the kernarg segment: indexed in unrolled batches of a by-value parameter, the optimiser makes a private copy
@@ -119,20 +120,60 @@ __device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, fl
 struct Sums {
   float acc[8], m, den;
 };
+// Where a lane's elements are, and their row's lse: in the states' own memory, or of all states in the LDS (kRows values a state), where the workgroup
+// brings them while the first states' elements are on their way.
+constexpr int kWaves = kThreads / 64;
+template <int kRows>
+struct Place {
+  int64_t elem;
+  uint32_t row, bhs;
+  float* lses;                  // lse of state i at [i * kRows + mine]
+  int mine;
+  bool staged;
+  static constexpr int kAhead = 2;
+  float ahead[kAhead];          // of the states wave and wave + kWaves, row `lane` of the tile
+  uint32_t as_bsh, as_bhs;      // that row's place
+
+  __device__ __forceinline__ float brought(KernArgs& a, int i) const { return a.lse[i][(a.bsh_mask >> i) & 1 ? as_bsh : as_bhs]; }
+  __device__ __forceinline__ void begin(KernArgs& a, int wave, int lane) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = wave + k * kWaves;
+      if (i < a.n && lane < kRows) ahead[k] = brought(a, i);
+    }
+  }
+  __device__ __forceinline__ void stage(KernArgs& a) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (lane < kRows) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (wave + k * kWaves < a.n) lses[(wave + k * kWaves) * kRows + lane] = ahead[k];
+      for (int i = wave + kAhead * kWaves; i < a.n; i += kWaves) lses[i * kRows + lane] = brought(a, i);
+    }
+    // (the elements stay on their way: a __syncthreads() would wait for them)
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    staged = true;
+  }
+};
 
 // NB states' loads are in flight together, and nothing between them and the folding branches: behind a branch on the lse the compiler would issue
 // the other loads after the lse's have come.
-template <int kBytes, int NB>
-__device__ __forceinline__ void batch(int i0, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+template <int kBytes, int NB, int kRows>
+__device__ __forceinline__ void batch(int i0, Place<kRows>& at, Sums& s) {
   KernArgs& a = kernel_args();
   Raw<kBytes> r[NB];
   float l[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    l[j] = a.lse[i0 + j][(a.bsh_mask >> (i0 + j)) & 1 ? row : bhs];
-    load<kBytes>(a, i0 + j, elem, r[j]);
+    if constexpr (kRows == 0) l[j] = a.lse[i0 + j][(a.bsh_mask >> (i0 + j)) & 1 ? at.row : at.bhs];
+    load<kBytes>(a, i0 + j, at.elem, r[j]);
   }
   __builtin_amdgcn_sched_barrier(0);
+  if constexpr (kRows > 0) {
+    if (!at.staged) at.stage(a);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) l[j] = at.lses[(i0 + j) * kRows + at.mine];
+  }
   const uint32_t kinds = (uint32_t)(a.kind_mask >> i0);
   float m = s.m;
 #pragma unroll
@@ -150,17 +191,17 @@ __device__ __forceinline__ void batch(int i0, int64_t elem, uint32_t row, uint32
   }
   s.m = m;
 }
-template <int kBytes, int NB>
-__device__ __forceinline__ void rest(int i0, int n, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
+template <int kBytes, int NB, int kRows>
+__device__ __forceinline__ void rest(int i0, int n, Place<kRows>& at, Sums& s) {
   if constexpr (NB >= 1) {
-    if (n == NB) batch<kBytes, NB>(i0, elem, row, bhs, s);
-    else rest<kBytes, NB - 1>(i0, n, elem, row, bhs, s);
+    if (n == NB) batch<kBytes, NB>(i0, at, s);
+    else rest<kBytes, NB - 1>(i0, n, at, s);
   }
 }
-template <int kBytes, int kBatch>
-__device__ __forceinline__ void states(int i0, int i1, int64_t elem, uint32_t row, uint32_t bhs, Sums& s) {
-  for (; i0 + kBatch <= i1; i0 += kBatch) batch<kBytes, kBatch>(i0, elem, row, bhs, s);
-  rest<kBytes, kBatch - 1>(i0, i1 - i0, elem, row, bhs, s);
+template <int kBytes, int kBatch, int kRows>
+__device__ __forceinline__ void states(int i0, int i1, Place<kRows>& at, Sums& s) {
+  for (; i0 + kBatch <= i1; i0 += kBatch) batch<kBytes, kBatch>(i0, at, s);
+  rest<kBytes, kBatch - 1>(i0, i1 - i0, at, s);
 }
 
 // The other lanes of a quad: lane ^ 1, lane ^ 2.
@@ -237,15 +278,17 @@ __device__ __forceinline__ void store(KernArgs& a, int64_t elem, bool live, int6
   }
 }
 
-// The first element of this lane.  The lse of consecutive queries share a line of the [B,H,Sq] layout, and workgroups go to the 8 XCDs in turn: so
+// This workgroup's place, and the first element of this lane.  The lse of consecutive queries share a line of the [B,H,Sq] layout, and workgroups go to the 8 XCDs in turn: so
 // that a line is read into one L2 only, kGroup workgroups that follow each other in memory are of one XCD.
 constexpr int kGroup = 64;
+__device__ __forceinline__ uint32_t workgroup() {
+  const uint32_t wg = blockIdx.x;
+  constexpr uint32_t kSpan = 8 * kGroup;
+  return (wg / kSpan + 1) * kSpan <= gridDim.x ? wg / kSpan * kSpan + (wg & 7u) * kGroup + (wg % kSpan >> 3) : wg;
+}
 template <int kUnits>
 __device__ __forceinline__ int64_t first_elem() {
-  uint32_t wg = blockIdx.x;
-  constexpr uint32_t kSpan = 8 * kGroup;
-  if ((wg / kSpan + 1) * kSpan <= gridDim.x) wg = wg / kSpan * kSpan + (wg & 7u) * kGroup + (wg % kSpan >> 3);
-  return ((int64_t)wg * (kThreads * kUnits) + threadIdx.x) * 8;
+  return ((int64_t)workgroup() * (kThreads * kUnits) + threadIdx.x) * 8;
 }
 
 __device__ __forceinline__ RowIndex rows_of(KernArgs& a) {
@@ -258,29 +301,63 @@ __device__ __forceinline__ RowIndex rows_of(KernArgs& a) {
   return at;
 }
 
-template <int D>
+// kTiles: a workgroup has the rows of kTileQueries queries and 512 / D heads, a wavefront one query's.  In the [B,H,Sq] layout the lse of neighbouring rows
+// are a sequence apart, and fetched by the rows' own lanes they cost as many requests as the elements; those of a tile come in 16-byte
+// runs, once for the four wavefronts, through the LDS.  us without and with: 14 882 x 24 heads of 128, 8 states of 8 bits 87.7 / 81.5, 6 and 2 of 16 bits
+// 111.8 / 104.8, 6 69.7 / 68.3, 2 38.4 / 42.2 (shorter runs of elements); heads of 64, 9000 x 48, 6 states 51.6 / 43.0, 2 25.5 / 24.8; 2222 x 48, 5 and 3 21.5 /
+// 18.5.  So heads of 64 always, heads of 128 from six states on.
+constexpr int kTileQueries = kThreads / 64;
+template <int D, bool kTiles>
 __global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs args_by_value) {
   (void)args_by_value;
+  constexpr int kHeads = 512 / D, kRows = kTiles ? kTileQueries * kHeads : 0;
   KernArgs& a = kernel_args();
   const RowIndex at = rows_of(a);
-  const int64_t elems = (int64_t)at.rows * D, elem = first_elem<1>();
-  const bool live = elem < elems;
-  const int64_t from = live ? elem : 0;          // (lanes behind the last row read the first one's and store nothing)
-  const uint32_t row = (uint32_t)(from / D), bhs = bhs_of(at, row);
+  const int64_t elems = (int64_t)at.rows * D;
+  int64_t elem;
+  Place<kRows> place;
+  bool live;
+  if constexpr (kTiles) {
+    __shared__ float lses[DT_MAX_MERGE * kRows];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t wg = workgroup();
+    const Quotient by_h = {a.by_h_tiles.mul, a.by_h_tiles.shift}, by_s = {a.by_s_tiles.mul, a.by_s_tiles.shift};
+    const uint32_t h_tiles = (uint32_t)at.H / kHeads, s_tiles = ((uint32_t)at.Sq + kTileQueries - 1) / kTileQueries;
+    const uint32_t bs = quotient(wg, by_h), h0 = (wg - bs * h_tiles) * kHeads, b = quotient(bs, by_s), s0 = (bs - b * s_tiles) * kTileQueries;
+    // lane r of a wavefront brings row r of every fourth state: query r % kTileQueries, head r / kTileQueries
+    const uint32_t q = min(s0 + lane % kTileQueries, (uint32_t)at.Sq - 1), h = h0 + lane / kTileQueries;
+    place.as_bsh = (b * (uint32_t)at.Sq + q) * (uint32_t)at.H + h;
+    place.as_bhs = (b * (uint32_t)at.H + h) * (uint32_t)at.Sq + q;
+    place.begin(a, wave, lane);
+    const uint32_t s = s0 + wave, mine = lane / (D / 8);
+    live = s < (uint32_t)at.Sq;
+    place.row = (b * (uint32_t)at.Sq + min(s, (uint32_t)at.Sq - 1)) * (uint32_t)at.H + h0 + mine;
+    place.bhs = (b * (uint32_t)at.H + h0 + mine) * (uint32_t)at.Sq + min(s, (uint32_t)at.Sq - 1);
+    place.elem = elem = (int64_t)place.row * D + 8 * (lane % (D / 8));
+    place.lses = lses;
+    place.mine = kTileQueries * mine + wave;
+    place.staged = false;
+  } else {
+    elem = first_elem<1>();
+    live = elem < elems;
+    place.elem = live ? elem : 0;          // (lanes behind the last row read the first one's and store nothing)
+    place.row = (uint32_t)(place.elem / D);
+    place.bhs = bhs_of(at, place.row);
+  }
   Sums s;
 #pragma unroll
   for (int e = 0; e < 8; ++e) s.acc[e] = 0.f;
   s.m = -INFINITY;
   s.den = 0.f;
-  states<1, 4>(0, a.n8, from, row, bhs, s);
-  states<2, 4>(a.n8, a.n16, from, row, bhs, s);
-  states<4, 2>(a.n16, a.n, from, row, bhs, s);
+  states<1, 4>(0, a.n8, place, s);
+  states<2, 4>(a.n8, a.n16, place, s);
+  states<4, 2>(a.n16, a.n, place, s);
   const float inv = s.den != 0.f ? 1.f / s.den : 0.f;
   float x[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = s.acc[e] * inv;
-  store(a, elem, live, elems, x);
-  if (live && elem % D == 0) a.dst_lse[a.dst_bsh ? row : bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
+  store(a, elem, live, live ? elems : kTiles ? 0 : elems, x);
+  if (live && elem % D == 0) a.dst_lse[a.dst_bsh ? place.row : place.bhs] = s.den != 0.f ? s.m + __logf(s.den) : -INFINITY;
 }
 
 // One state into another format, its lse bit for bit.  From kManyWorkgroups workgroups on, with twice the elements each.  A state of 14 882 x 24 heads of
@@ -404,9 +481,18 @@ extern "C" int dt_merge_block_states(int32_t n, const dt_state* states, const dt
     if (some) hipLaunchKernelGGL((copy_blocks_kernel<D, bytes, kCopyUnits>), fewer, block, 0, st, a);         \
     else DT_LAUNCH((copy_blocks_kernel<D, bytes, 1>));                                                        \
   } while (0)
-  if (n > 1) {
-    if (D == 128) DT_LAUNCH((merge_blocks_kernel<128>));
-    else DT_LAUNCH((merge_blocks_kernel<64>));
+  const int heads = 512 / D;
+  const uint64_t all = n == 64 ? ~0ull : (1ull << n) - 1;
+  const int s_tiles = (Sq - 1) / kTileQueries + 1;
+  if (n >= (D == 64 ? 2 : 6) && H % heads == 0 && Sq >= 16 && a.bsh_mask != all && (int64_t)B * s_tiles * (H / heads) < 1 << 24) {
+    a.by_h_tiles = quotient_by(H / heads);
+    a.by_s_tiles = quotient_by(s_tiles);
+    const dim3 tiles((unsigned)((int64_t)B * s_tiles * (H / heads)));
+    if (D == 128) hipLaunchKernelGGL((merge_blocks_kernel<128, true>), tiles, block, 0, st, a);
+    else hipLaunchKernelGGL((merge_blocks_kernel<64, true>), tiles, block, 0, st, a);
+  } else if (n > 1) {
+    if (D == 128) DT_LAUNCH((merge_blocks_kernel<128, false>));
+    else DT_LAUNCH((merge_blocks_kernel<64, false>));
   } else {
     const int bytes = element_bytes(states[0].dtype);
     if (D == 128) {

@@ -263,3 +263,37 @@ def test_more_than_2_to_the_31_elements(hip, fmt):
         piece = quantized(o, l, fmt)
         for whole, want in ((both, merge_any([piece, (o, l)], dst_dtype=torch.bfloat16)), (back, merge_any([piece], dst_dtype=torch.bfloat16))):
             assert torch.equal(whole[0][:, at], want[0]) and torch.equal(whole[1][:, :, at], want[1])
+
+
+@pytest.mark.parametrize("bsh", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kinds", ["e4m3 int8", "int8 bf16 f32 e4m3 int8 fp16", " ".join(["int8", "bf16", "e4m3"] * 13), " ".join(["e4m3"] * 64), " ".join(["f32"] * 7 + ["int8"] * 60)],
+                         ids=["two", "six", "39", "64", "67"])
+def test_merge_of_heads_in_tiles(hip, kinds, D, bsh):
+    """Heads and queries in tiles, whose lse come together: queries that do not fill the last one, lse in both layouts, more states than a launch takes."""
+    from ditango_amd.core.cache import BlockState, merge_any
+    g = torch.Generator().manual_seed(len(kinds) + D)
+    types = {"bf16": torch.bfloat16, "fp16": torch.float16, "f32": torch.float32}
+    for B, S, H in ((2, 37, 8), (1, 18, 24), (3, 16, 16)):
+        states, want = [], []
+        for i, kind in enumerate(kinds.split()):
+            o, l = _state(g, B, S, H, D, types.get(kind, torch.float32), 0.3)
+            if i % 3 == 1:
+                l[0, 0] = -math.inf
+            l[:, :, 5] = -math.inf
+            if kind in FORMATS:
+                state = BlockState.empty((B, S, H, D), kind, DEV)
+                merge_any([(o, l)], dst=state)
+                states.append(state)
+                want.append((L.value(state.elements.cpu(), state.scales.cpu().int() - 127), l.cpu()))
+            else:
+                states.append((o, l) if i % 2 else (o, l.transpose(1, 2).unsqueeze(-1).contiguous()))
+                want.append((o.cpu(), l.cpu()))
+        got, lse = merge_any(states, dst_dtype=torch.bfloat16, dst_lse_bsh=bsh)
+        _check_merge(got, lse.squeeze(-1).transpose(1, 2) if bsh else lse, want, torch.bfloat16)
+        if isinstance(states[0], BlockState):
+            first = states[0]
+            again, again_lse = merge_any(states, dst_dtype=torch.float32)
+            merge_any(states, dst=first)
+            assert torch.equal(first.lse, again_lse)
+            _exact(first, again)

@@ -34,7 +34,7 @@ def test_windowed_attention(resources):
         assert r["Occupancy [waves/SIMD]"] == (2 if "ILi128E" in name else 4), (name, r)
 
 
-@pytest.mark.parametrize("fragment, n", [("attn_window_fold_kernel", 4), ("merge_blocks_kernel", 2), ("copy_blocks_kernel", 12), ("qk_norm_rope_axes_kernel", 32)])
+@pytest.mark.parametrize("fragment, n", [("attn_window_fold_kernel", 4), ("merge_blocks_kernel", 4), ("copy_blocks_kernel", 12), ("qk_norm_rope_axes_kernel", 32)])
 def test_streaming_kernels_use_no_scratch(resources, fragment, n):
     for name, r in _kernels(resources, fragment, n).items():
         assert r["ScratchSize [bytes/lane]"] == 0 and r["VGPRs Spill"] == 0, (name, r)
