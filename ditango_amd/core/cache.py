@@ -70,8 +70,9 @@ def _parts(state):
 
 def merge_any(states, *, dst=None, dst_dtype: torch.dtype = torch.float32, dst_lse_bsh: bool = False):
     """N-way LSE merge of states of any format: each a ``BlockState`` or ``(out, lse)`` with out contiguous ``[B,S,H,D]`` (bf16, fp16, fp32) and
-    lse fp32 in ``[B,H,S]`` or ``[B,S,H(,1)]`` storage (three dimensions that fit both are the former).  One pass over HBM for up to ``DT_MAX_MERGE`` states; a single one is copied.  Into ``dst`` --
-    a ``BlockState`` or ``(out, lse)``, one of the states among them -- or a new ``(out, lse)`` of ``dst_dtype``.  Returns the destination."""
+    lse fp32 in ``[B,H,S]`` or ``[B,S,H(,1)]`` storage (three dimensions that fit both are the former).  One pass over HBM for up to
+    ``DT_MAX_MERGE`` states; a single one is copied.  Into ``dst`` -- a ``BlockState`` or ``(out, lse)``, one of the states among them -- or a new
+    ``(out, lse)`` of ``dst_dtype``.  Returns the destination."""
     if not states:
         raise ValueError("need at least one state")
     out, _, lse = _hip.merge_blocks([_parts(s) for s in states], None if dst is None else _parts(dst), dst_dtype, dst_lse_bsh)
