@@ -332,7 +332,7 @@ struct Loader {
   typedef Tiles<D, NKB> T;
   const uint16_t *k, *v;       // of this batch and key head
   int64_t k_ss, v_ss;
-  uint32_t k_off, v_off;       // lane's bytes within block 0
+  uint32_t k_row, k_chunk, v_off;     // lane's bytes within block 0; of K the row's and, apart from them, those inside the row
 
   __device__ __forceinline__ void open(const WindowArgs& a, int b, int hk, int lane) {
     k = a.k + b * a.k_sb + hk * a.k_sh;
@@ -340,7 +340,8 @@ struct Loader {
     k_ss = a.k_ss;
     v_ss = a.v_ss;
     const int row = lane / T::kRowLanes, chunk = lane % T::kRowLanes;
-    k_off = row * (uint32_t)(2 * k_ss) + 16 * (chunk ^ T::swz_k(row));
+    k_row = row * (uint32_t)(2 * k_ss);
+    k_chunk = 16 * (chunk ^ T::swz_k(row));
     v_off = row * (uint32_t)(2 * v_ss) + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
   }
   // Bytes of a tile in front of key `left` of the sample's: rows behind the last key arrive as zeros.
@@ -351,21 +352,24 @@ struct Loader {
   // that no offset needs more than 32 bits however long the cache is.  (The row is part of the lane's offset: a scalar offset beyond the
   // descriptor's end would wrap its range check.)
   template <int kCount>
-  __device__ __forceinline__ void issue(const uint16_t* from, uint32_t valid, uint32_t off, uint32_t flip, uint32_t row, int b0, int step, uint32_t to) const {
+  __device__ __forceinline__ void issue_k(const uint16_t* from, uint32_t valid, int b0, int step, uint32_t to) const {
     const u32x4 r = make_rsrc(from, valid);
 #pragma unroll
     for (int i = 0; i < kCount; ++i) {
       const int blk = b0 + i * step;
-      load_block_to_lds(r, (off ^ (64u * (blk & flip))) + blk * T::kBlockRows * row, 0, to + blk * 1024);
+      // (the block permutes the chunks of a row, whose own place may have any multiple of 16 bytes in it)
+      const uint32_t chunk = k_chunk ^ (64u * (blk & T::kBlockXor));
+      load_block_to_lds(r, k_row + chunk + blk * T::kBlockRows * (2 * (uint32_t)k_ss), 0, to + blk * 1024);
     }
   }
   template <int kCount>
-  __device__ __forceinline__ void issue_k(const uint16_t* from, uint32_t valid, int b0, int step, uint32_t to) const {
-    issue<kCount>(from, valid, k_off, T::kBlockXor, 2 * (uint32_t)k_ss, b0, step, to);
-  }
-  template <int kCount>
   __device__ __forceinline__ void issue_v(const uint16_t* from, uint32_t valid, int b0, int step, uint32_t to) const {
-    issue<kCount>(from, valid, v_off, 0u, 2 * (uint32_t)v_ss, b0, step, to);
+    const u32x4 r = make_rsrc(from, valid);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const int blk = b0 + i * step;
+      load_block_to_lds(r, v_off + blk * T::kBlockRows * (2 * (uint32_t)v_ss), 0, to + blk * 1024);
+    }
   }
 };
 
