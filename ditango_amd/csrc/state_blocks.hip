@@ -79,7 +79,7 @@ __device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, fl
   float x[8];
   if constexpr (kBytes == 1) {
     w = there ? w * scale_of(r.scale) : 0.f;       // (the scale may be infinite)
-    const uint32_t word[2] = {r.x.x, r.x.y};
+    const uint32_t word[2] = {there ? r.x.x : 0u, there ? r.x.y : 0u};     // (e4m3 has undefined elements of its own)
     if (kind) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = (float)((int32_t)(word[e / 4] << (24 - 8 * (e % 4))) >> 24);
@@ -307,8 +307,10 @@ __device__ __forceinline__ RowIndex rows_of(KernArgs& a) {
 // 111.8 / 104.8, 6 69.7 / 68.3, 2 38.4 / 42.2 (shorter runs of elements); heads of 64, 9000 x 48, 6 states 51.6 / 43.0, 2 25.5 / 24.8; 2222 x 48, 5 and 3 21.5 /
 // 18.5.  So heads of 64 always, heads of 128 from six states on.
 constexpr int kTileQueries = kThreads / 64;
+// (seven wavefronts a SIMD, but for tiles of heads of 128, which take 76 registers: left to itself the compiler takes 74 for heads of 64 and six fit, 17.9 -> 18.5 us for 5 + 3
+// states of 2222 x 48 heads)
 template <int D, bool kTiles>
-__global__ __launch_bounds__(kThreads) void merge_blocks_kernel(const BlockArgs args_by_value) {
+__global__ __launch_bounds__(kThreads, D == 128 && kTiles ? 6 : 7) void merge_blocks_kernel(const BlockArgs args_by_value) {
   (void)args_by_value;
   constexpr int kHeads = 512 / D, kRows = kTiles ? kTileQueries * kHeads : 0;
   KernArgs& a = kernel_args();
