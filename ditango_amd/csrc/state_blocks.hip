@@ -72,10 +72,10 @@ __device__ __forceinline__ void load(KernArgs& a, int i, int64_t elem, Raw<kByte
   }
 }
 
-// acc += w x; a weight of 0 leaves x out, whatever it is
+// acc += w x.  A state that is not there (an lse of -inf) is left out, whatever it holds.  The weight of one that is there is above 0, so its undefined
+// values stay undefined, also where fp32 has no number for the weight: in whatever order the states come.
 template <int kBytes>
-__device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, float w, float (&acc)[8]) {
-  const bool there = w != 0.f;
+__device__ __forceinline__ void add(const Raw<kBytes>& r, bool kind, bool there, float w, float (&acc)[8]) {
   float x[8];
   if constexpr (kBytes == 1) {
     w = there ? w * scale_of(r.scale) : 0.f;       // (the scale may be infinite)
@@ -187,7 +187,7 @@ __device__ __forceinline__ void batch(int i0, Place<kRows>& at, Sums& s) {
   for (int j = 0; j < NB; ++j) {
     const float w = __expf(l[j] - top);
     s.den += w;
-    add<kBytes>(r[j], (kinds >> j) & 1, w, s.acc);
+    add<kBytes>(r[j], (kinds >> j) & 1, l[j] != -INFINITY, w, s.acc);
   }
   s.m = m;
 }
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void copy_blocks_kernel(const BlockArgs a
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = -0.f;       // (-0 + -0 keeps its sign)
-    add<kBytes>(r[u], a.kind_mask & 1, 1.f, x);
+    add<kBytes>(r[u], a.kind_mask & 1, true, 1.f, x);
     store(a, e, live, elems, x);
     if (!flat && live && e % D == 0) a.dst_lse[a.dst_bsh ? (uint32_t)(e / D) : bhs[u]] = l[u];
   }

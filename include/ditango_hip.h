@@ -582,7 +582,8 @@ int dt_attn_window_fwd(const void* q, const void* k, const void* v, void* out, f
  * out is [B,Sq,H,D] contiguous, 16-byte aligned.  DT_BLOCK_E4M3 (OCP e4m3) and DT_BLOCK_INT8 have scales uint8 [B,Sq,H,D/32], one for every 32
  * elements along D: value = element * 2^(scale - 127), with the smallest scale for which no magnitude of the block is above the largest
  * element (448, 127), and elements rounded to nearest even.  A block that holds an infinite or undefined value has scale 255 and reads as NaN.
- * The other dtypes take scales = NULL.  States whose lse is -inf contribute nothing, whatever they hold.  dst may be one of the states (the
+ * The other dtypes take scales = NULL.  States whose lse is -inf contribute nothing, whatever they hold; what an infinite or undefined value of any other
+ * goes into is not finite, however small its weight and whatever the order of the states.  dst may be one of the states (the
  * same pointers, dtype and layout).  states is a HOST array; n <= DT_MAX_MERGE.
  */
 typedef struct {

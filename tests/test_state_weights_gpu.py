@@ -43,3 +43,34 @@ def test_memory_that_nobody_wrote_adds_nothing_without_weight(hip, B, S, H, n, D
                      torch.where(blank[..., None], torch.zeros((), dtype=torch.int32, device=DEV), some.scales.int() - 127).cpu())
     out, lse = merge_any(given + [some], dst_dtype=torch.bfloat16)
     _check_merge(out, lse, [(o.cpu(), l.cpu()) for o, l in given] + [(values, some.lse.cpu())], torch.bfloat16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D, H", [(64, 8), (128, 8), (64, 3)])        # in tiles (heads of 128 from six states on), and row by row
+@pytest.mark.parametrize("behind", [0.0, 40.0, 90.0, 120.0, 400.0])
+def test_undefined_values_are_seen_in_any_order(hip, behind, D, H, fmt):
+    """One state of many holds an infinity and a NaN and lies ``behind`` the others in its lse, beyond what fp32 has a weight for: wherever it comes among them,
+    these elements are not finite and all others are what they are without it."""
+    from ditango_amd.core.cache import BlockState, merge_any, quantized
+    g = torch.Generator().manual_seed(int(behind) + D)
+    B, S = 1, 18
+    for kind in (fmt, "bf16", "f32"):
+        for n in (1, 5, 9, 66):
+            others = [_state(g, B, S, H, D, (torch.bfloat16, torch.float32)[i % 2], 0.3) for i in range(n)]
+            others = [(o, l + 3.0 * i) for i, (o, l) in enumerate(others)]      # the largest lse comes late
+            others = [quantized(o, l, fmt) if i % 3 == 2 else (o, l) for i, (o, l) in enumerate(others)]
+            o, l = _state(g, B, S, H, D, torch.float32, 0.3)
+            l = torch.stack([s.lse if isinstance(s, BlockState) else s[1] for s in others]).amax(0) - behind
+            o[0, 3, 1, 7], o[0, 11, 2, D - 1] = math.inf, math.nan
+            odd = quantized(o, l, fmt) if kind in FORMATS else (o.to(dict(bf16=torch.bfloat16, f32=torch.float32)[kind]), l)
+            bad = ~o.isfinite()
+            if kind in FORMATS:                                # the whole block reads as NaN
+                bad = bad.unflatten(-1, (-1, 32)).any(-1, keepdim=True).expand(-1, -1, -1, -1, 32).flatten(-2)
+            clean = torch.where(bad, torch.zeros_like(o), o)
+            clean = quantized(clean, l, fmt) if kind in FORMATS else (clean.to(odd[0].dtype), l)
+            for at in sorted({0, n // 2, n}):
+                put = lambda s: others[:at] + [s] + others[at:]
+                got, lse = merge_any(put(odd), dst_dtype=torch.float32)
+                want, want_lse = merge_any(put(clean), dst_dtype=torch.float32)
+                assert torch.equal(got.isfinite(), ~bad), (kind, n, at)
+                assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse, want_lse)
