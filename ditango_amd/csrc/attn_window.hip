@@ -1123,6 +1123,8 @@ int launch_dim(WindowArgs& a, int64_t units, int n_cus, void* workspace, int64_t
   }
   if (plan.form == 0 || kXcds * plan.tail > n_counters) a.counters = nullptr;
   const unsigned grid = (unsigned)(kXcds * (a.tail_start + a.tail * a.ways));
+  std::unique_lock<std::mutex> lock;
+  if (a.ways > 1) lock = std::unique_lock<std::mutex>(workspace_lock(workspace));
   const int rc = plan.form == 0   ? launch<attn_window_kernel<D, kHalf>>(a, grid, kWavesShared, SharedLds<D>::kBytes, stream)
                  : plan.form == 1 ? launch<attn_window_few_kernel<D, kHalf, 8>>(a, grid, 8, FewLds<D, 8>::kAll, stream)
                                   : launch<attn_window_few_kernel<D, kHalf, 4>>(a, grid, 4, FewLds<D, 4>::kAll, stream);
