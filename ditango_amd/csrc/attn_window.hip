@@ -903,9 +903,8 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_window_few_kerne
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D, W>::kTile) + lane * 4 + q * 256);
-      if (w[j] != 0.f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);
+      for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(w[j], x[e], sum[e]);     // (a weight of 0 keeps what is undefined: some row's visible key is)
     }
     if (!live) continue;
     if (it.ways > 1) {

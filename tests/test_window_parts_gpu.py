@@ -43,3 +43,35 @@ def test_threads_that_launch_on_one_stream_share_its_workspace(hip):
         for i in range(2):
             o0, l0 = want[pair[i]]
             assert len(got[i]) == 60 and all(torch.equal(o, o0) and torch.equal(l, l0) for o, l in got[i])
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq, Sk, H, Hk", [(1, 256, 4, 4), (33, 300, 2, 1), (1, 30000, 2, 2), (9, 4000, 4, 2), (400, 410, 48, 1), (2100, 2100, 66, 66)])
+def test_undefined_values_of_keys_far_below_the_others_are_seen(hip, Sq, Sk, H, Hk, D, captured):
+    """Keys whose weight fp32 has no number for beside the others': their infinite and undefined values are those of visible keys all the same, whichever wavefront or part
+    has the keys, and no other element changes."""
+    from ditango_amd.window import window_attention
+    q, k, v = _tensors(1, Sq, Sk, H, Hk, D, torch.bfloat16, seed=31, sigma=0.5)
+    q += 4.0
+    k[:, :Sk // 2] -= 32.0                       # scores of -4 x 32 sqrt(D), beside some units
+    odd = v.clone()
+    odd[0, 5, 0, 3], odd[0, Sk // 2 - 1, Hk - 1, D - 2] = math.inf, math.nan
+    run = lambda x: window_attention(q, k, x)
+    clean, clean_lse = run(v)
+    if captured:
+        run(odd)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, lse = run(odd)
+        graph.replay()
+    else:
+        out, lse = run(odd)
+    torch.cuda.synchronize()
+    bad = torch.zeros(1, 1, H, D, dtype=torch.bool, device=DEV)
+    bad[0, 0, :H // Hk, 3] = True
+    bad[0, 0, H - H // Hk:, D - 2] = True
+    assert torch.equal(out.isfinite(), (~bad).expand_as(out))
+    if not captured:                             # (a captured launch adds its parts up in another order)
+        assert torch.equal(lse, clean_lse) and torch.equal(out[:, :, ~bad[0, 0]], clean[:, :, ~bad[0, 0]])
