@@ -536,13 +536,22 @@ class proAttention:
         B, Sq, H, D = query.shape
         cache = self.cache
         row = rm.chunk_mask[t, l]
-        have_arena = cache.ensure_arena(C, B, Sq, H, D, query.device)
-        compute = ([diag] if 0 <= diag < C else []) + [c for c in range(C) if c != diag and (row[c] == 0 or not have_arena)]
+        local = self.local_chunk_id if (self.local_chunk_id == diag and key is not None) else -1
+        if not cache.ensure_arena(C, B, Sq, H, D, query.device):
+            # no memory for the states: none of each chunk's own is made either, all chunks are one job
+            if self._exact_f32:
+                out, self.last_lse = merge_any(self._job_states_f32(query, [tuple(range(C))], key if local >= 0 else None, value), dst_dtype=self.out_dtype,
+                                               dst_lse_bsh=True)
+            else:
+                kv = [(key, value) if c == local else self.group.kv_chunk(c) for c in range(C)]
+                out = self._attn_uncached(query, [_as4d(k, B) for k, _ in kv], [_as4d(v, B) for _, v in kv])
+            rm.record_out_redundancy(timestep=t, layer_id=l, curr_out=out)
+            return out
+        compute = ([diag] if 0 <= diag < C else []) + [c for c in range(C) if c != diag and row[c] == 0]
         reuse = [c for c in range(C) if c not in compute]
         for c in reuse:
             if not cache.arena_valid[c]:
                 raise RuntimeError(f"T{t}L{l}: mask asks to reuse chunk {c} but no state was ever stored for it")
-        local = self.local_chunk_id if (self.local_chunk_id == diag and key is not None) else -1
         if not compute:
             fresh = []
         elif self._exact_f32:
@@ -559,11 +568,10 @@ class proAttention:
                                      self._MAX_JOB_CHUNKS, _hip.attn_workspace(query.device), self.q_prescaled, cu_q, cu_kv, dev_seg,
                                      _kernel_input)
         out, lse = merge_any([cache.arena_block(c) for c in reuse] + list(fresh), dst_dtype=self.out_dtype, dst_lse_bsh=True)
-        if have_arena:
-            for c, state in zip(compute, fresh):
-                if c != diag:
-                    merge_any([state], dst=cache.arena_block(c))
-                    cache.arena_valid[c] = True
+        for c, state in zip(compute, fresh):
+            if c != diag:
+                merge_any([state], dst=cache.arena_block(c))
+                cache.arena_valid[c] = True
         self.last_lse = lse
         rm.record_out_redundancy(timestep=t, layer_id=l, curr_out=out)
         return out
