@@ -37,7 +37,7 @@ from .. import _hip
 from ..logger import init_logger
 from ..timer import get_timer
 from ..utils import get_timestep
-from .cache import merge_any, merge_cached, proCache
+from .cache import BlockState, merge_any, merge_cached, proCache
 from .config import get_config
 from .parallel_state import LocalRingGroup
 from .redundancy_map import get_redundancy_map
@@ -408,14 +408,40 @@ class proAttention:
             states, out, lse = _hip.attn_states_merge(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, merge_outs, merge_lses, which, self.out_dtype,
                                                       workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
         else:
-            states = _hip.attn_states(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
-            fresh = [states[i] for i in which]
-            out, lse = merge_cached(merge_outs + [o for o, _ in fresh], merge_lses + [l for _, l in fresh], self.out_dtype)
+            slots = {i: job.store_slot for job, i in zip(plan.jobs, which) if job.store_slot is not None}
+            cached = [o if isinstance(o, BlockState) else (o, l) for o, l in zip(merge_outs, merge_lses)]
+            out, lse = self._merge_quantized(
+                query, cached, len(jobs), which,
+                lambda part: _hip.attn_states(query, ks, vs, [jobs[i] for i in part], self._MAX_JOB_CHUNKS, workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input),
+                lambda i, state: self.cache.store_block(slots[i], *state) if i in slots else None, len(slots),
+                lambda parts: merge_any(parts, dst_dtype=self.out_dtype, dst_lse_bsh=True) if any(isinstance(p, BlockState) for p in parts)
+                else _hip.merge_states([o for o, _ in parts], [l for _, l in parts], dst_dtype=self.out_dtype, dst_lse_bsh=True))
+            self.last_lse = lse
+            return out
         for job, i in zip(plan.jobs, which):
             if job.store_slot is not None:
                 self.cache.store_block(job.store_slot, *states[i])  # :207-211
         self.last_lse = lse
         return out
+
+    def _merge_quantized(self, query, cached, n: int, which, states_of, keep, kept: int, merge):
+        """(out, lse [B,S,H,1]) of the cached states, ``BlockState`` or ``(out, lse)``, and of the fresh states ``which[..]`` of ``n`` jobs, under a ``state_format``.
+        ``states_of(jobs)`` computes fresh ones, ``keep(job, state)`` quantises one into the cache, ``kept`` of them into new memory.  All of them at once, and one
+        ``merge``, unless the memory budget has no room for that: then in groups that one fp32 state takes up in turn (its sums are rounded once more a group)."""
+        parts, run = list(cached), None
+        at_once = self.cache.fresh_at_once(n, *query.shape, query.dtype.itemsize, kept) if n else 1
+        for first in range(0, max(n, 1), at_once):
+            jobs = range(first, min(first + at_once, n))
+            states = dict(zip(jobs, states_of(jobs))) if n else {}
+            parts += [states[i] for i in which if i in states]
+            if jobs.stop < n or (run is not None and self.out_dtype is torch.float32):
+                run = merge_any(parts, dst=run, dst_lse_bsh=True)
+            else:
+                run = merge(parts)
+            for i, state in states.items():
+                keep(i, state)
+            parts, states, state = [run], None, None         # (the group's states are gone before the next one's are made)
+        return run
 
     # ---- mask mode ----------------------------------------------------------------------------------
     def _attn_masked(self, query, key, value) -> torch.Tensor:
@@ -537,7 +563,7 @@ class proAttention:
         cache = self.cache
         row = rm.chunk_mask[t, l]
         local = self.local_chunk_id if (self.local_chunk_id == diag and key is not None) else -1
-        if not cache.ensure_arena(C, B, Sq, H, D, query.device):
+        if not cache.ensure_arena(C, B, Sq, H, D, query.device, fresh_bytes=query.dtype.itemsize):
             # no memory for the states: none of each chunk's own is made either, all chunks are one job
             if self._exact_f32:
                 out, self.last_lse = merge_any(self._job_states_f32(query, [tuple(range(C))], key if local >= 0 else None, value), dst_dtype=self.out_dtype,
@@ -553,25 +579,27 @@ class proAttention:
             if not cache.arena_valid[c]:
                 raise RuntimeError(f"T{t}L{l}: mask asks to reuse chunk {c} but no state was ever stored for it")
         if not compute:
-            fresh = []
+            states_of = None
         elif self._exact_f32:
-            fresh = self._job_states_f32(query, [(c,) for c in compute], key if local >= 0 else None, value)
+            states_of = lambda part: self._job_states_f32(query, [(compute[i],) for i in part], key if local >= 0 else None, value)
         else:
             kv = [(key, value) if c == local else self.group.kv_chunk(c) for c in compute]
+            ks, vs = [_as4d(k, B) for k, _ in kv], [_as4d(v, B) for _, v in kv]
             cu_q = cu_kv = dev_seg = None
             if isinstance(self._segments, _DeviceSegmentSource):
                 dev_seg = self._segments.over(compute)
             elif self._segments is not None:
                 cu_q, cu_kv_of = self._segments
                 cu_kv = [cu_kv_of(c) for c in compute]
-            fresh = _hip.attn_states(query, [_as4d(k, B) for k, _ in kv], [_as4d(v, B) for _, v in kv], [[i] for i in range(len(compute))],
-                                     self._MAX_JOB_CHUNKS, _hip.attn_workspace(query.device), self.q_prescaled, cu_q, cu_kv, dev_seg,
-                                     _kernel_input)
-        out, lse = merge_any([cache.arena_block(c) for c in reuse] + list(fresh), dst_dtype=self.out_dtype, dst_lse_bsh=True)
-        for c, state in zip(compute, fresh):
-            if c != diag:
-                merge_any([state], dst=cache.arena_block(c))
-                cache.arena_valid[c] = True
+            states_of = lambda part: _hip.attn_states(query, ks, vs, [[i] for i in part], self._MAX_JOB_CHUNKS, _hip.attn_workspace(query.device), self.q_prescaled,
+                                                      cu_q, cu_kv, dev_seg, _kernel_input)
+
+        def keep(i, state):
+            if compute[i] != diag:
+                merge_any([state], dst=cache.arena_block(compute[i]))
+                cache.arena_valid[compute[i]] = True
+        out, lse = self._merge_quantized(query, [cache.arena_block(c) for c in reuse], len(compute), range(len(compute)), states_of, keep, 0,
+                                         lambda parts: merge_any(parts, dst_dtype=self.out_dtype, dst_lse_bsh=True))
         self.last_lse = lse
         rm.record_out_redundancy(timestep=t, layer_id=l, curr_out=out)
         return out

@@ -147,6 +147,17 @@ class proCache:
         """Bytes of a cached (token, head)."""
         return 2 * D + 4 if self.state_format is None else D + D // BLOCK + 4
 
+    @staticmethod
+    def _fresh_mb(B: int, Sq: int, H: int, D: int, element_bytes: int) -> float:
+        """A state that is not in the cache."""
+        return B * Sq * H * (element_bytes * D + 4) / (1024 ** 2)
+
+    def fresh_at_once(self, n: int, B: int, Sq: int, H: int, D: int, element_bytes: int, kept: int = 0) -> int:
+        """How many of ``n`` fresh states of a call there may be at once before they are quantised, ``kept`` of them into new memory: as many as the memory
+        budget has room for beside the fp32 result, into which they are merged in turn where that is not all of them; at least one."""
+        room = self.memory_constraint - self.memory_probe() - kept * B * Sq * H * self._row_bytes(D) / (1024 ** 2)
+        return max(1, min(n, int((room - self._fresh_mb(B, Sq, H, D, 4)) / self._fresh_mb(B, Sq, H, D, element_bytes))))
+
     def pass_memory_check(self, next_isp_stride: int, layer_id: int) -> bool:
         """cache.py:103-128"""
         if next_isp_stride == self.isp_size:
@@ -280,9 +291,10 @@ class proCache:
 
     # ---- mask-mode arena --------------------------------------------------------------------------
     def ensure_arena(self, n_chunks: int, B: int, Sq: int, H: int, D: int, device,
-                     dtype: torch.dtype = torch.bfloat16) -> bool:
+                     dtype: torch.dtype = torch.bfloat16, fresh_bytes: int = 2) -> bool:
         """Make sure the mask-mode arena of this layer exists.  Returns False when it does not fit:
-        the arena (``n_chunks + 1`` states) is only allocated if the current allocation plus its size
+        the arena (``n_chunks + 1`` states; under a ``state_format`` ``n_chunks``, beside which a fresh one of ``fresh_bytes`` an element and
+        the fp32 result that it is merged into have to fit) is only allocated if the current allocation plus its size
         stays under ``memory_constraint`` -- the same probe and budget as ``pass_memory_check``
         (cache.py:103-128) -- and a layer without arena recomputes every chunk on every call, which is
         what the reference's guard falls back to (core/attention.py:97-98: stride forced to N)."""
@@ -295,8 +307,10 @@ class proCache:
         if self.arena_refused == shape:
             return False
         self.arena_out = self.arena_lse = self.diag_out = self.diag_lse = self.arena_scales = None
-        # (8-bit states are quantised from fresh ones of their own, the diagonal's among them)
         need_mb = (n_chunks + (self.state_format is None)) * B * Sq * H * self._row_bytes(D) / (1024 ** 2)
+        if self.state_format is not None:
+            # quantised from fresh states, the diagonal's among them, of which a call has at least one at a time (fresh_at_once)
+            need_mb += self._fresh_mb(B, Sq, H, D, fresh_bytes) + self._fresh_mb(B, Sq, H, D, 4)
         now = self.memory_probe()
         if now + need_mb > self.memory_constraint:
             logger.warning(f"T{get_timestep()}L{self.layer_id} | Memory check failed: {now + need_mb:.0f} > "

@@ -893,27 +893,28 @@ StateParts merge_blocks(const std::vector<StateParts>& states, std::optional<Sta
   auto state = [&](const StateParts& t, const Name& name) {
     return any_state({std::get<0>(t), std::get<2>(t), std::get<1>(t)}, d, first, name);
   };
-  if (!into) {
+  const bool own = !into;
+  if (own) {
     std::optional<Tensor> scales;
     if (dst_dtype == at::kFloat8_e4m3fn || dst_dtype == at::kChar) scales = empty({d.B, d.S, d.H, d.D / 32}, first.options().dtype(at::kByte));
     into = StateParts{new_out(d, dst_dtype, first), scales, new_lse(d, dst_bsh, first)};
   }
   const dt_state dst = state(*into, {"destination"});
   std::vector<dt_state> list;
-  Tensor run_out, run_lse;
   for (size_t i = 0; i < states.size(); ++i) list.push_back(state(states[i], {"states", (int64_t)i}));
   if (first.numel() == 0) return *into;
+  // the running state of several launches is the result's memory, where that is fp32 and none of the states
+  Tensor run_out, run_lse;
+  dt_state run = dst;
+  if (list.size() > DT_MAX_MERGE && !(own && dst.dtype == DT_FP32)) {
+    run_out = new_out(d, at::kFloat, first);
+    run_lse = new_lse(d, false, first);
+    run = {ptr(run_out), nullptr, static_cast<float*>(ptr(run_lse)), DT_FP32, DT_LSE_BHS};
+  }
   size_t at = 0;
-  while (list.size() - at > DT_MAX_MERGE) {
-    const bool again = run_out.defined();
-    if (!again) {
-      run_out = new_out(d, at::kFloat, first);
-      run_lse = new_lse(d, false, first);
-    }
-    const dt_state run = {ptr(run_out), nullptr, static_cast<float*>(ptr(run_lse)), DT_FP32, DT_LSE_BHS};
+  for (; list.size() - at > DT_MAX_MERGE; list[at] = run) {
     CALL(dt_merge_block_states, DT_MAX_MERGE, list.data() + at, &run, d.B, d.S, d.H, d.D, stream_of(stream));
     at += DT_MAX_MERGE - 1;      // the last one's place takes the running state
-    list[at] = run;
   }
   CALL(dt_merge_block_states, (int32_t)(list.size() - at), list.data() + at, &dst, d.B, d.S, d.H, d.D, stream_of(stream));
   return *into;
