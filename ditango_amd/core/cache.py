@@ -75,6 +75,8 @@ def merge_any(states, *, dst=None, dst_dtype: torch.dtype = torch.float32, dst_l
     ``(out, lse)`` of ``dst_dtype``.  Returns the destination."""
     if not states:
         raise ValueError("need at least one state")
+    if dst is None and dst_dtype in STATE_FORMATS.values():
+        raise ValueError(f"a new state of 8 bits has scales as well, which a pair of {dst_dtype} has no place for: quantized(), or dst = BlockState.empty()")
     out, _, lse = _hip.merge_blocks([_parts(s) for s in states], None if dst is None else _parts(dst), dst_dtype, dst_lse_bsh)
     return (out, lse) if dst is None else dst
 
