@@ -15,7 +15,7 @@ The reference's executors run these as chains of eager torch ops right before
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from decimal import Decimal, localcontext
 from functools import cached_property, lru_cache
 from typing import Optional, Sequence, Tuple
@@ -129,6 +129,9 @@ class RotaryAxes:
         step = 8 if by_section else 2
         if any(d <= 0 or d % step for d in self.dims):
             raise ValueError(f"{self.pairing} axes need positive multiples of {step} elements, got {self.dims}")
+
+    def __getstate__(self):
+        return {f.name: getattr(self, f.name) for f in fields(self)}       # (not what is made of them, which a copy makes again)
 
     @cached_property
     def turns(self):
