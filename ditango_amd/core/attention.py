@@ -380,6 +380,9 @@ class proAttention:
                 out, self.last_lse = self._result_f32(query, [c for job in plan.jobs for c in job.chunks], key, value)
                 return out
             distinct = list(dict.fromkeys(job.chunks for job in plan.jobs))
+            if self.cache.state_format is not None:
+                return self._execute_quantized(query, merge_outs, merge_lses, len(distinct), [(distinct.index(job.chunks), job.store_slot) for job in plan.jobs],
+                                               lambda part: self._job_states_f32(query, [distinct[i] for i in part], key, value))
             seen = dict(zip(distinct, self._job_states_f32(query, distinct, key, value)))
             for job in plan.jobs:
                 o, l = seen[job.chunks]
@@ -404,24 +407,29 @@ class proAttention:
                 cu_q, cu_kv_of = segments
                 cu_kv = [cu_kv_of(c) for c in needed]
         ks, vs, workspace = [k for k, _ in kv], [v for _, v in kv], _hip.attn_workspace(query.device)
-        if self.cache.state_format is None:
-            states, out, lse = _hip.attn_states_merge(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, merge_outs, merge_lses, which, self.out_dtype,
-                                                      workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
-        else:
-            slots = {i: job.store_slot for job, i in zip(plan.jobs, which) if job.store_slot is not None}
-            cached = [o if isinstance(o, BlockState) else (o, l) for o, l in zip(merge_outs, merge_lses)]
-            out, lse = self._merge_quantized(
-                query, cached, len(jobs), which,
-                lambda part: _hip.attn_states(query, ks, vs, [jobs[i] for i in part], self._MAX_JOB_CHUNKS, workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input),
-                lambda i, state: self.cache.store_block(slots[i], *state) if i in slots else None, len(slots),
-                lambda parts: merge_any(parts, dst_dtype=self.out_dtype, dst_lse_bsh=True) if any(isinstance(p, BlockState) for p in parts)
-                else _hip.merge_states([o for o, _ in parts], [l for _, l in parts], dst_dtype=self.out_dtype, dst_lse_bsh=True))
-            self.last_lse = lse
-            return out
+        if self.cache.state_format is not None:
+            return self._execute_quantized(query, merge_outs, merge_lses, len(jobs), [(i, job.store_slot) for job, i in zip(plan.jobs, which)],
+                                           lambda part: _hip.attn_states(query, ks, vs, [jobs[i] for i in part], self._MAX_JOB_CHUNKS, workspace, self.q_prescaled,
+                                                                         cu_q, cu_kv, dev_seg, _kernel_input))
+        states, out, lse = _hip.attn_states_merge(query, ks, vs, jobs, self._MAX_JOB_CHUNKS, merge_outs, merge_lses, which, self.out_dtype,
+                                                  workspace, self.q_prescaled, cu_q, cu_kv, dev_seg, _kernel_input)
         for job, i in zip(plan.jobs, which):
             if job.store_slot is not None:
                 self.cache.store_block(job.store_slot, *states[i])  # :207-211
         self.last_lse = lse
+        return out
+
+    def _execute_quantized(self, query, merge_outs, merge_lses, n: int, jobs, states_of) -> torch.Tensor:
+        """``_execute`` under a ``state_format``: ``jobs`` are (which of the ``n`` fresh states, slot that keeps it or None)."""
+        def keep(i, state):
+            for job, slot in jobs:
+                if job == i and slot is not None:
+                    self.cache.store_block(slot, *state)
+
+        def merge(parts):
+            return merge_cached([p if isinstance(p, BlockState) else p[0] for p in parts], [p.lse if isinstance(p, BlockState) else p[1] for p in parts], self.out_dtype)
+        cached = [o if isinstance(o, BlockState) else (o, l) for o, l in zip(merge_outs, merge_lses)]
+        out, self.last_lse = self._merge_quantized(query, cached, n, [i for i, _ in jobs], states_of, keep, sum(slot is not None for _, slot in jobs), merge)
         return out
 
     def _merge_quantized(self, query, cached, n: int, which, states_of, keep, kept: int, merge):

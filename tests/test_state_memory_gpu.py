@@ -135,8 +135,8 @@ def test_fresh_states_under_a_mask_stay_within_the_budget(env, C, room, mode):  
 
 
 @pytest.mark.parametrize("N, rank, col", [(8, 3, (1, 1, 4, 4, 2, 2, 1)), (4, 1, (1, 1, 2, 1, 4, 2, 1))])
-@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
-def test_fresh_states_under_the_stride_schedule_stay_within_the_budget(env, N, rank, col, out_dtype):  # noqa: F811
+@pytest.mark.parametrize("exact, out_dtype", [(False, torch.float32), (False, torch.bfloat16), (True, torch.float32)])
+def test_fresh_states_under_the_stride_schedule_stay_within_the_budget(env, N, rank, col, exact, out_dtype):  # noqa: F811
     from ditango_amd.core.attention import proAttention
     from ditango_amd.core.parallel_state import get_usp_group
     from ditango_amd.utils import update_timestep
@@ -145,11 +145,15 @@ def test_fresh_states_under_the_stride_schedule_stay_within_the_budget(env, N, r
     group = get_usp_group()
     tight, easy = proAttention(0, group), proAttention(0, group)
     tight.out_dtype = easy.out_dtype = out_dtype
-    each, running, slot = STATE, S * H * (4 * D + 4), S * H * (D + D // 32 + 4)
+    dtype = torch.bfloat16
+    if exact:
+        tight.fp32_inputs = easy.fp32_inputs = "exact"
+        dtype = torch.float32
+    each, running, slot = S * H * (dtype.itemsize * D + 4), S * H * (4 * D + 4), S * H * (D + D // 32 + 4)
     grouped = 0
     for t in range(len(col)):
         update_timestep(t)
-        q, ks, vs = _inputs(N, torch.bfloat16, seed=t)
+        q, ks, vs = _inputs(N, dtype, seed=t)
         group.set_kv_chunks(ks, vs)
         a, most_a = _peak(lambda: easy.attn(q, ks[rank], vs[rank]))
         jobs, stores = len(easy.last_plan.launch[1]), len(easy.last_plan.stores)
