@@ -15,9 +15,9 @@
 // Only a tile with a border in it is masked.  The last round of workgroups, or all of them, may be cut into parts along the keys, whose states the
 // last one of an item adds up (few rows, with counters) or a kernel behind the launch.
 //
-// Large launches are bound by the package's power cap: 14 400 queries of 24 heads of 128 over 8 frames of 3600 of 57 600 keys and the first frame 4.73 ms, 1.21
-// PFLOP/s of visible pairs at 1.60 GHz, MFMAs busy 73 % of the cycles (a library product of 16384^3: 1.36 PFLOP/s); 48 heads of 64, 17 550 queries over 5 frames of 1350
-// 1.41 ms, 0.97 PFLOP/s (vector ALU 76 %).  Single tokens by HBM: 4 x 24 heads of 128 over 4160 keys 44.2 us, 4.6 TB/s with the launch.
+// Large launches are bound by the package's power cap: 14 400 queries of 24 heads of 128 over 8 frames of 3600 of 57 600 keys and the first frame 4.69 ms, 1.22
+// PFLOP/s of visible pairs at 1.65 GHz, MFMAs busy 71 % of the cycles (a library product of 16384^3: 1.36 PFLOP/s); 48 heads of 64, 17 550 queries over 5 frames of 1350
+// 1.41 ms, 0.97 PFLOP/s (vector ALU 76 %).  Single tokens by HBM: 4 x 24 heads of 128 over 4160 keys 44.3 us, 4.6 TB/s with the launch, of 64 29.0 us, 3.5 TB/s.
 #include <algorithm>
 #include <cmath>
 
@@ -789,9 +789,13 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
   }
 }
 
-// Few rows, W wavefronts.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is on its
-// way while it has the softmax and the values of this one, V of the next from there on, and while it waits the others have theirs (8 x 16 KB a
+// Few rows, W wavefronts.  The LDS holds a tile (K and V) of each wavefront, then its state.  A wavefront needs nobody: K of its next tile is sent for
+// before the softmax of this one, V of the next behind its values, and while it waits the others have theirs (8 x 16 KB a
 // CU at D = 128; four wavefronts with two tiles each were 48 KB a us and CU, this is 70).
+// As the compiler builds the loop, more is waited for than that needs.  Q comes by loads that it counts, the tiles by loads that it does not, and its wait for
+// Q stands in front of the score MFMAs, in the loop: at D = 128 vmcnt(7) .. vmcnt(0) of every tile, so that V of a tile has landed before its softmax begins and K of
+// the next comes alone.  At D = 64, where four wavefronts a SIMD leave 128 registers, 4 to 6 are spilled around the loop, whose stores, counted as well, leave these
+// waits at vmcnt(8) .. vmcnt(4); the branch of the exact maximum, which the first tile takes, brings one of them back and waits for all loads.
 template <int D, int W>
 struct FewLds {
   static constexpr int kTile = 2 * Tiles<D, 1>::kBytes;
@@ -1056,15 +1060,19 @@ int launch(const WindowArgs& a, unsigned grid, int waves, int lds, hipStream_t s
 // estimate, from what the forms take here, in us: a step -- 64 keys of shared tiles, a 32-key tile of every wavefront of few rows -- with up to
 // eight wavefronts a CU, and with more (D = 64); an item beside its steps; parts, their states' way to memory and back, 2 bytes / 6.7 TB/s, and the
 // kernel that adds them up, or the last of them that does, 0.4 us a part (2 heads of 64, a token over 20 000: 20.9 us without that term, 13.3 with).
+// The constants lie inside what launches of one round measure (8 heads, no border, 8 to 32 steps; a workgroup on every fourth CU .. on every one, then as many as fit):
+//   us a step: shared tiles, D = 64 0.92 .. 1.19, then 2.1; D = 128 1.1 .. 1.7;  few rows, 8 wavefronts, D = 64 0.76 .. 0.92, then 1.6; D = 128 1.1 .. 1.5;
+//   4 wavefronts, D = 64 0.7 .. 0.78, then 1.6; D = 128 0.75 .. 1.0, then 1.5.  Beside the steps, with the launch's 4 to 5: 7 .. 12; 5 .. 10; 4 .. 9.
+// Keys that no two workgroups share cost more, from 128 workgroups on what HBM gives them, and rounds at the power cap do (1.86 a step of D = 128): both change all forms alike.
 struct Form {
   int rows, keys, per_cu;       // rows of a workgroup, keys of its step, workgroups a CU
   double step, full, once;
 };
 template <int D>
 constexpr Form kForms[3] = {
-    {kRowsShared, 64, D == 64 ? 2 : 1, D == 64 ? 1.15 : 1.4, 2.0, 8.0},
-    {kRowsFew, 256, D == 64 ? 2 : 1, D == 64 ? 1.0 : 1.6, 2.0, 5.0},
-    {kRowsFew, 128, D == 64 ? 4 : 2, D == 64 ? 1.0 : 1.6, 2.0, 4.0},
+    {kRowsShared, 64, D == 64 ? 2 : 1, D == 64 ? 1.15 : 1.4, D == 64 ? 2.0 : 1.4, 8.0},
+    {kRowsFew, 256, D == 64 ? 2 : 1, D == 64 ? 1.0 : 1.6, D == 64 ? 2.0 : 1.6, 5.0},
+    {kRowsFew, 128, D == 64 ? 4 : 2, D == 64 ? 1.0 : 1.6, D == 64 ? 2.0 : 1.6, 4.0},
 };
 struct Plan {
   int form, ways;
@@ -1082,7 +1090,7 @@ Plan plan_form(const WindowArgs& a, int form, int64_t units, int n_cus, int64_t 
   const int64_t seen = a.left < 0 || a.right < 0 ? a.Sk : std::min<int64_t>(a.Sk, (int64_t)a.left + a.right + a.sinks + queries / a.frame * a.frame);
   const int64_t steps = (seen + f.keys - 1) / f.keys;
   auto item = [&](int64_t n, int64_t workgroups) {     // us of an item of n steps, that many at once on an XCD
-    return (D == 64 && 2 * workgroups > slots ? f.full : f.step) * n + f.once;
+    return (2 * workgroups > slots ? f.full : f.step) * n + f.once;
   };
   const int64_t tail = (per_xcd - 1) % slots + 1;
   const double before = (double)((per_xcd - tail) / slots) * item(steps, slots);
