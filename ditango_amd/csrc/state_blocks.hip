@@ -8,7 +8,7 @@
 //
 // The merge is that of the 16-bit states: lse = log sum_i exp(lse_i), out = sum_i exp(lse_i - lse) out_i, fp32 sums, one pass; a single
 // state is copied.  Bound by HBM: D + D / 32 + 4 bytes a row and 8-bit state instead of 2 D + 4.
-// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 101.4 us, 6.5 TB/s; one stored and loaded 52.6 us, 5.4 TB/s.
+// 6 of 8 bits and 2 of 16 of 14 882 x 24 heads of 128 into fp32: 101.4 us, 6.5 TB/s; one stored and loaded 51.7 us, 5.5 TB/s; four merged into the first, in 8 bits, 49.4 us, 4.9 TB/s.
 //
 // A lane owns 8 consecutive elements, so 4 lanes hold a block and its maximum is two exchanges inside a quad; a row's lanes are
 // neighbours in a wavefront.  States come sorted by the size of their elements, each size in batches whose loads are in flight together.
@@ -305,10 +305,10 @@ __device__ __forceinline__ RowIndex rows_of(KernArgs& a) {
 // are a sequence apart, and fetched by the rows' own lanes they cost as many requests as the elements; those of a tile come in 16-byte
 // runs, once for the four wavefronts, through the LDS.  us without and with: 14 882 x 24 heads of 128, 8 states of 8 bits 87.7 / 81.5, 6 and 2 of 16 bits
 // 111.8 / 104.8, 6 69.7 / 68.3, 2 38.4 / 42.2 (shorter runs of elements); heads of 64, 9000 x 48, 6 states 51.6 / 43.0, 2 25.5 / 24.8; 2222 x 48, 5 and 3 21.5 /
-// 18.5.  So heads of 64 always, heads of 128 from six states on.
+// 18.5.  So heads of 64 always, heads of 128 from six states on.  From 16 queries on: 16 x 24 heads x 32 samples, 2 and 8 states of 64 3.40 / 3.21 and 5.93 / 5.62, 6 and 8
+// of 128 5.62 / 5.21 and 6.62 / 6.13; with 8 queries -0.3 .. 0, with 1 to 4 -0.6 .. +0.3 us.
 constexpr int kTileQueries = kThreads / 64;
-// (seven wavefronts a SIMD, but for tiles of heads of 128, which take 76 registers: left to itself the compiler takes 74 for heads of 64 and six fit, 17.9 -> 18.5 us for 5 + 3
-// states of 2222 x 48 heads)
+// (Seven wavefronts a SIMD are asked for, but for tiles of heads of 128, which take 74 registers: with six, 5 + 3 states of 2222 x 48 heads of 64 take 18.5 us instead of 17.9.)
 template <int D, bool kTiles>
 __global__ __launch_bounds__(kThreads, D == 128 && kTiles ? 6 : 7) void merge_blocks_kernel(const BlockArgs args_by_value) {
   (void)args_by_value;
@@ -363,7 +363,9 @@ __global__ __launch_bounds__(kThreads, D == 128 && kTiles ? 6 : 7) void merge_bl
 }
 
 // One state into another format, its lse bit for bit.  From kManyWorkgroups workgroups on, with twice the elements each.  A state of 14 882 x 24 heads of
-// 128, int8, stored and loaded: 52.6 us (one unit a lane 54.0, four 54.7; with the lse in the rows' first lanes 56.0).
+// 128, int8, stored and loaded: 52.6 us (one unit a lane 54.0, four 54.7; with the lse in the rows' first lanes 56.0).  us with one unit a lane and with two, a store of 24 heads of
+// 64, by workgroups: 750 2.71 / 3.02, 1500 3.27 / 3.42, 2048 4.21 / 3.77, 3000 5.41 / 4.98, 4095 6.77 / 6.39, 6000 8.77 / 8.79; of 128: 1500 3.29 / 3.45, 2250 4.63 / 4.28,
+// 4096 6.75 / 6.44, 6000 8.69 / 8.77, 22 323 25.35 / 25.05; loads alike.
 constexpr unsigned kManyWorkgroups = 2048;
 constexpr int kCopyUnits = 2;
 // kUnits times kThreads lanes' elements a workgroup.
