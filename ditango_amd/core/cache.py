@@ -158,7 +158,8 @@ class proCache:
         """How many of ``n`` fresh states of a call there may be at once before they are quantised, ``kept`` of them into new memory: as many as the memory
         budget has room for beside the fp32 result, into which they are merged in turn where that is not all of them; at least one."""
         room = self.memory_constraint - self.memory_probe() - kept * B * Sq * H * self._row_bytes(D) / (1024 ** 2)
-        return max(1, min(n, int((room - self._fresh_mb(B, Sq, H, D, 4)) / self._fresh_mb(B, Sq, H, D, element_bytes))))
+        each = self._fresh_mb(B, Sq, H, D, element_bytes)
+        return int(max(1, min(n, (room - self._fresh_mb(B, Sq, H, D, 4)) / each))) if each else n
 
     def pass_memory_check(self, next_isp_stride: int, layer_id: int) -> bool:
         """cache.py:103-128"""

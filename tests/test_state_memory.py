@@ -33,3 +33,13 @@ def test_how_many_fresh_states_there_may_be_at_once():
     assert at_once(516 + 3 * 260 + 5 * 136, 8, kept=5) == 3 and at_once(516 + 8 * 260 + 8 * 136, 8, kept=8) == 8
     assert at_once(516 + 3 * 516, 8, element_bytes=4) == 3
     assert at_once(0, 8) == 1 and _cache(-500.0).fresh_at_once(8, B, Sq, H, D, 2) == 1
+
+
+def test_no_bound_and_no_rows():
+    cache = _cache(0.0)
+    cache.memory_constraint = float("inf")
+    assert cache.fresh_at_once(8, B, Sq, H, D, 2) == 8 and cache.ensure_arena(8, B, Sq, H, D, torch.device("cpu"))
+    cache.memory_constraint = float("-inf")
+    assert cache.fresh_at_once(8, B, Sq, H, D, 2) == 1
+    for free in (100.0, 0.0, -100.0):
+        assert _cache(free).fresh_at_once(8, B, 0, H, D, 2) == 8
