@@ -124,6 +124,12 @@ _SIGNATURES = {
     "dt_merge_block_states": (ctypes.c_int, [c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp]),
     "dt_qk_norm_rope_axes": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32, c_vp, c_i64, c_i32, _P(ctypes.c_uint64),
                                             _P(ctypes.c_uint8), c_i32, _P(c_i32), c_i32, c_i32, c_vp]),
+    "dt_plan_pages": (ctypes.c_int, [c_vp, c_i64, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "dt_append_pages": (ctypes.c_int, [c_vp, c_vp, _P(c_i64), _P(c_i64), c_i32, c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "dt_prepare_pages": (ctypes.c_int, [c_vp, c_vp, _P(c_i64), c_i32, c_i32, c_i32, c_f32, c_vp, c_i32, _P(ctypes.c_uint64), _P(ctypes.c_uint8), c_i32,
+                                        _P(c_i32), c_i32, c_i32, c_vp, c_vp, c_vp]),
+    "dt_attn_pages_fwd": (ctypes.c_int, [c_vp, _P(c_i64), c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32,
+                                         c_vp, c_f32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -619,3 +625,31 @@ def rotary_table(turns: Sequence[int], axis_of_pair: Sequence[int], rope: int, s
 def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: float):
     """q and k in one launch of ``dt_qk_norm_rope_axes``; ``tensors``: one or two of ``(x, weight, bias, out, out_scale)``."""
     return _host().qk_norm_rope_axes(tensors, positions, table, norm, eps, _stream_at(tensors[0][0], "q"))
+
+
+# ---------------------------------------------------------------------------------------------
+# A cache of pages that several requests share
+# ---------------------------------------------------------------------------------------------
+
+def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, n_tokens: int, n_pages: int, page_size: int, in_place: bool):
+    """(lens, cu_seqlens, slots, served) of ``dt_plan_pages``; ``tables`` are extended in place, and with ``in_place`` ``lens`` as well."""
+    return _host().plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place, _stream_at(tables, "tables"))
+
+
+def append_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor) -> None:
+    _host().append_pages(k, v, k_pages, v_pages, slots, _stream_at(k, "k"))
+
+
+def prepare_pages(tensors, v: torch.Tensor, positions: torch.Tensor, table, norm: int, eps: float, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  slots: torch.Tensor) -> torch.Tensor:
+    """q of ``dt_prepare_pages``; ``tensors``: q and k as in ``qk_norm_rope_axes``, packed ``[T,H,D]``."""
+    return _host().prepare_pages(tensors, v, positions, table, norm, eps, k_pages, v_pages, slots, _stream_at(tensors[0][0], "q"))
+
+
+def attn_pages_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, cu_seqlens: torch.Tensor,
+                   max_seqlen_q: int, left: int, right: int, frame: int, sinks: int, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                   lse: Optional[torch.Tensor] = None):
+    """(out, lse) of ``dt_attn_pages_fwd``; -1 stands for a border that is not there."""
+    stream = _stream_at(q, "q")
+    return _host().attn_pages(q, k_pages, v_pages, tables, lens, cu_seqlens, max_seqlen_q, left, right, frame, sinks, float(softmax_scale), out, lse,
+                              None, None, stream)

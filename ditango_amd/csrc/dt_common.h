@@ -26,6 +26,20 @@ __device__ __forceinline__ uint32_t quotient(uint32_t n, const Quotient& by) {
   return by.shift < 0 ? n : __umulhi(n, by.mul) >> by.shift;
 }
 
+// Keys (0) and values (1) in pages, as the kernels take them; slot = page * tokens of a page + token.
+struct Pages {
+  uint16_t* base[2];
+  int64_t sp[2], ss[2], sh[2];  // strides of a page, a token, a head
+  int32_t n_pages, page;        // in the pool, tokens of one
+  Quotient by_page;
+  __device__ __forceinline__ bool has(int64_t slot) const { return (uint64_t)slot < (uint64_t)n_pages * (uint32_t)page; }
+  __device__ __forceinline__ uint16_t* row(int i, int64_t slot) const {      // of a slot that there is, which has 31 bits
+    const uint32_t p = quotient((uint32_t)slot, by_page);
+    return base[i] + p * sp[i] + (int64_t)((uint32_t)slot - p * page) * ss[i];
+  }
+};
+int check_pages(const dt_pages* p, int D, Pages& out);
+
 // One KV chunk, one reference of a job to a chunk, one job of an attention launch: a record each, so that a workgroup finds
 // what it needs in one or two cache lines.
 struct AttnChunk {

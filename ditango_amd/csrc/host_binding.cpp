@@ -930,27 +930,34 @@ struct RotaryTable {
 
 // ditango_amd._hip.qk_norm_rope_axes.  A tensor: (x, weight, bias, out, scale).
 using RotaryRows = std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>, std::optional<Tensor>, double>;
+// Norm parameters of a call in the tensors' own type are widened by the kernel as it reads them; others become fp32 here.
+struct NormParameters {
+  bool narrow = true;
+  at::TensorOptions options;
+  std::vector<Tensor> kept;
+  NormParameters(const std::vector<RotaryRows>& tensors, const Tensor& like, int64_t D) : options(like.options().dtype(at::kFloat)) {
+    for (const auto& t : tensors)
+      for (const auto* p : {&std::get<1>(t), &std::get<2>(t)})
+        if (*p) {
+          REQUIRE((*p)->numel() == D && at::isFloatingType((*p)->scalar_type()), "norm parameters must be floating-point [D]");
+          narrow = narrow && (*p)->scalar_type() == like.scalar_type() && same_device(**p, like) && (*p)->is_contiguous() &&
+                   reinterpret_cast<uintptr_t>(ptr(**p)) % 16 == 0;
+        }
+  }
+  const void* operator()(const std::optional<Tensor>& p) {
+    if (!p || narrow) return ptr(p);
+    kept.push_back(p->detach().to(options).contiguous());
+    return ptr(kept.back());
+  }
+};
 std::vector<Tensor> qk_norm_rope_axes(const std::vector<RotaryRows>& tensors, const Tensor& positions, const RotaryTable& table, int32_t norm, double eps,
                                       uint64_t stream) {
   REQUIRE(tensors.size() == 1 || tensors.size() == 2, "one or two tensors are needed");
   const Tensor& first = std::get<0>(tensors[0]);
   const Dims d = check_bshd(first, {"q"});
   dt_rotary_rows rows[2] = {};
-  std::vector<Tensor> outs, kept;
-  // norm parameters in the tensors' own type are widened by the kernel as it reads them; others become fp32 here
-  bool narrow = true;
-  for (const auto& t : tensors)
-    for (const auto* p : {&std::get<1>(t), &std::get<2>(t)})
-      if (*p) {
-        REQUIRE((*p)->numel() == d.D && at::isFloatingType((*p)->scalar_type()), "norm parameters must be floating-point [D]");
-        narrow = narrow && (*p)->scalar_type() == first.scalar_type() && same_device(**p, first) && (*p)->is_contiguous() &&
-                 reinterpret_cast<uintptr_t>(ptr(**p)) % 16 == 0;
-      }
-  auto parameter = [&](const std::optional<Tensor>& p) -> const void* {
-    if (!p || narrow) return ptr(p);
-    kept.push_back(p->detach().to(first.options().dtype(at::kFloat)).contiguous());
-    return ptr(kept.back());
-  };
+  std::vector<Tensor> outs;
+  NormParameters parameter(tensors, first, d.D);
   for (size_t i = 0; i < tensors.size(); ++i) {
     const auto& [x, weight, bias, given, scale] = tensors[i];
     const Dims dx = check_bshd(x, {i ? "k" : "q"});
@@ -970,11 +977,146 @@ std::vector<Tensor> qk_norm_rope_axes(const std::vector<RotaryRows>& tensors, co
   REQUIRE((int64_t)table.turns.size() == d.D / 2 && table.axis.size() == table.turns.size(), "the axes do not cover the head dim ", std::to_string(d.D));
   REQUIRE(d.S < (1ll << 31) && d.B < (1ll << 31), "too many tokens");
   if (first.numel() == 0) return outs;
-  const int32_t rounding = (first.scalar_type() == at::kHalf ? DT_IO_FP16 : 0) | (narrow ? DT_WEIGHTS_16 : 0);
+  const int32_t rounding = (first.scalar_type() == at::kHalf ? DT_IO_FP16 : 0) | (parameter.narrow ? DT_WEIGHTS_16 : 0);
   CALL(dt_qk_norm_rope_axes, rows, (int32_t)tensors.size(), (int32_t)d.B, (int32_t)d.S, (int32_t)d.D, norm, (float)eps,
        static_cast<const int32_t*>(ptr(positions)), positions.dim() == 3 ? positions.stride(0) : 0, (int32_t)n_axes, table.turns.data(),
        table.axis.data(), table.rope, table.sections.data(), (int32_t)table.sections.size(), rounding, stream_of(stream));
   return outs;
+}
+
+// ---- a cache of pages -----------------------------------------------------------------------------------------------
+
+struct Packed {
+  int64_t T, H, D;
+};
+Packed check_thd(const Tensor& t, const Name& name) {
+  REQUIRE(t.is_cuda(), name.str(), " must live on the GPU");
+  REQUIRE(is_half(t), name.str(), " must be bf16 or fp16");
+  REQUIRE(t.dim() == 3 && t.stride(2) == 1, name.str(), " must be [T,H,D] with contiguous D");
+  REQUIRE(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31), "too many tokens");
+  return {t.size(0), t.size(1), t.size(2)};
+}
+// (strides of dimensions of size one do not matter, and may be anything)
+int64_t stride_of(const Tensor& t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
+
+dt_pages pages_of(const Tensor& k, const Tensor& v, const Tensor& like, int64_t heads, int64_t D) {
+  REQUIRE(same_device(like, k) && same_device(like, v) && k.scalar_type() == like.scalar_type() && v.scalar_type() == like.scalar_type(),
+          "the pages must have the dtype and the device of the tokens");
+  REQUIRE(k.dim() == 4 && k.sizes() == v.sizes() && k.size(2) == heads && k.size(3) == D && k.stride(3) == 1 && v.stride(3) == 1,
+          "the pages must be [pages, page size, Hk, D] with contiguous D and the key heads and head dim of the tokens");
+  REQUIRE(k.size(0) < (1ll << 31) && k.size(1) < (1ll << 31), "too many pages");
+  dt_pages p = {ptr(k), ptr(v), {}, {}, (int32_t)k.size(0), (int32_t)k.size(1)};
+  for (int i = 0; i < 3; ++i) {
+    p.k_strides[i] = stride_of(k, i);
+    p.v_strides[i] = stride_of(v, i);
+  }
+  return p;
+}
+const int64_t* slots_of(const Tensor& slots, const Tensor& like, int64_t T) {
+  REQUIRE(same_device(like, slots) && slots.scalar_type() == at::kLong && slots.is_contiguous() && shape_is(slots, {T}),
+          "slots must be contiguous int64 [T] on the device of the tokens");
+  return static_cast<const int64_t*>(ptr(slots));
+}
+int32_t* ints_of(const Tensor& t, const Tensor& like, int64_t n, const char* name) {
+  REQUIRE(same_device(like, t) && t.scalar_type() == at::kInt && t.is_contiguous() && shape_is(t, {n}), name, " must be contiguous int32 [",
+          std::to_string(n), "] on the device of the other tensors");
+  return static_cast<int32_t*>(ptr(t));
+}
+void check_tables(const Tensor& tables) {
+  REQUIRE(tables.is_cuda() && tables.scalar_type() == at::kInt && tables.dim() == 2 && (tables.size(1) < 2 || tables.stride(1) == 1) &&
+              tables.size(0) < (1ll << 31) && tables.size(1) < (1ll << 31),
+          "tables must be int32 [requests, entries] on the GPU with contiguous rows");
+}
+int64_t row_stride(const Tensor& tables) { return tables.size(0) > 1 ? tables.stride(0) : tables.size(1); }
+
+// ditango_amd._hip.plan_pages
+std::tuple<Tensor, Tensor, Tensor, Tensor> plan_pages(const Tensor& tables, const Tensor& lens, const Tensor& new_lens, int64_t n_tokens, int64_t n_pages,
+                                                      int64_t page_size, bool in_place, uint64_t stream) {
+  check_tables(tables);
+  const int64_t B = tables.size(0);
+  int32_t* from = ints_of(lens, tables, B, "lens");
+  const int32_t* more = ints_of(new_lens, tables, B, "new_lens");
+  REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31) && n_pages >= 0 && n_pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31),
+          "n_tokens and n_pages must be whole numbers below 2^31, page_size a positive one");
+  const auto opt = tables.options();
+  Tensor lens_out = in_place ? lens : empty({B}, opt), cu = empty({B + 1}, opt), slots = empty({n_tokens}, opt.dtype(at::kLong)),
+         served = empty({B}, opt.dtype(at::kBool));
+  CALL(dt_plan_pages, static_cast<int32_t*>(ptr(tables)), row_stride(tables), (int32_t)tables.size(1), (const int32_t*)from, more, (int32_t)B,
+       (int32_t)n_pages, (int32_t)page_size, (int32_t)n_tokens, static_cast<int32_t*>(ptr(lens_out)), static_cast<int32_t*>(ptr(cu)),
+       static_cast<int64_t*>(ptr(slots)), static_cast<uint8_t*>(ptr(served)), stream_of(stream));
+  return {lens_out, cu, slots, served};
+}
+
+// ditango_amd._hip.append_pages
+void append_pages(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots, uint64_t stream) {
+  const Packed d = check_thd(k, {"k"}), dv = check_thd(v, {"v"});
+  REQUIRE(dv.T == d.T && dv.H == d.H && dv.D == d.D && v.scalar_type() == k.scalar_type() && same_device(k, v), "k and v must have one shape, dtype and device");
+  const dt_pages pages = pages_of(k_pages, v_pages, k, d.H, d.D);
+  const int64_t* to = slots_of(slots, k, d.T);
+  if (k.numel() == 0) return;
+  const int64_t ks[2] = {stride_of(k, 0), stride_of(k, 1)}, vs[2] = {stride_of(v, 0), stride_of(v, 1)};
+  CALL(dt_append_pages, (const void*)ptr(k), (const void*)ptr(v), ks, vs, (int32_t)d.T, (int32_t)d.H, (int32_t)d.D, &pages, to, stream_of(stream));
+}
+
+// ditango_amd._hip.prepare_pages
+Tensor prepare_pages(const std::vector<RotaryRows>& tensors, const Tensor& v, const Tensor& positions, const RotaryTable& table, int32_t norm, double eps,
+                     const Tensor& k_pages, const Tensor& v_pages, const Tensor& slots, uint64_t stream) {
+  REQUIRE(tensors.size() == 2, "q and k are needed");
+  const Tensor &q = std::get<0>(tensors[0]), &k = std::get<0>(tensors[1]);
+  const Packed d = check_thd(q, {"q"}), dk = check_thd(k, {"k"}), dv = check_thd(v, {"v"});
+  REQUIRE(dk.T == d.T && dk.D == d.D && k.scalar_type() == q.scalar_type() && same_device(q, k), "q and k must have one dtype, device, length and head dim");
+  REQUIRE(dv.T == dk.T && dv.H == dk.H && dv.D == dk.D && v.scalar_type() == k.scalar_type() && same_device(k, v), "k and v must have one shape, dtype and device");
+  const dt_pages pages = pages_of(k_pages, v_pages, k, dk.H, dk.D);
+  const int64_t* to = slots_of(slots, k, d.T);
+  NormParameters parameters(tensors, q, d.D);
+  Tensor y = std::get<3>(tensors[0]) ? *std::get<3>(tensors[0]) : empty({d.T, d.H, d.D}, q.options());
+  REQUIRE(same_device(y, q) && y.scalar_type() == q.scalar_type() && y.is_contiguous() && shape_is(y, {d.T, d.H, d.D}),
+          "out must be a contiguous [T,H,D] in the dtype of q");
+  const int64_t n_axes = positions.size(-1);
+  REQUIRE(same_device(positions, q) && positions.scalar_type() == at::kInt && positions.is_contiguous() && shape_is(positions, {d.T, n_axes}),
+          "positions must be contiguous int32 [T, axes] on the device of q");
+  REQUIRE((int64_t)table.turns.size() == d.D / 2 && table.axis.size() == table.turns.size(), "the axes do not cover the head dim ", std::to_string(d.D));
+  if (d.T == 0) return y;
+  dt_rotary_rows rows[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    const auto& [x, weight, bias, given, scale] = tensors[i];
+    rows[i] = {ptr(x), 0, stride_of(x, 0), stride_of(x, 1), i ? nullptr : ptr(y), parameters(weight), parameters(bias), (int32_t)x.size(1), (float)scale};
+  }
+  const int64_t vs[2] = {stride_of(v, 0), stride_of(v, 1)};
+  CALL(dt_prepare_pages, rows, (const void*)ptr(v), vs, (int32_t)d.T, (int32_t)d.D, norm, (float)eps, static_cast<const int32_t*>(ptr(positions)),
+       (int32_t)n_axes, table.turns.data(), table.axis.data(), table.rope, table.sections.data(), (int32_t)table.sections.size(),
+       (q.scalar_type() == at::kHalf ? DT_IO_FP16 : 0) | (parameters.narrow ? DT_WEIGHTS_16 : 0), &pages, to, stream_of(stream));
+  return y;
+}
+
+// ditango_amd._hip.attn_pages_fwd
+std::pair<Tensor, Tensor> attn_pages(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lens,
+                                     const Tensor& cu_seqlens, int64_t max_seqlen_q, int32_t left, int32_t right, int32_t frame, int32_t sinks, double scale,
+                                     std::optional<Tensor> out, std::optional<Tensor> lse, const std::optional<Tensor>& workspace,
+                                     const std::optional<Tensor>& counters, uint64_t stream) {
+  const Packed d = check_thd(q, {"q"});
+  REQUIRE(k_pages.dim() == 4 && k_pages.size(2) > 0 && d.H % k_pages.size(2) == 0,
+          "the pages must be [pages, page size, Hk, D] with a number of key heads that divides that of q");
+  const int64_t Hk = k_pages.size(2);
+  const dt_pages pages = pages_of(k_pages, v_pages, q, Hk, d.D);
+  check_tables(tables);
+  REQUIRE(same_device(q, tables), "tables must be on the device of q");
+  const int64_t B = tables.size(0);
+  const int32_t *len = ints_of(lens, q, B, "lens"), *cu = ints_of(cu_seqlens, q, B + 1, "cu_seqlens");
+  if (!out) out = empty({d.T, d.H, d.D}, q.options());
+  if (!lse) lse = empty({d.H, d.T}, q.options().dtype(at::kFloat));
+  REQUIRE(same_device(q, *out) && out->scalar_type() == q.scalar_type() && out->is_contiguous() && shape_is(*out, {d.T, d.H, d.D}),
+          "out must be a contiguous [T,H,D] in the dtype of q");
+  REQUIRE(same_device(q, *lse) && lse->scalar_type() == at::kFloat && lse->is_contiguous() && shape_is(*lse, {d.H, d.T}),
+          "lse must be contiguous fp32 [H,T] on the device of q");
+  if (q.numel() == 0) return {*out, *lse};
+  const int64_t qs[2] = {stride_of(q, 0), stride_of(q, 1)};
+  const dt_window w = {left, right, frame, sinks, -1, nullptr};
+  CALL(dt_attn_pages_fwd, (const void*)ptr(q), qs, ptr(*out), static_cast<float*>(ptr(*lse)), (int32_t)d.T, (int32_t)d.H, (int32_t)Hk, (int32_t)d.D, &pages,
+       static_cast<const int32_t*>(ptr(tables)), row_stride(tables), (int32_t)tables.size(1), (int32_t)B, len, cu,
+       (int32_t)std::min<int64_t>(max_seqlen_q, INT32_MAX), &w, (float)scale, q.scalar_type() == at::kHalf ? DT_ATTN_FP16 : 0, ptr(workspace),
+       bytes_of(workspace), static_cast<uint32_t*>(ptr(counters)), counters ? counters->numel() : 0, stream_of(stream));
+  return {*out, *lse};
 }
 
 // ---- host state of a call -------------------------------------------------------------------------------------
@@ -1052,6 +1194,10 @@ PYBIND11_MODULE(_ditango_host, m) {
         return RotaryTable{turns, axis, rope, sections};
       }));
   m.def("qk_norm_rope_axes", &qk_norm_rope_axes);
+  m.def("plan_pages", &plan_pages);
+  m.def("append_pages", &append_pages);
+  m.def("prepare_pages", &prepare_pages);
+  m.def("attn_pages", &attn_pages);
   m.def("element", &element);
   m.def("allocated_bytes", &allocated_bytes);
 }

@@ -9,6 +9,9 @@
 // HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
 // runs of 4 half a section apart with rotate-half.  It has their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of
 // 128 with an RMS norm: 64.4 us, 5.7 TB/s (two launches of the kernel with tables: 68.2, and the tables' making).
+#include <initializer_list>
+#include <type_traits>
+
 #include "producer_math.h"
 
 namespace dt {
@@ -60,19 +63,37 @@ __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d,
   }
 }
 
+// A launch whose keys go into the pages of a cache, and values beside them: rows[0] are q, rows[1] k, `v` values, of which nothing but their place
+// changes.  Tokens are packed, B = 1.  A lane group finds its token's slot with its rows under way.
+struct PagedArgs : RotaryArgs {
+  Rows v;
+  Pages to;
+  const int64_t* slots;
+};
+
 // kRms: with an RMS norm, which does without the 20 registers of means and biases (14 882 x 48 heads of 128 66.6 -> 64.4 us; a form of its own for rows
 // without a norm, with as few, is 3 % slower than the common one).
-template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const RotaryArgs a) {
+template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms, typename Args>
+__device__ __forceinline__ void rotate_rows(const Args& a) {
+  constexpr bool kPages = std::is_same<Args, PagedArgs>::value;
   constexpr int G = D / 8;
   const int c = threadIdx.x % G;
   const uint32_t item = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (item >= a.items) return;   // a lane group leaves as a whole; the exchanges below stay inside a group
   const uint32_t bs = quotient(item, a.by_groups);
-  int hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups));
+  int hg, values = 0;
+  if constexpr (kPages) {
+    hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups + a.v.groups));
+    values = hg >= a.rows[0].groups + a.rows[1].groups;
+    if (values) hg -= a.rows[1].groups;      // (and those of q, below)
+  } else {
+    hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups));
+  }
   const bool second = hg >= a.rows[0].groups;
   if (second) hg -= a.rows[0].groups;
-  const Rows& t = second ? a.rows[1] : a.rows[0];
+  const Rows* of = second ? &a.rows[1] : &a.rows[0];
+  if constexpr (kPages) of = values ? &a.v : of;
+  const Rows& t = *of;
   const uint32_t b = quotient(bs, a.by_s), s = bs - b * (uint32_t)a.S;
   const int h0 = hg * kHeads, nh = min(t.H - h0, kHeads);
   const int ea = kHalves ? a.a0[c] : 8 * c, eb = kHalves ? a.b0[c] : 8 * c + 4;
@@ -91,6 +112,31 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
       } else {
         raw[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + ea));
       }
+    }
+  }
+  uint16_t* yp;
+  int64_t y_sh = D;
+  if constexpr (kPages) {
+    yp = t.y + ((int64_t)bs * t.H + h0) * D;
+    if (second) {
+      const int64_t slot = a.slots[bs];
+      if (!a.to.has(slot)) return;
+      y_sh = a.to.sh[values];
+      yp = a.to.row(values, slot) + h0 * y_sh;
+    }
+    if (values) {
+#pragma unroll
+      for (int r = 0; r < kHeads; ++r)
+        if (r < nh) {
+          uint16_t* p = yp + r * y_sh;
+          if constexpr (kHalves) {
+            *reinterpret_cast<u32x2*>(p + ea) = u32x2{raw[r].x, raw[r].y};
+            *reinterpret_cast<u32x2*>(p + eb) = u32x2{raw[r].z, raw[r].w};
+          } else {
+            *reinterpret_cast<u32x4*>(p + ea) = raw[r];
+          }
+        }
+      return;
     }
   }
   // the angles of this lane's pairs; t mod 2^32 of the upper half of n F
@@ -143,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
       for (int i = 0; i < 4; ++i) rs[r + i] = four[i];
     }
   }
-  uint16_t* yp = t.y + ((int64_t)bs * t.H + h0) * D;
+  if constexpr (!kPages) yp = t.y + ((int64_t)bs * t.H + h0) * D;
 #pragma unroll
   for (int r = 0; r < kHeads; ++r) {
     if (r >= nh) break;
@@ -161,7 +207,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
       y[ib] = rotated(v[ib], v[ia], cs[i], sn[i]) * t.scale;
     }
     const u32x4 o = u32x4{pack2<kHalf>(y[0], y[1]), pack2<kHalf>(y[2], y[3]), pack2<kHalf>(y[4], y[5]), pack2<kHalf>(y[6], y[7])};
-    uint16_t* q = yp + r * D;
+    uint16_t* q = yp + r * y_sh;
     if constexpr (kHalves) {
       __builtin_nontemporal_store(u32x2{o.x, o.y}, reinterpret_cast<u32x2*>(q + ea));
       __builtin_nontemporal_store(u32x2{o.z, o.w}, reinterpret_cast<u32x2*>(q + eb));
@@ -171,21 +217,21 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
   }
 }
 
+template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms>
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const RotaryArgs a) {
+  rotate_rows<D, kHalf, kHalves, kHeads, kRms>(a);
+}
+template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms>
+__global__ __launch_bounds__(kThreads) void prepare_pages_kernel(const PagedArgs a) {
+  rotate_rows<D, kHalf, kHalves, kHeads, kRms>(a);
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-}  // namespace
-}  // namespace dt
-
-using namespace dt;
-
-extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, int32_t S, int32_t D, int32_t norm, float eps,
-                                    const int32_t* positions, int64_t pos_stride_b, int32_t n_axes, const uint64_t* turns,
-                                    const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections, int32_t n_sections,
-                                    int32_t rounding, void* stream) {
-  if (!rows || n_rows < 1 || n_rows > 2 || B <= 0 || S <= 0) {
-    set_error("need one or two tensors and positive B and S (got %d, %d, %d)", n_rows, B, S);
-    return DT_ERR_INVALID;
-  }
+// What the entry points have in common: everything but the number of rows.  `pages`: row 1 has no y of its own.
+int fill_rotary(RotaryArgs& a, const dt_rotary_rows* rows, int32_t n_rows, int32_t D, int32_t norm, float eps, const int32_t* positions,
+                int64_t pos_stride_b, int32_t n_axes, const uint64_t* turns, const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections,
+                int32_t n_sections, int32_t rounding, bool pages) {
   if (D != 64 && D != 128) {
     set_error("head dim %d not built (64 and 128 are)", D);
     return DT_ERR_UNSUPPORTED;
@@ -199,7 +245,6 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
     set_error("positions, turns and axis_of_pair must be non-null, with 1..%d axes and a stride that is not negative", kMostAxes);
     return DT_ERR_INVALID;
   }
-  RotaryArgs a{};
   for (int j = 0; j < D / 2; ++j)
     if (axis_of_pair[j] >= n_axes) {
       set_error("pair %d is on axis %d of %d", j, axis_of_pair[j], n_axes);
@@ -242,7 +287,8 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
   }
   for (int i = 0; i < n_rows; ++i) {
     const dt_rotary_rows& r = rows[i];
-    if (r.H <= 0 || !r.x || !r.y || !aligned16(r.x) || !aligned16(r.y) || ((r.stride_b | r.stride_s | r.stride_h) & 7)) {
+    const void* y = pages && i == 1 ? r.x : r.y;
+    if (r.H <= 0 || !r.x || !y || !aligned16(r.x) || !aligned16(y) || (((pages ? 0 : r.stride_b) | r.stride_s | r.stride_h) & 7)) {
       set_error("tensor %d: x and y must be non-null, 16-byte aligned, with strides that are multiples of 8 elements and a positive number of heads", i);
       return DT_ERR_INVALID;
     }
@@ -257,60 +303,122 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
     Rows& d = a.rows[i];
     d.x = static_cast<const uint16_t*>(r.x);
     d.y = static_cast<uint16_t*>(r.y);
-    d.sb = r.stride_b; d.ss = r.stride_s; d.sh = r.stride_h;
+    d.sb = pages ? 0 : r.stride_b; d.ss = r.stride_s; d.sh = r.stride_h;
     d.w = r.weight; d.bias = r.bias;
     d.scale = r.out_scale;
     d.H = r.H;
     d.groups = (r.H - 1) / 4 + 1;
   }
+  a.pos = positions;
+  a.pos_sb = pos_stride_b;
+  a.n_axes = n_axes;
+  a.norm = norm;
+  a.w16 = (rounding & DT_WEIGHTS_16) != 0;
+  a.eps = eps;
+  return DT_OK;
+}
+
+// Lane groups of `groups` (of four heads, per token) x tokens; eight heads a lane group where that pays, which halves the groups of `rows`.
+template <typename Args>
+bool eight_heads(Args& a, int64_t& groups, __int128& items, int D, std::initializer_list<Rows*> rows) {
+  bool eight = items > (int64_t)kManyWorkgroups * (kThreads / (D / 8));
+  for (const Rows* r : rows) eight = eight && r->groups % 2 == 0;
+  if (!eight) return false;
+  for (Rows* r : rows) r->groups /= 2;
+  groups /= 2;
+  items /= 2;
+  return true;
+}
+
+#define DT_LAUNCH_L(kernel, D, half, halves, rms)                                                                         \
+  do {                                                                                                                     \
+    if (eight) hipLaunchKernelGGL((kernel<D, half, halves, 8, rms>), grid, block, 0, st, a);                              \
+    else hipLaunchKernelGGL((kernel<D, half, halves, 4, rms>), grid, block, 0, st, a);                                    \
+  } while (0)
+#define DT_LAUNCH(kernel, D, half, halves)                        \
+  do {                                                            \
+    if (rms) DT_LAUNCH_L(kernel, D, half, halves, true);          \
+    else DT_LAUNCH_L(kernel, D, half, halves, false);             \
+  } while (0)
+#define DT_LAUNCH_D(kernel, D)                                           \
+  do {                                                                   \
+    if (half && halves) DT_LAUNCH(kernel, D, true, true);                \
+    else if (half) DT_LAUNCH(kernel, D, true, false);                    \
+    else if (halves) DT_LAUNCH(kernel, D, false, true);                  \
+    else DT_LAUNCH(kernel, D, false, false);                             \
+  } while (0)
+#define DT_LAUNCH_ROTARY(kernel)                                                                                    \
+  do {                                                                                                               \
+    const int per_wg = kThreads / (D / 8);                                                                          \
+    const dim3 grid((unsigned)((items + per_wg - 1) / per_wg)), block(kThreads);                                    \
+    const hipStream_t st = (hipStream_t)stream;                                                                     \
+    const bool half = (rounding & DT_IO_FP16) != 0, halves = rope == DT_ROPE_HALVES, rms = norm == DT_NORM_RMS;     \
+    if (D == 128) DT_LAUNCH_D(kernel, 128);                                                                         \
+    else DT_LAUNCH_D(kernel, 64);                                                                                   \
+  } while (0)
+
+}  // namespace
+}  // namespace dt
+
+using namespace dt;
+
+extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, int32_t S, int32_t D, int32_t norm, float eps,
+                                    const int32_t* positions, int64_t pos_stride_b, int32_t n_axes, const uint64_t* turns,
+                                    const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections, int32_t n_sections,
+                                    int32_t rounding, void* stream) {
+  if (!rows || n_rows < 1 || n_rows > 2 || B <= 0 || S <= 0) {
+    set_error("need one or two tensors and positive B and S (got %d, %d, %d)", n_rows, B, S);
+    return DT_ERR_INVALID;
+  }
+  RotaryArgs a{};
+  if (int rc = fill_rotary(a, rows, n_rows, D, norm, eps, positions, pos_stride_b, n_axes, turns, axis_of_pair, rope, sections, n_sections, rounding, false))
+    return rc;
   int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
   __int128 items = (__int128)B * S * groups;
   if (items * (D / 8) > (1ll << 32) - kThreads || items >= (1ll << 31)) {      // (a grid holds fewer than 2^32 lanes)
     set_error("too many rows");
     return DT_ERR_INVALID;
   }
-  const int per_wg = kThreads / (D / 8);
-  const bool eight = items > (int64_t)kManyWorkgroups * per_wg && a.rows[0].groups % 2 == 0 && a.rows[1].groups % 2 == 0;
-  if (eight) {
-    for (Rows& r : a.rows) r.groups /= 2;
-    groups /= 2;
-    items /= 2;
-  }
-  a.pos = positions;
-  a.pos_sb = pos_stride_b;
+  const bool eight = eight_heads(a, groups, items, D, {&a.rows[0], &a.rows[1]});
   a.S = S;
-  a.n_axes = n_axes;
-  a.norm = norm;
-  a.w16 = (rounding & DT_WEIGHTS_16) != 0;
-  a.eps = eps;
   a.items = (uint32_t)items;
   a.by_groups = quotient_by((int32_t)groups);
   a.by_s = quotient_by(S);
-  const dim3 grid((unsigned)((items + per_wg - 1) / per_wg)), block(kThreads);
-  const hipStream_t st = (hipStream_t)stream;
-  const bool half = (rounding & DT_IO_FP16) != 0, halves = rope == DT_ROPE_HALVES;
-  const bool rms = norm == DT_NORM_RMS;
-#define DT_LAUNCH_L(D, half, halves, rms)                                                                                  \
-  do {                                                                                                                       \
-    if (eight) hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves, 8, rms>), grid, block, 0, st, a);             \
-    else hipLaunchKernelGGL((qk_norm_rope_axes_kernel<D, half, halves, 4, rms>), grid, block, 0, st, a);                   \
-  } while (0)
-#define DT_LAUNCH(D, half, halves)                          \
-  do {                                                      \
-    if (rms) DT_LAUNCH_L(D, half, halves, true);          \
-    else DT_LAUNCH_L(D, half, halves, false);               \
-  } while (0)
-#define DT_LAUNCH_D(D)                                                           \
-  do {                                                                           \
-    if (half && halves) DT_LAUNCH(D, true, true);                                \
-    else if (half) DT_LAUNCH(D, true, false);                                    \
-    else if (halves) DT_LAUNCH(D, false, true);                                  \
-    else DT_LAUNCH(D, false, false);                                             \
-  } while (0)
-  if (D == 128) DT_LAUNCH_D(128);
-  else DT_LAUNCH_D(64);
-#undef DT_LAUNCH_D
-#undef DT_LAUNCH
-#undef DT_LAUNCH_L
+  DT_LAUNCH_ROTARY(qk_norm_rope_axes_kernel);
   return hip_fail(hipGetLastError(), "qk_norm_rope_axes launch");
+}
+
+extern "C" int dt_prepare_pages(const dt_rotary_rows* rows, const void* v, const int64_t* v_strides, int32_t T, int32_t D, int32_t norm, float eps,
+                                const int32_t* positions, int32_t n_axes, const uint64_t* turns, const uint8_t* axis_of_pair, int32_t rope,
+                                const int32_t* sections, int32_t n_sections, int32_t rounding, const dt_pages* pages, const int64_t* slots,
+                                void* stream) {
+  if (!rows || T <= 0) {
+    set_error("need q, k and a positive number of tokens (got %d)", T);
+    return DT_ERR_INVALID;
+  }
+  PagedArgs a{};
+  if (int rc = check_pages(pages, D, a.to)) return rc;
+  if (int rc = fill_rotary(a, rows, 2, D, norm, eps, positions, 0, n_axes, turns, axis_of_pair, rope, sections, n_sections, rounding, true)) return rc;
+  if (!v || !v_strides || !slots || !aligned16(v) || ((v_strides[0] | v_strides[1]) & 7)) {
+    set_error("v, its strides and slots must be non-null, v 16-byte aligned with strides that are multiples of 8 elements");
+    return DT_ERR_INVALID;
+  }
+  a.v = a.rows[1];
+  a.v.x = static_cast<const uint16_t*>(v);
+  a.v.ss = v_strides[0];
+  a.v.sh = v_strides[1];
+  a.slots = slots;
+  int64_t groups = (int64_t)a.rows[0].groups + 2 * a.rows[1].groups;
+  __int128 items = (__int128)T * groups;
+  if (items * (D / 8) > (1ll << 32) - kThreads || items >= (1ll << 31)) {
+    set_error("too many rows");
+    return DT_ERR_INVALID;
+  }
+  const bool eight = eight_heads(a, groups, items, D, {&a.rows[0], &a.rows[1], &a.v});
+  a.S = T;
+  a.items = (uint32_t)items;
+  a.by_groups = quotient_by((int32_t)groups);
+  a.by_s = quotient_by(T);
+  DT_LAUNCH_ROTARY(prepare_pages_kernel);
+  return hip_fail(hipGetLastError(), "prepare_pages launch");
 }

@@ -622,6 +622,66 @@ int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, 
                          const uint8_t* axis_of_pair, int32_t rope, const int32_t* sections, int32_t n_sections,
                          int32_t rounding, void* stream);
 
+/*
+ * A cache of pages that several requests share: keys and values of `page_size` tokens a page (a multiple of 16), [page, token, key head, D] with
+ * element strides {page, token, head} of their own (multiples of 8; token strides 0..2^23), bfloat16 or IEEE half, k and v 16-byte aligned.  A request's
+ * token j lies in page table[j / page_size], at its place j % page_size; slot = page * page_size + place.  n_pages * page_size < 2^31.
+ * No counterpart in the reference, whose caches hold whole blocks (core/cache.py:75-84).
+ */
+typedef struct {
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3];
+  int32_t n_pages, page_size;
+} dt_pages;
+
+/*
+ * Pages for the new tokens of B requests; everything is device memory.  Request b has lens[b] tokens (clamped to 0..width * page_size) and gets new_lens[b]
+ * (below 0: 0) more, whose rows lie one request behind the other:
+ *   cu_seqlens[0] = 0, cu_seqlens[b + 1] = min(cu_seqlens[b] + new_lens[b], n_tokens)   (rows behind n_tokens are not there)
+ * tables: int32, row b at b * table_stride, `width` entries.  A request holds the ceil(len / page_size) first entries of its row, whatever stands behind
+ * them; a page 0..n_pages-1 that no request holds is free.  Requests take what they need of the free pages in order, the lowest ones first; one whose
+ * tokens do not fit its row gets none, and from the first one that finds too few on, none gets any.  served[b] = 1 where request b has pages for
+ * all of its tokens, and then tables (in place, new entries only) and lens_out[b] (its new length) say so; else served[b] = 0, lens_out[b] its old length.
+ * slots[t], t < n_tokens: where the keys and values of row t go; -1 for rows of requests that are not served, rows behind the last one, and tokens whose
+ * entry is no page.  lens_out may be lens.  At most 2048 requests, 2^20 pages, 2^29 tokens a request, 2^30 new ones.
+ * No counterpart in the reference.
+ */
+int dt_plan_pages(int32_t* tables, int64_t table_stride, int32_t width, const int32_t* lens, const int32_t* new_lens, int32_t B,
+                  int32_t n_pages, int32_t page_size, int32_t n_tokens, int32_t* lens_out, int32_t* cu_seqlens, int64_t* slots,
+                  uint8_t* served, void* stream);
+
+/*
+ * Keys and values into their slots: row t of k and v [T,Hk,D] (HOST strides {token, head}) goes to slots[t] (device int64 [T]); a slot that is none of
+ * the pool's is left out.  Rows that share a slot leave either one's elements there.  Stands beside proCache.store_block (core/cache.py:75-84).
+ */
+int dt_append_pages(const void* k, const void* v, const int64_t* k_strides, const int64_t* v_strides, int32_t T, int32_t Hk, int32_t D,
+                    const dt_pages* pages, const int64_t* slots, void* stream);
+
+/*
+ * dt_qk_norm_rope_axes whose keys go straight into their slots, and the values with them, in one launch: q [T,H,D] (rows[0], packed: stride_b is not
+ * read) into its y, k [T,Hk,D] (rows[1], whose y is not read) and v as in dt_append_pages.  positions: device int32 [T, n_axes].  Values are copied.
+ * executor/hunyuanvideo/hunyuan_transformer.py:177-191 and executor/step/blocks.py:66-75 with the writes of core/cache.py:75-84.
+ */
+int dt_prepare_pages(const dt_rotary_rows* rows, const void* v, const int64_t* v_strides, int32_t T, int32_t D, int32_t norm, float eps,
+                     const int32_t* positions, int32_t n_axes, const uint64_t* turns, const uint8_t* axis_of_pair, int32_t rope,
+                     const int32_t* sections, int32_t n_sections, int32_t rounding, const dt_pages* pages, const int64_t* slots, void* stream);
+
+/*
+ * Attention of each request's new tokens over its pages.  q [T,H,D] (HOST strides {token, head}) holds the new tokens of request b in rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1], the last ones of its lens[b] tokens: row i of n stands at position lens[b] - n + i and sees what `window`
+ * (q_begin and kv_lens are not read) leaves of the keys 0 .. lens[b] - 1, as in dt_attn_window_fwd.  H is a multiple of Hk.
+ * cu_seqlens (int32 [B + 1], never falling), lens (int32 [B]) and tables (int32, row b at b * table_stride, `width` entries) are device memory, read by the
+ * kernel, which clamps lengths and boundaries to what is there; an entry that is no page of the pool reads as keys and values of zeros.
+ * out [T,H,D] contiguous in the dtype of q, lse fp32 [H,T]; a row that sees no key, or that no request owns, gets out = 0, lse = -inf.  A masked key
+ * adds nothing, whatever it and its value hold.  out may be q where that is contiguous.
+ * max_seqlen_q: the most rows a request has, which the launch is made for; requests with more come out right, only later.
+ * workspace and counters as for dt_attn_window_fwd; nothing is cut without either.  No counterpart in the reference.
+ */
+int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
+                      const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
+                      const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale, int32_t flags,
+                      void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
