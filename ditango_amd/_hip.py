@@ -631,6 +631,9 @@ def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: f
 # A cache of pages that several requests share
 # ---------------------------------------------------------------------------------------------
 
+CAPTURED_COUNTERS = 1 << 14      # words: 16 384 workgroups of few rows, or 2048 of 256
+
+
 def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, n_tokens: int, n_pages: int, page_size: int, in_place: bool):
     """(lens, cu_seqlens, slots, served) of ``dt_plan_pages``; ``tables`` are extended in place, and with ``in_place`` ``lens`` as well."""
     return _host().plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place, _stream_at(tables, "tables"))
@@ -651,5 +654,10 @@ def attn_pages_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    lse: Optional[torch.Tensor] = None):
     """(out, lse) of ``dt_attn_pages_fwd``; -1 stands for a border that is not there."""
     stream = _stream_at(q, "q")
+    workspace, counters = attn_scratch(q.device)
+    if counters is None:
+        counters = _stream_counters(q.device, 1)
+    if counters is None:          # under capture: the graph's own, which every replay clears
+        counters = torch.zeros(CAPTURED_COUNTERS, dtype=torch.int32, device=q.device)
     return _host().attn_pages(q, k_pages, v_pages, tables, lens, cu_seqlens, max_seqlen_q, left, right, frame, sinks, float(softmax_scale), out, lse,
-                              None, None, stream)
+                              workspace, counters, stream)

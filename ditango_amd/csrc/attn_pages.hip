@@ -1,17 +1,28 @@
 // Attention of requests' new tokens over the pages of a cache that they share (gfx950).
 //
 // Row i of the n new tokens of a request with len tokens stands at position len - n + i among its keys; which of them it sees is a window as of
-// attn_window.hip, and the result is a state (out, lse) like its.
+// attn_window.hip, and the result is a state (out, lse) like its.  The rows' arithmetic is attn_rows.h's, in the same two forms:
+//   * shared tiles: 256 rows of one request and key head a workgroup, which walks the 64-key tiles that some row sees;
+//   * few rows: 32 rows, whose four wavefronts take 32-key tiles in turn.
+// Requests of at most kFewRows rows (new tokens x query heads of a key head) take the second, the others the first; a batch with both is two launches.
+//
+// Which page holds a tile is read by scalar loads one tile ahead, so that no tile waits for it; a page is a multiple of 16 tokens, and 16 rows of a tile
+// are what a load's descriptor covers.  No host knows the lengths, so every workgroup finds its share of the work by itself: it reads all lengths and
+// boundaries, a lane a request, prices some lengths of parts to cut the keys into, and numbers row tiles, key heads and parts through (`find`).
 #include <algorithm>
 #include <cmath>
 
-#include "attn_tiles.h"
+#include "attn_rows.h"
 #include "dt_common.h"
 
 namespace dt {
 namespace {
 
 constexpr int32_t kMostTokens = 1 << 29;   // positions, spans and lengths: their sums stay in 32 bits
+constexpr int kXcds = 8;
+constexpr int kWavesFew = 4;
+constexpr int kFewRows = 96;
+constexpr int kMostWays = 64;              // parts of an item
 
 struct PagesArgs {
   const uint16_t* q;
@@ -25,82 +36,772 @@ struct PagesArgs {
   int32_t width, B, T, H, Hk, group;
   int32_t left, right;          // spans in tokens; -1: no border
   int32_t frame, sinks;
-  Quotient by_frame;
+  Quotient by_group, by_frame;
   float scale_log2;
+  // ---- a launch's share
+  int32_t least_rows, most_rows;   // of the requests that it takes
+  int32_t fill;                    // it writes the rows that no request owns
+  int32_t block;                   // row tiles of a key head that run one behind the other on an XCD
+  int32_t groups;                  // of `block` workgroups, that the grid has
+  int32_t cut_groups;              // up to how many of them items may be cut into parts
+  float slots;                     // workgroups at once
+  float step, once, part;          // us: of a step of keys, of a workgroup beside them, of a part's way to memory and back
+  float* part_out;                 // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
+  float* part_ml;
+  uint32_t* counters;              // of an item's parts that are done, zero before and after the launch
 };
 
-// One wavefront a row and head: a lane has a key's score, then its columns.
+// The rows of a request, by the names of attn_rows.h
+struct Queries {
+  const uint16_t* q;
+  int64_t q_sb, q_ss, q_sh;
+  int32_t Sq, rows, group, left, right, frame, sinks, q_begin;
+  Quotient by_group, by_frame;
+  float scale_log2;
+};
+__device__ __forceinline__ Queries queries_of(const PagesArgs& a, int begin, int n) {
+  return Queries{a.q + begin * a.q_ss, 0, a.q_ss, a.q_sh, n, n * a.group, a.group, a.left, a.right, a.frame, a.sinks, -1, a.by_group, a.by_frame, a.scale_log2};
+}
+
+// A workgroup's work: row tile `row0` .. of a request and key head, and of its keys the part [tiles part / ways, tiles (part + 1) / ways)
+struct Work {
+  int b, begin, n, len;         // request, its first row, its rows' and its keys' number
+  int hk, row0, part, ways;
+  int first, apart;             // slot of the item's first part, slots between its parts
+  template <typename List>
+  __device__ __forceinline__ void share(List& list) const {      // (2^24 tiles, 64 parts: 32 bits hold the products)
+    const uint32_t n = list.end;
+    if (ways > 1) {
+      list.begin = (int)(n * part / ways);
+      list.end = (int)(n * (part + 1) / ways);
+    }
+  }
+};
+
+// a lane's request
+struct Request {
+  int begin, n, len, tiles, steps;     // ... row tiles, and steps of keys that the last of them sees
+};
+template <int kRows, int kKeys>
+__device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
+  Request r = {};
+  if (b >= a.B) return r;
+  r.begin = min(max(a.cu[b], 0), a.T);
+  r.n = max(min(max(a.cu[b + 1], 0), a.T) - r.begin, 0);
+  r.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.kv.page);
+  const int rows = r.n * a.group;
+  if (rows < a.least_rows || rows > a.most_rows) return r;
+  r.tiles = (rows + kRows - 1) / kRows;
+  const Queries qs = queries_of(a, 0, r.n);
+  const Span first = span_of(qs, r.len, query_of(qs, (r.tiles - 1) * kRows)), last = span_of(qs, r.len, r.n - 1);
+  const int sinks = min(a.sinks, last.hi);
+  r.steps = (sinks + max(last.hi - max(first.lo, sinks), 0) + kKeys - 1) / kKeys;
+  return r;
+}
+__device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+// Parts of an item of that many steps, where a part has 1 / inv of them.  (In floating point: nothing depends on it but that all agree.)
+__device__ __forceinline__ int ways_of(int steps, float inv) { return min(max((int)__builtin_ceilf((float)steps * inv - 0.001f), 1), kMostWays); }
+
+// Finds workgroup blockIdx.x's work; false: it has none.  [*from, *to): the rows that requests own.
+template <int kRows, int kKeys>
+__device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int* to) {
+  const int lane = threadIdx.x & 63;
+  // (index of a group, place in it): groups go round the XCDs, a group's workgroups one behind the other on one
+  const int xcd = blockIdx.x % kXcds, i = blockIdx.x / kXcds, g = xcd + kXcds * (i / a.block), j = i % a.block;
+  Request r = request_of<kRows, kKeys>(a, lane);
+  int lo = r.n > 0 ? r.begin : a.T, hi = r.begin + r.n, most = r.steps;
+  float work = (float)r.tiles * (float)r.steps, items = (float)r.tiles;
+  for (int b0 = 64; b0 < a.B; b0 += 64) {
+    const Request x = request_of<kRows, kKeys>(a, b0 + lane);
+    if (x.n > 0) lo = min(lo, x.begin);
+    hi = max(hi, x.begin + x.n);
+    most = max(most, x.steps);
+    work += (float)x.tiles * (float)x.steps;
+    items += (float)x.tiles;
+  }
+  *to = wave_max(hi);
+  *from = min(-wave_max(-lo), *to);
+  most = wave_max(most);
+  work = wave_sum(work) * (float)a.Hk;
+  // steps of a part, as 1 / them
+  float inv = 0.f;
+  if (a.cut_groups > 0 && most > 1) {
+    if (a.B <= 64) {
+      // a lane prices 1 .. 64 parts of the longest item
+      const float ways = (float)(lane + 1), steps = __builtin_ceilf((float)most / ways), mine = 1.f / steps;
+      float n = 0.f;
+      for (int b = 0; b < a.B; ++b) {
+        const int tiles = lane_value(r.tiles, b);
+        if (tiles > 0) n += (float)((tiles + a.block - 1) / a.block) * (float)ways_of(lane_value(r.steps, b), mine);
+      }
+      n *= (float)a.Hk;
+      const bool fits = lane == 0 || n <= (float)a.cut_groups;
+      n *= (float)a.block;
+      const float once = steps * a.step + a.once;
+      float us = n <= a.slots ? once : min(__builtin_ceilf(n / a.slots) * once, (work * a.step + n * a.once) / a.slots + 0.5f * once);
+      if (lane > 0) us += 2.f + 0.4f * ways + n * a.part;
+      if (!fits) us = INFINITY;
+      float best = us;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) best = fminf(best, __shfl_xor(best, d));
+      const int at = __builtin_ctzll(__ballot(us == best));
+      inv = at == 0 ? 0.f : __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, mine), at));
+    } else {
+      // room for cuts beside one part of every item, shared out by their steps
+      items = wave_sum(items) * (float)a.Hk;
+      const float room = 0.99f * min((float)a.cut_groups, 2.f * a.slots) - items;      // (below what there is by more than the sums' roundings)
+      if (room > 0.f) inv = 1.f / max(max(work / room, (float)most / kMostWays), 8.f);
+    }
+  }
+  // groups in front of a lane's request
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    if (b0 > 0) r = request_of<kRows, kKeys>(a, b0 + lane);
+    const int blocks = (r.tiles + a.block - 1) / a.block, ways = ways_of(r.steps, inv);
+    const int mine = r.tiles > 0 ? a.Hk * blocks * ways : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(sum, d);
+      if (lane >= d) sum += y;
+    }
+    const uint64_t passed = __ballot(before + sum <= g);
+    if (passed == ~0ull) {
+      before += lane_value(sum, 63);
+      continue;
+    }
+    const int at = __builtin_ctzll(~passed);
+    const int group0 = before + lane_value(sum, at) - lane_value(mine, at), nblk = lane_value(blocks, at);
+    w.b = b0 + at;
+    w.begin = lane_value(r.begin, at);
+    w.n = lane_value(r.n, at);
+    w.len = lane_value(r.len, at);
+    w.ways = lane_value(ways, at);
+    const int unit = (g - group0) / nblk, blk = (g - group0) % nblk, tile = blk * a.block + j, tiles = lane_value(r.tiles, at);
+    w.hk = unit / w.ways;
+    w.part = unit % w.ways;
+    w.row0 = (tiles - 1 - tile) * kRows;      // the last ones first: under a causal border they see most
+    w.first = ((group0 + w.hk * w.ways * nblk + blk) * a.block) + j;
+    w.apart = nblk * a.block;
+    for (int* x : {&w.hk, &w.part, &w.row0, &w.first}) *x = __builtin_amdgcn_readfirstlane(*x);
+    return tile < tiles;
+  }
+  return false;
+}
+
+// Zeros, and -inf, in the rows that no request owns.
+__device__ __forceinline__ void fill_rows(const PagesArgs& a, int D, int from, int to) {
+  const int row = a.H * D / 8;          // 16-byte chunks
+  for (int r = blockIdx.x; r < a.T - (to - from); r += gridDim.x) {
+    const int64_t t = r < from ? r : r + (to - from);
+    for (int c = threadIdx.x; c < row; c += blockDim.x) *reinterpret_cast<u32x4*>(a.out + (t * row + c) * 8) = u32x4{0, 0, 0, 0};
+    for (int h = threadIdx.x; h < a.H; h += blockDim.x) a.lse[(int64_t)h * a.T + t] = -INFINITY;
+  }
+}
+
+// A request's keys (0) and values (1) of a key head.
+struct Keys {
+  const uint16_t* base[2];
+  int64_t sp[2], ss[2];
+  const __attribute__((address_space(4))) int32_t* table;      // (constant while the launch runs: scalar loads)
+  int len, page, n_pages;
+  Quotient by_page;
+  __device__ __forceinline__ Keys(const PagesArgs& a, const Work& w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      base[i] = a.kv.base[i] + w.hk * a.kv.sh[i];
+      sp[i] = a.kv.sp[i];
+      ss[i] = a.kv.ss[i];
+    }
+    table = (const __attribute__((address_space(4))) int32_t*)(a.tables + w.b * a.table_stride);
+    len = w.len;
+    page = a.kv.page;
+    n_pages = a.kv.n_pages;
+    by_page = a.kv.by_page;
+  }
+  // Row of key j < len, each lane's own; null where its entry is no page.
+  __device__ __forceinline__ const uint16_t* row(int i, int j) const {
+    const int at = (int)quotient(j, by_page), p = reinterpret_cast<const int32_t*>(reinterpret_cast<uintptr_t>(table))[at];
+    return (uint32_t)p < (uint32_t)n_pages ? base[i] + p * sp[i] + (int64_t)(j - at * page) * ss[i] : nullptr;
+  }
+};
+
+// 16 keys of a tile, which are in one page.
+struct Sixteen {
+  int id, place;                // page, and the first key's place in it
+  int left;                     // keys from the first one to the last of the request; not above 0: none of them is there
+  __device__ __forceinline__ void find(const Keys& ks, int key, bool there) {
+    key = __builtin_amdgcn_readfirstlane(key);
+    left = there ? ks.len - key : 0;
+    key = left > 0 ? key : 0;
+    const int at = (int)quotient(key, ks.by_page);
+    place = key - at * ks.page;
+    id = ks.table[__builtin_amdgcn_readfirstlane(at)];
+  }
+  // rows behind the last key, and those of no page, arrive as zeros
+  template <int D>
+  __device__ __forceinline__ u32x4 rsrc(const Keys& ks, int i) const {
+    const bool there = (left > 0) & ((uint32_t)id < (uint32_t)ks.n_pages);
+    const uint16_t* from = ks.base[i] + (there ? id : 0) * ks.sp[i] + place * ks.ss[i];
+    return make_rsrc(from, there ? (uint32_t)(min(left, 16) - 1) * (2 * (uint32_t)ks.ss[i]) + 2 * D : 0u);
+  }
+};
+
+// What a lane needs to bring its 16 bytes of every 1 KB block of a tile; blocks are numbered through the tile, kOf of them a sixteen.
+template <int D, int NKB>
+struct PageLoader {
+  typedef Tiles<D, NKB> T;
+  static constexpr int kOf = 16 / T::kBlockRows;
+  uint32_t k_row, k_chunk, v_off, k_block, v_block;
+  __device__ __forceinline__ void open(const Keys& ks, int lane) {
+    const int row = lane / T::kRowLanes, chunk = lane % T::kRowLanes;
+    k_row = row * (uint32_t)(2 * ks.ss[0]);
+    k_chunk = 16 * (chunk ^ T::swz_k(row));
+    v_off = row * (uint32_t)(2 * ks.ss[1]) + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
+    k_block = T::kBlockRows * (uint32_t)(2 * ks.ss[0]);
+    v_block = T::kBlockRows * (uint32_t)(2 * ks.ss[1]);
+  }
+  __device__ __forceinline__ void issue_k(const u32x4& r, int blk, uint32_t to) const {
+    load_block_to_lds(r, k_row + (k_chunk ^ (64u * (blk & T::kBlockXor))) + (blk % kOf) * k_block, 0, to + blk * 1024);
+  }
+  __device__ __forceinline__ void issue_v(const u32x4& r, int blk, uint32_t to) const {
+    load_block_to_lds(r, v_off + (blk % kOf) * v_block, 0, to + blk * 1024);
+  }
+};
+
+// Parts as they lie in the registers: 4 floats a lane, (register group) x (lane).  `at`: of a row's column d.
+template <int D>
+__device__ __forceinline__ int part_at(int row, int d) { return ((d >> 3) * 64 + 32 * ((d >> 2) & 1) + row) * 4 + (d & 3); }
+
+// The 32 rows of a wavefront without matrix instructions, visible keys of [begin, end) only, from the maxima (in powers of two) and inverse sums that lane r
+// and r + 32 hold of row r: a lane has a key's score, then its columns.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(64) void attn_pages_kernel(const PagesArgs a) {
+__device__ __forceinline__ void rows_one_by_one(const PagesArgs& a, const Work& w, const Queries& qs, const Keys& ks, int row0, float m, float inv, int begin,
+                                                int end, float* part, int lane) {
   typedef Elem<kHalf> E;
   constexpr int kCols = D / 64;
-  const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y;
-  int b = -1, begin = 0, n = 0;
-  for (int i = 0; i < a.B; ++i) {
-    const int lo = min(max(a.cu[i], 0), a.T), hi = min(max(a.cu[i + 1], 0), a.T);
-    if (row >= lo && row < hi) {
-      b = i;
-      begin = lo;
-      n = hi - lo;
-      break;
-    }
-  }
-  typename E::t* out = reinterpret_cast<typename E::t*>(a.out) + ((int64_t)row * a.H + head) * D + lane * kCols;
-  float m = -INFINITY, l = 0.f, acc[kCols] = {};
-  if (b >= 0) {
-    const int len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.kv.page);
-    const int x = len - n + row - begin - a.sinks;
-    const int f = x >= 0 ? (int)quotient(x, a.by_frame) : -1 - (int)quotient(-1 - x, a.by_frame);
-    const int start = a.sinks + f * a.frame;
-    const int lo = a.left < 0 ? 0 : max(start - a.left, 0), hi = a.right < 0 ? len : min(max(start + a.right, 0), len);
-    const int hk = head / a.group;
-    const uint16_t* q = a.q + row * a.q_ss + head * a.q_sh;
-    auto place = [&](int j, int i) -> const uint16_t* {      // of key j (0) or its value (1), null where it has no page
-      const int at = (int)quotient(j, a.kv.by_page), p = a.tables[b * a.table_stride + at];
-      if ((uint32_t)p >= (uint32_t)a.kv.n_pages) return nullptr;
-      return a.kv.base[i] + p * a.kv.sp[i] + (int64_t)(j - at * a.kv.page) * a.kv.ss[i] + hk * a.kv.sh[i];
-    };
-    for (int j0 = 0; j0 < hi; j0 += 64) {
-      if (j0 + 64 <= lo && j0 >= a.sinks) continue;
+#pragma unroll 1
+  for (int r = 0; r < 32 && row0 + r < qs.rows; ++r) {
+    const int s = query_of(qs, row0 + r), head = w.hk * a.group + row0 + r - s * a.group;
+    const Span span = uniform_span(qs, ks.len, s);
+    const uint16_t* q = qs.q + s * a.q_ss + head * a.q_sh;
+    const float top = __shfl(m, r), norm = __shfl(inv, r);
+    float acc[kCols] = {};
+#pragma unroll 1
+    for (int j0 = begin; j0 < min(end, span.hi); j0 += 64) {
+      if (j0 + 64 <= span.lo && j0 >= a.sinks) continue;
       const int j = j0 + lane;
-      const bool seen = j < hi && (j >= lo || j < a.sinks);
-      float s = -INFINITY;
+      const bool seen = j < min(end, span.hi) && (j >= span.lo || j < a.sinks);
+      float weight = 0.f;
       if (seen) {
-        s = 0.f;
-        if (const uint16_t* k = place(j, 0))
+        float score = 0.f;
+        if (const uint16_t* k = ks.row(0, j))
+#pragma unroll 1
           for (int d = 0; d < D; d += 8) {
-            const typename E::x8 u = *reinterpret_cast<const typename E::x8*>(q + d), w = *reinterpret_cast<const typename E::x8*>(k + d);
+            const typename E::x8 x = *reinterpret_cast<const typename E::x8*>(q + d), y = *reinterpret_cast<const typename E::x8*>(k + d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float)u[e], (float)w[e], s);
+            for (int e = 0; e < 8; ++e) score = __builtin_fmaf((float)x[e], (float)y[e], score);
           }
-        s *= a.scale_log2;
+        weight = __builtin_amdgcn_exp2f(__builtin_fmaf(score, a.scale_log2, -top));
       }
-      float top = s;
+      uint64_t some = __ballot(seen);
+#pragma unroll 1
+      while (some) {
+        const int i = __builtin_ctzll(some);
+        some &= some - 1;
+        const float wi = __shfl(weight, i);
+        if (const uint16_t* v = ks.row(1, j0 + i))
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-      const float m_new = fmaxf(m, top), ref = m_new > -INFINITY ? m_new : 0.f;
-      const float alpha = __builtin_amdgcn_exp2f(m - ref), w = seen ? __builtin_amdgcn_exp2f(s - ref) : 0.f;
-      m = m_new;
-      float sum = w;
+          for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(wi, (float)reinterpret_cast<const typename E::t*>(v)[lane * kCols + e], acc[e]);
+      }
+    }
+    if (part) {
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-      l = l * alpha + sum;
+      for (int e = 0; e < kCols; ++e) store_device(part + part_at<D>(r, lane * kCols + e), acc[e]);
+    } else {
+      typename E::t* out = reinterpret_cast<typename E::t*>(a.out) + ((int64_t)(w.begin + s) * a.H + head) * D + lane * kCols;
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) acc[e] *= alpha;
-      for (int i = 0; i < 64; ++i) {
-        const int key = j0 + i;
-        if (key >= hi || !(key >= lo || key < a.sinks)) continue;
-        const float wi = __shfl(w, i);
-        if (const uint16_t* v = place(key, 1))
+      for (int e = 0; e < kCols; ++e) out[e] = (typename E::t)(acc[e] * norm);
+    }
+  }
+}
+
+// Whether a tile that some row of the wavefront does not see whole holds infinite or undefined values.
+template <int D, bool kHalf>
+__device__ __forceinline__ bool masked_not_finite(const Keys& ks, const RowState<D, kHalf, 2>& st, const TileList<64>& list, int lane) {
+  typedef RowState<D, kHalf, 2> State;
+  typedef Tiles<D, 2> T;
+  uint32_t over = 0;
+#pragma unroll 1
+  for (int t = list.begin; t < list.end; ++t) {
+    const int k0 = list.key(t);
+    if (st.whole(k0)) continue;
+#pragma unroll 1
+    for (int j = k0 + lane / T::kRowLanes; j < min(k0 + T::kKeys, ks.len); j += T::kBlockRows)
+      if (const uint16_t* v = ks.row(1, j)) over |= State::ones(*reinterpret_cast<const u32x4*>(v + 8 * (lane % T::kRowLanes)));
+  }
+  return __any((over & 0x80008000u) != 0);
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
+  typedef Tiles<D, 2> T;
+  typedef SharedLds<D> S;
+  typedef Elem<kHalf> E;
+  typedef PageLoader<D, 2> L;
+  extern __shared__ __align__(1024) uint8_t lds[];
+  Work w;
+  int own_from, own_to;
+  const bool some = find<kRowsShared, 64>(a, w, &own_from, &own_to);
+  if (a.fill) fill_rows(a, D, own_from, own_to);
+  if (!some) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+  const Queries qs = queries_of(a, w.begin, w.n);
+  const Span all_first = uniform_span(qs, w.len, query_of(qs, w.row0)), all_last = uniform_span(qs, w.len, query_of(qs, min(w.row0 + kRowsShared - 1, qs.rows - 1)));
+  TileList<64> list(qs, all_first, all_last, 0, 1);
+  w.share(list);
+  const int n = list.end - list.begin;
+  const Keys ks(a, w);
+  L ld;
+  ld.open(ks, lane);
+  // A wavefront's blocks of a tile are wave, wave + 8 ..: kPer of them, each of its own sixteen.  Tile t + 1 of K goes with tile t of V.
+  constexpr int kPer = T::kBlocks / kWavesShared;
+  Sixteen of_v[kPer], of_k[kPer], of_next[kPer];
+  int t_next = list.begin;       // whose pages are found next
+  auto look = [&](Sixteen (&x)[kPer]) __attribute__((always_inline)) {
+    const int key = list.key(t_next) + 16 * (wave / L::kOf);
 #pragma unroll
-          for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(wi, (float)reinterpret_cast<const typename E::t*>(v + lane * kCols)[e], acc[e]);
+    for (int i = 0; i < kPer; ++i) x[i].find(ks, key + 16 * i * (kWavesShared / L::kOf), t_next < list.end);
+    ++t_next;
+  };
+  auto load_k = [&](int pair) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      ld.issue_k(of_k[i].template rsrc<D>(ks, 0), wave + kWavesShared * i, lds0 + pair_at<D>(pair) + T::kBytes);
+      of_v[i] = of_k[i];
+      of_k[i] = of_next[i];
+    }
+    look(of_next);
+  };
+  auto load_pair = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ld.issue_v(of_v[i].template rsrc<D>(ks, 1), wave + kWavesShared * i, lds0 + pair_at<D>(t));
+    load_k(t);
+  };
+  RowState<D, kHalf, 2> st;
+  const int row0 = w.row0 + 32 * wave;
+  if (n > 0) {
+    look(of_k);
+    look(of_next);
+    const uint16_t* q = qs.q + (int64_t)w.hk * a.group * a.q_sh;
+    queries_to_lds<D>(lds0, row0, wave, lane, [&](int r) __attribute__((always_inline)) {
+      const int row = min(r, qs.rows - 1);
+      const int s = query_of(qs, row), g = row - s * a.group;
+      return q + s * a.q_ss + g * a.q_sh;
+    });
+    load_k(-1);
+    load_pair(0);
+    load_pair(1);
+  }
+  st.open(qs, 0, w.hk, row0, w.len, lane, false);
+  if (n > 0) walk_tiles<D, kHalf>(st, lds, list, all_first, all_last, wave, lane, load_pair);
+  const int col = lane & 31, hh = lane >> 5;
+  float m = st.m_ref * st.c, l = st.l_run + __shfl_xor(st.l_run, 32);
+  float undefined = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) undefined = __builtin_fmaf(st.o[i][r], 0.f, undefined);
+  bool hurt = __builtin_expect(__any(undefined != 0.f && l == l), 0) && masked_not_finite<D, kHalf>(ks, st, list, lane);
+  const bool live = row0 + col < qs.rows;
+  if (w.ways > 1) {
+    // A part's sums, fp32; the wavefront that completes the parts of its rows adds them all up, in order.
+    constexpr int kPartFloats = 32 * D;
+    const int mine = w.first + w.part * w.apart;
+    float* part = a.part_out + ((int64_t)mine * kWavesShared + wave) * kPartFloats;
+    if (hurt) {
+      rows_one_by_one<D, kHalf>(a, w, qs, ks, row0, m, 0.f, list.begin < list.end ? list.key(list.begin) : 0,
+                                list.begin < list.end ? list.key(list.end - 1) + T::kKeys : 0, part, lane);
+    } else {
+      const Rsrc to = buffer_of(part, kPartFloats * 4);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          u32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(uint32_t, (float)st.o[i][4 * g + e]);
+          __builtin_amdgcn_raw_buffer_store_b128(x, to, (4 * i + g) * 1024 + lane * 16, 0, kDevice);
+        }
+    }
+    float* ml = a.part_ml + (((int64_t)mine * kWavesShared + wave) * 32 + col) * 2;
+    if (hh == 0) {
+      store_device(ml, m);
+      store_device(ml + 1, l);
+    }
+    wait_loads();                // (stores as well)
+    int done = 0;
+    if (lane == 0) {
+      uint32_t* counter = a.counters + (int64_t)w.first * kWavesShared + wave;
+      done = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
+      if (done) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!__builtin_amdgcn_readfirstlane(done)) return;
+    asm volatile("" ::: "memory");
+    const float* mls = a.part_ml + (((int64_t)w.first * kWavesShared + wave) * 32 + col) * 2;
+    const int64_t ml_apart = (int64_t)w.apart * kWavesShared * 64;
+    float top = -INFINITY;
+    for (int p = 0; p < w.ways; ++p) top = fmaxf(top, load_device(mls + p * ml_apart));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[i][r] = 0.f;
+    l = 0.f;
+#pragma unroll 1
+    for (int p = 0; p < w.ways; ++p) {
+      const float lp = load_device(mls + p * ml_apart + 1), wp = weight_of(load_device(mls + p * ml_apart), lp, top);
+      const Rsrc from = buffer_of(a.part_out + ((int64_t)(w.first + p * w.apart) * kWavesShared + wave) * kPartFloats, kPartFloats * 4);
+      l = __builtin_fmaf(wp, lp, l);
+      f32x4 x[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, i * 1024 + lane * 16, 0, kDevice));
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[i / 4][4 * (i % 4) + e] = __builtin_fmaf(wp, x[i][e], st.o[i / 4][4 * (i % 4) + e]);
+    }
+    m = top;
+    hurt = false;
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;      // (an undefined sum stays one)
+  if (hh == 0 && live) {
+    const int s = query_of(qs, row0 + col), g = row0 + col - s * a.group;
+    a.lse[(int64_t)(w.hk * a.group + g) * a.T + w.begin + s] = l != 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+  }
+  if (__builtin_expect(hurt, 0)) {
+    rows_one_by_one<D, kHalf>(a, w, qs, ks, row0, m, inv, 0, w.len, nullptr, lane);
+    return;
+  }
+  // Rows of the result through the LDS, so that a store covers whole lines: half of the columns at a time.
+  uint8_t* stage = lds + S::kStage + wave * 32 * D;
+  constexpr int kChunks = D / 16, kPass = 64 / kChunks;       // 16-byte chunks of half a row, rows of a store
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        typename E::x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(st.o[half * (D / 64) + i][4 * g + e] * inv);
+        *reinterpret_cast<typename E::x4*>(stage + col * D + (((4 * i + g) ^ S::swz_o(col)) << 4) + 8 * hh) = h;
+      }
+#pragma unroll
+    for (int i = 0; i < 32 / kPass; ++i) {
+      const int r = i * kPass + lane / kChunks, chunk = lane % kChunks;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * D + ((chunk ^ S::swz_o(r)) << 4));
+      const int row = row0 + r;
+      if (row < qs.rows) {
+        const int s = query_of(qs, row), g = row - s * a.group;
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(a.out + ((int64_t)(w.begin + s) * a.H + w.hk * a.group + g) * D + half * (D / 2) + 8 * chunk));
       }
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+}
+
+// Few rows: as attn_window.hip's, a wavefront takes every fourth tile of its item, or of a part of it, K of the next tile sent for before the softmax of
+// this one, V of the next behind its values; the states of the four meet in the LDS, those of parts in memory, where the last part adds them up.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
+  constexpr int W = kWavesFew;
+  typedef Tiles<D, 1> T;
+  typedef Elem<kHalf> E;
+  typedef PageLoader<D, 1> L;
+  extern __shared__ __align__(1024) uint8_t lds[];
+  Work w;
+  int own_from, own_to;
+  const bool some = find<kRowsFew, 32 * W>(a, w, &own_from, &own_to);
+  if (a.fill) fill_rows(a, D, own_from, own_to);
+  if (!some) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 31, hh = lane >> 5;
+  const Queries qs = queries_of(a, w.begin, w.n);
+  RowState<D, kHalf, 1> st;
+  st.open(qs, 0, w.hk, w.row0, w.len, lane, true);
+  TileList<T::kKeys> list(qs, st.first, st.last, 0, 1);
+  w.share(list);                // ... every W-th tile
+  const uint8_t* kt = lds + wave * FewLds<D, W>::kTile;
+  const uint8_t* vt = kt + T::kBytes;
+  const uint32_t kt0 = (uint32_t)(uintptr_t)(lds_ptr_t)(lds + wave * FewLds<D, W>::kTile);
+  const Keys ks(a, w);
+  L ld;
+  ld.open(ks, lane);
+  Sixteen here[2], next[2];
+  auto look = [&](Sixteen (&x)[2], int t) __attribute__((always_inline)) {
 #pragma unroll
-  for (int e = 0; e < kCols; ++e) out[e] = (typename E::t)(acc[e] * inv);
-  if (lane == 0) a.lse[(int64_t)head * a.T + row] = l != 0.f ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
+    for (int i = 0; i < 2; ++i) x[i].find(ks, list.key(t) + 16 * i, t < list.end);
+  };
+  auto load_k = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x4 r = x[i].template rsrc<D>(ks, 0);
+#pragma unroll
+      for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_k(r, blk, kt0);
+    }
+  };
+  auto load_v = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const u32x4 r = x[i].template rsrc<D>(ks, 1);
+#pragma unroll
+      for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_v(r, blk, kt0 + T::kBytes);
+    }
+  };
+  int t = list.begin + wave;
+  if (t < list.end) {
+    look(here, t);
+    look(next, t + W);
+    load_k(here);
+    load_v(here);
+  }
+  for (; t < list.end; t += W) {
+    const int k0 = list.key(t);
+    const bool masked = !st.whole(k0);
+    f32x16 s[1];
+    typename E::x8 p[1][2];
+    wait_oldest<T::kBlocks>();
+    st.scores(kt, s);
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");      // (the tile has been read)
+    load_k(next);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) here[i] = next[i];
+    look(next, t + 2 * W);
+    st.softmax(s, p, k0, masked, lane);
+    wait_oldest<T::kBlocks>();
+    if (masked && st.any_not_finite(vt, lane)) st.values_not_finite(vt, p, k0, lane);
+    else st.values(vt, p);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    load_v(here);
+  }
+  // The states as they lie in the registers; a wavefront then adds up its share of the columns.
+  float l = st.l_run + __shfl_xor(st.l_run, 32);
+  wait_loads();
+  float* slot = reinterpret_cast<float*>(lds + wave * FewLds<D, W>::kTile) + lane * 4;
+  float* ml = reinterpret_cast<float*>(lds + FewLds<D, W>::kBytes);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      f32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = st.o[i][4 * g + e];
+      *reinterpret_cast<f32x4*>(slot + (4 * i + g) * 256) = x;
+    }
+  if (hh == 0) {
+    ml[wave * 64 + col] = st.m_ref * st.c;
+    ml[wave * 64 + 32 + col] = l;
+  }
+  __syncthreads();
+  float m[W], weight[W], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    m[i] = ml[i * 64 + col];
+    top = fmaxf(top, m[i]);
+  }
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const float li = ml[i * 64 + 32 + col];
+    weight[i] = weight_of(m[i], li, top);
+    l = __builtin_fmaf(weight[i], li, l);
+  }
+  constexpr int kCols = D / 8 / W, kSome = 4;          // register groups of a wavefront's share, parts under way together
+  f32x4 sum[kCols];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + j * FewLds<D, W>::kTile) + lane * 4 + (wave * kCols + i) * 256);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(weight[j], x[e], sum[i][e]);     // (a weight of 0 keeps what is undefined: some row's visible key is)
+    }
+  }
+  if (w.ways > 1) {
+    constexpr int kPartFloats = kRowsFew * D;
+    const int64_t mine = w.first + w.part * w.apart;
+    const Rsrc to = buffer_of(a.part_out + mine * kPartFloats, kPartFloats * 4);
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), to, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice);
+    if (wave == 0 && hh == 0) {
+      store_device(a.part_ml + (mine * kRowsFew + col) * 2, top);
+      store_device(a.part_ml + (mine * kRowsFew + col) * 2 + 1, l);
+    }
+    int* flag = reinterpret_cast<int*>(lds + FewLds<D, W>::kFlag);
+    wait_loads();                // (stores as well)
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t* counter = a.counters + w.first;
+      const bool last = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
+      if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *flag = last;
+    }
+    __syncthreads();
+    if (!*flag) return;
+    const float* mls = a.part_ml + ((int64_t)w.first * kRowsFew + col) * 2;
+    top = -INFINITY;
+    for (int p0 = 0; p0 < w.ways; p0 += kSome) {
+      float x[kSome];
+#pragma unroll
+      for (int p = 0; p < kSome; ++p) x[p] = load_device(mls + (int64_t)min(p0 + p, w.ways - 1) * w.apart * (2 * kRowsFew));
+#pragma unroll
+      for (int p = 0; p < kSome; ++p) top = fmaxf(top, x[p]);
+    }
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+    for (int p0 = 0; p0 < w.ways; p0 += kSome) {
+      float pm[kSome], pl[kSome];
+      f32x4 x[kSome][kCols];
+#pragma unroll
+      for (int p = 0; p < kSome; ++p) {
+        const int64_t at = (int64_t)min(p0 + p, w.ways - 1) * w.apart;
+        pm[p] = load_device(mls + at * (2 * kRowsFew));
+        pl[p] = load_device(mls + at * (2 * kRowsFew) + 1);
+        const Rsrc from = buffer_of(a.part_out + (w.first + at) * kPartFloats, kPartFloats * 4);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+          x[p][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice));
+      }
+#pragma unroll
+      for (int p = 0; p < kSome; ++p) {
+        if (p0 + p >= w.ways) continue;
+        const float wp = weight_of(pm[p], pl[p], top);
+        l = __builtin_fmaf(wp, pl[p], l);
+#pragma unroll
+        for (int i = 0; i < kCols; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(wp, x[p][i][e], sum[i][e]);
+      }
+    }
+  }
+  const int row = w.row0 + col;
+  if (row >= qs.rows) return;
+  const int s = query_of(qs, row), g0 = row - s * a.group;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int64_t head = w.hk * a.group + g0;
+  uint16_t* out = a.out + ((int64_t)(w.begin + s) * a.H + head) * D;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    typename E::x4 h;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(sum[i][e] * inv);
+    *reinterpret_cast<typename E::x4*>(out + 8 * (wave * kCols + i) + 4 * hh) = h;
+  }
+  if (wave == 0 && hh == 0) a.lse[head * a.T + w.begin + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+int cus() {
+  static thread_local int cached_dev = -1, cached = 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 0;
+  if (dev != cached_dev) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+    cached = n;
+    cached_dev = dev;
+  }
+  return cached;
+}
+
+template <void (*kernel)(const PagesArgs)>
+int launch(const PagesArgs& a, int64_t grid, int waves, int lds, hipStream_t stream) {
+  // more than 64 KB of LDS has to be allowed once per kernel and device
+  static thread_local int allowed_dev = -1;
+  int dev = 0;
+  if (int rc = hip_fail(hipGetDevice(&dev), "hipGetDevice")) return rc;
+  if (lds > 65536 && allowed_dev != dev) {
+    if (int rc = hip_fail(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+                          "hipFuncSetAttribute"))
+      return rc;
+    allowed_dev = dev;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(waves * 64), lds, stream, a);
+  return hip_fail(hipGetLastError(), "attn_pages launch");
+}
+
+// A launch of one form: its grid holds what there can be.  `requests` at most have rows for it, `tiles` row tiles in all.
+struct Scratch {
+  void* workspace;
+  int64_t bytes;
+  uint32_t* counters;
+  int64_t n_counters;
+};
+template <int D, bool kHalf, bool kFew>
+int launch_form(PagesArgs a, int64_t requests, int64_t tiles, int n_cus, const Scratch& scratch, hipStream_t stream) {
+  constexpr int kRows = kFew ? kRowsFew : kRowsShared, kCounters = kFew ? 1 : kWavesShared;
+  constexpr int kPerCu = kFew ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1);
+  constexpr int64_t kPartBytes = (int64_t)kRows * (D + 2) * 4;
+  // (tiles of a group share keys in their XCD's L2; 64 groups or more, to go round)
+  const int64_t each = (tiles + requests - 1) / requests;
+  a.block = 1;
+  while (a.block < 8 && 2 * a.block <= each && a.Hk * (tiles / (2 * a.block)) >= 64) a.block *= 2;
+  const int64_t uncut = (int64_t)a.Hk * std::min(tiles, tiles / a.block + requests);
+  a.slots = (float)(n_cus * kPerCu);
+  int64_t room = std::min(scratch.workspace ? scratch.bytes / kPartBytes : 0, scratch.counters ? scratch.n_counters / kCounters : 0) / a.block;
+  room = std::min(room, std::max<int64_t>(2 * n_cus * kPerCu, 3 * uncut));
+  a.cut_groups = room > uncut ? (int32_t)room : 0;
+  a.groups = (int32_t)std::max(uncut, (int64_t)a.cut_groups);
+  const int64_t grid = (int64_t)kXcds * a.block * ((a.groups + kXcds - 1) / kXcds);
+  if (grid > (1 << 23) - 1) {
+    set_error("too many query rows");
+    return DT_ERR_INVALID;
+  }
+  a.step = D == 64 ? (kFew ? 1.0f : 1.15f) : (kFew ? 1.6f : 1.4f);
+  a.once = kFew ? 4.f : 8.f;
+  a.part = (float)(2.0 * kPartBytes / 6.7e6);
+  if (a.cut_groups) {
+    a.part_out = static_cast<float*>(scratch.workspace);
+    a.part_ml = a.part_out + room * a.block * kRows * D;
+    a.counters = scratch.counters;
+  }
+  if constexpr (kFew) return launch<attn_pages_few_kernel<D, kHalf>>(a, grid, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
+  else return launch<attn_pages_kernel<D, kHalf>>(a, grid, kWavesShared, SharedLds<D>::kBytes, stream);
+}
+
+template <int D, bool kHalf>
+int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.T * a.group;
+  most_rows = std::min(most_rows, rows);
+  a.least_rows = 1;
+  a.most_rows = INT32_MAX;
+  a.fill = 1;
+  if (most_rows <= kFewRows) return launch_form<D, kHalf, true>(a, a.B, rows / kRowsFew + std::min<int64_t>(a.B, rows), n_cus, scratch, stream);
+  if (a.B > 1) {
+    PagesArgs few = a;
+    few.most_rows = kFewRows;
+    const int64_t requests = std::min<int64_t>(a.B, a.T);
+    if (int rc = launch_form<D, kHalf, true>(few, requests, std::min(rows / kRowsFew + requests, requests * ((kFewRows + kRowsFew - 1) / kRowsFew)), n_cus,
+                                             scratch, stream))
+      return rc;
+    a.least_rows = kFewRows + 1;
+    a.fill = 0;
+  }
+  const int64_t requests = std::min<int64_t>(a.B, rows / a.least_rows);
+  return requests > 0 ? launch_form<D, kHalf, false>(a, requests, rows / kRowsShared + requests, n_cus, scratch, stream) : DT_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -153,7 +854,7 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
     set_error("counters must be 4-byte aligned with a non-negative number");
     return DT_ERR_INVALID;
   }
-  if ((int64_t)T * (H / Hk) > (1ll << 30) || H > 65535 || T > (1 << 25)) {
+  if ((int64_t)T * (H / Hk) > (1ll << 30) || (int64_t)T * H * D > (1ll << 40)) {
     set_error("too many query rows");
     return DT_ERR_INVALID;
   }
@@ -178,13 +879,17 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
   a.left = w.left < 0 ? -1 : (int32_t)std::min<int64_t>((int64_t)w.left * w.frame, 1 << 30);
   a.right = w.right < 0 ? -1 : (int32_t)std::min<int64_t>(((int64_t)w.right + 1) * w.frame, 1 << 30);
   a.by_frame = quotient_by(a.frame);
+  a.by_group = quotient_by(a.group);
   a.scale_log2 = (softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt((float)D)) * 1.4426950408889634f;
   const hipStream_t st = (hipStream_t)stream;
   const bool half = (flags & DT_ATTN_FP16) != 0;
-  const dim3 grid(T, H), block(64);
-  if (D == 128 && half) hipLaunchKernelGGL((attn_pages_kernel<128, true>), grid, block, 0, st, a);
-  else if (D == 128) hipLaunchKernelGGL((attn_pages_kernel<128, false>), grid, block, 0, st, a);
-  else if (half) hipLaunchKernelGGL((attn_pages_kernel<64, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((attn_pages_kernel<64, false>), grid, block, 0, st, a);
-  return hip_fail(hipGetLastError(), "attn_pages launch");
+  const int n_cus = cus();
+  if (n_cus <= 0) {
+    set_error("no current device");
+    return DT_ERR_HIP;
+  }
+  const Scratch scratch = {workspace, workspace_bytes, counters, n_counters};
+  const int64_t most_rows = (int64_t)std::max(max_seqlen_q, 0) * a.group;
+  if (D == 128) return half ? launch_dim<128, true>(a, most_rows, n_cus, scratch, st) : launch_dim<128, false>(a, most_rows, n_cus, scratch, st);
+  return half ? launch_dim<64, true>(a, most_rows, n_cus, scratch, st) : launch_dim<64, false>(a, most_rows, n_cus, scratch, st);
 }
