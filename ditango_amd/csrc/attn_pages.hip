@@ -41,10 +41,10 @@ struct PagesArgs {
   // ---- a launch's share
   int32_t least_rows, most_rows;   // of the requests that it takes
   int32_t fill;                    // it writes the rows that no request owns
-  int32_t block;                   // row tiles of a key head that run one behind the other on an XCD
-  int32_t groups;                  // of `block` workgroups, that the grid has
-  int32_t cut_groups;              // up to how many of them items may be cut into parts
-  float slots;                     // workgroups at once
+  int32_t block;                   // row tiles of a key head that run one behind the other on an XCD: a group
+  int32_t groups;                  // that the grid has
+  int32_t cut_groups;              // for how many of them there is room for parts
+  float round;                     // groups at once
   float step, once, part;          // us: of a step of keys, of a workgroup beside them, of a part's way to memory and back
   float* part_out;                 // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
   float* part_ml;
@@ -99,15 +99,41 @@ __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   return r;
 }
 __device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
+// Reductions and sums along the wavefront inside the vector instructions (__shfl is an LDS access): lane i of a row of 16 reads lane i - n, then the
+// rows behind the first read the row in front of them, or the half.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int moved(int x, int none) { return __builtin_amdgcn_update_dpp(none, x, kCtrl, kRows, 0xf, false); }
+template <typename Op>
+__device__ __forceinline__ int along(int x, int none, Op op) {      // lane i: of lanes 0 .. i
+  x = op(x, moved<0x111, 0xf>(x, none));
+  x = op(x, moved<0x112, 0xf>(x, none));
+  x = op(x, moved<0x114, 0xf>(x, none));
+  x = op(x, moved<0x118, 0xf>(x, none));
+  x = op(x, moved<0x142, 0xa>(x, none));
+  return op(x, moved<0x143, 0xc>(x, none));
 }
+__device__ __forceinline__ int sums_along(int x) {
+  return along(x, 0, [](int u, int v) { return u + v; });
+}
+__device__ __forceinline__ int wave_max(int x) {
+  return lane_value(along(x, INT32_MIN, [](int u, int v) { return max(u, v); }), 63);
+}
+__device__ __forceinline__ float as_float(int x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ int as_int(float x) { return __builtin_bit_cast(int, x); }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
+  return as_float(lane_value(along(as_int(x), 0, [](int u, int v) { return as_int(as_float(u) + as_float(v)); }), 63));
+}
+__device__ __forceinline__ float wave_min(float x) {
+  return as_float(lane_value(along(as_int(x), as_int(INFINITY), [](int u, int v) { return as_int(fminf(as_float(u), as_float(v))); }), 63));
+}
+// n / d and n % d, n < 2^23
+__device__ __forceinline__ int divided(int n, int d, int* rest) {
+  int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
+  q -= q * d > n;
+  q += (q + 1) * d <= n;
+  q = __builtin_amdgcn_readfirstlane(q);
+  *rest = n - q * d;
+  return q;
 }
 // Parts of an item of that many steps, where a part has 1 / inv of them.  (In floating point: nothing depends on it but that all agree.)
 __device__ __forceinline__ int ways_of(int steps, float inv) { return min(max((int)__builtin_ceilf((float)steps * inv - 0.001f), 1), kMostWays); }
@@ -116,65 +142,89 @@ __device__ __forceinline__ int ways_of(int steps, float inv) { return min(max((i
 template <int kRows, int kKeys>
 __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int* to) {
   const int lane = threadIdx.x & 63;
-  // (index of a group, place in it): groups go round the XCDs, a group's workgroups one behind the other on one
-  const int xcd = blockIdx.x % kXcds, i = blockIdx.x / kXcds, g = xcd + kXcds * (i / a.block), j = i % a.block;
+  // (group, workgroup of it): groups go round the XCDs, there and back and each time from another one on, as the groups of a key head come from the one
+  // with the most keys to the one with the fewest; a group's workgroups run one behind the other on its XCD
+  int g, j = 0;
+  {
+    const int xcd = blockIdx.x % kXcds;
+    int turn = blockIdx.x / kXcds;
+    if (a.block > 1) {
+      j = turn & (a.block - 1);
+      turn >>= __builtin_ctz(a.block);
+    }
+    const int place = (xcd + (turn >> 1)) % kXcds;
+    g = turn * kXcds + (turn & 1 ? kXcds - 1 - place : place);
+  }
   Request r = request_of<kRows, kKeys>(a, lane);
   int lo = r.n > 0 ? r.begin : a.T, hi = r.begin + r.n, most = r.steps;
-  float work = (float)r.tiles * (float)r.steps, items = (float)r.tiles;
+  float work = (float)r.tiles * (float)r.steps, items = (float)((r.tiles + a.block - 1) / a.block);
   for (int b0 = 64; b0 < a.B; b0 += 64) {
     const Request x = request_of<kRows, kKeys>(a, b0 + lane);
     if (x.n > 0) lo = min(lo, x.begin);
     hi = max(hi, x.begin + x.n);
     most = max(most, x.steps);
     work += (float)x.tiles * (float)x.steps;
-    items += (float)x.tiles;
+    items += (float)((x.tiles + a.block - 1) / a.block);
   }
   *to = wave_max(hi);
   *from = min(-wave_max(-lo), *to);
   most = wave_max(most);
-  work = wave_sum(work) * (float)a.Hk;
-  // steps of a part, as 1 / them
-  float inv = 0.f;
-  if (a.cut_groups > 0 && most > 1) {
+  float inv = 0.f;                          // 1 / steps of a part
+  int tail = INT32_MAX, tail_ways = 1;      // the groups from `tail` on are cut into that many
+  if (a.cut_groups > 0 && most > 3) {
+    work = wave_sum(work) * (float)a.Hk / (float)a.block;      // of group steps
+    items = wave_sum(items) * (float)a.Hk;
     if (a.B <= 64) {
-      // a lane prices 1 .. 64 parts of the longest item
-      const float ways = (float)(lane + 1), steps = __builtin_ceilf((float)most / ways), mine = 1.f / steps;
+      // A lane prices 1 .. 64 parts of the longest item, and of the groups of the last round.  Unlike items fill the rounds as they come, and wait
+      // for half of the longest one at the end.
+      const float ways = (float)(lane + 1), steps = __builtin_ceilf((float)most / ways), mine = 1.f / steps, fold = lane > 0 ? 2.f + 0.4f * ways : 0.f;
+      const float part = lane > 0 ? a.part * (float)a.block : 0.f;
       float n = 0.f;
       for (int b = 0; b < a.B; ++b) {
         const int tiles = lane_value(r.tiles, b);
         if (tiles > 0) n += (float)((tiles + a.block - 1) / a.block) * (float)ways_of(lane_value(r.steps, b), mine);
       }
       n *= (float)a.Hk;
-      const bool fits = lane == 0 || n <= (float)a.cut_groups;
-      n *= (float)a.block;
       const float once = steps * a.step + a.once;
-      float us = n <= a.slots ? once : min(__builtin_ceilf(n / a.slots) * once, (work * a.step + n * a.once) / a.slots + 0.5f * once);
-      if (lane > 0) us += 2.f + 0.4f * ways + n * a.part;
-      if (!fits) us = INFINITY;
-      float best = us;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) best = fminf(best, __shfl_xor(best, d));
-      const int at = __builtin_ctzll(__ballot(us == best));
-      inv = at == 0 ? 0.f : __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, mine), at));
+      float us = n <= a.round ? once : min(__builtin_ceilf(n / a.round) * once, (work * a.step + n * a.once) / a.round + 0.5f * once);
+      us += fold + n * part;
+      if (lane > 0 && n > (float)a.cut_groups) us = INFINITY;
+      const float whole = __builtin_floorf(items / a.round), rest = items - whole * a.round, each = work / items;
+      float tail_us = whole * (each * a.step + a.once) + 0.5f * ((float)most - each) * a.step;
+      if (rest > 0.f) tail_us += __builtin_ceilf(each / ways) * a.step + a.once + fold + rest * ways * part;
+      if (whole < 1.f || rest * ways > min(a.round, (float)a.cut_groups) || lane == 0) tail_us = INFINITY;
+      const float best = wave_min(us), tail_best = wave_min(tail_us);
+      if (tail_best < best) {
+        tail = (int)(whole * a.round);
+        tail_ways = 1 + __builtin_ctzll(__ballot(tail_us == tail_best));
+      } else {
+        const uint64_t these = __ballot(us == best);
+        const int at = these ? __builtin_ctzll(these) : 0;
+        inv = at == 0 ? 0.f : as_float(lane_value(as_int(mine), at));
+      }
     } else {
       // room for cuts beside one part of every item, shared out by their steps
-      items = wave_sum(items) * (float)a.Hk;
-      const float room = 0.99f * min((float)a.cut_groups, 2.f * a.slots) - items;      // (below what there is by more than the sums' roundings)
+      const float room = 0.99f * min((float)a.cut_groups, 2.f * a.round) - items;      // (below what there is by more than the sums' roundings)
       if (room > 0.f) inv = 1.f / max(max(work / room, (float)most / kMostWays), 8.f);
     }
+  }
+  w.ways = 1;
+  w.part = 0;
+  int slot = -1;
+  if (g >= tail) {
+    int rest;
+    const int item = divided(g - tail, tail_ways, &rest);
+    slot = item * tail_ways;
+    g = tail + item;
+    w.part = rest;
+    w.ways = tail_ways;
   }
   // groups in front of a lane's request
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     if (b0 > 0) r = request_of<kRows, kKeys>(a, b0 + lane);
     const int blocks = (r.tiles + a.block - 1) / a.block, ways = ways_of(r.steps, inv);
-    const int mine = r.tiles > 0 ? a.Hk * blocks * ways : 0;
-    int sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(sum, d);
-      if (lane >= d) sum += y;
-    }
+    const int mine = r.tiles > 0 ? a.Hk * blocks * ways : 0, sum = sums_along(mine);
     const uint64_t passed = __ballot(before + sum <= g);
     if (passed == ~0ull) {
       before += lane_value(sum, 63);
@@ -186,14 +236,20 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int
     w.begin = lane_value(r.begin, at);
     w.n = lane_value(r.n, at);
     w.len = lane_value(r.len, at);
-    w.ways = lane_value(ways, at);
-    const int unit = (g - group0) / nblk, blk = (g - group0) % nblk, tile = blk * a.block + j, tiles = lane_value(r.tiles, at);
-    w.hk = unit / w.ways;
-    w.part = unit % w.ways;
+    int blk, part, tiles = lane_value(r.tiles, at);
+    const int unit = divided(g - group0, nblk, &blk), cuts = lane_value(ways, at);
+    w.hk = divided(unit, cuts, &part);
+    w.apart = 1;
+    if (slot < 0) {
+      w.ways = cuts;
+      w.part = part;
+      w.apart = nblk;
+      slot = group0 + w.hk * cuts * nblk + blk;
+    }
+    w.first = slot * a.block + j;
+    w.apart *= a.block;
+    const int tile = blk * a.block + j;
     w.row0 = (tiles - 1 - tile) * kRows;      // the last ones first: under a causal border they see most
-    w.first = ((group0 + w.hk * w.ways * nblk + blk) * a.block) + j;
-    w.apart = nblk * a.block;
-    for (int* x : {&w.hk, &w.part, &w.row0, &w.first}) *x = __builtin_amdgcn_readfirstlane(*x);
     return tile < tiles;
   }
   return false;
@@ -212,27 +268,31 @@ __device__ __forceinline__ void fill_rows(const PagesArgs& a, int D, int from, i
 // A request's keys (0) and values (1) of a key head.
 struct Keys {
   const uint16_t* base[2];
-  int64_t sp[2], ss[2];
+  uint32_t sp[2], ss[2];        // bytes
   const __attribute__((address_space(4))) int32_t* table;      // (constant while the launch runs: scalar loads)
-  int len, page, n_pages;
+  int len, page, n_pages, width;
   Quotient by_page;
   __device__ __forceinline__ Keys(const PagesArgs& a, const Work& w) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       base[i] = a.kv.base[i] + w.hk * a.kv.sh[i];
-      sp[i] = a.kv.sp[i];
-      ss[i] = a.kv.ss[i];
+      sp[i] = 2 * (uint32_t)a.kv.sp[i];
+      ss[i] = 2 * (uint32_t)a.kv.ss[i];
     }
     table = (const __attribute__((address_space(4))) int32_t*)(a.tables + w.b * a.table_stride);
     len = w.len;
     page = a.kv.page;
     n_pages = a.kv.n_pages;
+    width = a.width;
     by_page = a.kv.by_page;
+  }
+  __device__ __forceinline__ const uint16_t* at(int i, uint32_t p, uint32_t place) const {
+    return reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(base[i]) + (uint64_t)p * sp[i] + (uint64_t)place * ss[i]);
   }
   // Row of key j < len, each lane's own; null where its entry is no page.
   __device__ __forceinline__ const uint16_t* row(int i, int j) const {
-    const int at = (int)quotient(j, by_page), p = reinterpret_cast<const int32_t*>(reinterpret_cast<uintptr_t>(table))[at];
-    return (uint32_t)p < (uint32_t)n_pages ? base[i] + p * sp[i] + (int64_t)(j - at * page) * ss[i] : nullptr;
+    const int e = (int)quotient(j, by_page), p = reinterpret_cast<const int32_t*>(reinterpret_cast<uintptr_t>(table))[e];
+    return (uint32_t)p < (uint32_t)n_pages ? at(i, p, j - e * page) : nullptr;
   }
 };
 
@@ -240,20 +300,53 @@ struct Keys {
 struct Sixteen {
   int id, place;                // page, and the first key's place in it
   int left;                     // keys from the first one to the last of the request; not above 0: none of them is there
-  __device__ __forceinline__ void find(const Keys& ks, int key, bool there) {
-    key = __builtin_amdgcn_readfirstlane(key);
-    left = there ? ks.len - key : 0;
-    key = left > 0 ? key : 0;
-    const int at = (int)quotient(key, ks.by_page);
-    place = key - at * ks.page;
-    id = ks.table[__builtin_amdgcn_readfirstlane(at)];
-  }
-  // rows behind the last key, and those of no page, arrive as zeros
+  // (rows behind the last key, and those of no page, arrive as zeros)
   template <int D>
   __device__ __forceinline__ u32x4 rsrc(const Keys& ks, int i) const {
-    const bool there = (left > 0) & ((uint32_t)id < (uint32_t)ks.n_pages);
-    const uint16_t* from = ks.base[i] + (there ? id : 0) * ks.sp[i] + place * ks.ss[i];
-    return make_rsrc(from, there ? (uint32_t)(min(left, 16) - 1) * (2 * (uint32_t)ks.ss[i]) + 2 * D : 0u);
+    uint32_t valid = 15 * ks.ss[i] + 2 * D;
+    if (__builtin_expect(left < 16, 0)) {
+      asm volatile("" ::: "memory");
+      valid = left > 0 ? (uint32_t)(left - 1) * ks.ss[i] + 2 * D : 0u;
+    }
+    return make_rsrc(ks.at(i, id, place), (uint32_t)id < (uint32_t)ks.n_pages ? valid : 0u);
+  }
+};
+// Finds a sixteen of each tile of a list, every kStep keys between two stops: the first key of the window, the list's end.  An entry is asked for when it
+// is found, and used a tile later.
+template <int kKeys, int kTiles>
+struct Finder {
+  int entry, place, left, t, stop;      // of the next one: its table entry, ...
+  int over, more;                       // kStep % page, kStep / page
+  static constexpr int kStep = kKeys * kTiles;
+  __device__ __forceinline__ void open(const Keys& ks, const TileList<kKeys>& list, int first, int offset) {
+    t = first;
+    more = (int)quotient(kStep, ks.by_page);
+    over = kStep - more * ks.page;
+    seek(ks, list, offset);
+  }
+  __device__ __forceinline__ void seek(const Keys& ks, const TileList<kKeys>& list, int offset) {
+    const int key = list.key(t) + offset;
+    left = t < list.end ? ks.len - key : 0;
+    entry = left > 0 ? (int)quotient(key, ks.by_page) : 0;
+    place = left > 0 ? key - entry * ks.page : 0;
+    stop = t < list.n_sink ? min(list.n_sink, list.end) : t < list.end ? list.end : INT32_MAX;
+    for (int* x : {&entry, &place, &left, &stop}) *x = __builtin_amdgcn_readfirstlane(*x);
+  }
+  __device__ __forceinline__ Sixteen next(const Keys& ks, const TileList<kKeys>& list, int offset) {
+    Sixteen x;
+    x.place = place;
+    x.left = left;
+    x.id = ks.table[min(entry, ks.width - 1)];
+    t += kTiles;
+    entry += more;
+    place += over;
+    left -= kStep;
+    if (place >= ks.page) {
+      place -= ks.page;
+      ++entry;
+    }
+    if (__builtin_expect(t >= stop, 0)) seek(ks, list, offset);
+    return x;
   }
 };
 
@@ -265,11 +358,11 @@ struct PageLoader {
   uint32_t k_row, k_chunk, v_off, k_block, v_block;
   __device__ __forceinline__ void open(const Keys& ks, int lane) {
     const int row = lane / T::kRowLanes, chunk = lane % T::kRowLanes;
-    k_row = row * (uint32_t)(2 * ks.ss[0]);
+    k_row = row * ks.ss[0];
     k_chunk = 16 * (chunk ^ T::swz_k(row));
-    v_off = row * (uint32_t)(2 * ks.ss[1]) + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
-    k_block = T::kBlockRows * (uint32_t)(2 * ks.ss[0]);
-    v_block = T::kBlockRows * (uint32_t)(2 * ks.ss[1]);
+    v_off = row * ks.ss[1] + 64 * ((chunk >> 2) ^ T::swz_v(row)) + 16 * (chunk & 3);
+    k_block = T::kBlockRows * ks.ss[0];
+    v_block = T::kBlockRows * ks.ss[1];
   }
   __device__ __forceinline__ void issue_k(const u32x4& r, int blk, uint32_t to) const {
     load_block_to_lds(r, k_row + (k_chunk ^ (64u * (blk & T::kBlockXor))) + (blk % kOf) * k_block, 0, to + blk * 1024);
@@ -377,37 +470,33 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
   const Keys ks(a, w);
   L ld;
   ld.open(ks, lane);
-  // A wavefront's blocks of a tile are wave, wave + 8 ..: kPer of them, each of its own sixteen.  Tile t + 1 of K goes with tile t of V.
+  // A wavefront brings kPer neighbouring blocks of a tile, which are of one sixteen.  Tile t + 1 of K goes with tile t of V.
   constexpr int kPer = T::kBlocks / kWavesShared;
-  Sixteen of_v[kPer], of_k[kPer], of_next[kPer];
-  int t_next = list.begin;       // whose pages are found next
-  auto look = [&](Sixteen (&x)[kPer]) __attribute__((always_inline)) {
-    const int key = list.key(t_next) + 16 * (wave / L::kOf);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i].find(ks, key + 16 * i * (kWavesShared / L::kOf), t_next < list.end);
-    ++t_next;
-  };
+  const int offset = 16 * (kPer * wave / L::kOf);
+  Finder<64, 1> finder;
+  Sixteen of_v, of_k, of_next;
   auto load_k = [&](int pair) __attribute__((always_inline)) {
+    const u32x4 r = of_k.template rsrc<D>(ks, 0);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      ld.issue_k(of_k[i].template rsrc<D>(ks, 0), wave + kWavesShared * i, lds0 + pair_at<D>(pair) + T::kBytes);
-      of_v[i] = of_k[i];
-      of_k[i] = of_next[i];
-    }
-    look(of_next);
+    for (int i = 0; i < kPer; ++i) ld.issue_k(r, kPer * wave + i, lds0 + pair_at<D>(pair) + T::kBytes);
+    of_v = of_k;
+    of_k = of_next;
+    of_next = finder.next(ks, list, offset);
   };
   auto load_pair = [&](int t) __attribute__((always_inline)) {
+    const u32x4 r = of_v.template rsrc<D>(ks, 1);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) ld.issue_v(of_v[i].template rsrc<D>(ks, 1), wave + kWavesShared * i, lds0 + pair_at<D>(t));
+    for (int i = 0; i < kPer; ++i) ld.issue_v(r, kPer * wave + i, lds0 + pair_at<D>(t));
     load_k(t);
   };
   RowState<D, kHalf, 2> st;
   const int row0 = w.row0 + 32 * wave;
   if (n > 0) {
-    look(of_k);
-    look(of_next);
+    finder.open(ks, list, list.begin, offset);
+    of_k = finder.next(ks, list, offset);
+    of_next = finder.next(ks, list, offset);
     const uint16_t* q = qs.q + (int64_t)w.hk * a.group * a.q_sh;
-    queries_to_lds<D>(lds0, row0, wave, lane, [&](int r) __attribute__((always_inline)) {
+    queries_to_lds<D, true>(lds0, row0, wave, lane, [&](int r) __attribute__((always_inline)) {
       const int row = min(r, qs.rows - 1);
       const int s = query_of(qs, row), g = row - s * a.group;
       return q + s * a.q_ss + g * a.q_sh;
@@ -417,7 +506,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
     load_pair(1);
   }
   st.open(qs, 0, w.hk, row0, w.len, lane, false);
-  if (n > 0) walk_tiles<D, kHalf>(st, lds, list, all_first, all_last, wave, lane, load_pair);
+  if (n > 0) walk_tiles<D, kHalf, true>(st, lds, list, all_first, all_last, wave, lane, load_pair);
   const int col = lane & 31, hh = lane >> 5;
   float m = st.m_ref * st.c, l = st.l_run + __shfl_xor(st.l_run, 32);
   float undefined = 0.f;
@@ -549,10 +638,11 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
   const Keys ks(a, w);
   L ld;
   ld.open(ks, lane);
+  Finder<T::kKeys, W> finder[2];
   Sixteen here[2], next[2];
-  auto look = [&](Sixteen (&x)[2], int t) __attribute__((always_inline)) {
+  auto look = [&](Sixteen (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i].find(ks, list.key(t) + 16 * i, t < list.end);
+    for (int i = 0; i < 2; ++i) x[i] = finder[i].next(ks, list, 16 * i);
   };
   auto load_k = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
 #pragma unroll
@@ -572,8 +662,10 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
   };
   int t = list.begin + wave;
   if (t < list.end) {
-    look(here, t);
-    look(next, t + W);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) finder[i].open(ks, list, t, 16 * i);
+    look(here);
+    look(next);
     load_k(here);
     load_v(here);
   }
@@ -588,7 +680,7 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
     load_k(next);
 #pragma unroll
     for (int i = 0; i < 2; ++i) here[i] = next[i];
-    look(next, t + 2 * W);
+    look(next);
     st.softmax(s, p, k0, masked, lane);
     wait_oldest<T::kBlocks>();
     if (masked && st.any_not_finite(vt, lane)) st.values_not_finite(vt, p, k0, lane);
@@ -759,12 +851,12 @@ int launch_form(PagesArgs a, int64_t requests, int64_t tiles, int n_cus, const S
   const int64_t each = (tiles + requests - 1) / requests;
   a.block = 1;
   while (a.block < 8 && 2 * a.block <= each && a.Hk * (tiles / (2 * a.block)) >= 64) a.block *= 2;
-  const int64_t uncut = (int64_t)a.Hk * std::min(tiles, tiles / a.block + requests);
-  a.slots = (float)(n_cus * kPerCu);
+  const int64_t uncut = (int64_t)a.Hk * std::min(tiles, tiles / a.block + requests), round = std::max<int64_t>((int64_t)n_cus * kPerCu / a.block, 1);
+  a.round = (float)round;
   int64_t room = std::min(scratch.workspace ? scratch.bytes / kPartBytes : 0, scratch.counters ? scratch.n_counters / kCounters : 0) / a.block;
-  room = std::min(room, std::max<int64_t>(2 * n_cus * kPerCu, 3 * uncut));
-  a.cut_groups = room > uncut ? (int32_t)room : 0;
-  a.groups = (int32_t)std::max(uncut, (int64_t)a.cut_groups);
+  room = std::min(room, std::max<int64_t>(2 * round, 3 * uncut));
+  a.cut_groups = (int32_t)room;
+  a.groups = (int32_t)(room > 0 ? std::max(uncut + round, room) : uncut);
   const int64_t grid = (int64_t)kXcds * a.block * ((a.groups + kXcds - 1) / kXcds);
   if (grid > (1 << 23) - 1) {
     set_error("too many query rows");

@@ -342,18 +342,21 @@ __device__ __forceinline__ int pair_at(int t) { return (t & (kPairs - 1)) * Shar
 // The wavefront's rows of Q come as whole lines through the LDS: half of them through its staging rows, a quarter each through its own shares
 // of V of pairs 3 and 2, which nothing but its own later loads writes.  (As fragments from memory, a load instruction touches 32 lines for 32
 // bytes each, and the compiler's wait for them would be one for every tile load behind them.)
-template <int D>
+// Block i of the wavefront's share of a tile: every eighth, or (kRun) kPer neighbours.
+template <int D, bool kRun>
+__device__ __forceinline__ int share_at(int wave, int i) { return kRun ? Tiles<D, 2>::kBlocks / kWavesShared * wave + i : wave + kWavesShared * i; }
+template <int D, bool kRun = false>
 __device__ __forceinline__ int query_at(int wave, int r) {      // row r; a quarter is kPer blocks of 1 KB
   typedef Tiles<D, 2> T;
   typedef SharedLds<D> S;
   constexpr int kPer = T::kBlocks / kWavesShared, kQRows = T::kBlockRows;
   const int in_half = S::kStage + wave * 32 * D + r * T::kRowBytes;
   const int blk = r / kQRows, i = blk % kPer;
-  const int apart = (blk / kPer == 2 ? pair_at<D>(3) : pair_at<D>(2)) + (wave + kWavesShared * i) * 1024 + r % kQRows * T::kRowBytes;
+  const int apart = (blk / kPer == 2 ? pair_at<D>(3) : pair_at<D>(2)) + share_at<D, kRun>(wave, i) * 1024 + r % kQRows * T::kRowBytes;
   return r < 16 ? in_half : apart;
 }
 // from(r): where row r of the batch and key head begins.
-template <int D, typename From>
+template <int D, bool kRun = false, typename From>
 __device__ __forceinline__ void queries_to_lds(uint32_t lds0, int row0, int wave, int lane, From from) {
   typedef Tiles<D, 2> T;
   typedef SharedLds<D> S;
@@ -361,7 +364,7 @@ __device__ __forceinline__ void queries_to_lds(uint32_t lds0, int row0, int wave
 #pragma unroll
   for (int blk = 0; blk < 4 * kPer; ++blk) {
     const int quarter = blk / kPer, i = blk % kPer;
-    const int to = quarter < 2 ? S::kStage + wave * 32 * D + blk * 1024 : pair_at<D>(5 - quarter) + (wave + kWavesShared * i) * 1024;
+    const int to = quarter < 2 ? S::kStage + wave * 32 * D + blk * 1024 : pair_at<D>(5 - quarter) + share_at<D, kRun>(wave, i) * 1024;
     const int r = blk * T::kBlockRows + lane / T::kRowLanes;
     load_rows_to_lds(from(row0 + r) + 8 * ((lane % T::kRowLanes) ^ T::swz_k(r)), lds0 + to);
   }
@@ -369,7 +372,7 @@ __device__ __forceinline__ void queries_to_lds(uint32_t lds0, int row0, int wave
 
 // The rows of a wavefront over the tiles of a list that is not empty.  In front of it go the loads of Q, K of tile 0 and pairs 0 and 1, in this order, of
 // kLoads / 2 and kLoads loads a wavefront; load_pair(t) sends for pair t.
-template <int D, bool kHalf, typename LoadPair>
+template <int D, bool kHalf, bool kRun = false, typename LoadPair>
 __device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint8_t* lds, const TileList<64>& list, const Span& all_first, const Span& all_last,
                                            int wave, int lane, LoadPair load_pair) {
   typedef Tiles<D, 2> T;
@@ -428,7 +431,7 @@ __device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint
   {
     const int r = lane & 31, hh = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) st.qf[i] = *reinterpret_cast<const ex8*>(lds + query_at<D>(wave, r) + 16 * ((2 * i + hh) ^ T::swz_k(r)));
+    for (int i = 0; i < D / 16; ++i) st.qf[i] = *reinterpret_cast<const ex8*>(lds + query_at<D, kRun>(wave, r) + 16 * ((2 * i + hh) ^ T::swz_k(r)));
   }
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.qf[i]));

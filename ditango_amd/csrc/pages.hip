@@ -252,6 +252,10 @@ int check_pages(const dt_pages* p, int D, Pages& out) {
       set_error("token strides of the pages must be in 0..2^23 elements");
       return DT_ERR_INVALID;
     }
+    if (strides[i][0] < 0 || strides[i][0] > INT32_MAX) {
+      set_error("page strides must be in 0..2^31 - 1 elements");
+      return DT_ERR_INVALID;
+    }
     out.base[i] = static_cast<uint16_t*>(i ? p->v : p->k);
     out.sp[i] = strides[i][0];
     out.ss[i] = strides[i][1];

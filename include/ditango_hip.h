@@ -624,7 +624,7 @@ int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, int32_t B, 
 
 /*
  * A cache of pages that several requests share: keys and values of `page_size` tokens a page (a multiple of 16), [page, token, key head, D] with
- * element strides {page, token, head} of their own (multiples of 8; token strides 0..2^23), bfloat16 or IEEE half, k and v 16-byte aligned.  A request's
+ * element strides {page, token, head} of their own (multiples of 8; token strides 0..2^23, page strides 0..2^31 - 1), bfloat16 or IEEE half, k and v 16-byte aligned.  A request's
  * token j lies in page table[j / page_size], at its place j % page_size; slot = page * page_size + place.  n_pages * page_size < 2^31.
  * No counterpart in the reference, whose caches hold whole blocks (core/cache.py:75-84).
  */
