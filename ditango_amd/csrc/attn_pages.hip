@@ -3,12 +3,13 @@
 // Row i of the n new tokens of a request with len tokens stands at position len - n + i among its keys; which of them it sees is a window as of
 // attn_window.hip, and the result is a state (out, lse) like its.  The rows' arithmetic is attn_rows.h's, in the same two forms:
 //   * shared tiles: 256 rows of one request and key head a workgroup, which walks the 64-key tiles that some row sees;
-//   * few rows: 32 rows, whose four wavefronts take 32-key tiles in turn.
-// Requests of at most kFewRows rows (new tokens x query heads of a key head) take the second, the others the first; a batch with both is two launches.
+//   * few rows: 32 rows, whose four or eight wavefronts take 32-key tiles in turn.
+// A request's rows (new tokens x query heads of a key head) go in tiles of 256, and what is left over in tiles of 32 where that is at most kFewRows.
+// Batches of requests that have no more rows than that run in a kernel with few rows only; in the other one both forms run side by side.
 //
 // Which page holds a tile is read by scalar loads one tile ahead, so that no tile waits for it; a page is a multiple of 16 tokens, and 16 rows of a tile
 // are what a load's descriptor covers.  No host knows the lengths, so every workgroup finds its share of the work by itself: it reads all lengths and
-// boundaries, a lane a request, prices some lengths of parts to cut the keys into, and numbers row tiles, key heads and parts through (`find`).
+// boundaries, a lane a request, prices some lengths of parts to cut the keys into, and numbers row tiles, parts and key heads through (`find`).
 #include <algorithm>
 #include <cmath>
 
@@ -38,17 +39,15 @@ struct PagesArgs {
   int32_t frame, sinks;
   Quotient by_group, by_frame;
   float scale_log2;
-  // ---- a launch's share
-  int32_t least_rows, most_rows;   // of the requests that it takes
-  int32_t fill;                    // it writes the rows that no request owns
-  int32_t block;                   // row tiles of a key head that run one behind the other on an XCD: a group
-  int32_t groups;                  // that the grid has
-  int32_t cut_groups;              // for how many of them there is room for parts
-  float round;                     // groups at once
-  float step, once, part;          // us: of a step of keys, of a workgroup beside them, of a part's way to memory and back
-  float* part_out;                 // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
-  float* part_ml;
-  uint32_t* counters;              // of an item's parts that are done, zero before and after the launch
+  // ---- how the launch runs
+  int32_t mixed;                // tiles of 256 rows as well as few rows
+  int32_t groups;               // workgroups of the grid
+  int32_t most_parts[2];        // for how many of them, of 256 rows (0) and of few (1), there is room for parts
+  float slots;                  // workgroups at once
+  float step[2], once[2], part[2];     // us: of 64 keys, of a workgroup beside them, of a part's way to memory and back
+  float* part_out[2];           // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
+  float* part_ml[2];
+  uint32_t* counters[2];        // of an item's parts that are done, zero before and after the launch
 };
 
 // The rows of a request, by the names of attn_rows.h
@@ -66,6 +65,7 @@ __device__ __forceinline__ Queries queries_of(const PagesArgs& a, int begin, int
 // A workgroup's work: row tile `row0` .. of a request and key head, and of its keys the part [tiles part / ways, tiles (part + 1) / ways)
 struct Work {
   int b, begin, n, len;         // request, its first row, its rows' and its keys' number
+  int few;                      // 32 rows, not 256
   int hk, row0, part, ways;
   int first, apart;             // slot of the item's first part, slots between its parts
   template <typename List>
@@ -78,11 +78,12 @@ struct Work {
   }
 };
 
-// a lane's request
+// A lane's request: its rows, keys, tiles of 256 rows (0) and of 32 (1), and about how long one of them takes.
 struct Request {
-  int begin, n, len, tiles, steps;     // ... row tiles, and steps of keys that the last of them sees
+  int begin, n, len;
+  int tiles[2];
+  float us[2];
 };
-template <int kRows, int kKeys>
 __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   Request r = {};
   if (b >= a.B) return r;
@@ -90,12 +91,21 @@ __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   r.n = max(min(max(a.cu[b + 1], 0), a.T) - r.begin, 0);
   r.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.kv.page);
   const int rows = r.n * a.group;
-  if (rows < a.least_rows || rows > a.most_rows) return r;
-  r.tiles = (rows + kRows - 1) / kRows;
+  int whole = 0;
+  if (a.mixed) {
+    r.tiles[0] = rows / kRowsShared + (rows % kRowsShared > kFewRows);
+    whole = min(r.tiles[0] * kRowsShared, rows);
+  }
+  r.tiles[1] = (rows - whole + kRowsFew - 1) / kRowsFew;
   const Queries qs = queries_of(a, 0, r.n);
-  const Span first = span_of(qs, r.len, query_of(qs, (r.tiles - 1) * kRows)), last = span_of(qs, r.len, r.n - 1);
-  const int sinks = min(a.sinks, last.hi);
-  r.steps = (sinks + max(last.hi - max(first.lo, sinks), 0) + kKeys - 1) / kKeys;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (r.tiles[i] > 0) {      // what its last tile sees
+      const int end = i ? rows : whole;
+      const Span first = span_of(qs, r.len, query_of(qs, i ? whole : max(end - kRowsShared, 0))), last = span_of(qs, r.len, query_of(qs, end - 1));
+      const int sinks = min(a.sinks, last.hi);
+      r.us[i] = (float)((sinks + max(last.hi - max(first.lo, sinks), 0) + 63) / 64) * a.step[i];
+    }
   return r;
 }
 __device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
@@ -135,122 +145,150 @@ __device__ __forceinline__ int divided(int n, int d, int* rest) {
   *rest = n - q * d;
   return q;
 }
-// Parts of an item of that many steps, where a part has 1 / inv of them.  (In floating point: nothing depends on it but that all agree.)
-__device__ __forceinline__ int ways_of(int steps, float inv) { return min(max((int)__builtin_ceilf((float)steps * inv - 0.001f), 1), kMostWays); }
+// Parts of an item that takes `us`, where a part takes 1 / inv of them.  (In floating point: nothing depends on it but that all agree.)
+__device__ __forceinline__ int ways_of(float us, float inv) { return min(max((int)__builtin_ceilf(us * inv - 0.001f), 1), kMostWays); }
 
 // Finds workgroup blockIdx.x's work; false: it has none.  [*from, *to): the rows that requests own.
-template <int kRows, int kKeys>
 __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int* to) {
   const int lane = threadIdx.x & 63;
-  // (group, workgroup of it): groups go round the XCDs, there and back and each time from another one on, as the groups of a key head come from the one
-  // with the most keys to the one with the fewest; a group's workgroups run one behind the other on its XCD
-  int g, j = 0;
-  {
-    const int xcd = blockIdx.x % kXcds;
-    int turn = blockIdx.x / kXcds;
-    if (a.block > 1) {
-      j = turn & (a.block - 1);
-      turn >>= __builtin_ctz(a.block);
-    }
-    const int place = (xcd + (turn >> 1)) % kXcds;
-    g = turn * kXcds + (turn & 1 ? kXcds - 1 - place : place);
+  // The workgroup's number.  They are dealt round the XCDs and counted through key heads first, then parts, then row tiles, from those with the most keys on: a
+  // multiple of eight key heads stay on an XCD each, whose L2 its row tiles share; else every other turn goes back, or the first XCD would always get
+  // the longer one.
+  const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
+  int g = turn * kXcds + ((turn & 1) && a.Hk % kXcds ? kXcds - 1 - xcd : xcd);
+  Request r = request_of(a, lane);
+  int lo = r.n > 0 ? r.begin : a.T, hi = r.begin + r.n;
+  float most = max(r.us[0], r.us[1]), work[2], items[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    work[i] = (float)r.tiles[i] * r.us[i];
+    items[i] = (float)r.tiles[i];
   }
-  Request r = request_of<kRows, kKeys>(a, lane);
-  int lo = r.n > 0 ? r.begin : a.T, hi = r.begin + r.n, most = r.steps;
-  float work = (float)r.tiles * (float)r.steps, items = (float)((r.tiles + a.block - 1) / a.block);
   for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const Request x = request_of<kRows, kKeys>(a, b0 + lane);
+    const Request x = request_of(a, b0 + lane);
     if (x.n > 0) lo = min(lo, x.begin);
     hi = max(hi, x.begin + x.n);
-    most = max(most, x.steps);
-    work += (float)x.tiles * (float)x.steps;
-    items += (float)((x.tiles + a.block - 1) / a.block);
+    most = max(most, max(x.us[0], x.us[1]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      work[i] += (float)x.tiles[i] * x.us[i];
+      items[i] += (float)x.tiles[i];
+    }
   }
   *to = wave_max(hi);
   *from = min(-wave_max(-lo), *to);
-  most = wave_max(most);
-  float inv = 0.f;                          // 1 / steps of a part
-  int tail = INT32_MAX, tail_ways = 1;      // the groups from `tail` on are cut into that many
-  if (a.cut_groups > 0 && most > 3) {
-    work = wave_sum(work) * (float)a.Hk / (float)a.block;      // of group steps
-    items = wave_sum(items) * (float)a.Hk;
+  most = as_float(wave_max(as_int(most)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    work[i] = wave_sum(work[i]) * (float)a.Hk;
+    items[i] = wave_sum(items[i]) * (float)a.Hk;
+  }
+  float inv[2] = {0.f, 0.f};                // 1 / us of a part
+  int tail = INT32_MAX, tail_ways = 1, tail_end = 0;      // items of 256 rows from `tail` on are cut into that many
+  if (a.most_parts[1] > 0 && most > 4.f * min(a.step[0], a.step[1])) {
     if (a.B <= 64) {
-      // A lane prices 1 .. 64 parts of the longest item, and of the groups of the last round.  Unlike items fill the rounds as they come, and wait
+      // A lane prices 1 .. 64 parts of the longest item, and of the items of 256 rows of the last round.  Unlike items fill the rounds as they come, and wait
       // for half of the longest one at the end.
-      const float ways = (float)(lane + 1), steps = __builtin_ceilf((float)most / ways), mine = 1.f / steps, fold = lane > 0 ? 2.f + 0.4f * ways : 0.f;
-      const float part = lane > 0 ? a.part * (float)a.block : 0.f;
-      float n = 0.f;
-      for (int b = 0; b < a.B; ++b) {
-        const int tiles = lane_value(r.tiles, b);
-        if (tiles > 0) n += (float)((tiles + a.block - 1) / a.block) * (float)ways_of(lane_value(r.steps, b), mine);
+      const float ways = (float)(lane + 1), us = most / ways, mine = 1.f / us, fold = lane > 0 ? 2.f + 0.4f * ways : 0.f;
+      float n[2] = {0.f, 0.f};
+      for (int b = 0; b < a.B; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) n[i] += (float)lane_value(r.tiles[i], b) * (float)ways_of(as_float(lane_value(as_int(r.us[i]), b)), mine);
+      float beside = 0.f, parts = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        n[i] *= (float)a.Hk;
+        beside += n[i] * a.once[i];
+        parts += lane > 0 ? n[i] * a.part[i] : 0.f;
       }
-      n *= (float)a.Hk;
-      const float once = steps * a.step + a.once;
-      float us = n <= a.round ? once : min(__builtin_ceilf(n / a.round) * once, (work * a.step + n * a.once) / a.round + 0.5f * once);
-      us += fold + n * part;
-      if (lane > 0 && n > (float)a.cut_groups) us = INFINITY;
-      const float whole = __builtin_floorf(items / a.round), rest = items - whole * a.round, each = work / items;
-      float tail_us = whole * (each * a.step + a.once) + 0.5f * ((float)most - each) * a.step;
-      if (rest > 0.f) tail_us += __builtin_ceilf(each / ways) * a.step + a.once + fold + rest * ways * part;
-      if (whole < 1.f || rest * ways > min(a.round, (float)a.cut_groups) || lane == 0) tail_us = INFINITY;
-      const float best = wave_min(us), tail_best = wave_min(tail_us);
+      const float all = n[0] + n[1], once = us + (items[0] > 0.f ? a.once[0] : a.once[1]);
+      float cost = all <= a.slots ? once : min(__builtin_ceilf(all / a.slots) * once, (work[0] + work[1] + beside) / a.slots + 0.5f * once);
+      cost += fold + parts;
+      if (lane > 0 && (n[0] > (float)a.most_parts[0] || n[1] > (float)a.most_parts[1] || all > (float)a.groups)) cost = INFINITY;
+      const float best = wave_min(cost);
+      float tail_cost = INFINITY, tail_best = INFINITY;
+      const float whole = __builtin_floorf(items[0] / a.slots), rest = items[0] - whole * a.slots, each = work[0] / max(items[0], 1.f);
+      if (whole >= 1.f) {
+        const float mine_us = each / ways, cuts = rest * ways;
+        float m = 0.f;      // parts of the few rows, as long as those of the tail
+        for (int b = 0; b < a.B; ++b) m += (float)lane_value(r.tiles[1], b) * (float)ways_of(as_float(lane_value(as_int(r.us[1]), b)), 1.f / mine_us);
+        m *= (float)a.Hk;
+        const float end = rest * each + work[1] + cuts * a.once[0] + m * a.once[1];
+        tail_cost = whole * (each + a.once[0]) + 0.5f * max(most - each, 0.f) + end / a.slots + fold + (lane > 0 ? cuts * a.part[0] + m * a.part[1] : 0.f);
+        if (cuts + m > 0.f) tail_cost += cuts + m <= a.slots ? max(mine_us + a.once[0] - end / a.slots, 0.f) : 0.5f * (mine_us + a.once[0]);
+        if (cuts > (float)a.most_parts[0] || m > (float)a.most_parts[1] || whole * a.slots + cuts + m > (float)a.groups) tail_cost = INFINITY;
+        tail_best = wave_min(tail_cost);
+      }
       if (tail_best < best) {
-        tail = (int)(whole * a.round);
-        tail_ways = 1 + __builtin_ctzll(__ballot(tail_us == tail_best));
+        const int at = __builtin_ctzll(__ballot(tail_cost == tail_best));
+        tail = (int)(whole * a.slots);
+        tail_ways = 1 + at;
+        tail_end = tail + (int)rest * tail_ways;
+        inv[1] = 1.f / as_float(lane_value(as_int(each / ways), at));
       } else {
-        const uint64_t these = __ballot(us == best);
+        const uint64_t these = __ballot(cost == best);
         const int at = these ? __builtin_ctzll(these) : 0;
-        inv = at == 0 ? 0.f : as_float(lane_value(as_int(mine), at));
+        inv[0] = inv[1] = at == 0 ? 0.f : as_float(lane_value(as_int(mine), at));
       }
     } else {
-      // room for cuts beside one part of every item, shared out by their steps
-      const float room = 0.99f * min((float)a.cut_groups, 2.f * a.round) - items;      // (below what there is by more than the sums' roundings)
-      if (room > 0.f) inv = 1.f / max(max(work / room, (float)most / kMostWays), 8.f);
+      // room for cuts beside one part of every item, shared out by their time; less than there is by more than the sums' roundings
+      const float room = 0.99f * min((float)a.groups, 2.f * a.slots) - items[0] - items[1];
+      if (room > 0.f) {
+        const float mine = 1.f / max(max((work[0] + work[1]) / room, most / kMostWays), 8.f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (items[i] + work[i] * mine < 0.99f * (float)a.most_parts[i]) inv[i] = mine;
+      }
     }
   }
   w.ways = 1;
   w.part = 0;
   int slot = -1;
-  if (g >= tail) {
-    int rest;
-    const int item = divided(g - tail, tail_ways, &rest);
+  if (g >= tail && g < tail_end) {
+    int part;
+    const int item = divided(g - tail, tail_ways, &part);
     slot = item * tail_ways;
     g = tail + item;
-    w.part = rest;
+    w.part = part;
     w.ways = tail_ways;
+  } else if (g >= tail) {
+    g += tail + (tail_end - tail) / tail_ways - tail_end;      // among the few rows, as if none of the others were cut
   }
-  // groups in front of a lane's request
+  // items, or their parts, in front of a lane's request: those of 256 rows, then the few rows
   int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    if (b0 > 0) r = request_of<kRows, kKeys>(a, b0 + lane);
-    const int blocks = (r.tiles + a.block - 1) / a.block, ways = ways_of(r.steps, inv);
-    const int mine = r.tiles > 0 ? a.Hk * blocks * ways : 0, sum = sums_along(mine);
-    const uint64_t passed = __ballot(before + sum <= g);
-    if (passed == ~0ull) {
-      before += lane_value(sum, 63);
-      continue;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (i == 0 && !a.mixed) continue;
+    const int first = before;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      if (a.B > 64) r = request_of(a, b0 + lane);
+      const int ways = ways_of(r.us[i], inv[i]), mine = a.Hk * r.tiles[i] * ways, sum = sums_along(mine);
+      const uint64_t passed = __ballot(before + sum <= g);
+      if (passed == ~0ull) {
+        before += lane_value(sum, 63);
+        continue;
+      }
+      const int at = __builtin_ctzll(~passed);
+      const int group0 = before + lane_value(sum, at) - lane_value(mine, at);
+      w.b = b0 + at;
+      w.begin = lane_value(r.begin, at);
+      w.n = lane_value(r.n, at);
+      w.len = lane_value(r.len, at);
+      w.few = i;
+      const int tiles = lane_value(r.tiles[i], at), cuts = lane_value(ways, at);
+      int part;
+      const int rest = divided(g - group0, a.Hk, &w.hk), tile = tiles - 1 - divided(rest, cuts, &part);      // the last ones first: under a causal border they see most
+      w.apart = 1;
+      if (slot < 0) {
+        w.ways = cuts;
+        w.part = part;
+        w.apart = a.Hk;
+        slot = group0 - first + (tiles - 1 - tile) * cuts * a.Hk + w.hk;
+      }
+      w.first = slot;
+      w.row0 = i ? lane_value(r.tiles[0], at) * kRowsShared + tile * kRowsFew : tile * kRowsShared;
+      return true;
     }
-    const int at = __builtin_ctzll(~passed);
-    const int group0 = before + lane_value(sum, at) - lane_value(mine, at), nblk = lane_value(blocks, at);
-    w.b = b0 + at;
-    w.begin = lane_value(r.begin, at);
-    w.n = lane_value(r.n, at);
-    w.len = lane_value(r.len, at);
-    int blk, part, tiles = lane_value(r.tiles, at);
-    const int unit = divided(g - group0, nblk, &blk), cuts = lane_value(ways, at);
-    w.hk = divided(unit, cuts, &part);
-    w.apart = 1;
-    if (slot < 0) {
-      w.ways = cuts;
-      w.part = part;
-      w.apart = nblk;
-      slot = group0 + w.hk * cuts * nblk + blk;
-    }
-    w.first = slot * a.block + j;
-    w.apart *= a.block;
-    const int tile = blk * a.block + j;
-    w.row0 = (tiles - 1 - tile) * kRows;      // the last ones first: under a causal border they see most
-    return tile < tiles;
   }
   return false;
 }
@@ -449,17 +487,11 @@ __device__ __forceinline__ bool masked_not_finite(const Keys& ks, const RowState
 constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
+__device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, uint8_t* lds) {
   typedef Tiles<D, 2> T;
   typedef SharedLds<D> S;
   typedef Elem<kHalf> E;
   typedef PageLoader<D, 2> L;
-  extern __shared__ __align__(1024) uint8_t lds[];
-  Work w;
-  int own_from, own_to;
-  const bool some = find<kRowsShared, 64>(a, w, &own_from, &own_to);
-  if (a.fill) fill_rows(a, D, own_from, own_to);
-  if (!some) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
   const Queries qs = queries_of(a, w.begin, w.n);
@@ -520,7 +552,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
     // A part's sums, fp32; the wavefront that completes the parts of its rows adds them all up, in order.
     constexpr int kPartFloats = 32 * D;
     const int mine = w.first + w.part * w.apart;
-    float* part = a.part_out + ((int64_t)mine * kWavesShared + wave) * kPartFloats;
+    float* part = a.part_out[0] + ((int64_t)mine * kWavesShared + wave) * kPartFloats;
     if (hurt) {
       rows_one_by_one<D, kHalf>(a, w, qs, ks, row0, m, 0.f, list.begin < list.end ? list.key(list.begin) : 0,
                                 list.begin < list.end ? list.key(list.end - 1) + T::kKeys : 0, part, lane);
@@ -536,7 +568,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
           __builtin_amdgcn_raw_buffer_store_b128(x, to, (4 * i + g) * 1024 + lane * 16, 0, kDevice);
         }
     }
-    float* ml = a.part_ml + (((int64_t)mine * kWavesShared + wave) * 32 + col) * 2;
+    float* ml = a.part_ml[0] + (((int64_t)mine * kWavesShared + wave) * 32 + col) * 2;
     if (hh == 0) {
       store_device(ml, m);
       store_device(ml + 1, l);
@@ -544,13 +576,13 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
     wait_loads();                // (stores as well)
     int done = 0;
     if (lane == 0) {
-      uint32_t* counter = a.counters + (int64_t)w.first * kWavesShared + wave;
+      uint32_t* counter = a.counters[0] + (int64_t)w.first * kWavesShared + wave;
       done = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
       if (done) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (!__builtin_amdgcn_readfirstlane(done)) return;
     asm volatile("" ::: "memory");
-    const float* mls = a.part_ml + (((int64_t)w.first * kWavesShared + wave) * 32 + col) * 2;
+    const float* mls = a.part_ml[0] + (((int64_t)w.first * kWavesShared + wave) * 32 + col) * 2;
     const int64_t ml_apart = (int64_t)w.apart * kWavesShared * 64;
     float top = -INFINITY;
     for (int p = 0; p < w.ways; ++p) top = fmaxf(top, load_device(mls + p * ml_apart));
@@ -562,7 +594,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
 #pragma unroll 1
     for (int p = 0; p < w.ways; ++p) {
       const float lp = load_device(mls + p * ml_apart + 1), wp = weight_of(load_device(mls + p * ml_apart), lp, top);
-      const Rsrc from = buffer_of(a.part_out + ((int64_t)(w.first + p * w.apart) * kWavesShared + wave) * kPartFloats, kPartFloats * 4);
+      const Rsrc from = buffer_of(a.part_out[0] + ((int64_t)(w.first + p * w.apart) * kWavesShared + wave) * kPartFloats, kPartFloats * 4);
       l = __builtin_fmaf(wp, lp, l);
       f32x4 x[D / 8];
 #pragma unroll
@@ -613,18 +645,11 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages
 
 // Few rows: as attn_window.hip's, a wavefront takes every fourth tile of its item, or of a part of it, K of the next tile sent for before the softmax of
 // this one, V of the next behind its values; the states of the four meet in the LDS, those of parts in memory, where the last part adds them up.
-template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
-  constexpr int W = kWavesFew;
+template <int D, bool kHalf, int W>
+__device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint8_t* lds) {
   typedef Tiles<D, 1> T;
   typedef Elem<kHalf> E;
   typedef PageLoader<D, 1> L;
-  extern __shared__ __align__(1024) uint8_t lds[];
-  Work w;
-  int own_from, own_to;
-  const bool some = find<kRowsFew, 32 * W>(a, w, &own_from, &own_to);
-  if (a.fill) fill_rows(a, D, own_from, own_to);
-  if (!some) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, hh = lane >> 5;
   const Queries qs = queries_of(a, w.begin, w.n);
@@ -720,7 +745,9 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
     weight[i] = weight_of(m[i], li, top);
     l = __builtin_fmaf(weight[i], li, l);
   }
-  constexpr int kCols = D / 8 / W, kSome = 4;          // register groups of a wavefront's share, parts under way together
+  constexpr int kCols = D / 8 / W, kSome = 8;          // register groups of a wavefront's share, parts under way together
+  const int row = w.row0 + col;
+  const bool live = row < qs.rows;
   f32x4 sum[kCols];
 #pragma unroll
   for (int i = 0; i < kCols; ++i) {
@@ -735,25 +762,26 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
   if (w.ways > 1) {
     constexpr int kPartFloats = kRowsFew * D;
     const int64_t mine = w.first + w.part * w.apart;
-    const Rsrc to = buffer_of(a.part_out + mine * kPartFloats, kPartFloats * 4);
+    const Rsrc to = buffer_of(a.part_out[1] + mine * kPartFloats, kPartFloats * 4);
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), to, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice);
-    if (wave == 0 && hh == 0) {
-      store_device(a.part_ml + (mine * kRowsFew + col) * 2, top);
-      store_device(a.part_ml + (mine * kRowsFew + col) * 2 + 1, l);
+    for (int i = 0; i < kCols; ++i)
+      if (live) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), to, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice);
+    if (wave == 0 && hh == 0 && live) {
+      store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2, top);
+      store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2 + 1, l);
     }
     int* flag = reinterpret_cast<int*>(lds + FewLds<D, W>::kFlag);
     wait_loads();                // (stores as well)
     __syncthreads();
     if (threadIdx.x == 0) {
-      uint32_t* counter = a.counters + w.first;
+      uint32_t* counter = a.counters[1] + w.first;
       const bool last = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
       if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       *flag = last;
     }
     __syncthreads();
-    if (!*flag) return;
-    const float* mls = a.part_ml + ((int64_t)w.first * kRowsFew + col) * 2;
+    if (!*flag || !live) return;
+    const float* mls = a.part_ml[1] + ((int64_t)w.first * kRowsFew + col) * 2;
     top = -INFINITY;
     for (int p0 = 0; p0 < w.ways; p0 += kSome) {
       float x[kSome];
@@ -773,7 +801,7 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
         const int64_t at = (int64_t)min(p0 + p, w.ways - 1) * w.apart;
         pm[p] = load_device(mls + at * (2 * kRowsFew));
         pl[p] = load_device(mls + at * (2 * kRowsFew) + 1);
-        const Rsrc from = buffer_of(a.part_out + (w.first + at) * kPartFloats, kPartFloats * 4);
+        const Rsrc from = buffer_of(a.part_out[1] + (w.first + at) * kPartFloats, kPartFloats * 4);
 #pragma unroll
         for (int i = 0; i < kCols; ++i)
           x[p][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice));
@@ -790,8 +818,7 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
       }
     }
   }
-  const int row = w.row0 + col;
-  if (row >= qs.rows) return;
+  if (!live) return;
   const int s = query_of(qs, row), g0 = row - s * a.group;
   const float inv = l != 0.f ? 1.f / l : 0.f;
   const int64_t head = w.hk * a.group + g0;
@@ -804,6 +831,27 @@ __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_fe
     *reinterpret_cast<typename E::x4*>(out + 8 * (wave * kCols + i) + 4 * hh) = h;
   }
   if (wave == 0 && hh == 0) a.lse[head * a.T + w.begin + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+}
+
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  Work w;
+  int own_from, own_to;
+  const bool some = find(a, w, &own_from, &own_to);
+  fill_rows(a, D, own_from, own_to);
+  if (some) few_rows<D, kHalf, kWavesFew>(a, w, lds);
+}
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  Work w;
+  int own_from, own_to;
+  const bool some = find(a, w, &own_from, &own_to);
+  fill_rows(a, D, own_from, own_to);
+  if (!some) return;
+  if (w.few) few_rows<D, kHalf, kWavesShared>(a, w, lds);
+  else shared_tiles<D, kHalf>(a, w, lds);
 }
 
 int cus() {
@@ -835,65 +883,55 @@ int launch(const PagesArgs& a, int64_t grid, int waves, int lds, hipStream_t str
   return hip_fail(hipGetLastError(), "attn_pages launch");
 }
 
-// A launch of one form: its grid holds what there can be.  `requests` at most have rows for it, `tiles` row tiles in all.
 struct Scratch {
   void* workspace;
   int64_t bytes;
   uint32_t* counters;
   int64_t n_counters;
 };
-template <int D, bool kHalf, bool kFew>
-int launch_form(PagesArgs a, int64_t requests, int64_t tiles, int n_cus, const Scratch& scratch, hipStream_t stream) {
-  constexpr int kRows = kFew ? kRowsFew : kRowsShared, kCounters = kFew ? 1 : kWavesShared;
-  constexpr int kPerCu = kFew ? (D == 64 ? 4 : 2) : (D == 64 ? 2 : 1);
-  constexpr int64_t kPartBytes = (int64_t)kRows * (D + 2) * 4;
-  // (tiles of a group share keys in their XCD's L2; 64 groups or more, to go round)
-  const int64_t each = (tiles + requests - 1) / requests;
-  a.block = 1;
-  while (a.block < 8 && 2 * a.block <= each && a.Hk * (tiles / (2 * a.block)) >= 64) a.block *= 2;
-  const int64_t uncut = (int64_t)a.Hk * std::min(tiles, tiles / a.block + requests), round = std::max<int64_t>((int64_t)n_cus * kPerCu / a.block, 1);
-  a.round = (float)round;
-  int64_t room = std::min(scratch.workspace ? scratch.bytes / kPartBytes : 0, scratch.counters ? scratch.n_counters / kCounters : 0) / a.block;
-  room = std::min(room, std::max<int64_t>(2 * round, 3 * uncut));
-  a.cut_groups = (int32_t)room;
-  a.groups = (int32_t)(room > 0 ? std::max(uncut + round, room) : uncut);
-  const int64_t grid = (int64_t)kXcds * a.block * ((a.groups + kXcds - 1) / kXcds);
+
+// The grid holds what there can be, cut or not.  us of 64 keys as launches that fill the chip take them; see attn_window.hip's forms.
+template <int D, bool kHalf>
+int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.T * a.group, requests = std::min<int64_t>(a.B, a.T);
+  a.mixed = std::min(most_rows, rows) > kFewRows;
+  const int64_t slots = (int64_t)n_cus * (a.mixed ? 1 : 2) * (D == 64 ? 2 : 1);
+  const int64_t big = a.mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
+  const int64_t small = std::min(rows / kRowsFew + requests, a.mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
+  const int64_t uncut = a.Hk * (big + small);
+  a.slots = (float)slots;
+  const float full = D == 64 ? 2.0f : 1.0f;      // workgroups that share a CU
+  a.step[0] = (D == 64 ? 1.0f : 1.4f) * full;
+  a.step[1] = (D == 64 ? 1.0f : 1.6f) * full * (a.mixed ? 0.25f : 0.5f);
+  a.once[0] = 8.f;
+  a.once[1] = 4.f;
+  constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
+  for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
+  // few rows first, whose parts are small
+  int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;
+  const int64_t groups = std::max(uncut + slots, 2 * slots);
+  int64_t parts[2];
+  parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups});
+  parts[0] = a.mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;
+  float* at = static_cast<float*>(scratch.workspace);
+  uint32_t* counter = scratch.counters;
+  for (int i : {1, 0}) {
+    const int64_t floats = parts[i] * kBytes[i] / 4, sums = floats / (D + 2) * D;
+    a.most_parts[i] = (int32_t)parts[i];
+    a.part_out[i] = at;
+    a.part_ml[i] = at + sums;
+    a.counters[i] = counter;
+    at += floats;
+    counter += parts[i] * (i ? 1 : kWavesShared);
+  }
+  const int64_t grid = (parts[1] > 0 ? groups : uncut) + kXcds - 1;
   if (grid > (1 << 23) - 1) {
     set_error("too many query rows");
     return DT_ERR_INVALID;
   }
-  a.step = D == 64 ? (kFew ? 1.0f : 1.15f) : (kFew ? 1.6f : 1.4f);
-  a.once = kFew ? 4.f : 8.f;
-  a.part = (float)(2.0 * kPartBytes / 6.7e6);
-  if (a.cut_groups) {
-    a.part_out = static_cast<float*>(scratch.workspace);
-    a.part_ml = a.part_out + room * a.block * kRows * D;
-    a.counters = scratch.counters;
-  }
-  if constexpr (kFew) return launch<attn_pages_few_kernel<D, kHalf>>(a, grid, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
-  else return launch<attn_pages_kernel<D, kHalf>>(a, grid, kWavesShared, SharedLds<D>::kBytes, stream);
-}
-
-template <int D, bool kHalf>
-int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.T * a.group;
-  most_rows = std::min(most_rows, rows);
-  a.least_rows = 1;
-  a.most_rows = INT32_MAX;
-  a.fill = 1;
-  if (most_rows <= kFewRows) return launch_form<D, kHalf, true>(a, a.B, rows / kRowsFew + std::min<int64_t>(a.B, rows), n_cus, scratch, stream);
-  if (a.B > 1) {
-    PagesArgs few = a;
-    few.most_rows = kFewRows;
-    const int64_t requests = std::min<int64_t>(a.B, a.T);
-    if (int rc = launch_form<D, kHalf, true>(few, requests, std::min(rows / kRowsFew + requests, requests * ((kFewRows + kRowsFew - 1) / kRowsFew)), n_cus,
-                                             scratch, stream))
-      return rc;
-    a.least_rows = kFewRows + 1;
-    a.fill = 0;
-  }
-  const int64_t requests = std::min<int64_t>(a.B, rows / a.least_rows);
-  return requests > 0 ? launch_form<D, kHalf, false>(a, requests, rows / kRowsShared + requests, n_cus, scratch, stream) : DT_OK;
+  a.groups = (int32_t)(grid / kXcds * kXcds);
+  return a.mixed ? launch<attn_pages_kernel<D, kHalf>>(a, a.groups, kWavesShared, SharedLds<D>::kBytes, stream)
+                 : launch<attn_pages_few_kernel<D, kHalf>>(a, a.groups, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
