@@ -9,7 +9,7 @@
 //
 // Which page holds a tile is read by scalar loads one tile ahead, so that no tile waits for it; a page is a multiple of 16 tokens, and 16 rows of a tile
 // are what a load's descriptor covers.  No host knows the lengths, so every workgroup finds its share of the work by itself: it reads all lengths and
-// boundaries, a lane a request, prices some lengths of parts to cut the keys into, and numbers row tiles, parts and key heads through (`find`).
+// boundaries, a lane a request, settles how long a part of the keys is, and numbers row tiles, parts and key heads through (`find`).
 #include <algorithm>
 #include <cmath>
 
@@ -34,17 +34,17 @@ struct PagesArgs {
   const int32_t* tables;
   int64_t table_stride;
   const int32_t *lens, *cu;
-  int32_t width, B, T, H, Hk, group;
+  int32_t width, most_len, B, T, H, Hk, group;
   int32_t left, right;          // spans in tokens; -1: no border
   int32_t frame, sinks;
   Quotient by_group, by_frame;
   float scale_log2;
   // ---- how the launch runs
-  int32_t mixed;                // tiles of 256 rows as well as few rows
   int32_t groups;               // workgroups of the grid
   int32_t most_parts[2];        // for how many of them, of 256 rows (0) and of few (1), there is room for parts
   float slots;                  // workgroups at once
   float step[2], once[2], part[2];     // us: of 64 keys, of a workgroup beside them, of a part's way to memory and back
+  float least;                  // ... of a part of few rows
   float* part_out[2];           // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
   float* part_ml[2];
   uint32_t* counters[2];        // of an item's parts that are done, zero before and after the launch
@@ -84,28 +84,33 @@ struct Request {
   int tiles[2];
   float us[2];
 };
+template <bool kMixed>
 __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   Request r = {};
   if (b >= a.B) return r;
-  r.begin = min(max(a.cu[b], 0), a.T);
-  r.n = max(min(max(a.cu[b + 1], 0), a.T) - r.begin, 0);
-  r.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.kv.page);
+  const int from = a.cu[b], to = a.cu[b + 1], len = a.lens[b];
+  r.begin = min(max(from, 0), a.T);
+  r.n = max(min(max(to, 0), a.T) - r.begin, 0);
+  r.len = min(max(len, 0), a.most_len);
   const int rows = r.n * a.group;
   int whole = 0;
-  if (a.mixed) {
+  if (kMixed) {
     r.tiles[0] = rows / kRowsShared + (rows % kRowsShared > kFewRows);
     whole = min(r.tiles[0] * kRowsShared, rows);
   }
   r.tiles[1] = (rows - whole + kRowsFew - 1) / kRowsFew;
-  const Queries qs = queries_of(a, 0, r.n);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (r.tiles[i] > 0) {      // what its last tile sees
-      const int end = i ? rows : whole;
-      const Span first = span_of(qs, r.len, query_of(qs, i ? whole : max(end - kRowsShared, 0))), last = span_of(qs, r.len, query_of(qs, end - 1));
-      const int sinks = min(a.sinks, last.hi);
-      r.us[i] = (float)((sinks + max(last.hi - max(first.lo, sinks), 0) + 63) / 64) * a.step[i];
+  for (int i = kMixed ? 0 : 1; i < 2; ++i) {      // 64-key tiles that its last tile sees
+    const Queries qs = queries_of(a, 0, r.n);
+    const int end = i ? rows : whole;
+    const int hi = a.right < 0 ? r.len : span_of(qs, r.len, query_of(qs, max(end - 1, 0))).hi;
+    int keys = hi;
+    if (a.left >= 0) {
+      const int sinks = min(a.sinks, hi);
+      keys = sinks + max(hi - max(span_of(qs, r.len, query_of(qs, i ? whole : max(end - kRowsShared, 0))).lo, sinks), 0);
     }
+    r.us[i] = r.tiles[i] > 0 ? (float)((keys + 63) / 64) * a.step[i] : 0.f;
+  }
   return r;
 }
 __device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
@@ -133,6 +138,9 @@ __device__ __forceinline__ int as_int(float x) { return __builtin_bit_cast(int, 
 __device__ __forceinline__ float wave_sum(float x) {
   return as_float(lane_value(along(as_int(x), 0, [](int u, int v) { return as_int(as_float(u) + as_float(v)); }), 63));
 }
+__device__ __forceinline__ float wave_max(float x) {
+  return as_float(lane_value(along(as_int(x), 0, [](int u, int v) { return as_int(fmaxf(as_float(u), as_float(v))); }), 63));
+}
 __device__ __forceinline__ float wave_min(float x) {
   return as_float(lane_value(along(as_int(x), as_int(INFINITY), [](int u, int v) { return as_int(fminf(as_float(u), as_float(v))); }), 63));
 }
@@ -147,121 +155,100 @@ __device__ __forceinline__ int divided(int n, int d, int* rest) {
 }
 // Parts of an item that takes `us`, where a part takes 1 / inv of them.  (In floating point: nothing depends on it but that all agree.)
 __device__ __forceinline__ int ways_of(float us, float inv) { return min(max((int)__builtin_ceilf(us * inv - 0.001f), 1), kMostWays); }
+__device__ __forceinline__ float over(float x, float y) { return x * __builtin_amdgcn_rcpf(y); }      // to 2^-22 or so
 
-// Finds workgroup blockIdx.x's work; false: it has none.  [*from, *to): the rows that requests own.
-__device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int* to) {
+// Finds workgroup blockIdx.x's work; false: it has none.  *none: whether there are rows that no request owns.
+template <bool kMixed>
+__device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
   const int lane = threadIdx.x & 63;
   // The workgroup's number.  They are dealt round the XCDs and counted through key heads first, then parts, then row tiles, from those with the most keys on: a
   // multiple of eight key heads stay on an XCD each, whose L2 its row tiles share; else every other turn goes back, or the first XCD would always get
   // the longer one.
   const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
   int g = turn * kXcds + ((turn & 1) && a.Hk % kXcds ? kXcds - 1 - xcd : xcd);
-  Request r = request_of(a, lane);
-  int lo = r.n > 0 ? r.begin : a.T, hi = r.begin + r.n;
-  float most = max(r.us[0], r.us[1]), work[2], items[2];
+  Request r = request_of<kMixed>(a, lane);
+  int owned = r.n;
+  float most = r.us[0], keys = r.us[1], work[2] = {}, items[2] = {};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = kMixed ? 0 : 1; i < 2; ++i) {
     work[i] = (float)r.tiles[i] * r.us[i];
     items[i] = (float)r.tiles[i];
   }
   for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const Request x = request_of(a, b0 + lane);
-    if (x.n > 0) lo = min(lo, x.begin);
-    hi = max(hi, x.begin + x.n);
-    most = max(most, max(x.us[0], x.us[1]));
+    const Request x = request_of<kMixed>(a, b0 + lane);
+    owned += x.n;
+    most = max(most, x.us[0]);
+    keys += x.us[1];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = kMixed ? 0 : 1; i < 2; ++i) {
       work[i] += (float)x.tiles[i] * x.us[i];
       items[i] += (float)x.tiles[i];
     }
   }
-  *to = wave_max(hi);
-  *from = min(-wave_max(-lo), *to);
-  most = as_float(wave_max(as_int(most)));
+  *none = lane_value(sums_along(owned), 63) != a.T;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = kMixed ? 0 : 1; i < 2; ++i) {
     work[i] = wave_sum(work[i]) * (float)a.Hk;
     items[i] = wave_sum(items[i]) * (float)a.Hk;
   }
   float inv[2] = {0.f, 0.f};                // 1 / us of a part
   int tail = INT32_MAX, tail_ways = 1, tail_end = 0;      // items of 256 rows from `tail` on are cut into that many
-  if (a.most_parts[1] > 0 && most > 4.f * min(a.step[0], a.step[1])) {
-    if (a.B <= 64) {
-      // A lane prices 1 .. 64 parts of the longest item, and of the items of 256 rows of the last round.  Unlike items fill the rounds as they come, and wait
-      // for half of the longest one at the end.
-      const float ways = (float)(lane + 1), us = most / ways, mine = 1.f / us, fold = lane > 0 ? 2.f + 0.4f * ways : 0.f;
-      float n[2] = {0.f, 0.f};
-      for (int b = 0; b < a.B; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) n[i] += (float)lane_value(r.tiles[i], b) * (float)ways_of(as_float(lane_value(as_int(r.us[i]), b)), mine);
-      float beside = 0.f, parts = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        n[i] *= (float)a.Hk;
-        beside += n[i] * a.once[i];
-        parts += lane > 0 ? n[i] * a.part[i] : 0.f;
-      }
-      const float all = n[0] + n[1], once = us + (items[0] > 0.f ? a.once[0] : a.once[1]);
-      float cost = all <= a.slots ? once : min(__builtin_ceilf(all / a.slots) * once, (work[0] + work[1] + beside) / a.slots + 0.5f * once);
-      cost += fold + parts;
-      if (lane > 0 && (n[0] > (float)a.most_parts[0] || n[1] > (float)a.most_parts[1] || all > (float)a.groups)) cost = INFINITY;
-      const float best = wave_min(cost);
-      float tail_cost = INFINITY, tail_best = INFINITY;
-      const float whole = __builtin_floorf(items[0] / a.slots), rest = items[0] - whole * a.slots, each = work[0] / max(items[0], 1.f);
-      if (whole >= 1.f) {
-        const float mine_us = each / ways, cuts = rest * ways;
-        float m = 0.f;      // parts of the few rows, as long as those of the tail
-        for (int b = 0; b < a.B; ++b) m += (float)lane_value(r.tiles[1], b) * (float)ways_of(as_float(lane_value(as_int(r.us[1]), b)), 1.f / mine_us);
-        m *= (float)a.Hk;
-        const float end = rest * each + work[1] + cuts * a.once[0] + m * a.once[1];
-        tail_cost = whole * (each + a.once[0]) + 0.5f * max(most - each, 0.f) + end / a.slots + fold + (lane > 0 ? cuts * a.part[0] + m * a.part[1] : 0.f);
-        if (cuts + m > 0.f) tail_cost += cuts + m <= a.slots ? max(mine_us + a.once[0] - end / a.slots, 0.f) : 0.5f * (mine_us + a.once[0]);
-        if (cuts > (float)a.most_parts[0] || m > (float)a.most_parts[1] || whole * a.slots + cuts + m > (float)a.groups) tail_cost = INFINITY;
-        tail_best = wave_min(tail_cost);
-      }
-      if (tail_best < best) {
-        const int at = __builtin_ctzll(__ballot(tail_cost == tail_best));
-        tail = (int)(whole * a.slots);
-        tail_ways = 1 + at;
-        tail_end = tail + (int)rest * tail_ways;
-        inv[1] = 1.f / as_float(lane_value(as_int(each / ways), at));
-      } else {
-        const uint64_t these = __ballot(cost == best);
-        const int at = these ? __builtin_ctzll(these) : 0;
-        inv[0] = inv[1] = at == 0 ? 0.f : as_float(lane_value(as_int(mine), at));
-      }
-    } else {
-      // room for cuts beside one part of every item, shared out by their time; less than there is by more than the sums' roundings
-      const float room = 0.99f * min((float)a.groups, 2.f * a.slots) - items[0] - items[1];
-      if (room > 0.f) {
-        const float mine = 1.f / max(max((work[0] + work[1]) / room, most / kMostWays), 8.f);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (items[i] + work[i] * mine < 0.99f * (float)a.most_parts[i]) inv[i] = mine;
-      }
+  // Few rows: as many parts a slot as make their own time and the wait for the last of them least.  (What there is room for, below by more than the
+  // sums' roundings: an item makes at most its time over that of a part, and one more.)
+  const float per_slot = over(work[0] + work[1], a.slots);
+  if (items[1] > 0.f) {
+    const float room = 0.99f * min((float)a.most_parts[1], (float)a.groups - items[0]) - items[1];
+    float us = 0.03f * per_slot;
+    if (!kMixed) {
+      const float rounds = __builtin_amdgcn_sqrtf(0.05f * over(wave_sum(keys) * (float)a.Hk, a.slots));
+      us = rounds > 2.f ? over(per_slot, rounds) : over(work[1], max(a.slots - items[1], 0.3f * a.slots));
+    }
+    us = max(us, a.least);
+    if (room > 0.f) inv[1] = __builtin_amdgcn_rcpf(max(us, over(work[1], room)));
+  }
+  if (kMixed && items[0] > 0.f) {
+    // Tiles of 256 rows: a lane prices 1 .. 64 parts of those of the last round, or of the longest where there is but one.
+    most = wave_max(most);
+    const float ways = (float)(lane + 1), whole = __builtin_floorf(over(items[0], a.slots) + 1e-4f), rest = items[0] - whole * a.slots;
+    const float each = whole > 0.f ? over(work[0], items[0]) : most;
+    // (unlike items, cut to one length: half a part more each, at most a whole one)
+    const float like = over(work[0], most), parts = whole > 0.f ? rest * ways : lane == 0 ? rest : like * ways + 0.5f * (rest - like), at_most = whole > 0.f ? parts : like * ways + rest;
+    float cost = __builtin_ceilf(over(parts, a.slots) - 1e-4f) * (each * __builtin_amdgcn_rcpf(ways) + a.once[0]);
+    if (lane > 0) cost += 2.f + 0.4f * ways + parts * a.part[0];
+    if (lane > 0 && at_most > 0.99f * min((float)a.most_parts[0], (float)a.groups - whole * a.slots - items[1])) cost = INFINITY;
+    const uint64_t these = __ballot(cost == wave_min(cost));
+    const int at = these ? __builtin_ctzll(these) : 0;
+    if (at > 0 && whole > 0.f) {
+      tail = (int)(whole * a.slots);
+      tail_ways = 1 + at;
+      tail_end = tail + (int)rest * tail_ways;
+      inv[1] = min(inv[1], over(0.99f * min((float)a.most_parts[1], (float)a.groups - (float)tail_end) - items[1], work[1] + 1e-9f));
+      inv[1] = max(inv[1], 0.f);
+    } else if (at > 0) {
+      inv[0] = (float)(at + 1) * __builtin_amdgcn_rcpf(most);
+      inv[1] = max(min(inv[1], over(0.99f * ((float)a.groups - (over(work[0] * (float)(at + 1), most) + items[0])) - items[1], work[1] + 1e-9f)), 0.f);
     }
   }
   w.ways = 1;
   w.part = 0;
   int slot = -1;
-  if (g >= tail && g < tail_end) {
+  if (kMixed && g >= tail && g < tail_end) {
     int part;
     const int item = divided(g - tail, tail_ways, &part);
     slot = item * tail_ways;
     g = tail + item;
     w.part = part;
     w.ways = tail_ways;
-  } else if (g >= tail) {
+  } else if (kMixed && g >= tail) {
     g += tail + (tail_end - tail) / tail_ways - tail_end;      // among the few rows, as if none of the others were cut
   }
   // items, or their parts, in front of a lane's request: those of 256 rows, then the few rows
   int before = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (i == 0 && !a.mixed) continue;
+  for (int i = kMixed ? 0 : 1; i < 2; ++i) {
     const int first = before;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-      if (a.B > 64) r = request_of(a, b0 + lane);
+      if (a.B > 64) r = request_of<kMixed>(a, b0 + lane);
       const int ways = ways_of(r.us[i], inv[i]), mine = a.Hk * r.tiles[i] * ways, sum = sums_along(mine);
       const uint64_t passed = __ballot(before + sum <= g);
       if (passed == ~0ull) {
@@ -286,15 +273,25 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, int* from, int
         slot = group0 - first + (tiles - 1 - tile) * cuts * a.Hk + w.hk;
       }
       w.first = slot;
-      w.row0 = i ? lane_value(r.tiles[0], at) * kRowsShared + tile * kRowsFew : tile * kRowsShared;
+      w.row0 = i ? (kMixed ? lane_value(r.tiles[0], at) * kRowsShared : 0) + tile * kRowsFew : tile * kRowsShared;
       return true;
     }
   }
   return false;
 }
 
-// Zeros, and -inf, in the rows that no request owns.
-__device__ __forceinline__ void fill_rows(const PagesArgs& a, int D, int from, int to) {
+// Zeros, and -inf, in the rows that no request owns: those in front of the first one's and behind the last one's.
+__device__ __forceinline__ void fill_rows(const PagesArgs& a, int D) {
+  const int lane = threadIdx.x & 63;
+  int lo = a.T, hi = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int from = min(max(a.cu[b], 0), a.T), to = min(max(a.cu[b + 1], 0), a.T);
+    if (to > from) {
+      lo = min(lo, from);
+      hi = max(hi, to);
+    }
+  }
+  const int to = wave_max(hi), from = min(-wave_max(-lo), to);
   const int row = a.H * D / 8;          // 16-byte chunks
   for (int r = blockIdx.x; r < a.T - (to - from); r += gridDim.x) {
     const int64_t t = r < from ? r : r + (to - from);
@@ -745,7 +742,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
     weight[i] = weight_of(m[i], li, top);
     l = __builtin_fmaf(weight[i], li, l);
   }
-  constexpr int kCols = D / 8 / W, kSome = 8;          // register groups of a wavefront's share, parts under way together
+  constexpr int kCols = D / 8 / W;          // register groups of a wavefront's share
   const int row = w.row0 + col;
   const bool live = row < qs.rows;
   f32x4 sum[kCols];
@@ -759,96 +756,145 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
       for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(weight[j], x[e], sum[i][e]);     // (a weight of 0 keeps what is undefined: some row's visible key is)
     }
   }
-  if (w.ways > 1) {
-    constexpr int kPartFloats = kRowsFew * D;
-    const int64_t mine = w.first + w.part * w.apart;
-    const Rsrc to = buffer_of(a.part_out[1] + mine * kPartFloats, kPartFloats * 4);
+  if (w.ways == 1) {
+    if (!live) return;
+    const int s = query_of(qs, row), g0 = row - s * a.group;
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    const int64_t head = w.hk * a.group + g0;
+    uint16_t* out = a.out + ((int64_t)(w.begin + s) * a.H + head) * D;
 #pragma unroll
-    for (int i = 0; i < kCols; ++i)
-      if (live) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), to, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice);
-    if (wave == 0 && hh == 0 && live) {
-      store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2, top);
-      store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2 + 1, l);
+    for (int i = 0; i < kCols; ++i) {
+      typename E::x4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(sum[i][e] * inv);
+      *reinterpret_cast<typename E::x4*>(out + 8 * (wave * kCols + i) + 4 * hh) = h;
     }
-    int* flag = reinterpret_cast<int*>(lds + FewLds<D, W>::kFlag);
-    wait_loads();                // (stores as well)
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t* counter = a.counters[1] + w.first;
-      const bool last = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
-      if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      *flag = last;
-    }
-    __syncthreads();
-    if (!*flag || !live) return;
-    const float* mls = a.part_ml[1] + ((int64_t)w.first * kRowsFew + col) * 2;
-    top = -INFINITY;
-    for (int p0 = 0; p0 < w.ways; p0 += kSome) {
-      float x[kSome];
+    if (wave == 0 && hh == 0) a.lse[head * a.T + w.begin + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
+    return;
+  }
+  // A part's rows, [row][D]; the workgroup that completes an item's parts adds them all up, in an order of the sizes' own.
+  constexpr int kPartFloats = kRowsFew * D, kThreads = W * 64;
+  const int64_t mine = w.first + w.part * w.apart;
+  const Rsrc to = buffer_of(a.part_out[1] + mine * kPartFloats, kPartFloats * 4);
 #pragma unroll
-      for (int p = 0; p < kSome; ++p) x[p] = load_device(mls + (int64_t)min(p0 + p, w.ways - 1) * w.apart * (2 * kRowsFew));
+  for (int i = 0; i < kCols; ++i)
+    if (live) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum[i]), to, (col * D + 8 * (wave * kCols + i) + 4 * hh) * 4, 0, kDevice);
+  if (wave == 0 && hh == 0 && live) {
+    store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2, top);
+    store_device(a.part_ml[1] + (mine * kRowsFew + col) * 2 + 1, l);
+  }
+  int* flag = reinterpret_cast<int*>(lds + FewLds<D, W>::kFlag);
+  wait_loads();                // (stores as well)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* counter = a.counters[1] + w.first;
+    const bool last = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
+    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  if (!*flag) return;
+  // Everything that is asked for comes from memory, so as much of it as there is is under way together: maxima and sums of all parts, a thread each, then
+  // 16 bytes of a row a thread, of every `by`-th part where the rows are fewer than the threads.
+  const int tid = threadIdx.x, rows = min(qs.rows - w.row0, kRowsFew);
+  float* weights = reinterpret_cast<float*>(lds);                  // [part][row] maxima, then weights
+  float* sums = weights + kMostWays * kRowsFew;                    // [part][row]
+  float* norms = sums + kMostWays * kRowsFew;                      // [row]
+  f32x4* halves = reinterpret_cast<f32x4*>(norms + kRowsFew);      // [by][16 bytes of the rows]
+  static_assert((2 * kMostWays * kRowsFew + kRowsFew) * 4 + kThreads * 16 <= FewLds<D, W>::kBytes, "the parts' meeting fits the tiles");
+  float pm[kMostWays * kRowsFew / kThreads], pl[kMostWays * kRowsFew / kThreads];
 #pragma unroll
-      for (int p = 0; p < kSome; ++p) top = fmaxf(top, x[p]);
-    }
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    l = 0.f;
-    for (int p0 = 0; p0 < w.ways; p0 += kSome) {
-      float pm[kSome], pl[kSome];
-      f32x4 x[kSome][kCols];
-#pragma unroll
-      for (int p = 0; p < kSome; ++p) {
-        const int64_t at = (int64_t)min(p0 + p, w.ways - 1) * w.apart;
-        pm[p] = load_device(mls + at * (2 * kRowsFew));
-        pl[p] = load_device(mls + at * (2 * kRowsFew) + 1);
-        const Rsrc from = buffer_of(a.part_out[1] + (w.first + at) * kPartFloats, kPartFloats * 4);
-#pragma unroll
-        for (int i = 0; i < kCols; ++i)
-          x[p][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (wave * kCols + i) * 1024 + lane * 16, 0, kDevice));
-      }
-#pragma unroll
-      for (int p = 0; p < kSome; ++p) {
-        if (p0 + p >= w.ways) continue;
-        const float wp = weight_of(pm[p], pl[p], top);
-        l = __builtin_fmaf(wp, pl[p], l);
-#pragma unroll
-        for (int i = 0; i < kCols; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[i][e] = __builtin_fmaf(wp, x[p][i][e], sum[i][e]);
-      }
+  for (int i = 0; i < kMostWays * kRowsFew / kThreads; ++i) {
+    const int at = tid + i * kThreads, p = at / kRowsFew, r = at % kRowsFew;
+    if (p < w.ways && r < rows) {
+      const float* ml = a.part_ml[1] + ((w.first + (int64_t)p * w.apart) * kRowsFew + r) * 2;
+      pm[i] = load_device(ml);
+      pl[i] = load_device(ml + 1);
     }
   }
-  if (!live) return;
-  const int s = query_of(qs, row), g0 = row - s * a.group;
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  const int64_t head = w.hk * a.group + g0;
-  uint16_t* out = a.out + ((int64_t)(w.begin + s) * a.H + head) * D;
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) {
+  for (int i = 0; i < kMostWays * kRowsFew / kThreads; ++i) {
+    const int at = tid + i * kThreads;
+    if (at / kRowsFew < w.ways && at % kRowsFew < rows) {
+      weights[at] = pm[i];
+      sums[at] = pl[i];
+    }
+  }
+  __syncthreads();
+  if (tid < rows) {
+    float high = -INFINITY, all = 0.f;
+    for (int p = 0; p < w.ways; ++p) high = fmaxf(high, weights[p * kRowsFew + tid]);
+    for (int p = 0; p < w.ways; ++p) {
+      const float lp = sums[p * kRowsFew + tid], wp = weight_of(weights[p * kRowsFew + tid], lp, high);
+      all = __builtin_fmaf(wp, lp, all);
+      weights[p * kRowsFew + tid] = wp;
+    }
+    norms[tid] = all != 0.f ? 1.f / all : 0.f;
+    const int s = query_of(qs, w.row0 + tid), head = w.hk * a.group + w.row0 + tid - s * a.group;
+    a.lse[(int64_t)head * a.T + w.begin + s] = all != 0.f ? (high + __builtin_amdgcn_logf(all)) * kLn2 : -INFINITY;
+  }
+  __syncthreads();
+  constexpr int kSixteens = D / 4, kSome = 8;          // 16-byte pieces of a row, parts under way together
+  const int pieces = rows * kSixteens;
+  auto added = [&](int e, int first, int by) {      // piece e of the parts first, first + by ..
+    const Rsrc from = buffer_of(a.part_out[1] + (int64_t)w.first * kPartFloats, 0x7fffffff);
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int p0 = first; p0 < w.ways; p0 += kSome * by) {
+      f32x4 x[kSome];
+#pragma unroll
+      for (int i = 0; i < kSome; ++i) {
+        const uint32_t at = (uint32_t)min(p0 + i * by, w.ways - 1) * (uint32_t)w.apart * (kPartFloats * 4);
+        x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at + e * 16, 0, kDevice));
+      }
+#pragma unroll
+      for (int i = 0; i < kSome; ++i)
+        if (p0 + i * by < w.ways) {
+          const float wp = weights[(p0 + i * by) * kRowsFew + e / kSixteens];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[c] = __builtin_fmaf(wp, x[i][c], acc[c]);
+        }
+    }
+    return acc;
+  };
+  auto store = [&](int e, const f32x4& acc) {
+    const int r = e / kSixteens, s = query_of(qs, w.row0 + r), head = w.hk * a.group + w.row0 + r - s * a.group;
     typename E::x4 h;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = (typename E::t)(sum[i][e] * inv);
-    *reinterpret_cast<typename E::x4*>(out + 8 * (wave * kCols + i) + 4 * hh) = h;
+    for (int c = 0; c < 4; ++c) h[c] = (typename E::t)(acc[c] * norms[r]);
+    *reinterpret_cast<typename E::x4*>(a.out + ((int64_t)(w.begin + s) * a.H + head) * D + 4 * (e % kSixteens)) = h;
+  };
+  if (2 * pieces <= kThreads) {
+    const int by = kThreads / pieces, first = tid / pieces, e = tid - first * pieces;
+    if (first < by) halves[first * pieces + e] = added(e, first, by);
+    __syncthreads();
+    if (tid < pieces) {
+      f32x4 acc = halves[tid];
+      for (int i = 1; i < by; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += halves[i * pieces + tid][c];
+      store(tid, acc);
+    }
+  } else {
+    for (int e = tid; e < pieces; e += kThreads) store(e, added(e, 0, 1));
   }
-  if (wave == 0 && hh == 0) a.lse[head * a.T + w.begin + s] = l != 0.f ? (top + __builtin_amdgcn_logf(l)) * kLn2 : -INFINITY;
 }
 
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   Work w;
-  int own_from, own_to;
-  const bool some = find(a, w, &own_from, &own_to);
-  fill_rows(a, D, own_from, own_to);
+  bool none;
+  const bool some = find<false>(a, w, &none);
+  if (none) fill_rows(a, D);
   if (some) few_rows<D, kHalf, kWavesFew>(a, w, lds);
 }
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   Work w;
-  int own_from, own_to;
-  const bool some = find(a, w, &own_from, &own_to);
-  fill_rows(a, D, own_from, own_to);
+  bool none;
+  const bool some = find<true>(a, w, &none);
+  if (none) fill_rows(a, D);
   if (!some) return;
   if (w.few) few_rows<D, kHalf, kWavesShared>(a, w, lds);
   else shared_tiles<D, kHalf>(a, w, lds);
@@ -894,25 +940,26 @@ struct Scratch {
 template <int D, bool kHalf>
 int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
   const int64_t rows = (int64_t)a.T * a.group, requests = std::min<int64_t>(a.B, a.T);
-  a.mixed = std::min(most_rows, rows) > kFewRows;
-  const int64_t slots = (int64_t)n_cus * (a.mixed ? 1 : 2) * (D == 64 ? 2 : 1);
-  const int64_t big = a.mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
-  const int64_t small = std::min(rows / kRowsFew + requests, a.mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
+  const bool mixed = std::min(most_rows, rows) > kFewRows;
+  const int64_t slots = (int64_t)n_cus * (mixed ? 1 : 2) * (D == 64 ? 2 : 1);
+  const int64_t big = mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
+  const int64_t small = std::min(rows / kRowsFew + requests, mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
   const int64_t uncut = a.Hk * (big + small);
   a.slots = (float)slots;
-  const float full = D == 64 ? 2.0f : 1.0f;      // workgroups that share a CU
-  a.step[0] = (D == 64 ? 1.0f : 1.4f) * full;
-  a.step[1] = (D == 64 ? 1.0f : 1.6f) * full * (a.mixed ? 0.25f : 0.5f);
+  a.step[0] = D == 64 ? 2.2f : 1.6f;
+  a.step[1] = mixed ? (D == 64 ? 0.5f : 0.6f) : 3.2f;
+  a.least = mixed ? 12.f : 16 * a.step[1];
   a.once[0] = 8.f;
   a.once[1] = 4.f;
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
   // few rows first, whose parts are small
   int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;
-  const int64_t groups = std::max(uncut + slots, 2 * slots);
+  // (an empty workgroup takes a slot for 1.1 us: there are no more than what the longest row of the tables could be cut into)
+  const int64_t groups = uncut + std::min<int64_t>(3 * slots, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
   int64_t parts[2];
   parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups});
-  parts[0] = a.mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;
+  parts[0] = mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;
   float* at = static_cast<float*>(scratch.workspace);
   uint32_t* counter = scratch.counters;
   for (int i : {1, 0}) {
@@ -930,7 +977,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
     return DT_ERR_INVALID;
   }
   a.groups = (int32_t)(grid / kXcds * kXcds);
-  return a.mixed ? launch<attn_pages_kernel<D, kHalf>>(a, a.groups, kWavesShared, SharedLds<D>::kBytes, stream)
+  return mixed ? launch<attn_pages_kernel<D, kHalf>>(a, a.groups, kWavesShared, SharedLds<D>::kBytes, stream)
                  : launch<attn_pages_few_kernel<D, kHalf>>(a, a.groups, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
 }
 
@@ -998,6 +1045,7 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
   a.lens = lens;
   a.cu = cu_seqlens;
   a.width = width;
+  a.most_len = width * pages->page_size;
   a.B = B;
   a.T = T;
   a.H = H;
