@@ -63,13 +63,35 @@ __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d,
   }
 }
 
-// A launch whose keys go into the pages of a cache, and values beside them: rows[0] are q, rows[1] k, `v` values, of which nothing but their place
-// changes.  Tokens are packed, B = 1.  A lane group finds its token's slot with its rows under way.
+// A launch whose keys go into the pages of a cache, and values beside them: rows[0] are q, rows[1] k.  Tokens are packed, B = 1.  A lane group finds its
+// token's slot with its rows under way.  Values are only copied, by workgroups of their own behind the others, 16 bytes a lane.
+constexpr int kCopies = 4;       // of a lane
 struct PagedArgs : RotaryArgs {
-  Rows v;
   Pages to;
   const int64_t* slots;
+  const uint16_t* v;
+  int64_t v_ss, v_sh;
+  uint32_t first_copy, copies;   // workgroup, and 16-byte pieces in all
+  Quotient by_pieces;
+  int32_t pieces, head_shift;    // of a token, log2 of those of a head
 };
+__device__ __forceinline__ void copy_values(const PagedArgs& a) {
+  const uint32_t first = (blockIdx.x - a.first_copy) * (kThreads * kCopies) + threadIdx.x;
+  u32x4 x[kCopies];
+  int64_t slot[kCopies];
+  int head[kCopies], d[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const uint32_t at = min(first + i * kThreads, a.copies - 1), t = quotient(at, a.by_pieces), c = at - t * a.pieces;
+    head[i] = c >> a.head_shift;
+    d[i] = 8 * (c & ((1 << a.head_shift) - 1));
+    slot[i] = first + i * kThreads < a.copies ? a.slots[t] : -1;
+    x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.v + t * a.v_ss + head[i] * a.v_sh + d[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i)
+    if (a.to.has(slot[i])) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(a.to.row(1, slot[i]) + head[i] * a.to.sh[1] + d[i]));
+}
 
 // kRms: with an RMS norm, which does without the 20 registers of means and biases (14 882 x 48 heads of 128 66.6 -> 64.4 us; a form of its own for rows
 // without a norm, with as few, is 3 % slower than the common one).
@@ -81,19 +103,10 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
   const uint32_t item = blockIdx.x * (kThreads / G) + threadIdx.x / G;
   if (item >= a.items) return;   // a lane group leaves as a whole; the exchanges below stay inside a group
   const uint32_t bs = quotient(item, a.by_groups);
-  int hg, values = 0;
-  if constexpr (kPages) {
-    hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups + a.v.groups));
-    values = hg >= a.rows[0].groups + a.rows[1].groups;
-    if (values) hg -= a.rows[1].groups;      // (and those of q, below)
-  } else {
-    hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups));
-  }
+  int hg = (int)(item - bs * (uint32_t)(a.rows[0].groups + a.rows[1].groups));
   const bool second = hg >= a.rows[0].groups;
   if (second) hg -= a.rows[0].groups;
-  const Rows* of = second ? &a.rows[1] : &a.rows[0];
-  if constexpr (kPages) of = values ? &a.v : of;
-  const Rows& t = *of;
+  const Rows& t = second ? a.rows[1] : a.rows[0];
   const uint32_t b = quotient(bs, a.by_s), s = bs - b * (uint32_t)a.S;
   const int h0 = hg * kHeads, nh = min(t.H - h0, kHeads);
   const int ea = kHalves ? a.a0[c] : 8 * c, eb = kHalves ? a.b0[c] : 8 * c + 4;
@@ -121,22 +134,8 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
     if (second) {
       const int64_t slot = a.slots[bs];
       if (!a.to.has(slot)) return;
-      y_sh = a.to.sh[values];
-      yp = a.to.row(values, slot) + h0 * y_sh;
-    }
-    if (values) {
-#pragma unroll
-      for (int r = 0; r < kHeads; ++r)
-        if (r < nh) {
-          uint16_t* p = yp + r * y_sh;
-          if constexpr (kHalves) {
-            *reinterpret_cast<u32x2*>(p + ea) = u32x2{raw[r].x, raw[r].y};
-            *reinterpret_cast<u32x2*>(p + eb) = u32x2{raw[r].z, raw[r].w};
-          } else {
-            *reinterpret_cast<u32x4*>(p + ea) = raw[r];
-          }
-        }
-      return;
+      y_sh = a.to.sh[0];
+      yp = a.to.row(0, slot) + h0 * y_sh;
     }
   }
   // the angles of this lane's pairs; t mod 2^32 of the upper half of n F
@@ -223,7 +222,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(const Rotar
 }
 template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms>
 __global__ __launch_bounds__(kThreads) void prepare_pages_kernel(const PagedArgs a) {
-  rotate_rows<D, kHalf, kHalves, kHeads, kRms>(a);
+  if (blockIdx.x >= a.first_copy) copy_values(a);
+  else rotate_rows<D, kHalf, kHalves, kHeads, kRms>(a);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -347,10 +347,10 @@ bool eight_heads(Args& a, int64_t& groups, __int128& items, int D, std::initiali
     else if (halves) DT_LAUNCH(kernel, D, false, true);                  \
     else DT_LAUNCH(kernel, D, false, false);                             \
   } while (0)
-#define DT_LAUNCH_ROTARY(kernel)                                                                                    \
+#define DT_LAUNCH_ROTARY(kernel, copies)                                                                            \
   do {                                                                                                               \
     const int per_wg = kThreads / (D / 8);                                                                          \
-    const dim3 grid((unsigned)((items + per_wg - 1) / per_wg)), block(kThreads);                                    \
+    const dim3 grid((unsigned)((items + per_wg - 1) / per_wg) + copies), block(kThreads);                           \
     const hipStream_t st = (hipStream_t)stream;                                                                     \
     const bool half = (rounding & DT_IO_FP16) != 0, halves = rope == DT_ROPE_HALVES, rms = norm == DT_NORM_RMS;     \
     if (D == 128) DT_LAUNCH_D(kernel, 128);                                                                         \
@@ -384,7 +384,7 @@ extern "C" int dt_qk_norm_rope_axes(const dt_rotary_rows* rows, int32_t n_rows, 
   a.items = (uint32_t)items;
   a.by_groups = quotient_by((int32_t)groups);
   a.by_s = quotient_by(S);
-  DT_LAUNCH_ROTARY(qk_norm_rope_axes_kernel);
+  DT_LAUNCH_ROTARY(qk_norm_rope_axes_kernel, 0);
   return hip_fail(hipGetLastError(), "qk_norm_rope_axes launch");
 }
 
@@ -403,22 +403,28 @@ extern "C" int dt_prepare_pages(const dt_rotary_rows* rows, const void* v, const
     set_error("v, its strides and slots must be non-null, v 16-byte aligned with strides that are multiples of 8 elements");
     return DT_ERR_INVALID;
   }
-  a.v = a.rows[1];
-  a.v.x = static_cast<const uint16_t*>(v);
-  a.v.ss = v_strides[0];
-  a.v.sh = v_strides[1];
+  a.v = static_cast<const uint16_t*>(v);
+  a.v_ss = v_strides[0];
+  a.v_sh = v_strides[1];
   a.slots = slots;
-  int64_t groups = (int64_t)a.rows[0].groups + 2 * a.rows[1].groups;
+  int64_t groups = (int64_t)a.rows[0].groups + a.rows[1].groups;
+  const __int128 copies = (__int128)T * a.rows[1].H * (D / 8);
   __int128 items = (__int128)T * groups;
-  if (items * (D / 8) > (1ll << 32) - kThreads || items >= (1ll << 31)) {
+  if (items * (D / 8) + copies > (1ll << 31)) {
     set_error("too many rows");
     return DT_ERR_INVALID;
   }
-  const bool eight = eight_heads(a, groups, items, D, {&a.rows[0], &a.rows[1], &a.v});
+  const bool eight = eight_heads(a, groups, items, D, {&a.rows[0], &a.rows[1]});
   a.S = T;
   a.items = (uint32_t)items;
   a.by_groups = quotient_by((int32_t)groups);
   a.by_s = quotient_by(T);
-  DT_LAUNCH_ROTARY(prepare_pages_kernel);
+  a.first_copy = (uint32_t)((items + kThreads / (D / 8) - 1) / (kThreads / (D / 8)));
+  a.copies = (uint32_t)copies;
+  a.pieces = a.rows[1].H * (D / 8);
+  a.by_pieces = quotient_by(a.pieces);
+  a.head_shift = D == 128 ? 4 : 3;
+  const unsigned copy_groups = (unsigned)((copies + kThreads * kCopies - 1) / (kThreads * kCopies));
+  DT_LAUNCH_ROTARY(prepare_pages_kernel, copy_groups);
   return hip_fail(hipGetLastError(), "prepare_pages launch");
 }
