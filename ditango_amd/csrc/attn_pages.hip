@@ -879,14 +879,14 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
   }
 }
 
-template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesFew * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
+template <int D, bool kHalf, int W>
+__global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel(const PagesArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   Work w;
   bool none;
   const bool some = find<false>(a, w, &none);
   if (none) fill_rows(a, D);
-  if (some) few_rows<D, kHalf, kWavesFew>(a, w, lds);
+  if (some) few_rows<D, kHalf, W>(a, w, lds);
 }
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
@@ -941,13 +941,15 @@ template <int D, bool kHalf>
 int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
   const int64_t rows = (int64_t)a.T * a.group, requests = std::min<int64_t>(a.B, a.T);
   const bool mixed = std::min(most_rows, rows) > kFewRows;
-  const int64_t slots = (int64_t)n_cus * (mixed ? 1 : 2) * (D == 64 ? 2 : 1);
   const int64_t big = mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
   const int64_t small = std::min(rows / kRowsFew + requests, mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
   const int64_t uncut = a.Hk * (big + small);
+  // Few rows of few requests, which leave CUs without one, have eight wavefronts each.
+  const bool eight = !mixed && uncut <= n_cus / 2;
+  const int64_t slots = (int64_t)n_cus * (mixed || eight ? 1 : 2) * (D == 64 ? 2 : 1);
   a.slots = (float)slots;
   a.step[0] = D == 64 ? 2.2f : 1.6f;
-  a.step[1] = mixed ? (D == 64 ? 0.5f : 0.6f) : 3.2f;
+  a.step[1] = mixed ? (D == 64 ? 0.5f : 0.6f) : eight ? 1.6f : 3.2f;
   a.least = mixed ? 12.f : 16 * a.step[1];
   a.once[0] = 8.f;
   a.once[1] = 4.f;
@@ -978,7 +980,8 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   }
   a.groups = (int32_t)(grid / kXcds * kXcds);
   return mixed ? launch<attn_pages_kernel<D, kHalf>>(a, a.groups, kWavesShared, SharedLds<D>::kBytes, stream)
-                 : launch<attn_pages_few_kernel<D, kHalf>>(a, a.groups, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
+         : eight ? launch<attn_pages_few_kernel<D, kHalf, kWavesShared>>(a, a.groups, kWavesShared, FewLds<D, kWavesShared>::kAll, stream)
+                 : launch<attn_pages_few_kernel<D, kHalf, kWavesFew>>(a, a.groups, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -38,31 +38,32 @@ struct PlanArgs {
 };
 
 __device__ __forceinline__ int held_pages(const PlanArgs& a, int tokens) { return (int)quotient(tokens + a.page - 1, a.by_page); }
-__device__ __forceinline__ int kept_len(const PlanArgs& a, int b) {
-  return (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.width * a.page);
-}
 
-// Sums over the threads in front of this one; *total is that of all of them.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* waves, int64_t* total) {
+// Sums along the threads that stop at `most`, and are still sums then: of x, 0 .. 2^30, over the threads in front of this one; *total over all.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
+__device__ __forceinline__ int block_scan(int x, int most, int* waves, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t sum = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(sum, d);
-    if (lane >= d) sum += y;
-  }
+  int sum = x;      // rows of 16 lanes, then across them
+  sum = min(sum + moved<0x111, 0xf>(sum), most);
+  sum = min(sum + moved<0x112, 0xf>(sum), most);
+  sum = min(sum + moved<0x114, 0xf>(sum), most);
+  sum = min(sum + moved<0x118, 0xf>(sum), most);
+  sum = min(sum + moved<0x142, 0xa>(sum), most);
+  sum = min(sum + moved<0x143, 0xc>(sum), most);
   if (lane == 63) waves[wave] = sum;
+  const int mine = __shfl_up(sum, 1);
   __syncthreads();
-  int64_t before = 0, all = 0;
+  int before = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < kPlanWaves; ++i) {
-    const int64_t w = waves[i];
-    if (i < wave) before += w;
-    all += w;
+    const int w = waves[i];
+    if (i < wave) before = min(before + w, most);
+    all = min(all + w, most);
   }
   __syncthreads();
   *total = all;
-  return before + sum - x;
+  return min(before + (lane > 0 ? mine : 0), most);
 }
 
 // The last of the n values of x, which never fall, that is at most v (x[0] is).
@@ -82,51 +83,54 @@ __device__ __forceinline__ int64_t slot_of(const PlanArgs& a, int b, int j) {
   return (uint32_t)p < (uint32_t)a.n_pages ? (int64_t)p * a.page + (j - i * a.page) : -1;
 }
 
-// One workgroup: the free pages are in its LDS, a bit a page.
+// One workgroup: the free pages are in its LDS, a bit a page.  Latency all the way: 8 requests' next tokens PLANTOKEN us, of which an empty launch is 2.4; 64
+// requests that hold 29 300 pages and get 1250 PLANFRAMES (their 86 400 slots, by a launch behind it, 4.2).
 __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs a, int slots_too) {
   extern __shared__ __align__(16) uint8_t lds[];
-  __shared__ int64_t waves[kPlanWaves];
+  __shared__ int32_t waves[kPlanWaves];
   __shared__ int32_t before[kPlanThreads];          // free pages in front of a thread's words
   uint32_t* taken = reinterpret_cast<uint32_t*>(lds);
   int32_t* cu = reinterpret_cast<int32_t*>(taken + a.words);      // [B + 1]
   int32_t* start = cu + a.B + 1;                                  // [B]: pages that the requests in front of it need
   int32_t* len = start + a.B;                                     // [B], its complement where the request is not served
-  const int tid = threadIdx.x;
-  for (int i = tid; i < a.words; i += kPlanThreads) taken[i] = 0;
-  int64_t tokens = 0, pages = 0;
+  const int tid = threadIdx.x, most_len = a.width * a.page;
+  int tokens = 0, pages = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     const bool there = b < a.B;
-    const int l = there ? kept_len(a, b) : 0;
-    int64_t total;
-    const int64_t c0 = tokens + block_scan(there ? max(a.new_lens[b], 0) : 0, waves, &total);
-    const int from = (int)min(c0, (int64_t)a.n_tokens);
-    tokens += total;
-    const int64_t to64 = c0 + (there ? max(a.new_lens[b], 0) : 0);
-    const int n = (int)min(to64, (int64_t)a.n_tokens) - from;
-    const bool fits = (int64_t)l + n <= (int64_t)a.width * a.page;
-    const int64_t s0 = pages + block_scan(there && fits ? held_pages(a, l + n) - held_pages(a, l) : 0, waves, &total);
-    pages += total;
+    const int l = there ? min(max(a.lens[b], 0), most_len) : 0, asked = there ? min(max(a.new_lens[b], 0), a.n_tokens) : 0;
+    if (b0 == 0)
+      for (int i = tid; i < a.words; i += kPlanThreads) taken[i] = 0;
+    int total;
+    const int from = min(tokens + block_scan(asked, a.n_tokens, waves, &total), a.n_tokens), n = min(asked, a.n_tokens - from);
+    tokens = min(tokens + total, a.n_tokens);
+    const bool fits = n <= most_len - l;
+    const int before_me = block_scan(there && fits ? min(held_pages(a, l + n) - held_pages(a, l), kMostPages + 1) : 0, kMostPages + 1, waves, &total);
     if (there) {
       cu[b] = from;
       len[b] = fits ? l : ~l;
-      start[b] = (int)min(s0, (int64_t)kMostPages + 1);
+      start[b] = min(pages + before_me, kMostPages + 1);
     }
+    pages = min(pages + total, kMostPages + 1);
   }
-  if (tid == 0) cu[a.B] = (int)min(tokens, (int64_t)a.n_tokens);
+  if (tid == 0) cu[a.B] = tokens;
   __syncthreads();
-  // the pages that somebody holds; a.lanes threads a request
+  // the pages that somebody holds; a.lanes threads a request, 16 entries of each under way together
+  constexpr int kSome = 16;
   for (int b = tid / a.lanes; b < a.B; b += kPlanThreads / a.lanes) {
     const int l = len[b], n = held_pages(a, l < 0 ? ~l : l);
     const int32_t* row = a.tables + b * a.table_stride;
-    for (int i = tid % a.lanes; i < n; i += a.lanes) {
-      const int p = row[i];
-      if ((uint32_t)p < (uint32_t)a.n_pages) atomicOr(&taken[p >> 5], 1u << (p & 31));
+    for (int i = tid % a.lanes; i < n; i += kSome * a.lanes) {
+      int p[kSome];
+#pragma unroll
+      for (int j = 0; j < kSome; ++j) p[j] = row[min(i + j * a.lanes, n - 1)];
+#pragma unroll
+      for (int j = 0; j < kSome; ++j)
+        if (i + j * a.lanes < n && (uint32_t)p[j] < (uint32_t)a.n_pages) atomicOr(&taken[p[j] >> 5], 1u << (p[j] & 31));
     }
   }
-  __syncthreads();
   // behind the last page there is none
-  if (tid == 0 && (a.n_pages & 31)) taken[a.words - 1] |= ~0u << (a.n_pages & 31);
+  if (tid == 0 && (a.n_pages & 31)) atomicOr(&taken[a.words - 1], ~0u << (a.n_pages & 31));
   __syncthreads();
   const int each = (a.words + kPlanThreads - 1) / kPlanThreads;
   int mine = 0;
@@ -134,23 +138,23 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs
     const int w = tid * each + i;
     if (w < a.words) mine += __popc(~taken[w]);
   }
-  int64_t n_free;
-  before[tid] = (int)block_scan(mine, waves, &n_free);
+  int n_free;
+  before[tid] = block_scan(mine, kMostPages + 1, waves, &n_free);
   // who is served: in order, from the first one that finds too few on none that needs any
-  int64_t granted = 0;
+  int granted = 0;
   for (int b = tid; b < a.B; b += kPlanThreads) {
     const int l = len[b], at = l < 0 ? ~l : l, n = cu[b + 1] - cu[b];
     const int need = l < 0 ? 0 : held_pages(a, at + n) - held_pages(a, at);
-    const bool yes = l >= 0 && (need == 0 || start[b] + need <= n_free);
+    const bool yes = l >= 0 && (need == 0 || need <= n_free - start[b]);
     if (!yes) len[b] = ~at;
-    else if (need > 0) granted = max(granted, (int64_t)start[b] + need);
+    else if (need > 0) granted = max(granted, start[b] + need);
     a.served[b] = yes;
     a.lens_out[b] = yes ? at + n : at;
     a.cu[b] = cu[b];
   }
   if (tid == 0) a.cu[a.B] = cu[a.B];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) granted = max(granted, (int64_t)__shfl_xor((int)granted, d));
+  for (int d = 1; d < 64; d <<= 1) granted = max(granted, __shfl_xor(granted, d));
   if ((tid & 63) == 0) waves[tid >> 6] = granted;
   __syncthreads();
 #pragma unroll
@@ -284,8 +288,8 @@ extern "C" int dt_plan_pages(int32_t* tables, int64_t table_stride, int32_t widt
     return DT_ERR_INVALID;
   }
   if (B > kMostRequests || n_pages > kMostPages || (int64_t)width * page_size > (1 << 29) || (int64_t)n_pages * page_size > INT32_MAX ||
-      n_tokens > (1 << 30)) {
-    set_error("more than %d requests, %d pages, 2^29 tokens of a request, 2^31 - 1 of the pool or 2^30 new ones are not supported", kMostRequests, kMostPages);
+      n_tokens > (1 << 29)) {
+    set_error("more than %d requests, %d pages, 2^29 tokens of a request, 2^31 - 1 of the pool or 2^29 new ones are not supported", kMostRequests, kMostPages);
     return DT_ERR_UNSUPPORTED;
   }
   PlanArgs a{};

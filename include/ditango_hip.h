@@ -643,7 +643,7 @@ typedef struct {
  * tokens do not fit its row gets none, and from the first one that finds too few on, none gets any.  served[b] = 1 where request b has pages for
  * all of its tokens, and then tables (in place, new entries only) and lens_out[b] (its new length) say so; else served[b] = 0, lens_out[b] its old length.
  * slots[t], t < n_tokens: where the keys and values of row t go; -1 for rows of requests that are not served, rows behind the last one, and tokens whose
- * entry is no page.  lens_out may be lens.  At most 2048 requests, 2^20 pages, 2^29 tokens a request, 2^30 new ones.
+ * entry is no page.  lens_out may be lens.  At most 2048 requests, 2^20 pages, 2^29 tokens a request, 2^29 new ones.
  * No counterpart in the reference.
  */
 int dt_plan_pages(int32_t* tables, int64_t table_stride, int32_t width, const int32_t* lens, const int32_t* new_lens, int32_t B,
