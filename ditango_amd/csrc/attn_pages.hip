@@ -24,6 +24,7 @@ constexpr int kXcds = 8;
 constexpr int kWavesFew = 4;
 constexpr int kFewRows = 96;
 constexpr int kMostWays = 64;              // parts of an item
+constexpr int kMostRequests = 2048;        // every workgroup reads all lengths
 
 struct PagesArgs {
   const uint16_t* q;
@@ -127,8 +128,9 @@ __device__ __forceinline__ int along(int x, int none, Op op) {      // lane i: o
   x = op(x, moved<0x142, 0xa>(x, none));
   return op(x, moved<0x143, 0xc>(x, none));
 }
+constexpr int kMost = 1 << 24;      // sums stop here, beyond every workgroup of a grid
 __device__ __forceinline__ int sums_along(int x) {
-  return along(x, 0, [](int u, int v) { return u + v; });
+  return along(x, 0, [](int u, int v) { return min(u + v, kMost); });
 }
 __device__ __forceinline__ int wave_max(int x) {
   return lane_value(along(x, INT32_MIN, [](int u, int v) { return max(u, v); }), 63);
@@ -167,7 +169,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
   const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
   int g = turn * kXcds + ((turn & 1) && a.Hk % kXcds ? kXcds - 1 - xcd : xcd);
   Request r = request_of<kMixed>(a, lane);
-  int owned = r.n;
+  uint32_t owned = r.n;
   float most = r.us[0], keys = r.us[1], work[2] = {}, items[2] = {};
 #pragma unroll
   for (int i = kMixed ? 0 : 1; i < 2; ++i) {
@@ -185,7 +187,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
       items[i] += (float)x.tiles[i];
     }
   }
-  *none = lane_value(sums_along(owned), 63) != a.T;
+  *none = lane_value(along((int)owned, 0, [](int u, int v) { return (int)((uint32_t)u + (uint32_t)v); }), 63) != a.T;
 #pragma unroll
   for (int i = kMixed ? 0 : 1; i < 2; ++i) {
     work[i] = wave_sum(work[i]) * (float)a.Hk;
@@ -249,14 +251,14 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     const int first = before;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
       if (a.B > 64) r = request_of<kMixed>(a, b0 + lane);
-      const int ways = ways_of(r.us[i], inv[i]), mine = a.Hk * r.tiles[i] * ways, sum = sums_along(mine);
+      const int ways = ways_of(r.us[i], inv[i]), sum = sums_along((int)min((int64_t)a.Hk * r.tiles[i] * ways, (int64_t)kMost));
       const uint64_t passed = __ballot(before + sum <= g);
       if (passed == ~0ull) {
         before += lane_value(sum, 63);
         continue;
       }
       const int at = __builtin_ctzll(~passed);
-      const int group0 = before + lane_value(sum, at) - lane_value(mine, at);
+      const int group0 = before + (at > 0 ? lane_value(sum, at - 1) : 0);
       w.b = b0 + at;
       w.begin = lane_value(r.begin, at);
       w.n = lane_value(r.n, at);
@@ -960,7 +962,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   // (an empty workgroup takes a slot for 1.1 us: there are no more than what the longest row of the tables could be cut into)
   const int64_t groups = uncut + std::min<int64_t>(3 * slots, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
   int64_t parts[2];
-  parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups});
+  parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups, (int64_t)INT32_MAX / kBytes[1]});      // (a part's place in 32 bits)
   parts[0] = mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;
   float* at = static_cast<float*>(scratch.workspace);
   uint32_t* counter = scratch.counters;
@@ -1017,6 +1019,10 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
   if (w.left < -1 || w.right < -1 || w.frame < 1 || w.sinks < 0) {
     set_error("window: left and right must be -1 (no border) or frames, frame at least 1, sinks not negative");
     return DT_ERR_INVALID;
+  }
+  if (B > kMostRequests) {
+    set_error("more than %d requests are not supported", kMostRequests);
+    return DT_ERR_UNSUPPORTED;
   }
   if ((int64_t)width * pages->page_size > kMostTokens || T > kMostTokens || w.sinks > kMostTokens || w.frame > kMostTokens) {
     set_error("lengths, sinks and frames beyond 2^29 tokens are not supported");

@@ -675,7 +675,7 @@ int dt_prepare_pages(const dt_rotary_rows* rows, const void* v, const int64_t* v
  * out [T,H,D] contiguous in the dtype of q, lse fp32 [H,T]; a row that sees no key, or that no request owns, gets out = 0, lse = -inf.  A masked key
  * adds nothing, whatever it and its value hold.  out may be q where that is contiguous.
  * max_seqlen_q: the most rows a request has, which the launch is made for; requests with more come out right, only later.
- * workspace and counters as for dt_attn_window_fwd; nothing is cut without either.  No counterpart in the reference.
+ * At most 2048 requests.  workspace and counters as for dt_attn_window_fwd; nothing is cut without either.  No counterpart in the reference.
  */
 int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
                       const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,

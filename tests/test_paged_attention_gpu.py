@@ -178,6 +178,18 @@ def test_boundaries_and_lengths_that_cannot_be(hip, rows):
         _check(out, lse, q, kp, vp, tables, [min(n, width * 16) for n in lens], cu, right=0)
 
 
+def test_overlapping_requests_end(hip):
+    """Boundaries that fall: more rows in all than there are.  What comes out is not said, but the launch ends and touches nothing else."""
+    q, kp, vp, tables, _ = _setup([100] * 200, [3] * 200, 2, 1, 64, 16, torch.bfloat16, junk=0.25)
+    for cu in ([0, 600] * 100 + [0], [600, 0] * 100 + [600]):
+        guard = torch.full((602, 2, 64), 5.0, device=DEV).bfloat16()
+        out = guard[1:601]
+        from ditango_amd.pages import paged_attention
+        paged_attention(q, kp, vp, _i32(tables), _i32([100] * 200), _i32(cu), right=0, out=out)
+        torch.cuda.synchronize()
+        assert bool((guard[0] == 5).all()) and bool((guard[601] == 5).all())
+
+
 @pytest.mark.parametrize("new", [1, 200])
 def test_entries_that_are_no_pages_read_as_zeros(hip, new):
     lens = [333, 200]
