@@ -537,7 +537,7 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
     load_pair(1);
   }
   st.open(qs, 0, w.hk, row0, w.len, lane, false);
-  if (n > 0) walk_tiles<D, kHalf, true>(st, lds, list, all_first, all_last, wave, lane, load_pair);
+  if (n > 0) walk_tiles<D, kHalf, true>(st, lds, list, all_first, all_last, n, wave, lane, load_pair);
   const int col = lane & 31, hh = lane >> 5;
   float m = st.m_ref * st.c, l = st.l_run + __shfl_xor(st.l_run, 32);
   float undefined = 0.f;
@@ -960,7 +960,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   // few rows first, whose parts are small
   int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;
   // (an empty workgroup takes a slot for 1.1 us: there are no more than what the longest row of the tables could be cut into)
-  const int64_t groups = uncut + std::min<int64_t>(3 * slots, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
+  const int64_t groups = uncut + std::min<int64_t>((mixed ? 3 : 6) * slots / 2, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
   int64_t parts[2];
   parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups, (int64_t)INT32_MAX / kBytes[1]});      // (a part's place in 32 bits)
   parts[0] = mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;

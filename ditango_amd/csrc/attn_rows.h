@@ -373,13 +373,13 @@ __device__ __forceinline__ void queries_to_lds(uint32_t lds0, int row0, int wave
 // The rows of a wavefront over the tiles of a list that is not empty.  In front of it go the loads of Q, K of tile 0 and pairs 0 and 1, in this order, of
 // kLoads / 2 and kLoads loads a wavefront; load_pair(t) sends for pair t.
 template <int D, bool kHalf, bool kRun = false, typename LoadPair>
-__device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint8_t* lds, const TileList<64>& list, const Span& all_first, const Span& all_last,
-                                           int wave, int lane, LoadPair load_pair) {
+__device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint8_t* lds, TileList<64> list, Span all_first, Span all_last,
+                                           int n, int wave, int lane, LoadPair load_pair) {
   typedef Tiles<D, 2> T;
   typedef SharedLds<D> S;
   typedef Elem<kHalf> E;
   typedef typename E::x8 ex8;
-  const int group = wave >> 2, n = list.end - list.begin;
+  const int group = wave >> 2;
   f32x16 s[2];
   ex8 p[2][2];
   // The products of a tile and the scores of the next as one stream of MFMAs, fed by reads from the LDS that run kRing fragments ahead.

@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_windo
     load_pair(1);
   }
   st.open(a, it.b, it.hk, row0, len, lane, false);
-  if (n > 0) walk_tiles<D, kHalf>(st, lds, list, all_first, all_last, wave, lane, load_pair);
+  if (n > 0) walk_tiles<D, kHalf>(st, lds, list, all_first, all_last, n, wave, lane, load_pair);
   // Rows of the result through the LDS, so that a store covers whole lines: half of the columns at a time.
   const int col = lane & 31, hh = lane >> 5;
   const float l = st.l_run + __shfl_xor(st.l_run, 32);
