@@ -46,6 +46,7 @@ struct PagesArgs {
   float slots;                  // workgroups at once
   float step[2], once[2], part[2];     // us: of 64 keys, of a workgroup beside them, of a part's way to memory and back
   float least;                  // ... of a part of few rows
+  float cached;                 // ... of as many keys of all key heads as the last cache holds
   float* part_out[2];           // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
   float* part_ml[2];
   uint32_t* counters[2];        // of an item's parts that are done, zero before and after the launch
@@ -66,7 +67,7 @@ __device__ __forceinline__ Queries queries_of(const PagesArgs& a, int begin, int
 // A workgroup's work: row tile `row0` .. of a request and key head, and of its keys the part [tiles part / ways, tiles (part + 1) / ways)
 struct Work {
   int b, begin, n, len;         // request, its first row, its rows' and its keys' number
-  int few;                      // 32 rows, not 256
+  int few, once;                // 32 rows, not 256; whose keys are read by this item only, of a launch of many
   int hk, row0, part, ways;
   int first, apart;             // slot of the item's first part, slots between its parts
   template <typename List>
@@ -193,6 +194,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     work[i] = wave_sum(work[i]) * (float)a.Hk;
     items[i] = wave_sum(items[i]) * (float)a.Hk;
   }
+  keys = wave_sum(keys);
   float inv[2] = {0.f, 0.f};                // 1 / us of a part
   int tail = INT32_MAX, tail_ways = 1, tail_end = 0;      // items of 256 rows from `tail` on are cut into that many
   // Few rows: as many parts a slot as make their own time and the wait for the last of them least.  (What there is room for, below by more than the
@@ -202,7 +204,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     const float room = 0.99f * min((float)a.most_parts[1], (float)a.groups - items[0]) - items[1];
     float us = 0.03f * per_slot;
     if (!kMixed) {
-      const float rounds = __builtin_amdgcn_sqrtf(0.05f * over(wave_sum(keys) * (float)a.Hk, a.slots));
+      const float rounds = __builtin_amdgcn_sqrtf(0.05f * over(keys * (float)a.Hk, a.slots));
       us = rounds > 2.f ? over(per_slot, rounds) : over(work[1], max(a.slots - items[1], 0.3f * a.slots));
     }
     us = max(us, a.least);
@@ -264,6 +266,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
       w.n = lane_value(r.n, at);
       w.len = lane_value(r.len, at);
       w.few = i;
+      w.once = i && keys > a.cached && lane_value(r.tiles[0] * 2 + r.tiles[1], at) == 1;
       const int tiles = lane_value(r.tiles[i], at), cuts = lane_value(ways, at);
       int part;
       const int rest = divided(g - group0, a.Hk, &w.hk), tile = tiles - 1 - divided(rest, cuts, &part);      // the last ones first: under a causal border they see most
@@ -401,12 +404,17 @@ struct PageLoader {
     k_block = T::kBlockRows * ks.ss[0];
     v_block = T::kBlockRows * ks.ss[1];
   }
+  template <bool kOnce = false>
+  __device__ __forceinline__ static void load(const u32x4& r, uint32_t off, uint32_t to) {
+    if constexpr (kOnce) load_block_once_to_lds(r, off, to);
+    else load_block_to_lds(r, off, 0, to);
+  }
+  template <bool kOnce = false>
   __device__ __forceinline__ void issue_k(const u32x4& r, int blk, uint32_t to) const {
-    load_block_to_lds(r, k_row + (k_chunk ^ (64u * (blk & T::kBlockXor))) + (blk % kOf) * k_block, 0, to + blk * 1024);
+    load<kOnce>(r, k_row + (k_chunk ^ (64u * (blk & T::kBlockXor))) + (blk % kOf) * k_block, to + blk * 1024);
   }
-  __device__ __forceinline__ void issue_v(const u32x4& r, int blk, uint32_t to) const {
-    load_block_to_lds(r, v_off + (blk % kOf) * v_block, 0, to + blk * 1024);
-  }
+  template <bool kOnce = false>
+  __device__ __forceinline__ void issue_v(const u32x4& r, int blk, uint32_t to) const { load<kOnce>(r, v_off + (blk % kOf) * v_block, to + blk * 1024); }
 };
 
 // Parts as they lie in the registers: 4 floats a lane, (register group) x (lane).  `at`: of a row's column d.
@@ -642,6 +650,8 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
   }
 }
 
+// (kOnce: no other workgroup reads these keys, and they are more than the last cache holds; 8 tokens over 10 000 keys of 24 heads of 128 each 187 -> 167 us, 5.9
+// TB/s.  With keys that are in the cache yet, 64 tokens over 300 keys of 24 heads again and again, 45 -> 48; with two row tiles to a head, 120 -> 140.)
 // Few rows: as attn_window.hip's, a wavefront takes every fourth tile of its item, or of a part of it, K of the next tile sent for before the softmax of
 // this one, V of the next behind its values; the states of the four meet in the LDS, those of parts in memory, where the last part adds them up.
 template <int D, bool kHalf, int W>
@@ -662,6 +672,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
   const Keys ks(a, w);
   L ld;
   ld.open(ks, lane);
+  const bool once = __builtin_amdgcn_readfirstlane(w.once);
   Finder<T::kKeys, W> finder[2];
   Sixteen here[2], next[2];
   auto look = [&](Sixteen (&x)[2]) __attribute__((always_inline)) {
@@ -672,16 +683,26 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const u32x4 r = x[i].template rsrc<D>(ks, 0);
+      if (once) {
 #pragma unroll
-      for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_k(r, blk, kt0);
+        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.template issue_k<true>(r, blk, kt0);
+      } else {
+#pragma unroll
+        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_k(r, blk, kt0);
+      }
     }
   };
   auto load_v = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const u32x4 r = x[i].template rsrc<D>(ks, 1);
+      if (once) {
 #pragma unroll
-      for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_v(r, blk, kt0 + T::kBytes);
+        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.template issue_v<true>(r, blk, kt0 + T::kBytes);
+      } else {
+#pragma unroll
+        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_v(r, blk, kt0 + T::kBytes);
+      }
     }
   };
   int t = list.begin + wave;
@@ -955,6 +976,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   a.least = mixed ? 12.f : 16 * a.step[1];
   a.once[0] = 8.f;
   a.once[1] = 4.f;
+  a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
   // few rows first, whose parts are small

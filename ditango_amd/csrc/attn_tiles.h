@@ -94,6 +94,19 @@ __device__ __forceinline__ void load_block_to_lds(u32x4 rsrc, uint32_t lane_off,
                : "memory", "m0");
 }
 
+// The same for bytes that nobody else reads: past the caches, which keep what others do.
+__device__ __forceinline__ void load_block_once_to_lds(u32x4 rsrc, uint32_t lane_off, uint32_t lds_addr) {
+  u32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane(rsrc.x);
+  r.y = __builtin_amdgcn_readfirstlane(rsrc.y);
+  r.z = __builtin_amdgcn_readfirstlane(rsrc.z);
+  r.w = __builtin_amdgcn_readfirstlane(rsrc.w);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+               :
+               : "v"(lane_off), "s"(r), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
+               : "memory", "m0");
+}
+
 // The same from an address of each lane's own.
 __device__ __forceinline__ void load_rows_to_lds(const uint16_t* from, uint32_t lds_addr) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
