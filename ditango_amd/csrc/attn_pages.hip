@@ -41,6 +41,7 @@ struct PagesArgs {
   Quotient by_group, by_frame;
   float scale_log2;
   // ---- how the launch runs
+  int32_t all_few;              // whether a grid with tiles of 256 rows has room for all rows as few rows
   int32_t groups;               // workgroups of the grid
   int32_t most_parts[2];        // for how many of them, of 256 rows (0) and of few (1), there is room for parts
   float slots;                  // workgroups at once
@@ -220,15 +221,28 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     float cost = __builtin_ceilf(over(parts, a.slots) - 1e-4f) * (each * __builtin_amdgcn_rcpf(ways) + a.once[0]);
     if (lane > 0) cost += 2.f + 0.4f * ways + parts * a.part[0];
     if (lane > 0 && at_most > 0.99f * min((float)a.most_parts[0], (float)a.groups - whole * a.slots - items[1])) cost = INFINITY;
-    const uint64_t these = __ballot(cost == wave_min(cost));
+    const float best = wave_min(cost);
+    const uint64_t these = __ballot(cost == best);
     const int at = these ? __builtin_ctzll(these) : 0;
+    bool all_few = false;
+    if (a.all_few && whole == 0.f) {
+      // Little work: all of it as few rows, which twice as many CUs share.
+      const Request f = request_of<false>(a, lane);
+      const float all = wave_sum((float)f.tiles[1] * f.us[1]) * (float)a.Hk, n = wave_sum((float)f.tiles[1]) * (float)a.Hk, longest = wave_max(f.us[1]);
+      all_few = a.once[1] + max(min(longest, a.least), over(all, a.slots)) + (longest > a.least ? 5.f : 0.f) < best;
+      if (all_few) {
+        r = f;
+        const float room = 0.99f * min((float)a.most_parts[1], (float)a.groups) - n;
+        inv[1] = room > 0.f ? __builtin_amdgcn_rcpf(max(max(over(all, max(a.slots - n, 0.3f * a.slots)), a.least), over(all, room))) : 0.f;
+      }
+    }
     if (at > 0 && whole > 0.f) {
       tail = (int)(whole * a.slots);
       tail_ways = 1 + at;
       tail_end = tail + (int)rest * tail_ways;
       inv[1] = min(inv[1], over(0.99f * min((float)a.most_parts[1], (float)a.groups - (float)tail_end) - items[1], work[1] + 1e-9f));
       inv[1] = max(inv[1], 0.f);
-    } else if (at > 0) {
+    } else if (at > 0 && !all_few) {
       inv[0] = (float)(at + 1) * __builtin_amdgcn_rcpf(most);
       inv[1] = max(min(inv[1], over(0.99f * ((float)a.groups - (over(work[0] * (float)(at + 1), most) + items[0])) - items[1], work[1] + 1e-9f)), 0.f);
     }
@@ -973,16 +987,19 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   a.slots = (float)slots;
   a.step[0] = D == 64 ? 2.2f : 1.6f;
   a.step[1] = mixed ? (D == 64 ? 0.5f : 0.6f) : eight ? 1.6f : 3.2f;
-  a.least = mixed ? 12.f : 16 * a.step[1];
+  a.least = mixed ? 8.f : 16 * a.step[1];
   a.once[0] = 8.f;
   a.once[1] = 4.f;
   a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
+  const int64_t as_few = a.Hk * (rows / kRowsFew + requests);
+  a.all_few = mixed && a.B <= 64 && as_few <= slots;
   // few rows first, whose parts are small
   int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;
   // (an empty workgroup takes a slot for 1.1 us: there are no more than what the longest row of the tables could be cut into)
-  const int64_t groups = uncut + std::min<int64_t>((mixed ? 3 : 6) * slots / 2, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
+  int64_t groups = uncut + std::min<int64_t>((mixed ? 3 : 6) * slots / 2, uncut * std::min<int64_t>(a.most_len / 512, kMostWays - 1));
+  if (a.all_few) groups = std::max(groups, as_few + slots);
   int64_t parts[2];
   parts[1] = std::min({bytes / 2 / kBytes[1], counters / 2, groups, (int64_t)INT32_MAX / kBytes[1]});      // (a part's place in 32 bits)
   parts[0] = mixed ? std::min({(bytes - parts[1] * kBytes[1]) / kBytes[0], (counters - parts[1]) / kWavesShared, groups}) : 0;
@@ -997,7 +1014,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
     at += floats;
     counter += parts[i] * (i ? 1 : kWavesShared);
   }
-  const int64_t grid = (parts[1] > 0 ? groups : uncut) + kXcds - 1;
+  const int64_t grid = (parts[1] > 0 || a.all_few ? groups : uncut) + kXcds - 1;
   if (grid > (1 << 23) - 1) {
     set_error("too many query rows");
     return DT_ERR_INVALID;
