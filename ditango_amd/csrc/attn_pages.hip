@@ -666,8 +666,21 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
 
 // (kOnce: no other workgroup reads these keys, and they are more than the last cache holds; 8 tokens over 10 000 keys of 24 heads of 128 each 187 -> 167 us, 5.9
 // TB/s.  With keys that are in the cache yet, 64 tokens over 300 keys of 24 heads again and again, 45 -> 48; with two row tiles to a head, 120 -> 140.)
+template <int N>
+__device__ __forceinline__ void wait_q() {     // all loads but those of a tile's K and V, of N each
+  static_assert(N == 4 || N == 8, "blocks of a half tile");
+  if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+}
 // Few rows: as attn_window.hip's, a wavefront takes every fourth tile of its item, or of a part of it, K of the next tile sent for before the softmax of
 // this one, V of the next behind its values; the states of the four meet in the LDS, those of parts in memory, where the last part adds them up.
+// Q comes once for all of them, through the LDS: loaded as fragments, by loads that the compiler counts among the tiles' that it does not know, it would be
+// waited for in the loop, and V of a tile with it.
+template <int D, int W>
+struct FewPagesLds {
+  typedef FewLds<D, W> F;
+  static constexpr int kQ = (F::kAll + 1023) / 1024 * 1024, kAll = kQ + 32 * 2 * D;
+};
 template <int D, bool kHalf, int W>
 __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint8_t* lds) {
   typedef Tiles<D, 1> T;
@@ -677,7 +690,17 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
   const int col = lane & 31, hh = lane >> 5;
   const Queries qs = queries_of(a, w.begin, w.n);
   RowState<D, kHalf, 1> st;
-  st.open(qs, 0, w.hk, w.row0, w.len, lane, true);
+  // (4 or 8 blocks of 1 KB: none, one or two a wavefront)
+  const uint32_t qt0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds + FewPagesLds<D, W>::kQ;
+#pragma unroll
+  for (int i = 0; i < (T::kBlocks + W - 1) / W; ++i) {
+    const int blk = wave + W * i, r = blk * T::kBlockRows + lane / T::kRowLanes;
+    if (blk < T::kBlocks) {
+      const int row = min(w.row0 + r, qs.rows - 1), s = query_of(qs, row);
+      load_rows_to_lds(qs.q + s * a.q_ss + (w.hk * a.group + row - s * a.group) * a.q_sh + 8 * ((lane % T::kRowLanes) ^ T::swz_k(r)), qt0 + blk * 1024);
+    }
+  }
+  st.open(qs, 0, w.hk, w.row0, w.len, lane, false);
   TileList<T::kKeys> list(qs, st.first, st.last, 0, 1);
   w.share(list);                // ... every W-th tile
   const uint8_t* kt = lds + wave * FewLds<D, W>::kTile;
@@ -727,7 +750,17 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
     look(next);
     load_k(here);
     load_v(here);
+    wait_q<T::kBlocks>();
+  } else {
+    wait_loads();
   }
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+    st.qf[i] = *reinterpret_cast<const typename E::x8*>(lds + FewPagesLds<D, W>::kQ + col * T::kRowBytes + 16 * ((2 * i + hh) ^ T::swz_k(col)));
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) asm volatile("" : "+v"(st.qf[i]));
   for (; t < list.end; t += W) {
     const int k0 = list.key(t);
     const bool masked = !st.whole(k0);
@@ -925,6 +958,7 @@ __global__ __launch_bounds__(W * 64, D == 64 ? 4 : 2) void attn_pages_few_kernel
   if (none) fill_rows(a, D);
   if (some) few_rows<D, kHalf, W>(a, w, lds);
 }
+static_assert(FewPagesLds<64, kWavesShared>::kAll <= SharedLds<64>::kBytes && FewPagesLds<128, kWavesShared>::kAll <= SharedLds<128>::kBytes, "both forms fit");
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kWavesShared * 64, D == 64 ? 4 : 2) void attn_pages_kernel(const PagesArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
@@ -1021,8 +1055,8 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   }
   a.groups = (int32_t)(grid / kXcds * kXcds);
   return mixed ? launch<attn_pages_kernel<D, kHalf>>(a, a.groups, kWavesShared, SharedLds<D>::kBytes, stream)
-         : eight ? launch<attn_pages_few_kernel<D, kHalf, kWavesShared>>(a, a.groups, kWavesShared, FewLds<D, kWavesShared>::kAll, stream)
-                 : launch<attn_pages_few_kernel<D, kHalf, kWavesFew>>(a, a.groups, kWavesFew, FewLds<D, kWavesFew>::kAll, stream);
+         : eight ? launch<attn_pages_few_kernel<D, kHalf, kWavesShared>>(a, a.groups, kWavesShared, FewPagesLds<D, kWavesShared>::kAll, stream)
+                 : launch<attn_pages_few_kernel<D, kHalf, kWavesFew>>(a, a.groups, kWavesFew, FewPagesLds<D, kWavesFew>::kAll, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
