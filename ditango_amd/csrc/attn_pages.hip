@@ -350,26 +350,31 @@ struct Keys {
   }
 };
 
-// 16 keys of a tile, which are in one page.
-struct Sixteen {
-  int id, place;                // page, and the first key's place in it
-  int left;                     // keys from the first one to the last of the request; not above 0: none of them is there
+// kCount times 16 keys of a tile; each sixteen is in one page.
+template <int kCount>
+struct Sixteens {
+  int id[kCount], place[kCount];      // page, and the first key's place in it
+  int left;                           // keys from the first one to the last of the request; not above 0: none of them is there
   // (rows behind the last key, and those of no page, arrive as zeros)
   template <int D>
-  __device__ __forceinline__ u32x4 rsrc(const Keys& ks, int i) const {
-    uint32_t valid = 15 * ks.ss[i] + 2 * D;
-    if (__builtin_expect(left < 16, 0)) {
+  __device__ __forceinline__ void rsrc(const Keys& ks, int i, u32x4 (&r)[kCount]) const {
+    uint32_t valid[kCount];
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) valid[j] = 15 * ks.ss[i] + 2 * D;
+    if (__builtin_expect(left < 16 * kCount, 0)) {
       asm volatile("" ::: "memory");
-      valid = left > 0 ? (uint32_t)(left - 1) * ks.ss[i] + 2 * D : 0u;
+#pragma unroll
+      for (int j = 0; j < kCount; ++j) valid[j] = left > 16 * j ? (uint32_t)(min(left - 16 * j, 16) - 1) * ks.ss[i] + 2 * D : 0u;
     }
-    return make_rsrc(ks.at(i, id, place), (uint32_t)id < (uint32_t)ks.n_pages ? valid : 0u);
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) r[j] = make_rsrc(ks.at(i, id[j], place[j]), (uint32_t)id[j] < (uint32_t)ks.n_pages ? valid[j] : 0u);
   }
 };
-// Finds a sixteen of each tile of a list, every kStep keys between two stops: the first key of the window, the list's end.  An entry is asked for when it
+// Finds the sixteens of each tile of a list, every kStep keys between two stops: the first key of the window, the list's end.  An entry is asked for when it
 // is found, and used a tile later.
-template <int kKeys, int kTiles>
+template <int kKeys, int kTiles, int kCount>
 struct Finder {
-  int entry, place, left, t, stop;      // of the next one: its table entry, ...
+  int entry, place, left, t, stop;      // of the next one: its first sixteen's table entry, ...
   int over, more;                       // kStep % page, kStep / page
   static constexpr int kStep = kKeys * kTiles;
   __device__ __forceinline__ void open(const Keys& ks, const TileList<kKeys>& list, int first, int offset) {
@@ -386,11 +391,23 @@ struct Finder {
     stop = t < list.n_sink ? min(list.n_sink, list.end) : t < list.end ? list.end : INT32_MAX;
     for (int* x : {&entry, &place, &left, &stop}) *x = __builtin_amdgcn_readfirstlane(*x);
   }
-  __device__ __forceinline__ Sixteen next(const Keys& ks, const TileList<kKeys>& list, int offset) {
-    Sixteen x;
-    x.place = place;
+  __device__ __forceinline__ Sixteens<kCount> next(const Keys& ks, const TileList<kKeys>& list, int offset) {
+    Sixteens<kCount> x;
     x.left = left;
-    x.id = ks.table[min(entry, ks.width - 1)];
+    int e = entry, p = place;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) {
+      if (j > 0) {
+        p += 16;
+        if (p >= ks.page) {
+          p = 0;
+          ++e;
+        }
+      }
+      x.place[j] = p;
+      x.id[j] = *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+          reinterpret_cast<const __attribute__((address_space(4))) char*>(ks.table) + 4u * (uint32_t)min(e, ks.width - 1));
+    }
     t += kTiles;
     entry += more;
     place += over;
@@ -526,20 +543,22 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
   // A wavefront brings kPer neighbouring blocks of a tile, which are of one sixteen.  Tile t + 1 of K goes with tile t of V.
   constexpr int kPer = T::kBlocks / kWavesShared;
   const int offset = 16 * (kPer * wave / L::kOf);
-  Finder<64, 1> finder;
-  Sixteen of_v, of_k, of_next;
+  Finder<64, 1, 1> finder;
+  Sixteens<1> of_v, of_k, of_next;
   auto load_k = [&](int pair) __attribute__((always_inline)) {
-    const u32x4 r = of_k.template rsrc<D>(ks, 0);
+    u32x4 r[1];
+    of_k.template rsrc<D>(ks, 0, r);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) ld.issue_k(r, kPer * wave + i, lds0 + pair_at<D>(pair) + T::kBytes);
+    for (int i = 0; i < kPer; ++i) ld.issue_k(r[0], kPer * wave + i, lds0 + pair_at<D>(pair) + T::kBytes);
     of_v = of_k;
     of_k = of_next;
     of_next = finder.next(ks, list, offset);
   };
   auto load_pair = [&](int t) __attribute__((always_inline)) {
-    const u32x4 r = of_v.template rsrc<D>(ks, 1);
+    u32x4 r[1];
+    of_v.template rsrc<D>(ks, 1, r);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) ld.issue_v(r, kPer * wave + i, lds0 + pair_at<D>(t));
+    for (int i = 0; i < kPer; ++i) ld.issue_v(r[0], kPer * wave + i, lds0 + pair_at<D>(t));
     load_k(t);
   };
   RowState<D, kHalf, 2> st;
@@ -710,44 +729,35 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
   L ld;
   ld.open(ks, lane);
   const bool once = __builtin_amdgcn_readfirstlane(w.once);
-  Finder<T::kKeys, W> finder[2];
-  Sixteen here[2], next[2];
-  auto look = [&](Sixteen (&x)[2]) __attribute__((always_inline)) {
+  Finder<T::kKeys, W, 2> finder;
+  Sixteens<2> here, next;
+  auto load_k = [&](const Sixteens<2>& x) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
+    u32x4 r[2];
+    x.template rsrc<D>(ks, 0, r);
+    if (once) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = finder[i].next(ks, list, 16 * i);
-  };
-  auto load_k = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {     // (past the end, with an empty descriptor: the waits count loads)
+      for (int blk = 0; blk < T::kBlocks; ++blk) ld.template issue_k<true>(r[blk / L::kOf], blk, kt0);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const u32x4 r = x[i].template rsrc<D>(ks, 0);
-      if (once) {
-#pragma unroll
-        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.template issue_k<true>(r, blk, kt0);
-      } else {
-#pragma unroll
-        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_k(r, blk, kt0);
-      }
+      for (int blk = 0; blk < T::kBlocks; ++blk) ld.issue_k(r[blk / L::kOf], blk, kt0);
     }
   };
-  auto load_v = [&](const Sixteen (&x)[2]) __attribute__((always_inline)) {
+  auto load_v = [&](const Sixteens<2>& x) __attribute__((always_inline)) {
+    u32x4 r[2];
+    x.template rsrc<D>(ks, 1, r);
+    if (once) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const u32x4 r = x[i].template rsrc<D>(ks, 1);
-      if (once) {
+      for (int blk = 0; blk < T::kBlocks; ++blk) ld.template issue_v<true>(r[blk / L::kOf], blk, kt0 + T::kBytes);
+    } else {
 #pragma unroll
-        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.template issue_v<true>(r, blk, kt0 + T::kBytes);
-      } else {
-#pragma unroll
-        for (int blk = i * L::kOf; blk < (i + 1) * L::kOf; ++blk) ld.issue_v(r, blk, kt0 + T::kBytes);
-      }
+      for (int blk = 0; blk < T::kBlocks; ++blk) ld.issue_v(r[blk / L::kOf], blk, kt0 + T::kBytes);
     }
   };
   int t = list.begin + wave;
   if (t < list.end) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) finder[i].open(ks, list, t, 16 * i);
-    look(here);
-    look(next);
+    finder.open(ks, list, t, 0);
+    here = finder.next(ks, list, 0);
+    next = finder.next(ks, list, 0);
     load_k(here);
     load_v(here);
     wait_q<T::kBlocks>();
@@ -770,13 +780,12 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Work& w, uint
     st.scores(kt, s);
     asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0]) : : "memory");      // (the tile has been read)
     load_k(next);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) here[i] = next[i];
-    look(next);
+    here = next;
+    next = finder.next(ks, list, 0);
     st.softmax(s, p, k0, masked, lane);
     wait_oldest<T::kBlocks>();
-    if (masked && st.any_not_finite(vt, lane)) st.values_not_finite(vt, p, k0, lane);
-    else st.values(vt, p);
+    if (masked && st.any_not_finite(vt, lane)) st.take_out_not_finite(const_cast<uint8_t*>(vt), k0, lane);
+    st.values(vt, p);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     load_v(here);
   }
