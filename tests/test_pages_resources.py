@@ -32,7 +32,7 @@ def test_paged_attention(resources):
         for name, r in _kernels(resources, fragment, n).items():
             # heads of 64: some registers around the few rows' loop, none within it
             assert r["ScratchSize [bytes/lane]"] <= (0 if "ILi128E" in name else 40), (name, r)
-            assert r["Occupancy [waves/SIMD]"] == (2 if "ILi128E" in name else 4), (name, r)
+            assert r["Occupancy [waves/SIMD]"] >= (2 if "ILi128E" in name else 4), (name, r)
 
 
 @pytest.mark.parametrize("fragment, n", [("plan_pages_kernel", 1), ("plan_slots_kernel", 1), ("append_pages_kernel", 1), ("prepare_pages_kernel", 32)])
