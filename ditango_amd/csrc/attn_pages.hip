@@ -7,6 +7,11 @@
 // A request's rows (new tokens x query heads of a key head) go in tiles of 256, and what is left over in tiles of 32 where that is at most kFewRows.
 // Batches of requests that have no more rows than that run in a kernel with few rows only; in the other one both forms run side by side.
 //
+// Many rows are bound by the matrix instructions at the power cap: two frames of 3600 tokens, 24 heads of 128, 32 400 keys each, 2.56 ms, 1.12 PFLOP/s at
+// 1.66 GHz (on contiguous keys 2.53); heads of 64 by softmax and products in turn (a frame of 1350 of two rollouts, 48 heads, 0.52 ms, 0.87 PFLOP/s).
+// Single tokens are bound by the memory: 8 over 3000 to 17 776 keys of 24 heads of 128, 176 us, 5.8 TB/s.  Small calls wait: 3 requests of 4 tokens 9.2 us,
+// of which 2.4 are an empty launch's, 2 go by until a workgroup has found its work, 3 until its first tile is there.
+//
 // Which page holds a tile is read by scalar loads one tile ahead, so that no tile waits for it; a page is a multiple of 16 tokens, and 16 rows of a tile
 // are what a load's descriptor covers.  No host knows the lengths, so every workgroup finds its share of the work by itself: it reads all lengths and
 // boundaries, a lane a request, settles how long a part of the keys is, and numbers row tiles, parts and key heads through (`find`).
@@ -22,6 +27,8 @@ namespace {
 constexpr int32_t kMostTokens = 1 << 29;   // positions, spans and lengths: their sums stay in 32 bits
 constexpr int kXcds = 8;
 constexpr int kWavesFew = 4;
+// Two tiles of 32 rows take less time than one of 256, three about as much.  Against 64, geometric means over draws of all sizes differ by less than 1 %:
+// 7 requests x 86 rows of 20 key heads of 64 over 14 000 keys 182 us with 64, 169 with 96; 16 x 80 of 8 of 128 239 and 270, of 6 227 and 205.
 constexpr int kFewRows = 96;
 constexpr int kMostWays = 64;              // parts of an item
 constexpr int kMostRequests = 2048;        // every workgroup reads all lengths
@@ -277,6 +284,8 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
       w.n = lane_value(r.n, at);
       w.len = lane_value(r.len, at);
       w.few = i;
+      // Keys that no other workgroup reads go past the caches where all of them are more than the last one holds: 8 tokens over 10 000 keys of 24 heads of 128
+      // each 187 -> 167 us.  Of keys that the last call has left there, 64 tokens over 300 keys of 24 heads, 45 -> 48; with two row tiles to a head 120 -> 140.
       w.once = i && keys > a.cached && lane_value(r.tiles[0] * 2 + r.tiles[1], at) == 1;
       const int tiles = lane_value(r.tiles[i], at), cuts = lane_value(ways, at);
       // Of tiles of 256 rows key heads are counted first, then parts, then row tiles, from those with the most keys on: a multiple of eight key heads stay on
@@ -699,8 +708,6 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
   }
 }
 
-// (kOnce: no other workgroup reads these keys, and they are more than the last cache holds; 8 tokens over 10 000 keys of 24 heads of 128 each 187 -> 167 us, 5.9
-// TB/s.  With keys that are in the cache yet, 64 tokens over 300 keys of 24 heads again and again, 45 -> 48; with two row tiles to a head, 120 -> 140.)
 template <int N>
 __device__ __forceinline__ void wait_q() {     // all loads but those of a tile's K and V, of N each
   static_assert(N == 4 || N == 8, "blocks of a half tile");
@@ -1032,7 +1039,9 @@ struct Scratch {
   int64_t n_counters;
 };
 
-// The grid holds what there can be, cut or not.  us of 64 keys as launches that fill the chip take them; see attn_window.hip's forms.
+// The grid holds what there can be, cut or not.  `step` is the time of 64 keys as traces of launches that fill the chip show it: 256 rows 1.6 us with heads
+// of 128 (alone on a CU), 2.2 with heads of 64 (two on a CU); 32 rows by the memory, of which eight wavefronts draw twice what four do.  `once` is a workgroup's
+// time beside them.  They only decide how keys are cut: parts of half or twice the length change a launch by a few per cent.
 template <int D, bool kHalf>
 int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
   const int64_t rows = (int64_t)a.T * a.group, requests = std::min<int64_t>(a.B, a.T);
@@ -1040,7 +1049,8 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   const int64_t big = mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
   const int64_t small = std::min(rows / kRowsFew + requests, mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
   const int64_t uncut = a.Hk * (big + small);
-  // Few rows of few requests, which leave CUs without one, have eight wavefronts each.
+  // Few rows of few requests, which leave CUs without one, have eight wavefronts each: 40 items of 30 rows, heads of 64, over 20 000 keys 40 us, with four 47;
+  // 144 items of a row, heads of 128, over 5000 keys 82, with four 69.
   const bool eight = !mixed && uncut <= n_cus / 2;
   const int64_t slots = (int64_t)n_cus * (mixed || eight ? 1 : 2) * (D == 64 ? 2 : 1);
   a.slots = (float)slots;
@@ -1049,7 +1059,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   a.least = mixed ? 8.f : 16 * a.step[1];
   a.once[0] = 8.f;
   a.once[1] = 4.f;
-  a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];
+  a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];      // (256 MB; 64 keys and values of a head are 256 D bytes)
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
   const int64_t as_few = a.Hk * (rows / kRowsFew + requests);
