@@ -4,7 +4,7 @@
 // attn_window.hip, and the result is a state (out, lse) like its.  The rows' arithmetic is attn_rows.h's, in the same two forms:
 //   * shared tiles: 256 rows of one request and key head a workgroup, which walks the 64-key tiles that some row sees;
 //   * few rows: 32 rows, whose four or eight wavefronts take 32-key tiles in turn.
-// A request's rows (new tokens x query heads of a key head) go in tiles of 256, and what is left over in tiles of 32 where that is at most kFewRows.
+// A request's rows (new tokens x query heads of a key head) go in tiles of 256, and what is left over in tiles of 32 where that is at most 64 or 96.
 // Batches of requests that have no more rows than that run in a kernel with few rows only; in the other one both forms run side by side.
 //
 // Many rows are bound by the matrix instructions at the power cap: two frames of 3600 tokens, 24 heads of 128, 32 400 keys each, 2.56 ms, 1.12 PFLOP/s at
@@ -27,9 +27,6 @@ namespace {
 constexpr int32_t kMostTokens = 1 << 29;   // positions, spans and lengths: their sums stay in 32 bits
 constexpr int kXcds = 8;
 constexpr int kWavesFew = 4;
-// Two tiles of 32 rows take less time than one of 256, three about as much.  Against 64, geometric means over draws of all sizes differ by less than 1 %:
-// 7 requests x 86 rows of 20 key heads of 64 over 14 000 keys 182 us with 64, 169 with 96; 16 x 80 of 8 of 128 239 and 270, of 6 227 and 205.
-constexpr int kFewRows = 96;
 constexpr int kMostWays = 64;              // parts of an item
 constexpr int kMostRequests = 2048;        // every workgroup reads all lengths
 
@@ -48,6 +45,7 @@ struct PagesArgs {
   Quotient by_group, by_frame;
   float scale_log2;
   // ---- how the launch runs
+  int32_t few_rows;             // rows that are left over of tiles of 256 go in tiles of 32 up to here
   int32_t all_few;              // whether a grid with tiles of 256 rows has room for all rows as few rows
   int32_t groups;               // workgroups of the grid
   int32_t most_parts[2];        // for how many of them, of 256 rows (0) and of few (1), there is room for parts
@@ -105,7 +103,7 @@ __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   const int rows = r.n * a.group;
   int whole = 0;
   if (kMixed) {
-    r.tiles[0] = rows / kRowsShared + (rows % kRowsShared > kFewRows);
+    r.tiles[0] = rows / kRowsShared + (rows % kRowsShared > a.few_rows);
     whole = min(r.tiles[0] * kRowsShared, rows);
   }
   r.tiles[1] = (rows - whole + kRowsFew - 1) / kRowsFew;
@@ -549,28 +547,29 @@ __device__ __forceinline__ bool masked_not_finite(const Keys& ks, const RowState
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D, bool kHalf>
-__device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, uint8_t* lds) {
+// A wavefront's share of the tiles of 256 rows: kPer neighbouring blocks of each, which are of one sixteen.  Tile t + 1 of K goes with tile t of V.
+template <int D>
+struct SharedLoads {
   typedef Tiles<D, 2> T;
-  typedef SharedLds<D> S;
-  typedef Elem<kHalf> E;
   typedef PageLoader<D, 2> L;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
-  const Queries qs = queries_of(a, w.begin, w.n);
-  const Span all_first = uniform_span(qs, w.len, query_of(qs, w.row0)), all_last = uniform_span(qs, w.len, query_of(qs, min(w.row0 + kRowsShared - 1, qs.rows - 1)));
-  TileList<64> list(qs, all_first, all_last, 0, 1);
-  w.share(list);
-  const int n = list.end - list.begin;
-  const Keys ks(a, w);
+  static constexpr int kPer = T::kBlocks / kWavesShared;
+  const Keys ks;
+  const TileList<64>& list;
+  const int wave, offset;
+  const uint32_t lds0;
   L ld;
-  ld.open(ks, lane);
-  // A wavefront brings kPer neighbouring blocks of a tile, which are of one sixteen.  Tile t + 1 of K goes with tile t of V.
-  constexpr int kPer = T::kBlocks / kWavesShared;
-  const int offset = 16 * (kPer * wave / L::kOf);
   Finder<64, 1, 1> finder;
   Sixteens<1> of_v, of_k, of_next;
-  auto load_k = [&](int pair) __attribute__((always_inline)) {
+  __device__ __forceinline__ SharedLoads(const PagesArgs& a, const Work& w, const TileList<64>& tiles, uint32_t lds_at, int wave_at, int lane)
+      : ks(a, w), list(tiles), wave(wave_at), offset(16 * (kPer * wave_at / L::kOf)), lds0(lds_at) {
+    ld.open(ks, lane);
+  }
+  __device__ __forceinline__ void open() {
+    finder.open(ks, list, list.begin, offset);
+    of_k = finder.next(ks, list, offset);
+    of_next = finder.next(ks, list, offset);
+  }
+  __device__ __forceinline__ void load_k(int pair) {
     u32x4 r[1];
     of_k.template rsrc<D>(ks, 0, r);
 #pragma unroll
@@ -578,32 +577,57 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
     of_v = of_k;
     of_k = of_next;
     of_next = finder.next(ks, list, offset);
-  };
-  auto load_pair = [&](int t) __attribute__((always_inline)) {
+  }
+  __device__ __forceinline__ void load_pair(int t) {
     u32x4 r[1];
     of_v.template rsrc<D>(ks, 1, r);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) ld.issue_v(r[0], kPer * wave + i, lds0 + pair_at<D>(t));
     load_k(t);
-  };
-  RowState<D, kHalf, 2> st;
+  }
+};
+
+template <int D, bool kHalf>
+__device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, uint8_t* lds) {
+  typedef Tiles<D, 2> T;
+  typedef SharedLds<D> S;
+  typedef Elem<kHalf> E;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+  const Queries qs = queries_of(a, w.begin, w.n);
+  const Span all_first = uniform_span(qs, w.len, query_of(qs, w.row0)), all_last = uniform_span(qs, w.len, query_of(qs, min(w.row0 + kRowsShared - 1, qs.rows - 1)));
+  TileList<64> list(qs, all_first, all_last, 0, 1);
+  w.share(list);
+  const int n = list.end - list.begin;
   const int row0 = w.row0 + 32 * wave;
+  if (__builtin_expect(row0 >= qs.rows, 0)) {      // (11 requests x 114 rows of 8 key heads of 128 over 8000 keys 158 -> 118 us: the others have the SIMDs, and the power)
+    if (n > 0) {
+      SharedLoads<D> loads(a, w, list, lds0, wave, lane);
+      loads.open();
+      loads.load_k(-1);
+      loads.load_pair(0);
+      loads.load_pair(1);
+      walk_idle<D>(n, wave, [&](int t) __attribute__((always_inline)) { loads.load_pair(t); });
+    }
+    return;
+  }
+  SharedLoads<D> loads(a, w, list, lds0, wave, lane);
+  const Keys& ks = loads.ks;
+  RowState<D, kHalf, 2> st;
   if (n > 0) {
-    finder.open(ks, list, list.begin, offset);
-    of_k = finder.next(ks, list, offset);
-    of_next = finder.next(ks, list, offset);
+    loads.open();
     const uint16_t* q = qs.q + (int64_t)w.hk * a.group * a.q_sh;
     queries_to_lds<D, true>(lds0, row0, wave, lane, [&](int r) __attribute__((always_inline)) {
       const int row = min(r, qs.rows - 1);
       const int s = query_of(qs, row), g = row - s * a.group;
       return q + s * a.q_ss + g * a.q_sh;
     });
-    load_k(-1);
-    load_pair(0);
-    load_pair(1);
+    loads.load_k(-1);
+    loads.load_pair(0);
+    loads.load_pair(1);
   }
   st.open(qs, 0, w.hk, row0, w.len, lane, false);
-  if (n > 0) walk_tiles<D, kHalf, true>(st, lds, list, all_first, all_last, n, wave, lane, load_pair);
+  if (n > 0) walk_tiles<D, kHalf, true>(st, lds, list, all_first, all_last, n, wave, lane, [&](int t) __attribute__((always_inline)) { loads.load_pair(t); });
   const int col = lane & 31, hh = lane >> 5;
   float m = st.m_ref * st.c, l = st.l_run + __shfl_xor(st.l_run, 32);
   float undefined = 0.f;
@@ -1045,9 +1069,15 @@ struct Scratch {
 template <int D, bool kHalf>
 int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratch, hipStream_t stream) {
   const int64_t rows = (int64_t)a.T * a.group, requests = std::min<int64_t>(a.B, a.T);
-  const bool mixed = std::min(most_rows, rows) > kFewRows;
-  const int64_t big = mixed ? rows / kRowsShared + std::min(requests, rows / (kFewRows + 1)) : 0;
-  const int64_t small = std::min(rows / kRowsFew + requests, mixed ? requests * (kFewRows / kRowsFew) : INT64_MAX);
+  // What is left over of tiles of 256 rows: as few rows up to 64 (heads of 128) or 96, else as a tile of 256 some of whose wavefronts have none.  Heads of 128,
+  // 16 requests x 80 rows of 8 key heads over 13 600 keys: with 96 270 us, with 64 174; 313 rows over 20 000 keys of 40 heads with 64 420, with 32 369, but over all
+  // sizes alike.  Heads of 64, 6 requests x 72 rows beside a prompt: with 96 1154, with 64 1541.  Little work goes by few rows alone up to 96: 63 requests x 96
+  // rows over 50 keys 9.5, with tiles of 256 13.8.
+  a.few_rows = D == 64 ? 96 : 64;
+  const int64_t as_few = a.Hk * (rows / kRowsFew + requests);
+  const bool mixed = std::min(most_rows, rows) > (as_few > n_cus ? a.few_rows : 96);
+  const int64_t big = mixed ? rows / kRowsShared + std::min(requests, rows / (a.few_rows + 1)) : 0;
+  const int64_t small = std::min(rows / kRowsFew + requests, mixed ? requests * (a.few_rows / kRowsFew) : INT64_MAX);
   const int64_t uncut = a.Hk * (big + small);
   // Few rows of few requests, which leave CUs without one, have eight wavefronts each: 40 items of 30 rows, heads of 64, over 20 000 keys 40 us, with four 47;
   // 144 items of a row, heads of 128, over 5000 keys 82, with four 69.
@@ -1062,7 +1092,6 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];      // (256 MB; 64 keys and values of a head are 256 D bytes)
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
-  const int64_t as_few = a.Hk * (rows / kRowsFew + requests);
   a.all_few = mixed && a.B <= 64 && as_few <= slots;
   // few rows first, whose parts are small
   int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;

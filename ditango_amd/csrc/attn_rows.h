@@ -519,6 +519,28 @@ __device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint
   wait_loads();     // those past the last tile, which store zeros: before the LDS is another workgroup's (and not behind the result's stores)
 }
 
+// A wavefront without rows among others that walk: its share of the loads, and everybody's barriers.
+template <int D, typename LoadPair>
+__device__ __forceinline__ void walk_idle(int n, int wave, LoadPair load_pair) {
+  typedef SharedLds<D> S;
+  const int group = wave >> 2;
+  wait_all_but<2 * S::kLoads>();
+  wait_lds_barrier();
+  wait_all_but<S::kLoads>();
+  if (group == 1) wait_lds_barrier();
+  wait_lds_barrier();
+  for (int t = 0; t < n - 1; ++t) {
+    load_pair(t + 2);
+    if (group == 1) wait_all_but<S::kLoads>();
+    wait_lds_barrier();
+    if (group == 0) wait_all_but<S::kLoads>();
+    wait_lds_barrier();
+  }
+  wait_lds_barrier();
+  if (group == 0) wait_lds_barrier();
+  wait_loads();
+}
+
 template <int D, int W>
 struct FewLds {
   static constexpr int kTile = 2 * Tiles<D, 1>::kBytes;
