@@ -22,6 +22,8 @@ from . import _hip
 from .producer import _NORMS, RotaryAxes
 from .window import _limit
 
+_INT32 = torch.int32
+
 
 class PagePlan(NamedTuple):
     lens: torch.Tensor          # int32 [B]: tokens of each request, the new ones among them where it is served
@@ -40,7 +42,7 @@ def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     order, the lowest first, and their entries go into ``tables``.  A request whose tokens do not fit its row gets none, and from the first one that finds too
     few free pages on, no request gets any: ``served`` says whose tokens have a place; the rows of the others stay without a slot, and their length as it was.  With ``in_place`` ``lens`` itself becomes the new lengths, for a
     captured step that is replayed."""
-    if lens.dtype is not torch.int32 or new_lens.dtype is not torch.int32 or tables.dtype is not torch.int32:
+    if lens.dtype is not _INT32 or new_lens.dtype is not _INT32 or tables.dtype is not _INT32:
         raise ValueError(f"tables, lens and new_lens must be int32, got {tables.dtype}, {lens.dtype}, {new_lens.dtype}")
     return PagePlan(*_hip.plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place))
 
@@ -60,7 +62,7 @@ def prepare_qkv_pages(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     ``append_pages`` of v, in one launch.  Returns q, contiguous; q of rows without a slot is computed as well."""
     if norm not in _NORMS:
         raise ValueError(f"unknown norm {norm!r}")
-    if positions.dtype is not torch.int32:
+    if positions.dtype is not _INT32:
         raise ValueError(f"positions must be int32, got {positions.dtype}")
     if positions.dim() != 2 or positions.size(-1) != len(axes.dims):
         raise ValueError(f"positions must be [T, {len(axes.dims)}] for these axes, got {tuple(positions.shape)}")
@@ -80,11 +82,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``window.window_attention`` (``right=0``: causal, by tokens or by whole frames).  Rows that see no key, and rows that belong to no request, get 0 and an
     lse of -inf.  ``max_seqlen_q`` is the most rows a request has, where the caller knows it: the launch is made for that; without it for ``T``.  An entry of
     ``tables`` that a window needs and that names no page stands for keys and values of zeros."""
-    for name, t in (("tables", tables), ("lens", lens), ("cu_seqlens", cu_seqlens)):
-        if t.dtype is not torch.int32:
-            raise ValueError(f"{name} must be int32, got {t.dtype}")
+    if tables.dtype is not _INT32 or lens.dtype is not _INT32 or cu_seqlens.dtype is not _INT32:
+        raise ValueError(f"tables, lens and cu_seqlens must be int32, got {tables.dtype}, {lens.dtype}, {cu_seqlens.dtype}")
     if frame < 1:
         raise ValueError(f"frame must be at least 1, got {frame}")
-    rows = -1 if max_seqlen_q is None else _limit("max_seqlen_q", max_seqlen_q)
-    return _hip.attn_pages_fwd(q, k_pages, v_pages, tables, lens, cu_seqlens, q.shape[0] if rows < 0 else rows, _limit("left", left),
+    rows = q.shape[0] if max_seqlen_q is None else _limit("max_seqlen_q", max_seqlen_q)
+    return _hip.attn_pages_fwd(q, k_pages, v_pages, tables, lens, cu_seqlens, rows, _limit("left", left),
                                _limit("right", right), _limit("frame", frame), _limit("sinks", sinks), softmax_scale, out, lse)
