@@ -115,3 +115,15 @@ def test_undefined_values_however_the_work_is_cut(hip, name, D):
     assert bool((got[0].isnan() == (out.isnan() | hurt)).all()) and bool((got[1].isnan() == hurt[..., 0].t()).all())
     # (the rows beside it stay within their bound, not the same bits: its tile is computed once more, from exact maxima)
     _check(torch.where(hurt, out, got[0]), torch.where(hurt[..., 0].t(), lse, got[1]), q, defined, vp, tables, lens, cu, **w)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [65, 97, 128, 129, 161, 225, 256, 257, 353])
+def test_tiles_that_are_not_full(hip, rows, D):
+    """Wavefronts of a tile of 256 rows that have none, beside others: with one part and with many, on short lists of tiles and on long ones."""
+    for B, len_, H, Hk, w in ((3, 9000, 2, 2, dict(right=0)), (40, 500, 8, 8, dict(right=0)), (5, 420, 20, 20, dict(left=30, right=0, sinks=7)), (66, rows, 4, 4, dict(right=0))):
+        lens, new = [len_ + b for b in range(B)], [rows] + [1] * (B - 2) + [rows]
+        q, kp, vp, tables, cu = _setup(lens, new, H, Hk, D, 32, torch.bfloat16, junk=float("inf"), seed=rows)
+        vp[tables[0][0], 3, 0, 0] = float("inf")
+        out, lse = _run(q, kp, vp, tables, lens, cu, rows, **w)
+        _check(out, lse, q, kp, vp, tables, lens, cu, **w)
