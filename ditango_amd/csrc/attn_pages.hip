@@ -28,6 +28,7 @@ constexpr int32_t kMostTokens = 1 << 29;   // positions, spans and lengths: thei
 constexpr int kXcds = 8;
 constexpr int kWavesFew = 4;
 constexpr int kMostWays = 64;              // parts of an item
+constexpr int kOneMeeting = 8;             // parts of 256 rows that meet all at once
 constexpr int kMostRequests = 2048;        // every workgroup reads all lengths
 
 struct PagesArgs {
@@ -51,6 +52,7 @@ struct PagesArgs {
   int32_t most_parts[2];        // for how many of them, of 256 rows (0) and of few (1), there is room for parts
   float slots;                  // workgroups at once
   float step[2], once[2], part[2];     // us: of 64 keys, of a workgroup beside them, of a part's way to memory and back
+  float join;                   // ... of one of 256 rows that one CU adds to others
   float least;                  // ... of a part of few rows
   float cached;                 // ... of as many keys of all key heads as the last cache holds
   float* part_out[2];           // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
@@ -221,7 +223,7 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     // (unlike items, cut to one length: half a part more each, at most a whole one)
     const float like = over(work[0], most), parts = whole > 0.f ? rest * ways : lane == 0 ? rest : like * ways + 0.5f * (rest - like), at_most = whole > 0.f ? parts : like * ways + rest;
     float cost = __builtin_ceilf(over(parts, a.slots) - 1e-4f) * (each * __builtin_amdgcn_rcpf(ways) + a.once[0]);
-    if (lane > 0) cost += 2.f + 0.4f * ways + parts * a.part[0];
+    if (lane > 0) cost += 2.f + a.join * (lane < kOneMeeting ? ways : 2.f * __builtin_amdgcn_sqrtf(ways)) + parts * a.part[0];
     if (lane > 0 && at_most > 0.99f * min((float)a.most_parts[0], (float)a.groups - whole * a.slots - items[1])) cost = INFINITY;
     const float best = wave_min(cost);
     const uint64_t these = __ballot(cost == best);
@@ -638,15 +640,20 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
   bool hurt = __builtin_expect(__any(undefined != 0.f && l == l), 0) && masked_not_finite<D, kHalf>(ks, st, list, lane);
   const bool live = row0 + col < qs.rows;
   if (w.ways > 1) {
-    // A part's sums, fp32; the wavefront that completes the parts of its rows adds them all up, in order.
+    // A part's sums, fp32; the wavefront that completes the parts of its rows adds them up, in order: of more than eight, neighbours in groups first, and what
+    // the groups come to then, so that several CUs read them (one reads 100 KB a us): 617 rows of 2 key heads of 128 over 38 000 keys, 39 parts, 97 -> 61 us.  A
+    // group's counter is its first part's, that of the groups part 1's.
     constexpr int kPartFloats = 32 * D;
-    const int mine = w.first + w.part * w.apart;
-    float* part = a.part_out[0] + ((int64_t)mine * kWavesShared + wave) * kPartFloats;
-    if (hurt) {
-      rows_one_by_one<D, kHalf>(a, w, qs, ks, row0, m, 0.f, list.begin < list.end ? list.key(list.begin) : 0,
-                                list.begin < list.end ? list.key(list.end - 1) + T::kKeys : 0, part, lane);
-    } else {
-      const Rsrc to = buffer_of(part, kPartFloats * 4);
+    auto part_of = [&](int at) __attribute__((always_inline)) { return (int64_t)(w.first + at * w.apart) * kWavesShared + wave; };
+    auto store_sums = [&](int64_t at) __attribute__((always_inline)) {
+      float* ml = a.part_ml[0] + (at * 32 + col) * 2;
+      if (hh == 0) {
+        store_device(ml, m);
+        store_device(ml + 1, l);
+      }
+    };
+    auto store_part = [&](int64_t at) __attribute__((always_inline)) {
+      const Rsrc to = buffer_of(a.part_out[0] + at * kPartFloats, kPartFloats * 4);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -656,44 +663,56 @@ __device__ __forceinline__ void shared_tiles(const PagesArgs& a, const Work& w, 
           for (int e = 0; e < 4; ++e) x[e] = __builtin_bit_cast(uint32_t, (float)st.o[i][4 * g + e]);
           __builtin_amdgcn_raw_buffer_store_b128(x, to, (4 * i + g) * 1024 + lane * 16, 0, kDevice);
         }
-    }
-    float* ml = a.part_ml[0] + (((int64_t)mine * kWavesShared + wave) * 32 + col) * 2;
-    if (hh == 0) {
-      store_device(ml, m);
-      store_device(ml + 1, l);
-    }
-    wait_loads();                // (stores as well)
-    int done = 0;
-    if (lane == 0) {
-      uint32_t* counter = a.counters[0] + (int64_t)w.first * kWavesShared + wave;
-      done = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == w.ways;
-      if (done) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (!__builtin_amdgcn_readfirstlane(done)) return;
-    asm volatile("" ::: "memory");
-    const float* mls = a.part_ml[0] + (((int64_t)w.first * kWavesShared + wave) * 32 + col) * 2;
-    const int64_t ml_apart = (int64_t)w.apart * kWavesShared * 64;
-    float top = -INFINITY;
-    for (int p = 0; p < w.ways; ++p) top = fmaxf(top, load_device(mls + p * ml_apart));
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) st.o[i][r] = 0.f;
-    l = 0.f;
+    };
+    const int64_t mine = part_of(w.part);
+    if (hurt)
+      rows_one_by_one<D, kHalf>(a, w, qs, ks, row0, m, 0.f, list.begin < list.end ? list.key(list.begin) : 0,
+                                list.begin < list.end ? list.key(list.end - 1) + T::kKeys : 0, a.part_out[0] + mine * kPartFloats, lane);
+    else store_part(mine);
+    store_sums(mine);
+    const int group = w.ways <= kOneMeeting ? w.ways : (int)__builtin_ceilf(__builtin_amdgcn_sqrtf((float)w.ways));
+    int lead = w.part / group * group, count = min(group, w.ways - lead), step = 1, counter_of = lead;
 #pragma unroll 1
-    for (int p = 0; p < w.ways; ++p) {
-      const float lp = load_device(mls + p * ml_apart + 1), wp = weight_of(load_device(mls + p * ml_apart), lp, top);
-      const Rsrc from = buffer_of(a.part_out[0] + ((int64_t)(w.first + p * w.apart) * kWavesShared + wave) * kPartFloats, kPartFloats * 4);
-      l = __builtin_fmaf(wp, lp, l);
-      f32x4 x[D / 8];
+    for (;;) {
+      wait_loads();                // (stores as well)
+      int done = 0;
+      if (lane == 0) {
+        uint32_t* counter = a.counters[0] + part_of(counter_of);
+        done = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == count;
+        if (done) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (!__builtin_amdgcn_readfirstlane(done)) return;
+      asm volatile("" ::: "memory");
+      const int64_t first = part_of(lead), apart = (int64_t)step * w.apart * kWavesShared;
+      const float* mls = a.part_ml[0] + (first * 32 + col) * 2;
+      m = -INFINITY;
+      for (int p = 0; p < count; ++p) m = fmaxf(m, load_device(mls + p * apart * 64));
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, i * 1024 + lane * 16, 0, kDevice));
+      for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
+        for (int r = 0; r < 16; ++r) st.o[i][r] = 0.f;
+      l = 0.f;
+#pragma unroll 1
+      for (int p = 0; p < count; ++p) {
+        const float lp = load_device(mls + p * apart * 64 + 1), wp = weight_of(load_device(mls + p * apart * 64), lp, m);
+        const Rsrc from = buffer_of(a.part_out[0] + (first + p * apart) * kPartFloats, kPartFloats * 4);
+        l = __builtin_fmaf(wp, lp, l);
+        f32x4 x[D / 8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[i / 4][4 * (i % 4) + e] = __builtin_fmaf(wp, x[i][e], st.o[i / 4][4 * (i % 4) + e]);
+        for (int i = 0; i < D / 8; ++i) x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, i * 1024 + lane * 16, 0, kDevice));
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) st.o[i / 4][4 * (i % 4) + e] = __builtin_fmaf(wp, x[i][e], st.o[i / 4][4 * (i % 4) + e]);
+      }
+      if (step > 1 || group == w.ways) break;
+      store_part(first);
+      store_sums(first);
+      lead = 0;
+      step = group;
+      count = (w.ways + group - 1) / group;
+      counter_of = 1;
     }
-    m = top;
     hurt = false;
   }
   const float inv = l != 0.f ? 1.f / l : 0.f;      // (an undefined sum stays one)
@@ -1092,6 +1111,7 @@ int launch_dim(PagesArgs& a, int64_t most_rows, int n_cus, const Scratch& scratc
   a.cached = 268435456.f / (256 * D) / a.Hk * a.step[1];      // (256 MB; 64 keys and values of a head are 256 D bytes)
   constexpr int64_t kBytes[2] = {(int64_t)kRowsShared * (D + 2) * 4, (int64_t)kRowsFew * (D + 2) * 4};
   for (int i = 0; i < 2; ++i) a.part[i] = (float)(2.0 * kBytes[i] / 6.7e6);
+  a.join = (float)(kBytes[0] / 1e5);
   a.all_few = mixed && a.B <= 64 && as_few <= slots;
   // few rows first, whose parts are small
   int64_t bytes = scratch.workspace && scratch.counters ? scratch.bytes : 0, counters = scratch.counters ? scratch.n_counters : 0;

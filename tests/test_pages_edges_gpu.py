@@ -127,3 +127,22 @@ def test_tiles_that_are_not_full(hip, rows, D):
         vp[tables[0][0], 3, 0, 0] = float("inf")
         out, lse = _run(q, kp, vp, tables, lens, cu, rows, **w)
         _check(out, lse, q, kp, vp, tables, lens, cu, **w)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("len_, rows, H, Hk", [(38000, 617, 2, 2), (20000, 255, 1, 1), (9000, 140, 6, 3), (60000, 300, 4, 1)])
+def test_many_parts_meet(hip, len_, rows, H, Hk, D):
+    """Tiles of 256 rows whose keys are cut into many parts, which meet in groups: within their bound, the same bits each time, counters left at zero."""
+    q, kp, vp, tables, cu = _setup([len_, 300], [rows, 1], H, Hk, D, 64, torch.bfloat16, junk=float("inf"), seed=rows)
+    out, lse = _run(q, kp, vp, tables, [len_, 300], cu, rows, right=0)
+    _check(out, lse, q, kp, vp, tables, [len_, 300], cu, right=0)
+    for _ in range(5):
+        again = _run(q, kp, vp, tables, [len_, 300], cu, rows, right=0)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    for counters in hip._counters.values():
+        assert not bool(counters.any())
+    vp[tables[0][0], 5, 0, 1] = -float("inf")
+    j = len_ - rows // 2
+    vp[tables[0][j // 64], j % 64, Hk - 1, D - 3] = float("inf")
+    out, lse = _run(q, kp, vp, tables, [len_, 300], cu, rows, right=0)
+    _check(out, lse, q, kp, vp, tables, [len_, 300], cu, right=0)
