@@ -7,7 +7,8 @@
 // included (4 million fractions all round the turn), where the row's 16 bits are off by 2^-9 to 2^-12 of a value.
 //
 // HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
-// runs of 4 half a section apart with rotate-half.  It has their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of
+// runs of 4 half a section apart with rotate-half, which two lanes load and store as 16 bytes each and exchange (4 x 1802 tokens of 3 x 48 heads of 128 111 -> 95
+// us; with 8 bytes a run where a section is no multiple of 16).  It has their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of
 // 128 with an RMS norm: 64.4 us, 5.7 TB/s (two launches of the kernel with tables: 68.2, and the tables' making).
 #include <initializer_list>
 #include <type_traits>
@@ -39,7 +40,8 @@ struct RotaryArgs {
   Rows rows[2];
   const int32_t* pos;
   int64_t pos_sb;
-  int32_t S, n_axes, norm, w16, halves;
+  int32_t S, n_axes, norm, w16;
+  int32_t wide;                   // halves: sections are multiples of 16, so that runs come in neighbouring pairs and 16 bytes a lane go
   float eps;
   uint32_t items;                 // B * S * groups of both
   Quotient by_groups, by_s;
@@ -65,7 +67,7 @@ __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d,
 
 // A launch whose keys go into the pages of a cache, and values beside them: rows[0] are q, rows[1] k.  Tokens are packed, B = 1.  A lane group finds its
 // token's slot with its rows under way.  Values are only copied, by workgroups of their own behind the others, 16 bytes a lane: 4 x 1802 tokens of 48 heads of
-// 128, 532 MB, 108 us, 4.9 TB/s (by the lanes that rotate the keys 129).
+// 128, 532 MB, 95 us, 5.6 TB/s (by the lanes that rotate the keys, when it took 109: 129).
 constexpr int kCopies = 4;       // of a lane
 struct PagedArgs : RotaryArgs {
   Pages to;
@@ -94,6 +96,15 @@ __device__ __forceinline__ void copy_values(const PagedArgs& a) {
     if (a.to.has(slot[i])) __builtin_nontemporal_store(x[i], reinterpret_cast<u32x4*>(a.to.row(1, slot[i]) + head[i] * a.to.sh[1] + d[i]));
 }
 
+// Of two neighbouring lanes' runs of 4 (x, y: in the first half of a section, z, w: in its second), or of chunks of 8 (of the first half in even lanes, of the
+// second in odd ones), the others.
+__device__ __forceinline__ u32x4 swapped(const u32x4& r, bool odd) {
+  uint32_t x = odd ? r.x : r.z, y = odd ? r.y : r.w;
+  x = __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false);      // lane ^ 1
+  y = __builtin_amdgcn_update_dpp(0, y, 0xb1, 0xf, 0xf, false);
+  return odd ? u32x4{x, y, r.z, r.w} : u32x4{r.x, r.y, x, y};
+}
+
 // kRms: with an RMS norm, which does without the 20 registers of means and biases (14 882 x 48 heads of 128 66.6 -> 64.4 us; a form of its own for rows
 // without a norm, with as few, is 3 % slower than the common one).
 template <int D, bool kHalf, bool kHalves, int kHeads, bool kRms, typename Args>
@@ -111,6 +122,8 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
   const uint32_t b = quotient(bs, a.by_s), s = bs - b * (uint32_t)a.S;
   const int h0 = hg * kHeads, nh = min(t.H - h0, kHeads);
   const int ea = kHalves ? a.a0[c] : 8 * c, eb = kHalves ? a.b0[c] : 8 * c + 4;
+  const bool odd = c & 1;
+  const int chunk = odd ? eb - 4 : ea;      // that a lane loads and stores where runs come in neighbouring pairs
 
   const uint16_t* xp = t.x + (int64_t)b * t.sb + (int64_t)s * t.ss + (int64_t)h0 * t.sh;
   u32x4 raw[kHeads];
@@ -120,9 +133,13 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
     if (r < nh) {
       const uint16_t* p = xp + (int64_t)r * t.sh;
       if constexpr (kHalves) {
-        const u32x2 lo = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + ea));
-        const u32x2 hi = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + eb));
-        raw[r] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        if (a.wide) {
+          raw[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + chunk));
+        } else {
+          const u32x2 lo = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + ea));
+          const u32x2 hi = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p + eb));
+          raw[r] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
       } else {
         raw[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + ea));
       }
@@ -168,6 +185,10 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
     load_weights4<kHalf>(t.bias, a.w16 != 0, ea, bias);
     load_weights4<kHalf>(t.bias, a.w16 != 0, eb, bias + 4);
   }
+  if (kHalves && a.wide) {
+#pragma unroll
+    for (int r = 0; r < kHeads; ++r) raw[r] = swapped(raw[r], odd);
+  }
   float mean[kHeads] = {}, rs[kHeads] = {}, ss[kHeads];
   if (kRms || a.norm != DT_NORM_NONE) {   // uniform
 #pragma unroll
@@ -208,7 +229,9 @@ __device__ __forceinline__ void rotate_rows(const Args& a) {
     }
     const u32x4 o = u32x4{pack2<kHalf>(y[0], y[1]), pack2<kHalf>(y[2], y[3]), pack2<kHalf>(y[4], y[5]), pack2<kHalf>(y[6], y[7])};
     uint16_t* q = yp + r * y_sh;
-    if constexpr (kHalves) {
+    if (kHalves && a.wide) {
+      __builtin_nontemporal_store(swapped(o, odd), reinterpret_cast<u32x4*>(q + chunk));
+    } else if (kHalves) {
       __builtin_nontemporal_store(u32x2{o.x, o.y}, reinterpret_cast<u32x2*>(q + ea));
       __builtin_nontemporal_store(u32x2{o.z, o.w}, reinterpret_cast<u32x2*>(q + eb));
     } else {
@@ -263,11 +286,13 @@ int fill_rotary(RotaryArgs& a, const dt_rotary_rows* rows, int32_t n_rows, int32
       return DT_ERR_INVALID;
     }
     int lo = 0, lane = 0;
+    a.wide = 1;
     for (int i = 0; i < n_sections; ++i) {
       if (sections[i] <= 0 || (sections[i] & 7) || sections[i] > D - lo) {
         set_error("section %d has %d elements: need positive multiples of 8 that sum to %d", i, sections[i], D);
         return DT_ERR_INVALID;
       }
+      if (sections[i] & 15) a.wide = 0;
       for (int e = 0; e < sections[i] / 2; e += 4, ++lane) {
         a.a0[lane] = (uint8_t)(lo + e);
         a.b0[lane] = (uint8_t)(lo + sections[i] / 2 + e);
