@@ -221,7 +221,8 @@ __device__ __forceinline__ bool find(const PagesArgs& a, Work& w, bool* none) {
     const float ways = (float)(lane + 1), whole = __builtin_floorf(over(items[0], a.slots) + 1e-4f), rest = items[0] - whole * a.slots;
     const float each = whole > 0.f ? over(work[0], items[0]) : most;
     // (unlike items, cut to one length: half a part more each, at most a whole one)
-    const float like = over(work[0], most), parts = whole > 0.f ? rest * ways : lane == 0 ? rest : like * ways + 0.5f * (rest - like), at_most = whole > 0.f ? parts : like * ways + rest;
+    const float like = over(work[0], most), parts = whole > 0.f ? rest * ways : lane == 0 ? rest : like * ways + 0.5f * (rest - like);
+    const float at_most = whole > 0.f ? parts : like * ways + rest;
     float cost = __builtin_ceilf(over(parts, a.slots) - 1e-4f) * (each * __builtin_amdgcn_rcpf(ways) + a.once[0]);
     if (lane > 0) cost += 2.f + a.join * (lane < kOneMeeting ? ways : 2.f * __builtin_amdgcn_sqrtf(ways)) + parts * a.part[0];
     if (lane > 0 && at_most > 0.99f * min((float)a.most_parts[0], (float)a.groups - whole * a.slots - items[1])) cost = INFINITY;

@@ -40,8 +40,8 @@ def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     A request holds the first ``ceil(len / page_size)`` entries of its row of ``tables``; what stands behind them means nothing.  Pages that no request
     holds are free: a request ends by its length going to 0, and requests may share the whole pages of a common beginning.  Requests take free pages in
     order, the lowest first, and their entries go into ``tables``.  A request whose tokens do not fit its row gets none, and from the first one that finds too
-    few free pages on, no request gets any: ``served`` says whose tokens have a place; the rows of the others stay without a slot, and their length as it was.  With ``in_place`` ``lens`` itself becomes the new lengths, for a
-    captured step that is replayed."""
+    few free pages on, no request gets any: ``served`` says whose tokens have a place; the rows of the others stay without a slot, and their length as it
+    was.  With ``in_place`` ``lens`` itself becomes the new lengths, for a captured step that is replayed."""
     if lens.dtype is not _INT32 or new_lens.dtype is not _INT32 or tables.dtype is not _INT32:
         raise ValueError(f"tables, lens and new_lens must be int32, got {tables.dtype}, {lens.dtype}, {new_lens.dtype}")
     return PagePlan(*_hip.plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place))
