@@ -39,18 +39,21 @@ struct PlanArgs {
 
 __device__ __forceinline__ int held_pages(const PlanArgs& a, int tokens) { return (int)quotient(tokens + a.page - 1, a.by_page); }
 
-// Sums along the threads that stop at `most`, and are still sums then: of x, 0 .. 2^30, over the threads in front of this one; *total over all.
+// Sums along the threads that stop at `most`, and are still sums then: of x, 0 .. 2^30, over the lanes up to this one, or over the threads in front of it;
+// *total over all.
 template <int kCtrl, int kRows>
 __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
-__device__ __forceinline__ int block_scan(int x, int most, int* waves, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int sum = x;      // rows of 16 lanes, then across them
+__device__ __forceinline__ int wave_scan(int sum, int most) {      // rows of 16 lanes, then across them
   sum = min(sum + moved<0x111, 0xf>(sum), most);
   sum = min(sum + moved<0x112, 0xf>(sum), most);
   sum = min(sum + moved<0x114, 0xf>(sum), most);
   sum = min(sum + moved<0x118, 0xf>(sum), most);
   sum = min(sum + moved<0x142, 0xa>(sum), most);
-  sum = min(sum + moved<0x143, 0xc>(sum), most);
+  return min(sum + moved<0x143, 0xc>(sum), most);
+}
+__device__ __forceinline__ int block_scan(int x, int most, int* waves, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sum = wave_scan(x, most);
   if (lane == 63) waves[wave] = sum;
   const int mine = __shfl_up(sum, 1);
   __syncthreads();
@@ -95,18 +98,25 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs
   int32_t* len = start + a.B;                                     // [B], its complement where the request is not served
   const int tid = threadIdx.x, most_len = a.width * a.page;
   int tokens = 0, pages = 0;
+  const bool one_wave = a.B <= 64;        // then every wavefront sums by itself, and none waits for another
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
+    const int b = one_wave ? tid & 63 : b0 + tid;
     const bool there = b < a.B;
     const int l = there ? min(max(a.lens[b], 0), most_len) : 0, asked = there ? min(max(a.new_lens[b], 0), a.n_tokens) : 0;
     if (b0 == 0)
       for (int i = tid; i < a.words; i += kPlanThreads) taken[i] = 0;
     int total;
-    const int from = min(tokens + block_scan(asked, a.n_tokens, waves, &total), a.n_tokens), n = min(asked, a.n_tokens - from);
+    auto in_front = [&](int x, int most) __attribute__((always_inline)) {
+      if (!one_wave) return block_scan(x, most, waves, &total);
+      const int sum = wave_scan(x, most);
+      total = __builtin_amdgcn_readlane(sum, 63);
+      return moved<0x138, 0xf>(sum);      // of the lane in front
+    };
+    const int from = min(tokens + in_front(asked, a.n_tokens), a.n_tokens), n = min(asked, a.n_tokens - from);
     tokens = min(tokens + total, a.n_tokens);
     const bool fits = n <= most_len - l;
-    const int before_me = block_scan(there && fits ? min(held_pages(a, l + n) - held_pages(a, l), kMostPages + 1) : 0, kMostPages + 1, waves, &total);
-    if (there) {
+    const int before_me = in_front(there && fits ? min(held_pages(a, l + n) - held_pages(a, l), kMostPages + 1) : 0, kMostPages + 1);
+    if (there && (tid < 64 || !one_wave)) {
       cu[b] = from;
       len[b] = fits ? l : ~l;
       start[b] = min(pages + before_me, kMostPages + 1);
@@ -160,22 +170,34 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs
 #pragma unroll
   for (int i = 0; i < kPlanWaves; ++i) granted = max(granted, waves[i]);
   // the r-th free page, for every r that is given away
+  const bool kept = granted <= kPlanThreads;      // then `before` keeps them for the slots
+  int page = 0, entry_of = 0, entry = 0;
   for (int r = tid; r < granted; r += kPlanThreads) {
     const int t = last_at_most(before, kPlanThreads, r);
     int k = r - before[t], w = t * each;
     for (; k >= __popc(~taken[w]); ++w) k -= __popc(~taken[w]);
     uint32_t bits = ~taken[w];
     for (; k > 0; --k) bits &= bits - 1;
-    const int b = last_at_most(start, a.B, r);
-    a.tables[b * a.table_stride + held_pages(a, len[b]) + r - start[b]] = 32 * w + __ffs(bits) - 1;
+    entry_of = last_at_most(start, a.B, r);
+    entry = held_pages(a, len[entry_of]) + r - start[entry_of];
+    page = 32 * w + __ffs(bits) - 1;
+    if (!kept || !slots_too) a.tables[entry_of * a.table_stride + entry] = page;
   }
   if (!slots_too) return;
   __syncthreads();
+  if (kept) {
+    if (tid < granted) before[tid] = page;
+    __syncthreads();
+    if (tid < granted) a.tables[entry_of * a.table_stride + entry] = page;
+  }
   for (int t = tid; t < a.n_tokens; t += kPlanThreads) {
     int64_t slot = -1;
     if (t < cu[a.B]) {
       const int b = last_at_most(cu, a.B, t);
-      if (len[b] >= 0) slot = slot_of(a, b, len[b] + t - cu[b]);
+      if (len[b] >= 0) {
+        const int j = len[b] + t - cu[b], held = held_pages(a, len[b]), i = (int)quotient(j, a.by_page);
+        slot = kept && i >= held ? (int64_t)before[start[b] + i - held] * a.page + (j - i * a.page) : slot_of(a, b, j);
+      }
     }
     a.slots[t] = slot;
   }
