@@ -69,13 +69,17 @@ __device__ __forceinline__ int block_scan(int x, int most, int* waves, int* tota
   return min(before + (lane > 0 ? mine : 0), most);
 }
 
-// The last of the n values of x, which never fall, that is at most v (x[0] is).
+// The last of the n values of x, which never fall, that is at most v (x[0] is): a quarter of them each time, as three reads under way together take no longer
+// than one.
 __device__ __forceinline__ int last_at_most(const int32_t* x, int n, int v) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (x[mid] <= v) lo = mid;
-    else hi = mid;
+  int lo = 0;
+  while (n > 1) {
+    const int quarter = (n + 3) >> 2, last = lo + n - 1;
+    const int p = min(lo + quarter, last), q = min(lo + 2 * quarter, last), r = min(lo + 3 * quarter, last);
+    const int u = x[p], w = x[q], y = x[r];
+    const int from = y <= v ? r : w <= v ? q : u <= v ? p : lo;
+    n = min(quarter, last + 1 - from);
+    lo = from;
   }
   return lo;
 }
@@ -125,18 +129,24 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs
   }
   if (tid == 0) cu[a.B] = tokens;
   __syncthreads();
-  // the pages that somebody holds; a.lanes threads a request, 16 entries of each under way together
-  constexpr int kSome = 16;
+  // the pages that somebody holds; a.lanes threads a request, up to 32 entries of each under way together
+  constexpr int kSome = 8, kTimes = 4;
   for (int b = tid / a.lanes; b < a.B; b += kPlanThreads / a.lanes) {
     const int l = len[b], n = held_pages(a, l < 0 ? ~l : l);
     const int32_t* row = a.tables + b * a.table_stride;
-    for (int i = tid % a.lanes; i < n; i += kSome * a.lanes) {
-      int p[kSome];
+    for (int i = tid % a.lanes; i < n; i += kTimes * kSome * a.lanes) {
+      int p[kTimes][kSome];
 #pragma unroll
-      for (int j = 0; j < kSome; ++j) p[j] = row[min(i + j * a.lanes, n - 1)];
+      for (int k = 0; k < kTimes; ++k)
+        if (i + k * kSome * a.lanes < n)
 #pragma unroll
-      for (int j = 0; j < kSome; ++j)
-        if (i + j * a.lanes < n && (uint32_t)p[j] < (uint32_t)a.n_pages) atomicOr(&taken[p[j] >> 5], 1u << (p[j] & 31));
+          for (int j = 0; j < kSome; ++j) p[k][j] = row[min(i + (k * kSome + j) * a.lanes, n - 1)];
+#pragma unroll
+      for (int k = 0; k < kTimes; ++k)
+        if (i + k * kSome * a.lanes < n)
+#pragma unroll
+          for (int j = 0; j < kSome; ++j)
+            if (i + (k * kSome + j) * a.lanes < n && (uint32_t)p[k][j] < (uint32_t)a.n_pages) atomicOr(&taken[p[k][j] >> 5], 1u << (p[k][j] & 31));
     }
   }
   // behind the last page there is none
