@@ -90,8 +90,9 @@ __device__ __forceinline__ int64_t slot_of(const PlanArgs& a, int b, int j) {
   return (uint32_t)p < (uint32_t)a.n_pages ? (int64_t)p * a.page + (j - i * a.page) : -1;
 }
 
-// One workgroup: the free pages are in its LDS, a bit a page.  Latency all the way: 8 requests' next tokens 6.5 us, of which an empty launch is 2.4; 64
-// requests that hold 29 300 pages and get 1250 12.8 (their 86 400 slots, by a launch behind it, 4.0).
+// One workgroup: the free pages are in its LDS, a bit a page.  Latency all the way: 8 requests' next tokens 5.7 us, of which an empty launch is 2.4, lengths and
+// their sums 1.2, the tables' entries 1.6; 64 requests that hold 29 300 pages and get 1250 11.8, of which the entries are 4.5 and what is given away 2.5 (their
+// 86 400 slots, by a launch behind it, 4.0).
 __global__ __launch_bounds__(kPlanThreads) void plan_pages_kernel(const PlanArgs a, int slots_too) {
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ int32_t waves[kPlanWaves];
