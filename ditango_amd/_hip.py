@@ -130,6 +130,8 @@ _SIGNATURES = {
                                         _P(c_i32), c_i32, c_i32, c_vp, c_vp, c_vp]),
     "dt_attn_pages_fwd": (ctypes.c_int, [c_vp, _P(c_i64), c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32,
                                          c_vp, c_f32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "dt_attn_pages_served_fwd": (ctypes.c_int, [c_vp, _P(c_i64), c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp,
+                                                c_i32, c_vp, c_f32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -651,13 +653,13 @@ def prepare_pages(tensors, v: torch.Tensor, positions: torch.Tensor, table, norm
 
 def attn_pages_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, cu_seqlens: torch.Tensor,
                    max_seqlen_q: int, left: int, right: int, frame: int, sinks: int, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
-                   lse: Optional[torch.Tensor] = None):
-    """(out, lse) of ``dt_attn_pages_fwd``; -1 stands for a border that is not there."""
+                   lse: Optional[torch.Tensor] = None, served: Optional[torch.Tensor] = None):
+    """(out, lse) of ``dt_attn_pages_served_fwd``; -1 stands for a border that is not there."""
     stream = _stream_at(q, "q")
     workspace, counters = attn_scratch(q.device)
     if counters is None:
         counters = _stream_counters(q.device, 1)
     if counters is None:          # under capture: the graph's own, which every replay clears
         counters = torch.zeros(CAPTURED_COUNTERS, dtype=torch.int32, device=q.device)
-    return _host().attn_pages(q, k_pages, v_pages, tables, lens, cu_seqlens, max_seqlen_q, left, right, frame, sinks, float(softmax_scale), out, lse,
+    return _host().attn_pages(q, k_pages, v_pages, tables, lens, served, cu_seqlens, max_seqlen_q, left, right, frame, sinks, float(softmax_scale), out, lse,
                               workspace, counters, stream)

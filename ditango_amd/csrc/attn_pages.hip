@@ -58,6 +58,8 @@ struct PagesArgs {
   float* part_out[2];           // of slot s: sums of its rows, and (maximum in powers of two, sum) of each
   float* part_ml[2];
   uint32_t* counters[2];        // of an item's parts that are done, zero before and after the launch
+  const uint8_t* served;        // 0: a request without keys, whatever its length
+  int32_t all_served;           // ... but for launches without `served`, which read any bytes there: a branch around the load waits for it by itself
 };
 
 // The rows of a request, by the names of attn_rows.h
@@ -98,10 +100,10 @@ template <bool kMixed>
 __device__ __forceinline__ Request request_of(const PagesArgs& a, int b) {
   Request r = {};
   if (b >= a.B) return r;
-  const int from = a.cu[b], to = a.cu[b + 1], len = a.lens[b];
+  const int from = a.cu[b], to = a.cu[b + 1], len = a.lens[b], served = a.served[b] | a.all_served;
   r.begin = min(max(from, 0), a.T);
   r.n = max(min(max(to, 0), a.T) - r.begin, 0);
-  r.len = min(max(len, 0), a.most_len);
+  r.len = served ? min(max(len, 0), a.most_len) : 0;
   const int rows = r.n * a.group;
   int whole = 0;
   if (kMixed) {
@@ -1151,10 +1153,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 using namespace dt;
 
-extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
-                                 const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
-                                 const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale, int32_t flags,
-                                 void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream) {
+extern "C" int dt_attn_pages_served_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
+                                        const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
+                                        const uint8_t* served, const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale,
+                                        int32_t flags, void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream) {
   if (T <= 0 || B <= 0 || H <= 0 || Hk <= 0 || H % Hk) {
     set_error("T, B, H, Hk must be positive and H a multiple of Hk (got %d, %d, %d, %d)", T, B, H, Hk);
     return DT_ERR_INVALID;
@@ -1210,6 +1212,8 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
   a.tables = tables;
   a.table_stride = table_stride;
   a.lens = lens;
+  a.served = served ? served : reinterpret_cast<const uint8_t*>(lens);
+  a.all_served = !served;
   a.cu = cu_seqlens;
   a.width = width;
   a.most_len = width * pages->page_size;
@@ -1237,4 +1241,12 @@ extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* 
   const int64_t most_rows = (int64_t)std::max(max_seqlen_q, 0) * a.group;
   if (D == 128) return half ? launch_dim<128, true>(a, most_rows, n_cus, scratch, st) : launch_dim<128, false>(a, most_rows, n_cus, scratch, st);
   return half ? launch_dim<64, true>(a, most_rows, n_cus, scratch, st) : launch_dim<64, false>(a, most_rows, n_cus, scratch, st);
+}
+
+extern "C" int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
+                                 const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
+                                 const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale, int32_t flags,
+                                 void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream) {
+  return dt_attn_pages_served_fwd(q, q_strides, out, lse, T, H, Hk, D, pages, tables, table_stride, width, B, lens, nullptr, cu_seqlens, max_seqlen_q, window,
+                                  softmax_scale, flags, workspace, workspace_bytes, counters, n_counters, stream);
 }

@@ -1101,7 +1101,7 @@ Tensor prepare_pages(const std::vector<RotaryRows>& tensors, const Tensor& v, co
 
 // ditango_amd._hip.attn_pages_fwd
 std::pair<Tensor, Tensor> attn_pages(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& lens,
-                                     const Tensor& cu_seqlens, int64_t max_seqlen_q, int32_t left, int32_t right, int32_t frame, int32_t sinks, double scale,
+                                     const std::optional<Tensor>& served, const Tensor& cu_seqlens, int64_t max_seqlen_q, int32_t left, int32_t right, int32_t frame, int32_t sinks, double scale,
                                      std::optional<Tensor> out, std::optional<Tensor> lse, const std::optional<Tensor>& workspace,
                                      const std::optional<Tensor>& counters, uint64_t stream) {
   const Packed d = check_thd(q, {"q"});
@@ -1113,6 +1113,8 @@ std::pair<Tensor, Tensor> attn_pages(const Tensor& q, const Tensor& k_pages, con
   REQUIRE(same_device(q, tables), "tables must be on the device of q");
   const int64_t B = tables.size(0);
   const int32_t *len = ints_of(lens, q, B, "lens"), *cu = ints_of(cu_seqlens, q, B + 1, "cu_seqlens");
+  REQUIRE(!served || (same_device(q, *served) && served->scalar_type() == at::kBool && served->is_contiguous() && shape_is(*served, {B})),
+          "served must be contiguous bool [requests] on the device of q");
   if (!out) out = empty({d.T, d.H, d.D}, q.options());
   if (!lse) lse = empty({d.H, d.T}, q.options().dtype(at::kFloat));
   REQUIRE(same_device(q, *out) && out->scalar_type() == q.scalar_type() && out->is_contiguous() && shape_is(*out, {d.T, d.H, d.D}),
@@ -1122,8 +1124,9 @@ std::pair<Tensor, Tensor> attn_pages(const Tensor& q, const Tensor& k_pages, con
   if (q.numel() == 0) return {*out, *lse};
   const int64_t qs[2] = {stride_of(q, 0), stride_of(q, 1)};
   const dt_window w = {left, right, frame, sinks, -1, nullptr};
-  CALL(dt_attn_pages_fwd, (const void*)ptr(q), qs, ptr(*out), static_cast<float*>(ptr(*lse)), (int32_t)d.T, (int32_t)d.H, (int32_t)Hk, (int32_t)d.D, &pages,
-       static_cast<const int32_t*>(ptr(tables)), row_stride(tables), (int32_t)tables.size(1), (int32_t)B, len, cu,
+  CALL(dt_attn_pages_served_fwd, (const void*)ptr(q), qs, ptr(*out), static_cast<float*>(ptr(*lse)), (int32_t)d.T, (int32_t)d.H, (int32_t)Hk, (int32_t)d.D, &pages,
+       static_cast<const int32_t*>(ptr(tables)), row_stride(tables), (int32_t)tables.size(1), (int32_t)B, len,
+       static_cast<const uint8_t*>(ptr(served)), cu,
        (int32_t)std::min<int64_t>(max_seqlen_q, INT32_MAX), &w, (float)scale, q.scalar_type() == at::kHalf ? DT_ATTN_FP16 : 0, ptr(workspace),
        bytes_of(workspace), static_cast<uint32_t*>(ptr(counters)), counters ? counters->numel() : 0, stream_of(stream));
   return {*out, *lse};

@@ -43,11 +43,11 @@ class Attention(nn.Module):
                         plan: PagePlan, causal: bool = False, **window) -> torch.Tensor:
         """q / k / v ``[T,H,D]``, the new tokens of all rollouts -> ``[T,H,D]``: k and v go into the pages where ``plan`` has a place for them, and q attends
         to its own rollout's, within the frames that ``window`` (the keyword arguments of ``paged_attention``) names; ``causal``: nothing behind the own
-        frame."""
+        frame.  Rows of a rollout that ``plan`` has no pages for are 0."""
         if causal and window.setdefault("right", 0) != 0:
             raise ValueError("a causal window has no frames behind the own one (right = 0)")
         append_pages(k, v, k_pages, v_pages, plan.slots)
-        return paged_attention(q, k_pages, v_pages, tables, plan.lens, plan.cu_seqlens, **window)[0]
+        return paged_attention(q, k_pages, v_pages, tables, plan.lens, plan.cu_seqlens, served=plan.served, **window)[0]
 
     def o_attn_func(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = False, **kwargs) -> torch.Tensor:
         """q / k / v ``[B,S,H,D]`` of this rank's shard -> ``[B,S,H,D]`` in q's dtype (:85-100).  The merge kernel

@@ -6,7 +6,7 @@ pages as it needs; ``tables[b]`` names request ``b``'s, in order, and ``lens[b]`
     plan = plan_pages(tables, lens, new_lens, q.shape[0], n_pages=k_pages.shape[0], page_size=k_pages.shape[1])      # once
     for each layer:
         q = prepare_qkv_pages(q, k, v, positions, axes, k_pages, v_pages, plan.slots, norm="rms", ...)               # or append_pages(k, v, ...)
-        out, lse = paged_attention(q, k_pages, v_pages, tables, plan.lens, plan.cu_seqlens, left=7, right=0, frame=1350, sinks=226)
+        out, lse = paged_attention(q, k_pages, v_pages, tables, plan.lens, plan.cu_seqlens, served=plan.served, left=7, right=0, frame=1350, sinks=226)
     lens = plan.lens
 
 The new tokens of all requests are packed, one request behind the other.  Nothing here reads device memory on the host, so a step can be captured in a
@@ -41,7 +41,7 @@ def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     holds are free: a request ends by its length going to 0, and requests may share the whole pages of a common beginning.  Requests take free pages in
     order, the lowest first, and their entries go into ``tables``.  A request whose tokens do not fit its row gets none, and from the first one that finds too
     few free pages on, no request gets any: ``served`` says whose tokens have a place; the rows of the others stay without a slot, and their length as it
-    was.  With ``in_place`` ``lens`` itself becomes the new lengths, for a captured step that is replayed."""
+    was, so that the attention behind it needs ``served`` as well.  With ``in_place`` ``lens`` itself becomes the new lengths, for a captured step that is replayed."""
     if lens.dtype is not _INT32 or new_lens.dtype is not _INT32 or tables.dtype is not _INT32:
         raise ValueError(f"tables, lens and new_lens must be int32, got {tables.dtype}, {lens.dtype}, {new_lens.dtype}")
     return PagePlan(*_hip.plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place))
@@ -71,7 +71,7 @@ def prepare_qkv_pages(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, cu_seqlens: torch.Tensor, *,
-                    max_seqlen_q: Optional[int] = None, left: Optional[int] = None, right: Optional[int] = None, frame: int = 1, sinks: int = 0,
+                    served: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None, left: Optional[int] = None, right: Optional[int] = None, frame: int = 1, sinks: int = 0,
                     softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
                     lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """q ``[T,H,D]`` (bf16 or fp16, D 64 or 128; H a multiple of the pages' key heads) holds the new tokens of request ``b`` in rows ``cu_seqlens[b] ..
@@ -80,12 +80,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Row ``i`` of a request's ``n`` stands at position ``lens[b] - n + i`` and sees the frames that ``left``, ``right``, ``frame`` and ``sinks`` name in
     ``window.window_attention`` (``right=0``: causal, by tokens or by whole frames).  Rows that see no key, and rows that belong to no request, get 0 and an
-    lse of -inf.  ``max_seqlen_q`` is the most rows a request has, where the caller knows it: the launch is made for that; without it for ``T``.  An entry of
+    lse of -inf; so do the rows of a request that ``served`` (bool ``[B]``, as ``plan_pages`` makes it) leaves out, whose keys are not in the pages.  Without
+    ``served`` every request's are.  ``max_seqlen_q`` is the most rows a request has, where the caller knows it: the launch is made for that; without it for ``T``.  An entry of
     ``tables`` that a window needs and that names no page stands for keys and values of zeros."""
     if tables.dtype is not _INT32 or lens.dtype is not _INT32 or cu_seqlens.dtype is not _INT32:
         raise ValueError(f"tables, lens and cu_seqlens must be int32, got {tables.dtype}, {lens.dtype}, {cu_seqlens.dtype}")
+    if served is not None and served.dtype is not torch.bool:
+        raise ValueError(f"served must be bool, got {served.dtype}")
     if frame < 1:
         raise ValueError(f"frame must be at least 1, got {frame}")
     rows = q.shape[0] if max_seqlen_q is None else _limit("max_seqlen_q", max_seqlen_q)
     return _hip.attn_pages_fwd(q, k_pages, v_pages, tables, lens, cu_seqlens, rows, _limit("left", left),
-                               _limit("right", right), _limit("frame", frame), _limit("sinks", sinks), softmax_scale, out, lse)
+                               _limit("right", right), _limit("frame", frame), _limit("sinks", sinks), softmax_scale, out, lse, served)

@@ -643,7 +643,7 @@ typedef struct {
  * tokens do not fit its row gets none, and from the first one that finds too few on, none gets any.  served[b] = 1 where request b has pages for
  * all of its tokens, and then tables (in place, new entries only) and lens_out[b] (its new length) say so; else served[b] = 0, lens_out[b] its old length.
  * slots[t], t < n_tokens: where the keys and values of row t go; -1 for rows of requests that are not served, rows behind the last one, and tokens whose
- * entry is no page.  lens_out may be lens.  At most 2048 requests, 2^20 pages, 2^29 tokens a request, 2^29 new ones.
+ * entry is no page.  cu_seqlens has the rows of requests that are not served as well: the attention behind it takes `served` (dt_attn_pages_served_fwd).  lens_out may be lens.  At most 2048 requests, 2^20 pages, 2^29 tokens a request, 2^29 new ones.
  * No counterpart in the reference.
  */
 int dt_plan_pages(int32_t* tables, int64_t table_stride, int32_t width, const int32_t* lens, const int32_t* new_lens, int32_t B,
@@ -676,11 +676,21 @@ int dt_prepare_pages(const dt_rotary_rows* rows, const void* v, const int64_t* v
  * adds nothing, whatever it and its value hold.  out may be q where that is contiguous.
  * max_seqlen_q: the most rows a request has, which the launch is made for; requests with more come out right, only later.
  * At most 2048 requests.  workspace and counters as for dt_attn_window_fwd; nothing is cut without either.  No counterpart in the reference.
+ * Rows of a request that dt_plan_pages has not served are taken for its last OLD tokens here, as its length is the old one.
  */
 int dt_attn_pages_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
                       const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
                       const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale, int32_t flags,
                       void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream);
+
+/*
+ * dt_attn_pages_fwd behind dt_plan_pages: a request b with served[b] = 0 (device uint8 [B], may be null) has no keys, and its rows get out = 0, lse = -inf.
+ * No counterpart in the reference.
+ */
+int dt_attn_pages_served_fwd(const void* q, const int64_t* q_strides, void* out, float* lse, int32_t T, int32_t H, int32_t Hk, int32_t D,
+                             const dt_pages* pages, const int32_t* tables, int64_t table_stride, int32_t width, int32_t B, const int32_t* lens,
+                             const uint8_t* served, const int32_t* cu_seqlens, int32_t max_seqlen_q, const dt_window* window, float softmax_scale,
+                             int32_t flags, void* workspace, int64_t workspace_bytes, uint32_t* counters, int64_t n_counters, void* stream);
 
 #ifdef __cplusplus
 }
