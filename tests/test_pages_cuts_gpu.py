@@ -1,9 +1,10 @@
 """How paged attention cuts the keys of its tiles of 256 rows, each way with cases that take it: parts of one length that meet in groups, a last round in parts behind one
-or two whole ones, more requests than a wavefront has lanes.
+or two whole ones, more requests than a wavefront has lanes; with room for all parts, for some and for none; captured, on several streams, from several threads.
 
 Which way a launch goes is seen from what it leaves in a workspace of the test's own: the slots of its parts.  ``_room`` knows where they lie, which the
 slots bear out (a part's sums and its maxima lie in different places and have to agree)."""
 import ctypes
+import threading
 
 import pytest
 import torch
@@ -128,3 +129,84 @@ def test_every_cut(hip, name, dtype):
     kp[tables[0][j // 64], j % 64, 0, 7] = float("nan")
     out, lse, big, few = launch(q, kp, vp, tables, lens, cu, max(new))
     _check(out, lse, q, kp, vp, tables, lens, cu, right=0)
+
+
+def _beside(seed, dtype=torch.bfloat16):
+    lens, new = [6000, 700, 5000, 44], [1000, 1, 3, 1]
+    return (*_setup(lens, new, 8, 8, 128, 64, dtype, seed=seed), lens, new)
+
+
+def test_room_for_some_parts(hip):
+    """32 items of 256 rows: without room for a part of each and one more they are not cut; with little they are cut less."""
+    q, kp, vp, tables, cu, lens, new = _beside(1)
+    whole = int(hip.load_library().dt_attn_workspace_bytes())
+    some = 504 * 32 * 130 * 4 + 110 * 256 * 130 * 4          # 504 slots of few rows, 110 of 256
+    for nbytes, words, parts in ((0, 0, 0), (whole, 0, 0), (0, WORDS, 0), (whole, 16, 0), (whole, 800, 0), (whole, 1400, 64), (some, WORDS, 64), (8 << 20, WORDS, 0),
+                                 (whole, WORDS, 256)):
+        launch = Launch(hip, nbytes, words)
+        out, lse, big, few = launch(q, kp, vp, tables, lens, cu, max(new))
+        assert len(big) == parts, (nbytes, words, len(big))
+        _check(out, lse, q, kp, vp, tables, lens, cu, right=0)
+
+
+def _attend(case, **w):
+    from ditango_amd.pages import paged_attention
+    q, kp, vp, tables, cu, lens, new = case
+    return paged_attention(q, kp, vp, tables, lens, cu, max_seqlen_q=1000, right=0, **w)
+
+
+def _three():
+    cases = [_beside(s, dtype) for s, dtype in ((2, torch.bfloat16), (3, torch.float16), (4, torch.bfloat16))]
+    on_gpu = [(q, kp, vp, _i32(tables), _i32(cu), _i32(lens), new) for q, kp, vp, tables, cu, lens, new in cases]
+    want = [_attend(c) for c in on_gpu]
+    torch.cuda.synchronize()
+    for (out, lse), (q, kp, vp, tables, cu, lens, new) in zip(want, cases):
+        _check(out, lse, q, kp, vp, tables, lens, cu, right=0)
+    return on_gpu, want
+
+
+def test_two_graphs_and_eager_launches(hip):
+    cases, want = _three()
+    assert len(Launch(hip)(*cases[0][:3], cases[0][3].tolist(), cases[0][5].tolist(), cases[0][4].tolist(), 1000)[2]) == 256      # tiles of 256 rows, in parts
+    graphs, outs = [], []
+    for c in cases[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_attend(c))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(5):
+        for t in outs[0] + outs[1]:
+            t.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs if turn % 2 else graphs[::-1], streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = _attend(cases[2])
+        torch.cuda.synchronize()
+        for got, ref in zip(outs + [eager], want):
+            assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+def test_threads_and_streams(hip):
+    cases, want = _three()
+    bad = []
+
+    def work(i, own_stream):
+        stream = torch.cuda.Stream() if own_stream else torch.cuda.default_stream()
+        with torch.cuda.stream(stream):
+            for _ in range(15):
+                out, lse = _attend(cases[i])
+                stream.synchronize()
+                if not (torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])):
+                    bad.append(i)
+
+    for own in (True, False):
+        threads = [threading.Thread(target=work, args=(i, own)) for i in range(3)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert not bad
+    torch.cuda.synchronize()
+    assert all(not bool(c.any()) for c in hip._counters.values())
