@@ -633,7 +633,9 @@ def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: f
 # A cache of pages that several requests share
 # ---------------------------------------------------------------------------------------------
 
-CAPTURED_COUNTERS = 1 << 14      # words: 16 384 workgroups of few rows, or 2048 of 256
+# Words: up to half of them for parts of few rows, one each, the others for parts of 256 rows, eight each.  The workspace has room for fewer of both, whatever the heads,
+# so that a captured launch is cut like an eager one, whose stream keeps more of them.
+CAPTURED_COUNTERS = 1 << 14
 
 
 def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor, n_tokens: int, n_pages: int, page_size: int, in_place: bool):
