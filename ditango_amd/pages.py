@@ -26,6 +26,8 @@ _INT32 = torch.int32
 
 
 class PagePlan(NamedTuple):
+    """What a step needs to know.  The results of a plan are parts of one allocation (``lens`` with ``in_place`` apart): whoever keeps ``lens`` for long keeps the 8 bytes
+    a row of ``slots`` with it, and ``torch.save``, which refuses tensors of different types in one storage, takes clones of them."""
     lens: torch.Tensor          # int32 [B]: tokens of each request, the new ones among them where it is served
     cu_seqlens: torch.Tensor    # int32 [B + 1]: rows of each request's new tokens
     slots: torch.Tensor         # int64 [n_tokens]: page * page_size + place of each row; -1: nowhere
