@@ -253,9 +253,8 @@ struct RowState {
     for (int i = 0; i < T::kBlocks; ++i) over |= ones(*reinterpret_cast<const u32x4*>(vt + i * 1024 + lane * 16));
     return __any((over & 0x80008000u) != 0);
   }
-  // The same ahead of the products: what the rows see of such values is added as it is, and the tile holds zeros for all of them.  (With products of its own
-  // the rare case made the compiler move all of O^T from registers to others and back in every turn.)
-  __device__ __forceinline__ void take_out_not_finite(uint8_t* vt, int k0, int lane) {
+  // What the rows see of such values, added as it is.
+  __device__ __forceinline__ void add_not_finite(const uint8_t* vt, int k0, int lane) {
     const int hh = lane >> 5;
 #pragma unroll 1
     for (int key = 0; key < T::kKeys; ++key) {
@@ -274,6 +273,11 @@ struct RowState {
           }
         }
     }
+  }
+  // The same ahead of the products: what the rows see of such values is added as it is, and the tile holds zeros for all of them.  (With products of its own
+  // the rare case made the compiler move all of O^T from registers to others and back in every turn.)
+  __device__ __forceinline__ void take_out_not_finite(uint8_t* vt, int k0, int lane) {
+    add_not_finite(vt, k0, lane);
 #pragma unroll 1
     for (int i = 0; i < T::kBlocks; ++i) {
       u32x4* at = reinterpret_cast<u32x4*>(vt + i * 1024 + lane * 16);
@@ -300,24 +304,7 @@ struct RowState {
         }
         o[db] = E::mfma(__builtin_bit_cast(ex8, v), p[step >> 1][step & 1], o[db]);
       }
-    const int hh = lane >> 5;
-#pragma unroll 1
-    for (int key = 0; key < T::kKeys; ++key) {
-      const int j = k0 + key;
-      const bool seen = j < mine.hi && (j >= mine.lo || j < sinks);
-      const uint8_t* row = vt + key * T::kRowBytes;
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const typename E::x4 v = *reinterpret_cast<const typename E::x4*>(row + 64 * (db ^ T::swz_v(key)) + 16 * g + 8 * hh);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float f = (float)v[e];
-            if (seen && !(__builtin_fabsf(f) < INFINITY)) o[db][4 * g + e] += f;
-          }
-        }
-    }
+    add_not_finite(vt, k0, lane);
   }
 };
 
