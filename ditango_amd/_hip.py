@@ -633,8 +633,8 @@ def qk_norm_rope_axes(tensors, positions: torch.Tensor, table, norm: int, eps: f
 # A cache of pages that several requests share
 # ---------------------------------------------------------------------------------------------
 
-# Words: up to half of them for parts of few rows, one each, the others for parts of 256 rows, eight each.  The workspace has room for fewer of both, whatever the heads,
-# so that a captured launch is cut like an eager one, whose stream keeps more of them.
+# Words: up to half of them for parts of few rows, one each, the others for parts of 256 rows, eight each.  The workspace has room for fewer of both,
+# whatever the heads, so that a captured launch is cut like an eager one, whose stream keeps more of them.
 CAPTURED_COUNTERS = 1 << 14
 
 

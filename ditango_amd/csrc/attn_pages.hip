@@ -7,10 +7,11 @@
 // A request's rows (new tokens x query heads of a key head) go in tiles of 256, and what is left over in tiles of 32 where that is at most 64 or 96.
 // Batches of requests that have no more rows than that run in a kernel with few rows only; in the other one both forms run side by side.
 //
-// Many rows are bound by the matrix instructions at the power cap: two frames of 3600 tokens, 24 heads of 128, 32 400 keys each, 2.56 .. 2.64 ms, 1.1 PFLOP/s at
-// 1.66 GHz (on contiguous keys 2.45 .. 2.53); heads of 64 by softmax and products in turn (a frame of 1350 of two rollouts, 48 heads, 0.53 ms, 0.86 PFLOP/s).
-// Single tokens are bound by the memory: 8 over 3000 to 17 776 keys of 24 heads of 128, 176 us, 5.8 TB/s.  Small calls wait: 3 requests of 4 tokens 9.2 us,
-// of which 2.4 are an empty launch's, 2 go by until a workgroup has found its work, 3 until its first tile is there.
+// Many rows are bound by the matrix instructions at the power cap: two frames of 3600 tokens, 24 heads of 128, 32 400 keys each, 2.54 .. 2.64 ms, 1.1
+// PFLOP/s at 1.66 GHz (on contiguous keys 2.47 .. 2.49); heads of 64 by softmax and products in turn (a frame of 1350 of two rollouts, 48 heads, 0.51 ..
+// 0.55 ms, 0.83 .. 0.90 PFLOP/s).  Single tokens are bound by the memory: 8 over 3000 to 17 776 keys of 24 heads of 128, 176 .. 190 us, 5.4 .. 5.8 TB/s; of
+// 24 heads of 64, over 8192 keys each, 79 us, 5.1 TB/s.  Small calls wait: 3 requests of 4 tokens 9.3 us, of which 2.4 are an empty launch's, 2 go by until
+// a workgroup has found its work, 3 until its first tile is there.
 //
 // Which page holds a tile is read by scalar loads one tile ahead, so that no tile waits for it; a page is a multiple of 16 tokens, and 16 rows of a tile
 // are what a load's descriptor covers.  No host knows the lengths, so every workgroup finds its share of the work by itself: it reads all lengths and

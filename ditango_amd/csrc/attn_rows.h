@@ -478,7 +478,7 @@ __device__ __forceinline__ void walk_tiles(RowState<D, kHalf, 2>& st, const uint
   };
   // (the last tile is apart: with a way out in the middle of the loop, the compiler moves O^T to other registers and back in every turn)
   // Where the loop begins does not go by the code in front of it: 16 bytes off, the windowed attention's same instructions with heads of 64 take 1.2 % longer
-  // (4096 rows over 8192 keys of 24 heads 225.0 against 227.7 us).  Over pages no place was better than another by more than the boxes differ.
+  // (4096 rows over 8192 keys of 24 heads 225.0 against 227.7 us).  Over pages no place was better than another by more than cards differ.
   if constexpr (!kRun) asm volatile(".p2align 6" ::: "memory");
   for (int t = 0; t < n - 1; ++t) {
     __builtin_amdgcn_s_setprio(D == 64 ? 0 : 1);

@@ -6,10 +6,11 @@
 // a signed fraction of a turn in fp32, is what the sine and cosine instructions take; they are off by 1.9e-7 at most, the fraction's rounding
 // included (4 million fractions all round the turn), where the row's 16 bits are off by 2^-9 to 2^-12 of a value.
 //
-// HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two
-// runs of 4 half a section apart with rotate-half, which two lanes load and store as 16 bytes each and exchange (4 x 1802 tokens of 3 x 48 heads of 128 111 -> 95
-// us; with 8 bytes a run where a section is no multiple of 16).  It has their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of
-// 128 with an RMS norm: 64.4 us, 5.7 TB/s (two launches of the kernel with tables: 68.2, and the tables' making).
+// HBM-bound: rows x D x 2 bytes in and out, 12 bytes of positions a token.  A lane owns 4 pairs of a row: 8 neighbours with interleaved pairs, two runs of
+// 4 half a section apart with rotate-half, which two lanes load and store as 16 bytes each and exchange (4 x 1802 tokens of 48 + 48 heads of 128 with an
+// RMS norm 80.7 -> 61.9 us); with 8 bytes a run where a section is no multiple of 16 (75.7; without a norm 75.8, and 75.3 without the choice).  It has
+// their angles once for the heads of its lane group.  14 882 tokens x (24 + 24) heads of 128 with an RMS norm: 64.4 us, 5.7 TB/s (two launches of the
+// kernel with tables: 68.2, and the tables' making).
 #include <initializer_list>
 #include <type_traits>
 
@@ -67,7 +68,7 @@ __device__ __forceinline__ void load_weights4(const void* base, bool w16, int d,
 
 // A launch whose keys go into the pages of a cache, and values beside them: rows[0] are q, rows[1] k.  Tokens are packed, B = 1.  A lane group finds its
 // token's slot with its rows under way.  Values are only copied, by workgroups of their own behind the others, 16 bytes a lane: 4 x 1802 tokens of 48 heads of
-// 128, 532 MB, 95 us, 5.6 TB/s (by the lanes that rotate the keys, when it took 109: 129).
+// 128, 532 MB, 91 us, 5.8 TB/s (by the lanes that rotate the keys, when it took 109: 129).
 constexpr int kCopies = 4;       // of a lane
 struct PagedArgs : RotaryArgs {
   Pages to;

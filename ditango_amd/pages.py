@@ -26,8 +26,9 @@ _INT32 = torch.int32
 
 
 class PagePlan(NamedTuple):
-    """What a step needs to know.  The results of a plan are parts of one allocation (``lens`` with ``in_place`` apart): whoever keeps ``lens`` for long keeps the 8 bytes
-    a row of ``slots`` with it, and ``torch.save``, which refuses tensors of different types in one storage, takes clones of them."""
+    """What a step needs to know.  The results of a plan are parts of one allocation (``lens`` with ``in_place`` apart): whoever keeps ``lens`` for long
+    keeps the 8 bytes a row of ``slots`` with it, and ``torch.save``, which refuses tensors of different types in one storage, takes clones of them."""
+
     lens: torch.Tensor          # int32 [B]: tokens of each request, the new ones among them where it is served
     cu_seqlens: torch.Tensor    # int32 [B + 1]: rows of each request's new tokens
     slots: torch.Tensor         # int64 [n_tokens]: page * page_size + place of each row; -1: nowhere
@@ -43,7 +44,8 @@ def plan_pages(tables: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     holds are free: a request ends by its length going to 0, and requests may share the whole pages of a common beginning.  Requests take free pages in
     order, the lowest first, and their entries go into ``tables``.  A request whose tokens do not fit its row gets none, and from the first one that finds too
     few free pages on, no request gets any: ``served`` says whose tokens have a place; the rows of the others stay without a slot, and their length as it
-    was, so that the attention behind it needs ``served`` as well.  With ``in_place`` ``lens`` itself becomes the new lengths, for a captured step that is replayed."""
+    was, so that the attention behind it needs ``served`` as well.  With ``in_place`` ``lens`` itself becomes the new lengths, for a captured step that is
+    replayed."""
     if lens.dtype is not _INT32 or new_lens.dtype is not _INT32 or tables.dtype is not _INT32:
         raise ValueError(f"tables, lens and new_lens must be int32, got {tables.dtype}, {lens.dtype}, {new_lens.dtype}")
     return PagePlan(*_hip.plan_pages(tables, lens, new_lens, n_tokens, n_pages, page_size, in_place))
@@ -73,8 +75,8 @@ def prepare_qkv_pages(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, cu_seqlens: torch.Tensor, *,
-                    served: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None, left: Optional[int] = None, right: Optional[int] = None, frame: int = 1, sinks: int = 0,
-                    softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
+                    served: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None, left: Optional[int] = None, right: Optional[int] = None,
+                    frame: int = 1, sinks: int = 0, softmax_scale: float = 0.0, out: Optional[torch.Tensor] = None,
                     lse: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """q ``[T,H,D]`` (bf16 or fp16, D 64 or 128; H a multiple of the pages' key heads) holds the new tokens of request ``b`` in rows ``cu_seqlens[b] ..
     cu_seqlens[b + 1]``: the last ones of its ``lens[b]`` tokens, whose keys and values are in the pages already.  Returns (out ``[T,H,D]``, lse fp32
@@ -83,8 +85,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Row ``i`` of a request's ``n`` stands at position ``lens[b] - n + i`` and sees the frames that ``left``, ``right``, ``frame`` and ``sinks`` name in
     ``window.window_attention`` (``right=0``: causal, by tokens or by whole frames).  Rows that see no key, and rows that belong to no request, get 0 and an
     lse of -inf; so do the rows of a request that ``served`` (bool ``[B]``, as ``plan_pages`` makes it) leaves out, whose keys are not in the pages.  Without
-    ``served`` every request's are.  ``max_seqlen_q`` is the most rows a request has, where the caller knows it: the launch is made for that; without it for ``T``.  An entry of
-    ``tables`` that a window needs and that names no page stands for keys and values of zeros."""
+    ``served`` every request's are.  ``max_seqlen_q`` is the most rows a request has, where the caller knows it: the launch is made for that; without it
+    for ``T``.  An entry of ``tables`` that a window needs and that names no page stands for keys and values of zeros."""
     if tables.dtype is not _INT32 or lens.dtype is not _INT32 or cu_seqlens.dtype is not _INT32:
         raise ValueError(f"tables, lens and cu_seqlens must be int32, got {tables.dtype}, {lens.dtype}, {cu_seqlens.dtype}")
     if served is not None and served.dtype is not torch.bool:
